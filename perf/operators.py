@@ -179,7 +179,8 @@ def plain_adjusted(s):
         begin = s["shown_begin"]
         row = torch.repeat_interleave(torch.arange(n, device=x.device), begin[1:] - begin[:-1], output_size=s["shown"].numel())
         count = torch.zeros(C * n, device=x.device).index_add_(0, s["shown"].long() * n + row, torch.ones(row.numel(), device=x.device)).view(C, n)
-        less = torch.where(x > 0, x / s["repetition"], x * s["repetition"]) - s["frequency"] * count - s["presence"]
+        by = torch.full((), s["repetition"], device=x.device)  # (a tensor, so that it is divided by, not multiplied by its inverse)
+        less = torch.where(x > 0, x / by, x * by) - s["frequency"] * count - s["presence"]
         x = torch.where(count > 0, less, x)
     if s["allowed"] is not None:
         cls = torch.arange(C, device=x.device)
@@ -307,7 +308,8 @@ def exact_adjusted(s):
         assert bool(((last - first) >= 0).all())
         pair, times = torch.unique(row * C + s["shown"].long(), return_counts=True)
         old = x.view(-1)[pair]
-        new = torch.where(old > 0, old / s["repetition"], old * s["repetition"])
+        strength = torch.tensor(s["repetition"], device=x.device)
+        new = torch.where(old > 0, torch.div(old, strength), old * strength)
         new = new - s["frequency"] * times.to(torch.float32)
         x.view(-1)[pair] = new - s["presence"]
     if s["allowed"] is not None:
