@@ -225,6 +225,49 @@ void tgbm_release_memory(void);
 int tgbm_cut_points(int row_size, int n_features, const float *val, const int *row_ptr, const int *col_ptr,
                     int max_num_bin, float *cut_val, int *cut_row_ptr, int *cut_fid, int *bin_id);
 
+/* ------------------------------------------------------- Part 3: operators on class scores
+ *
+ * They work on class scores that lie on the GPU (every pointer in this part is a device pointer of the current device,
+ * but for those to the structs themselves), go to the stream that they are given (a hipStream_t; NULL: the default stream), allocate nothing,
+ * wait for nothing and can be recorded into a HIP graph. Outputs do not depend on what else runs. They return 0, or 1
+ * with a message on stderr when an argument is refused (nothing is launched then), or 2 when a launch failed.
+ * They have no counterpart in the reference. */
+
+#define TGBM_F32 0
+#define TGBM_F16 1
+#define TGBM_BF16 2
+
+/* The score of class c in row i is data[c * class_stride + i * row_stride]; one of the strides is 1: row_stride where the
+ * rows of a class lie side by side, as trainers and predictors hold them, class_stride where the classes of a row do. */
+typedef struct tgbm_scores {
+    const void *data;
+    long long class_stride, row_stride;
+    int type; /* TGBM_F32, TGBM_F16, TGBM_BF16 */
+    int classes, rows;
+} tgbm_scores;
+
+/* What is known besides the scores. s = score + bias[class]; a class that the row was shown m > 0 times:
+ * s = (s > 0 ? s / repetition : s * repetition) - frequency * m - presence; a class that is not allowed: -infinity,
+ * whatever its score is. Each step is one operation in 32 bits.
+ * allowed: [allowed_sets][(classes + 31) / 32] words, bit c % 32 of word c / 32 says whether class c is allowed;
+ * allowed_set: the rows' sets, a negative number allows everything, one that is no set's nothing; without it there is one
+ * set for all rows, or one for each. shown: the rows' lists one behind the other, n_shown classes in all; row i's is
+ * [shown_begin[i], shown_begin[i + 1]); numbers that are no classes are skipped. Parts that are NULL are left out. */
+typedef struct tgbm_score_rules {
+    const float *bias;
+    const unsigned *allowed;
+    const int *allowed_set;
+    const int *shown;
+    const long long *shown_begin;
+    long long n_shown;
+    int allowed_sets;
+    float repetition, frequency, presence;
+} tgbm_score_rules;
+
+/* out = the scores as the rules leave them, rounded once to their type. out: another array of the same type, classes and
+ * rows, in either order, or `in` itself. */
+int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,101 @@
+"""Refusals of the operators on class scores: nothing is launched, so no GPU is needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import thundergbm_amd as T
+from thundergbm_amd import scores as S
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return T.load()
+
+
+ADDRESS = 1 << 20  # (never followed)
+
+
+def array(data=ADDRESS, class_stride=10, row_stride=1, kind=0, classes=4, rows=10):
+    return S._Scores(data, class_stride, row_stride, kind, classes, rows)
+
+
+def rules(**fields):
+    r = S._Rules(repetition=1.0)
+    for k, v in fields.items():
+        setattr(r, k, v)
+    return r
+
+
+BAD_ARRAYS = [
+    (dict(kind=3), "unknown type"),
+    (dict(kind=-1), "unknown type"),
+    (dict(classes=0), "0 classes"),
+    (dict(classes=(1 << 30) + 1), "classes"),
+    (dict(rows=-1), "-1 rows"),
+    (dict(data=None), "null data"),
+    (dict(class_stride=9), "strides 9 and 1"),
+    (dict(class_stride=0), "strides 0 and 1"),
+    (dict(class_stride=-10), "strides -10 and 1"),
+    (dict(class_stride=2, row_stride=8), "strides 2 and 8"),
+    (dict(class_stride=1, row_stride=3), "strides 1 and 3"),
+    (dict(class_stride=1, row_stride=0), "strides 1 and 0"),
+]
+BAD_RULES = [
+    (dict(allowed=ADDRESS, allowed_sets=0), "0 allowed sets"),
+    (dict(allowed=ADDRESS, allowed_sets=9), "9 allowed sets for 10 rows"),
+    (dict(allowed_set=ADDRESS), "allowed_set without allowed"),
+    (dict(shown=ADDRESS, n_shown=3), "shown without shown_begin"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=-1), "n_shown is -1"),
+    (dict(shown_begin=ADDRESS, n_shown=2), "shown_begin without shown"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=2, repetition=0.0), "repetition is 0"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=2, repetition=-1.0), "repetition is -1"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=2, repetition=float("nan")), "repetition is nan"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=2, frequency=float("inf")), "frequency inf"),
+    (dict(shown=ADDRESS, shown_begin=ADDRESS, n_shown=2, presence=float("nan")), "presence"),
+]
+
+
+@pytest.mark.parametrize("fields,msg", BAD_ARRAYS)
+def test_adjust_refuses_arrays(lib, capfd, fields, msg):
+    for pair in ((array(**fields), array()), (array(), array(**fields))):
+        assert lib.tgbm_scores_adjust(C.byref(pair[0]), C.byref(rules()), C.byref(pair[1]), None) == 1
+        err = capfd.readouterr().err
+        assert err.startswith("tgbm_scores_adjust: ") and msg in err
+
+
+@pytest.mark.parametrize("fields,msg", BAD_RULES)
+def test_adjust_refuses_rules(lib, capfd, fields, msg):
+    assert lib.tgbm_scores_adjust(C.byref(array()), C.byref(rules(**fields)), C.byref(array(data=2 * ADDRESS)), None) == 1
+    assert msg in capfd.readouterr().err
+
+
+def test_adjust_refuses_pairs_and_nulls(lib, capfd):
+    good, r = array(), rules()
+    for args in ((None, r, good), (good, None, good), (good, r, None), (good, r, array(rows=9)), (good, r, array(kind=1)),
+                 (good, r, array(classes=3)), (good, r, array(class_stride=1, row_stride=4))):
+        assert lib.tgbm_scores_adjust(*(C.byref(a) if a is not None else None for a in args), None) == 1
+        assert capfd.readouterr().err.startswith("tgbm_scores_adjust: ")
+
+
+def test_no_rows_are_no_work(lib):
+    assert lib.tgbm_scores_adjust(C.byref(array(rows=0, data=None)), C.byref(rules()), C.byref(array(rows=0, data=None)), None) == 0
+
+
+def test_tensors_on_the_host_are_refused():
+    x = torch.zeros(3, 5)
+    with pytest.raises(ValueError, match="on the GPU"):
+        S.adjust(x)
+    with pytest.raises(ValueError, match="torch tensor"):
+        S.adjust(np.zeros((3, 5), np.float32))
+
+
+def test_parts_of_one_array_are_told_apart():
+    at = lambda data, width, pitch: S._Scores(ADDRESS + data, pitch, 1, 0, 4, width)
+    assert S._apart(at(0, 4, 10), at(16, 4, 10), 4)
+    assert S._apart(at(16, 4, 10), at(0, 4, 10), 4)
+    assert S._apart(at(0, 5, 10), at(20, 5, 10), 4)
+    assert not S._apart(at(0, 4, 10), at(12, 4, 10), 4)
+    assert not S._apart(at(0, 4, 10), at(28, 4, 10), 4)
+    assert not S._apart(at(0, 4, 10), at(16, 4, 9), 4)

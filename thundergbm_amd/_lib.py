@@ -56,6 +56,7 @@ SIGNATURES = {
     "tgbm_predict_raw_noalloc": (C.c_int, [C.c_int, _P, _P, _P, _P, C.c_int, C.c_int, C.c_float, C.c_float, _P]),
     "tgbm_release_memory": (None, []),
     "tgbm_cut_points": (C.c_int, [C.c_int, C.c_int, _P, _P, _P, C.c_int, _P, _P, _P, _P]),
+    "tgbm_scores_adjust": (C.c_int, [_P, _P, _P, _P]),
 }
 
 

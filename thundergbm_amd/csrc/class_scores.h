@@ -1,0 +1,21 @@
+// Operators on class scores that lie on the GPU: adjusting them before an answer, the best classes of every row, and the
+// loss against a teacher's top scores (the tgbm_scores_* entry points). Launchers are stream-ordered, allocate nothing and
+// never synchronise; the entry points (scores_api.hip) have checked the arguments. None has a counterpart in the reference,
+// whose answers are its arg-max and its softmax over the raw scores (multiclass_obj.cu:44-88) and whose multi-class loss
+// knows labels only (multiclass_obj.cu:6-35).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/thundergbm.h"
+#include "common.h"
+
+namespace tgbm {
+
+constexpr int kTopMost = 128;      // classes that top lists
+constexpr int kTeacherMost = 128;  // entries of a teacher's row
+
+inline bool rows_side_by_side(const tgbm_scores &s) { return !(s.class_stride == 1 && (s.rows == 1 || s.row_stride != 1)); }
+
+void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out);
+
+}  // namespace tgbm

@@ -1,0 +1,82 @@
+// extern "C" layer of the operators on class scores (part 3 of include/thundergbm.h). Nothing here throws or aborts: what
+// cannot be done is said on stderr and returned.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "class_scores.h"
+
+using namespace tgbm;
+
+namespace {
+
+int refused(const char *entry, const char *fmt, ...) {
+    char text[256];
+    va_list args;
+    va_start(args, fmt);
+    std::vsnprintf(text, sizeof(text), fmt, args);
+    va_end(args);
+    std::fprintf(stderr, "%s: %s\n", entry, text);
+    std::fflush(stderr);
+    return 1;
+}
+
+int launched(const char *entry) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    std::fprintf(stderr, "%s: launch failed: %s\n", entry, hipGetErrorString(e));
+    std::fflush(stderr);
+    return 2;
+}
+
+// 0 when the array can be worked on
+int check_scores(const char *entry, const char *what, const tgbm_scores *s) {
+    if (s == nullptr) return refused(entry, "%s is null", what);
+    if (s->type != TGBM_F32 && s->type != TGBM_F16 && s->type != TGBM_BF16) return refused(entry, "%s: unknown type %d", what, s->type);
+    if (s->classes < 1 || s->classes > 1 << 30) return refused(entry, "%s: %d classes", what, s->classes);
+    if (s->rows < 0) return refused(entry, "%s: %d rows", what, s->rows);
+    if (s->rows > 0 && s->data == nullptr) return refused(entry, "%s: null data", what);
+    const bool columns = s->row_stride == 1 && (s->classes == 1 || s->class_stride >= s->rows);
+    const bool rows = s->class_stride == 1 && (s->rows <= 1 || s->row_stride >= s->classes);
+    const bool one_row = s->rows <= 1 && s->class_stride >= 1;
+    if (!columns && !rows && !one_row)
+        return refused(entry, "%s: strides %lld and %lld of %d classes and %d rows: one of them is 1, the other one at least as long", what, s->class_stride,
+                       s->row_stride, s->classes, s->rows);
+    return 0;
+}
+
+int check_rules(const char *entry, const tgbm_score_rules *r, int rows) {
+    if (r == nullptr) return refused(entry, "rules is null");
+    if (r->allowed != nullptr) {
+        if (r->allowed_sets < 1) return refused(entry, "%d allowed sets", r->allowed_sets);
+        if (r->allowed_set == nullptr && r->allowed_sets != 1 && r->allowed_sets < rows)
+            return refused(entry, "%d allowed sets for %d rows, and no allowed_set", r->allowed_sets, rows);
+    } else if (r->allowed_set != nullptr) {
+        return refused(entry, "allowed_set without allowed");
+    }
+    if (r->shown != nullptr) {
+        if (r->shown_begin == nullptr) return refused(entry, "shown without shown_begin");
+        if (r->n_shown < 0) return refused(entry, "n_shown is %lld", r->n_shown);
+        if (!(r->repetition > 0.f) || !std::isfinite(r->repetition)) return refused(entry, "repetition is %g: a number above 0 is wanted", r->repetition);
+        if (!std::isfinite(r->frequency) || !std::isfinite(r->presence)) return refused(entry, "frequency %g, presence %g", r->frequency, r->presence);
+    } else if (r->shown_begin != nullptr && r->n_shown != 0) {
+        return refused(entry, "shown_begin without shown");
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream) {
+    const char *entry = "tgbm_scores_adjust";
+    int rc = check_scores(entry, "in", in);
+    if (rc == 0) rc = check_scores(entry, "out", out);
+    if (rc == 0) rc = check_rules(entry, rules, in->rows);
+    if (rc != 0) return rc;
+    if (out->type != in->type || out->classes != in->classes || out->rows != in->rows) return refused(entry, "out is not of in's type and sizes");
+    if (in->data == out->data && (in->class_stride != out->class_stride || in->row_stride != out->row_stride))
+        return refused(entry, "out is in's memory with other strides");
+    if (in->rows == 0) return 0;
+    launch_scores_adjust(static_cast<hipStream_t>(stream), *in, *rules, *out);
+    return launched(entry);
+}

@@ -1,0 +1,184 @@
+"""Operators on class scores that lie on the GPU, as torch tensors (tgbm_scores_*): what is known besides the model is put on
+the scores (`adjust`). torch is imported by the caller, never here.
+
+Scores are [classes, rows], float32, float16 or bfloat16, in either order: the rows of a class side by side, as trainers and
+predictors hold them, or the classes of a row side by side (`x.t()` of a [rows, classes] tensor). Everything is launched on
+torch's current stream of the tensors' device; nothing waits, and calls can be captured into a graph. Wrong arguments
+raise ValueError before anything is launched. The calls take no part in autograd: a tensor that requires a gradient is refused.
+"""
+import ctypes as C
+import math
+import sys
+
+from . import _lib
+
+
+class _Scores(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("class_stride", C.c_longlong), ("row_stride", C.c_longlong), ("type", C.c_int),
+                ("classes", C.c_int), ("rows", C.c_int)]
+
+
+class _Rules(C.Structure):
+    _fields_ = [("bias", C.c_void_p), ("allowed", C.c_void_p), ("allowed_set", C.c_void_p), ("shown", C.c_void_p),
+                ("shown_begin", C.c_void_p), ("n_shown", C.c_longlong), ("allowed_sets", C.c_int), ("repetition", C.c_float),
+                ("frequency", C.c_float), ("presence", C.c_float)]
+
+
+_types = None
+
+
+def _torch():
+    """The caller's torch, and the numbers of the types."""
+    global _types
+    torch = sys.modules.get("torch")
+    if torch is None:
+        raise ValueError("the scores are torch tensors")
+    if _types is None:
+        _types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return torch
+
+
+def _is(condition, *what):
+    if not condition:
+        raise ValueError(what[0] % what[1:] if len(what) > 1 else what[0])
+
+
+def _on_gpu(torch, name, x):
+    if not isinstance(x, torch.Tensor):
+        raise ValueError("%s: a torch tensor is wanted, got %s" % (name, type(x).__name__))
+    if not x.is_cuda:
+        raise ValueError("%s: a tensor on the GPU is wanted" % name)
+    if x.requires_grad:
+        raise ValueError("%s requires a gradient: these operators take no part in autograd (detach it)" % name)
+
+
+def _scores(torch, name, x):
+    _on_gpu(torch, name, x)
+    kind = _types.get(x.dtype)
+    if kind is None:
+        raise ValueError("%s: float32, float16 or bfloat16 is wanted, got %s" % (name, x.dtype))
+    if x.dim() != 2:
+        raise ValueError("%s: [classes, rows] is wanted, got %d dimensions" % (name, x.dim()))
+    classes, rows = x.shape
+    by_class, by_row = x.stride()
+    if classes < 1 or classes > 1 << 30 or rows >= 1 << 31:
+        raise ValueError("%s: %d classes, %d rows" % (name, classes, rows))
+    if classes == 1:  # (the stride along a single class says nothing)
+        by_class = max(by_class, rows, 1) if by_row == 1 else 1
+    if rows <= 1:
+        by_row = max(by_row, classes) if by_class == 1 else 1
+    if not (by_row == 1 and by_class >= rows) and not (by_class == 1 and by_row >= classes):
+        raise ValueError("%s: strides %s of a tensor %s: the rows of a class or the classes of a row lie side by side"
+                         % (name, tuple(x.stride()), tuple(x.shape)))
+    return _Scores(x.data_ptr(), by_class, by_row, kind, classes, rows)
+
+
+def _plain(torch, name, x, like, dtype, shape):
+    """A contiguous tensor of one type, on the scores' device."""
+    _on_gpu(torch, name, x)
+    if x.dtype != dtype:
+        raise ValueError("%s: %s is wanted, got %s" % (name, dtype, x.dtype))
+    if x.device != like.device:
+        raise ValueError("%s is on %s, the scores are on %s" % (name, x.device, like.device))
+    if tuple(x.shape) != shape:
+        raise ValueError("%s: the shape %s is wanted, got %s" % (name, shape, tuple(x.shape)))
+    if not x.is_contiguous():
+        raise ValueError("%s: a contiguous tensor is wanted" % name)
+    return x.data_ptr()
+
+
+def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence):
+    classes, rows = scores.shape
+    r = _Rules(repetition=1.0)
+    if bias is not None:
+        r.bias = _plain(torch, "bias", bias, scores, torch.float32, (classes,))
+    if allowed is not None:
+        _on_gpu(torch, "allowed", allowed)
+        if allowed.dim() != 2 or allowed.shape[0] < 1:
+            raise ValueError("allowed: [sets, (classes + 31) // 32] is wanted, got %s" % (tuple(allowed.shape),))
+        sets = allowed.shape[0]
+        r.allowed = _plain(torch, "allowed", allowed, scores, torch.int32, (sets, (classes + 31) // 32))
+        r.allowed_sets = sets
+        if allowed_set is not None:
+            r.allowed_set = _plain(torch, "allowed_set", allowed_set, scores, torch.int32, (rows,))
+        elif sets != 1 and sets != rows:
+            raise ValueError("allowed: %d sets for %d rows: which one is a row's says allowed_set" % (sets, rows))
+    elif allowed_set is not None:
+        raise ValueError("allowed_set without allowed")
+    if (shown is None) != (shown_begin is None):
+        raise ValueError("shown and shown_begin belong together")
+    if shown is not None:
+        r.shown_begin = _plain(torch, "shown_begin", shown_begin, scores, torch.int64, (rows + 1,))
+        if shown.dim() != 1:
+            raise ValueError("shown: one dimension is wanted, got %d" % shown.dim())
+        r.n_shown = shown.numel()
+        # (an empty tensor has no address, and no list is like empty lists)
+        r.shown = _plain(torch, "shown", shown, scores, torch.int32, (shown.numel(),)) if shown.numel() else None
+        if not shown.numel():
+            r.shown_begin = None
+        if not (repetition > 0 and math.isfinite(repetition)):
+            raise ValueError("repetition is %r: a number above 0 is wanted" % (repetition,))
+        if not (math.isfinite(frequency) and math.isfinite(presence)):
+            raise ValueError("frequency is %r, presence is %r: numbers are wanted" % (frequency, presence))
+        r.repetition, r.frequency, r.presence = repetition, frequency, presence
+    return r
+
+
+def _call(torch, scores, name, *args):
+    """One call of the library on the current stream of the scores' device."""
+    fn = getattr(_lib.load(), name)
+    device = scores.device.index
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise (ValueError if rc == 1 else RuntimeError)("%s failed; it has said why on stderr" % name)
+
+
+def adjust(scores, bias=None, allowed=None, allowed_set=None, shown=None, shown_begin=None, repetition=1.0, frequency=0.0,
+           presence=0.0, out=None):
+    """The scores with what is known besides them, in their type and order.
+
+    bias: float32 [classes], added to every row's scores.
+    shown, shown_begin: classes that the rows were shown before, int32 lists one behind the other, and where they begin, int64
+      [rows + 1]. A score s of a class that the row was shown m times becomes (s / repetition if s > 0 else s * repetition) -
+      frequency * m - presence. Numbers that are no classes are skipped.
+    allowed: int32 [sets, (classes + 31) // 32], bit c % 32 of word c // 32 says whether class c is allowed; the others'
+      scores become -inf. One set for all rows, one for each, or with allowed_set, int32 [rows], the rows' sets: a negative
+      number allows everything, one that is no set's nothing.
+    out: where the result goes; `scores` itself, or memory apart from it."""
+    torch = _torch()
+    s = _scores(torch, "scores", scores)
+    r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
+    if out is None:
+        # (in the scores' order, without the gaps that a part of a larger array has)
+        if s.class_stride == 1 and s.rows > 1:
+            out = torch.empty((s.rows, s.classes), dtype=scores.dtype, device=scores.device).t()
+        else:
+            out = torch.empty((s.classes, s.rows), dtype=scores.dtype, device=scores.device)
+    elif not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != scores.device:
+        raise ValueError("out: a tensor of the scores' type, shape and device is wanted")
+    o = _scores(torch, "out", out)
+    if s.rows:
+        if o.data == s.data:
+            if (o.class_stride, o.row_stride) != (s.class_stride, s.row_stride):
+                raise ValueError("out is the scores' memory in another order")
+        else:
+            size = scores.element_size()
+            ends = [x.data + ((x.classes - 1) * x.class_stride + (x.rows - 1) * x.row_stride + 1) * size for x in (s, o)]
+            # (two parts of one array may lie between each other's rows: what counts is that they have the same strides then)
+            if o.data < ends[0] and s.data < ends[1] and not _apart(s, o, size):
+                raise ValueError("out overlaps the scores")
+        _call(torch, scores, "tgbm_scores_adjust", C.byref(s), C.byref(r), C.byref(o))
+    return out
+
+
+def _apart(s, o, size):
+    """Whether two arrays whose memory is interleaved share no element: parts of one larger array, side by side."""
+    if (s.class_stride, s.row_stride) != (o.class_stride, o.row_stride):
+        return False
+    pitch, width = (s.class_stride, s.rows) if s.row_stride == 1 else (s.row_stride, s.classes)
+    at = abs(o.data - s.data) // size % pitch
+    return width <= at <= pitch - width
