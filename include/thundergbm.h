@@ -268,6 +268,16 @@ typedef struct tgbm_score_rules {
  * rows, in either order, or `in` itself. */
 int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream);
 
+/* The k (1 to 128) best classes of every row by the scores as the rules leave them, and the logarithm of the sum of
+ * exp(score / temperature) over all classes: exp(value / temperature - lse) is a listed class's probability. values and
+ * classes are [rows][k], the best first, of equal scores the lower class; a class whose score is -infinity or NaN is not
+ * listed, and what is left of a list is class -1 with -infinity. lse, [rows], is -infinity where nothing is allowed and
+ * NaN where a score is that is not taken out. temperature: 1e-6 to 1e6. workspace: as many bytes as
+ * tgbm_scores_top_workspace says, whose only use is during the call's work on the stream. */
+size_t tgbm_scores_top_workspace(const tgbm_scores *in, int k);
+int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes,
+                    float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

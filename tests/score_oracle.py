@@ -54,3 +54,21 @@ def adjusted(z, bias=None, allowed=None, allowed_set=None, shown=None, shown_beg
         s = np.where(m > 0, less, s)
         assert s.dtype == f
         return np.where(allowed_table(allowed, allowed_set, C, n), s, f(-np.inf))
+
+
+def top(x, k, temperature=1.0):
+    """x: adjusted scores, float32 [classes, rows]. The k best of every row and the log-sum-exp."""
+    C, n = x.shape
+    values = np.full((n, k), -np.inf, np.float32)
+    classes = np.full((n, k), -1, np.int32)
+    lse = np.zeros(n)
+    for i in range(n):
+        s = x[:, i]
+        listed = np.flatnonzero(s > -np.inf)  # (no NaN either)
+        best = listed[np.argsort(-s[listed].astype(np.float64), kind="stable")][:k]
+        values[i, :len(best)], classes[i, :len(best)] = s[best], best
+        t = s.astype(np.float64) / temperature
+        m = t.max() if not np.isnan(t).any() else np.nan
+        with np.errstate(all="ignore"):
+            lse[i] = m if not np.isfinite(m) else m + np.log(np.exp(t - m).sum())
+    return values, classes, lse

@@ -99,3 +99,37 @@ def test_parts_of_one_array_are_told_apart():
     assert not S._apart(at(0, 4, 10), at(12, 4, 10), 4)
     assert not S._apart(at(0, 4, 10), at(28, 4, 10), 4)
     assert not S._apart(at(0, 4, 10), at(16, 4, 9), 4)
+
+
+def test_top_refuses(lib, capfd):
+    good, r = array(), rules()
+
+    def call(a=good, rule=r, k=3, temperature=1.0, outs=(ADDRESS,) * 3, room=ADDRESS, size=1 << 20):
+        return lib.tgbm_scores_top(C.byref(a), C.byref(rule), k, temperature, *outs, room, size, None)
+
+    for fields, msg in BAD_ARRAYS:
+        assert call(a=array(**fields)) == 1 and msg in capfd.readouterr().err
+    for fields, msg in BAD_RULES:
+        assert call(rule=rules(**fields)) == 1 and msg in capfd.readouterr().err
+    large = array(class_stride=1, row_stride=100_000, classes=100_000, rows=2)
+    needed = lib.tgbm_scores_top_workspace(C.byref(large), 5)
+    assert needed > 0
+    for more, msg in ((dict(k=0), "k is 0"), (dict(k=129), "k is 129"), (dict(temperature=0.0), "temperature"), (dict(temperature=float("inf")), "temperature"),
+                      (dict(outs=(None, ADDRESS, ADDRESS)), "null"), (dict(outs=(ADDRESS, ADDRESS, None)), "null"),
+                      (dict(a=large, k=5, size=needed - 1), "workspace"), (dict(a=large, k=5, room=None, size=needed), "workspace")):
+        assert call(**more) == 1 and msg in capfd.readouterr().err
+    assert call(a=array(rows=0)) == 0
+
+
+@pytest.mark.parametrize("by_class", [True, False])
+def test_top_workspace(lib, by_class):
+    """No workspace for a row that goes in one piece, none asked for by a call that is refused, and always room for the chunks."""
+    for classes in (1, 32, 33, 1024, 1025, 16_384, 16_385, 1 << 20, 1 << 30):
+        for rows in (1, 2, 100, 5000, 100_000):
+            a = array(class_stride=rows, row_stride=1, classes=classes, rows=rows) if by_class else array(class_stride=1, row_stride=classes, classes=classes, rows=rows)
+            for k in (1, 10, 128):
+                size = lib.tgbm_scores_top_workspace(C.byref(a), k)
+                chunks = (classes - 1) // (1024 if by_class and rows > 1 else 16_384) + 1
+                assert size >= (rows * chunks * (8 * k + 8) if chunks > 1 else 0)
+                assert classes > 32 or size == 0
+                assert lib.tgbm_scores_top_workspace(C.byref(a), 0) == lib.tgbm_scores_top_workspace(C.byref(a), 129) == 0

@@ -189,3 +189,124 @@ def test_adjust_on_a_stream_and_in_a_graph():
         torch.cuda.synchronize()
         same(captured, O.adjusted(z2, **r))
         same(other, O.adjusted(np.zeros_like(z2), **r))
+
+
+def check_top(got, x, k, temperature=1.0):
+    values, classes, lse = got
+    want_values, want_classes, want_lse = O.top(x, k, temperature)
+    np.testing.assert_array_equal(classes.cpu().numpy(), want_classes)
+    same(values, want_values)
+    # Half steps of 2^-24: three in the argument of an exponential, which its weight makes at most ln C of on average, two in
+    # its value, one for every addition in a row (at most 32 + 6 + 16 + 9), two in the quotient and the sum with it, four
+    # in the logarithm.
+    lse, C = lse.cpu().numpy().astype(np.float64), x.shape[0]
+    fine = np.isfinite(want_lse)
+    np.testing.assert_array_equal(lse[~fine], want_lse[~fine])
+    with np.errstate(all="ignore"):
+        largest = np.abs(np.where(fine, x.max(0), 0) / temperature)
+    room = 2.0**-24 * (7 * np.log(C) + 70 + np.where(fine, largest + np.abs(want_lse), 0))
+    assert np.all(np.abs(lse[fine] - want_lse[fine]) <= room[fine])
+
+
+@pytest.mark.parametrize("order", ["class", "row"])
+@pytest.mark.parametrize("C,n", SIZES + [(2, 300), (17, 77), (32, 500), (64, 130), (512, 9), (1024, 33), (2048, 5), (2049, 600)])
+def test_top(C, n, order):
+    rng = np.random.default_rng(C * 11 + n)
+    for j, dtype in enumerate(TYPES):
+        special = (0.1, 0.0, 0.02)[j]
+        z = rounded(D.scores(rng, C, n, special=special), dtype)
+        r = D.rules(rng, C, n, bias=j != 1, sets=("each", "none", "some")[j], shown=j != 2, longest=9)
+        x = O.adjusted(z, **r)
+        for k, temperature in ((1, 1.0), (min(C, 7), 0.5), (128 if j else 64, 3.0)):
+            check_top(S.top(place(z, order, dtype, pad=j, shift=j), k, temperature=temperature, **on_gpu(r)), x, k, temperature)
+
+
+@pytest.mark.parametrize("order", ["class", "row"])
+@pytest.mark.parametrize("C,n", [(30, 40), (1000, 20), (5000, 3), (40_000, 2)])
+def test_top_equal_scores(C, n, order):
+    """All equal, two values, one class allowed, nothing allowed, the lowest number, infinities."""
+    rng = np.random.default_rng(9)
+    z = np.zeros((C, n), np.float32)
+    for k in (1, 5, 128):
+        check_top(S.top(place(z, order), k), z, k)
+        z2 = (rng.random((C, n)) < 0.5).astype(np.float32) * np.where(rng.random((C, n)) < 0.5, 0.0, -0.0).astype(np.float32)
+        z2[rng.random((C, n)) < 0.01] = 1
+        check_top(S.top(place(z2, order), k), z2, k)
+        z3 = np.full((C, n), -np.inf, np.float32)
+        z3[rng.integers(0, C, n), np.arange(n)] = -3.4028235e38
+        check_top(S.top(place(z3, order), k), z3, k)
+        z3[:, ::2] = -np.inf
+        z3[C // 2:, 1::2] = 3.4028235e38
+        check_top(S.top(place(z3, order), k), z3, k)
+        z3[C // 3, :] = np.inf
+        z3[C // 4, 0] = np.inf
+        check_top(S.top(place(z3, order), k), z3, k)
+        z3[C // 5, 0] = np.nan
+        check_top(S.top(place(z3, order), k), z3, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["class", "row"])
+@pytest.mark.parametrize("C", [700, 1024, 2048, 8192, 16_384, 40_000])
+def test_top_best_in_few_threads(C, order, dtype):
+    """The best classes at distances at which one thread, or one wavefront, holds all of them: more candidates than the list takes."""
+    rng = np.random.default_rng(C)
+    rows = []
+    for step in (64, 256, 512, 1024, 2048, 4096):
+        for run in (1, 4, 8):
+            z = rng.standard_normal(C).astype(np.float32)
+            at = np.arange(C)
+            z[at % step < run] += 100
+            rows.append(z)
+            rows.append(np.where(at % step < run, 2.0, np.round(z / 50)).astype(np.float32))
+    rows.append(np.sort(rng.standard_normal(C)).astype(np.float32))
+    rows.append(rows[-1][::-1].copy())
+    z = rounded(np.stack(rows, 1), dtype)
+    for k in (3, 64, 128):
+        check_top(S.top(place(z, order, dtype), k), z, k)
+
+
+def test_top_chunks_of_chunks():
+    """So many classes that the chunks' best ones are joined twice."""
+    C = 300_000
+    z = D.scores(np.random.default_rng(1), C, 2)
+    check_top(S.top(place(z, "class"), 128), z, 128)
+    check_top(S.top(place(z, "row"), 128), z, 128)
+
+
+def test_top_refuses():
+    x = torch.zeros(8, 10, device="cuda")
+    for more, msg in ((dict(k=0), "k is 0"), (dict(k=129), "k is 129"), (dict(k=1.5), "k is 1.5"), (dict(k=2, temperature=0.0), "temperature"),
+                      (dict(k=2, temperature=float("nan")), "temperature"), (dict(k=2, bias=torch.zeros(7, device="cuda")), "bias"),
+                      (dict(scores=x.int(), k=2), "float32")):
+        with pytest.raises(ValueError, match=msg):
+            S.top(**dict(dict(scores=x), **more))
+    values, classes, lse = S.top(torch.zeros(5, 0, device="cuda"), 3)
+    assert values.shape == classes.shape == (0, 3) and lse.shape == (0,)
+
+
+def test_top_two_graphs():
+    """Two captured calls of different sizes and an eager one take turns: each has its own workspace."""
+    rng = np.random.default_rng(8)
+    shapes = [(40_000, 3, 64), (5000, 7, 20), (300, 500, 10)]
+    graphs = []
+    for C, n, k in shapes:
+        x = place(D.scores(rng, C, n), "row")
+        S.top(x, k)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = S.top(x, k)
+        graphs.append((graph, x, k, got))
+    for _ in range(3):
+        news = []
+        for graph, x, k, got in graphs:
+            z = D.scores(rng, *x.shape)
+            x.copy_(torch.from_numpy(z))
+            news.append(z)
+        for graph, *_ in graphs:
+            graph.replay()
+        eager = S.top(graphs[0][1], 5)
+        for (graph, x, k, got), z in zip(graphs, news):
+            check_top(got, z, k)
+        check_top(eager, news[0], 5)

@@ -18,4 +18,8 @@ inline bool rows_side_by_side(const tgbm_scores &s) { return !(s.class_stride ==
 
 void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out);
 
+size_t scores_top_workspace(bool columns, int classes, int rows, int k);
+void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
+                       void *workspace);
+
 }  // namespace tgbm

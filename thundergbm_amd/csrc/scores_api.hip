@@ -65,6 +65,10 @@ int check_rules(const char *entry, const tgbm_score_rules *r, int rows) {
     return 0;
 }
 
+int check_temperature(const char *entry, float t) {
+    return t >= 1e-6f && t <= 1e6f ? 0 : refused(entry, "temperature is %g: 1e-6 to 1e6 is wanted", t);
+}
+
 }  // namespace
 
 extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream) {
@@ -78,5 +82,26 @@ extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules 
         return refused(entry, "out is in's memory with other strides");
     if (in->rows == 0) return 0;
     launch_scores_adjust(static_cast<hipStream_t>(stream), *in, *rules, *out);
+    return launched(entry);
+}
+
+extern "C" size_t tgbm_scores_top_workspace(const tgbm_scores *in, int k) {
+    if (check_scores("tgbm_scores_top_workspace", "in", in) != 0 || k < 1 || k > kTopMost || in->rows == 0) return 0;
+    return scores_top_workspace(rows_side_by_side(*in), in->classes, in->rows, k);
+}
+
+extern "C" int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes, float *lse,
+                               void *workspace, size_t workspace_bytes, void *stream) {
+    const char *entry = "tgbm_scores_top";
+    int rc = check_scores(entry, "in", in);
+    if (rc == 0) rc = check_rules(entry, rules, in->rows);
+    if (rc == 0) rc = check_temperature(entry, temperature);
+    if (rc != 0) return rc;
+    if (k < 1 || k > kTopMost) return refused(entry, "k is %d: 1 to %d is wanted", k, kTopMost);
+    if (in->rows == 0) return 0;
+    if (values == nullptr || classes == nullptr || lse == nullptr) return refused(entry, "an output is null");
+    const size_t needed = scores_top_workspace(rows_side_by_side(*in), in->classes, in->rows, k);
+    if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
+    launch_scores_top(static_cast<hipStream_t>(stream), *in, *rules, k, temperature, values, classes, lse, workspace);
     return launched(entry);
 }

@@ -1,5 +1,5 @@
 """Operators on class scores that lie on the GPU, as torch tensors (tgbm_scores_*): what is known besides the model is put on
-the scores (`adjust`). torch is imported by the caller, never here.
+the scores (`adjust`), the best classes of every row are listed (`top`). torch is imported by the caller, never here.
 
 Scores are [classes, rows], float32, float16 or bfloat16, in either order: the rows of a class side by side, as trainers and
 predictors hold them, or the classes of a row side by side (`x.t()` of a [rows, classes] tensor). Everything is launched on
@@ -173,6 +173,34 @@ def adjust(scores, bias=None, allowed=None, allowed_set=None, shown=None, shown_
                 raise ValueError("out overlaps the scores")
         _call(torch, scores, "tgbm_scores_adjust", C.byref(s), C.byref(r), C.byref(o))
     return out
+
+
+def top(scores, k, bias=None, allowed=None, allowed_set=None, shown=None, shown_begin=None, repetition=1.0, frequency=0.0,
+        presence=0.0, temperature=1.0):
+    """The k (1 to 128) best classes of every row, by the scores as `adjust` would leave them: values float32 [rows, k], classes int32
+    [rows, k], lse float32 [rows].
+
+    The best come first, of equal scores the lower class. A class whose score is -inf or NaN is not listed; a list that is
+    not filled ends with class -1 and -inf. lse is the logarithm of the sum of exp(score / temperature) over all classes (-inf
+    where nothing is allowed, NaN where a score is NaN), so that exp(values / temperature - lse[:, None]) are probabilities."""
+    torch = _torch()
+    s = _scores(torch, "scores", scores)
+    r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
+    if not isinstance(k, int) or not 1 <= k <= 128:
+        raise ValueError("k is %r: 1 to 128 is wanted" % (k,))
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError("temperature is %r: 1e-6 to 1e6 is wanted" % (temperature,))
+    n, device = s.rows, scores.device
+    values = torch.empty((n, k), dtype=torch.float32, device=device)
+    classes = torch.empty((n, k), dtype=torch.int32, device=device)
+    lse = torch.empty(n, dtype=torch.float32, device=device)
+    if n:
+        size = _lib.load().tgbm_scores_top_workspace(C.byref(s), k)
+        # (torch keeps it until the stream's work that uses it is done, and a captured graph has its own)
+        room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _call(torch, scores, "tgbm_scores_top", C.byref(s), C.byref(r), k, temperature, values.data_ptr(), classes.data_ptr(), lse.data_ptr(),
+              room.data_ptr() if size else None, size)
+    return values, classes, lse
 
 
 def _apart(s, o, size):
