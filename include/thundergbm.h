@@ -278,6 +278,34 @@ size_t tgbm_scores_top_workspace(const tgbm_scores *in, int k);
 int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes,
                     float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
+/* A teacher's best scores: [rows][entries] (1 to 128) classes and scores, in any order, as tgbm_scores_top lists them.
+ * Entries whose class is negative or no class of the student, or whose score is -infinity, are left out; entries that name the
+ * same class add up. lse (may be NULL): the logarithm of the sum of exp(score / temperature) over all of the teacher's classes. */
+typedef struct tgbm_teacher {
+    const int *classes;
+    const void *scores;
+    const float *lse;
+    int type; /* of scores */
+    int entries;
+} tgbm_teacher;
+
+/* The loss of class scores z against a teacher t, and the gradient pairs for the trees of the next boosting round.
+ * With p = softmax(z / T) and the teacher's q = exp(t / T) over their sum, or exp(t / T - lse) where lse is given:
+ *   loss = weight * T^2 * [ sum of q (log q - log p) + r (log r - log R) ] + (1 - weight) * -log softmax(z)[label]
+ * r = 1 - sum of q (not below 0) is what the teacher left to the classes that it does not name, taken together, R their p;
+ * without lse, or where every class is named, there is no such part. A row without entries has no first part, one whose label is no class's
+ * number no second.
+ *   gradient = weight * T * (p - q) + (1 - weight) * (softmax(z) - [label]), q of a class that is not named being r p / R
+ *   hessian = max(2 (weight * p (1 - p) + (1 - weight) * s (1 - s)), 1e-16), s = softmax(z): the factor of two and the
+ * least value are those of the objective multi:softmax (multiclass_obj.cu:6-35).
+ * Where all scores of a row are -infinity every p is 0; a NaN or an infinite score or teacher's score makes its row NaN.
+ * in: float scores, the rows of a class side by side. labels (NULL only where weight is 1): [rows] class numbers as floats. loss (may be NULL): [rows].
+ * pairs (may be NULL): gradient and hessian of class c in row i at pairs[2 * (c * pair_stride + i)]. temperature: 1e-3 to
+ * 1e3, weight: 0 to 1. workspace: as for tgbm_scores_top. */
+size_t tgbm_scores_distill_workspace(const tgbm_scores *in, int entries);
+int tgbm_scores_distill(const tgbm_scores *in, const tgbm_teacher *teacher, const float *labels, float temperature, float weight,
+                        float *loss, float *pairs, long long pair_stride, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,3 +45,26 @@ def rules(rng, C, n, bias=True, sets="each", shown=True, longest=9):
         if begin[-1]:
             r.update(shown=lists, shown_begin=begin, repetition=1.3, frequency=0.2, presence=0.4)
     return r
+
+
+def teacher(rng, C, n, K, dtype=None, short=True, repeated=False):
+    """(classes [n, K], scores [n, K], the log-sum-exp of a teacher over all classes at a temperature of one): lists that end early, entries that are no
+    class, rows without entries, and on demand classes that several entries name."""
+    full = rng.standard_normal((n, C)).astype(np.float32) * 2.5
+    k = min(K, C)
+    at = np.argsort(-full, axis=1, kind="stable")[:, :k].astype(np.int32)
+    t = np.take_along_axis(full, at, 1)
+    if k < K:
+        at = np.concatenate([at, np.full((n, K - k), -1, np.int32)], 1)
+        t = np.concatenate([t, np.zeros((n, K - k), np.float32)], 1)
+    if short:
+        at[rng.random((n, K)) < 0.1] = -1
+        at[rng.random((n, K)) < 0.05] = C
+        t[rng.random((n, K)) < 0.05] = -np.inf
+        at[::7] = -1
+    if repeated:
+        from_ = rng.integers(0, K, (n, K))
+        at = np.where(rng.random((n, K)) < 0.5, np.take_along_axis(at, from_, 1), at)
+    shuffled = rng.permuted(np.broadcast_to(np.arange(K), (n, K)), axis=1)
+    of = lambda x: np.ascontiguousarray(np.take_along_axis(x, shuffled, 1))
+    return of(at), of(t), full

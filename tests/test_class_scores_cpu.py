@@ -133,3 +133,25 @@ def test_top_workspace(lib, by_class):
                 assert size >= (rows * chunks * (8 * k + 8) if chunks > 1 else 0)
                 assert classes > 32 or size == 0
                 assert lib.tgbm_scores_top_workspace(C.byref(a), 0) == lib.tgbm_scores_top_workspace(C.byref(a), 129) == 0
+
+
+def test_distill_refuses(lib, capfd):
+    def call(a=array(), teacher=True, classes=ADDRESS, scores=ADDRESS, kind=0, entries=3, labels=ADDRESS, temperature=1.0, weight=0.5, loss=ADDRESS, pairs=ADDRESS,
+             stride=10, room=ADDRESS, size=1 << 20):
+        t = S._Teacher(classes, scores, None, kind, entries)
+        return lib.tgbm_scores_distill(C.byref(a), C.byref(t) if teacher else None, labels, temperature, weight, loss, pairs, stride, room, size, None)
+
+    for fields, msg in BAD_ARRAYS:
+        assert call(a=array(**fields)) == 1 and msg in capfd.readouterr().err
+    large = array(class_stride=100, classes=100_000, rows=100)
+    needed = lib.tgbm_scores_distill_workspace(C.byref(large), 3)
+    assert needed > 0
+    for more, msg in ((dict(a=array(kind=1)), "float scores"), (dict(a=array(class_stride=1, row_stride=4)), "side by side"), (dict(teacher=False), "teacher"),
+                      (dict(kind=7), "unknown type"), (dict(entries=0), "0 entries"), (dict(entries=129), "129 entries"), (dict(classes=None), "null"),
+                      (dict(scores=None), "null"), (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+                      (dict(weight=-0.1), "weight"), (dict(weight=float("nan")), "weight"), (dict(labels=None), "labels"), (dict(stride=9), "pair_stride"),
+                      (dict(loss=None, pairs=None), "no output"), (dict(a=large, stride=100, size=needed - 1), "workspace"),
+                      (dict(a=large, stride=100, room=None), "workspace")):
+        assert call(**more) == 1 and msg in capfd.readouterr().err, more
+    assert call(a=array(rows=0)) == 0
+    assert lib.tgbm_scores_distill_workspace(C.byref(large), 0) == lib.tgbm_scores_distill_workspace(C.byref(large), 129) == 0

@@ -310,3 +310,201 @@ def test_top_two_graphs():
         for (graph, x, k, got), z in zip(graphs, news):
             check_top(got, z, k)
         check_top(eager, news[0], 5)
+
+
+def check_distill(got, want):
+    loss, pairs, loss_room, pairs_room = want
+    l = got[0].cpu().numpy().astype(np.float64)
+    with np.errstate(all="ignore"):
+        assert np.array_equal(np.isfinite(l), np.isfinite(loss)), (l, loss)
+        off = np.abs(l - loss)
+    fine = np.isfinite(loss)
+    assert np.array_equal(l[~fine & ~np.isnan(loss)], loss[~fine & ~np.isnan(loss)])
+    assert np.all(off[fine] <= loss_room[fine]), np.max(off[fine] / loss_room[fine])
+    if got[1] is not None:
+        p = got[1].cpu().numpy().astype(np.float64)
+        off = np.abs(p - pairs) / pairs_room
+        assert np.all(off <= 1), (off.max(), np.unravel_index(off.argmax(), off.shape))
+
+
+DISTILL_SIZES = [(1, 1, 1), (3, 1, 2), (8, 1, 8), (8, 1000, 5), (9, 257, 9), (31, 65, 40), (100, 16, 10), (129, 63, 64), (300, 300, 128), (1000, 40, 32), (1300, 17, 20),
+                 (5000, 5, 128), (20_000, 2, 7), (30_000, 1, 128), (40_000, 33, 16)]
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("C,n,K", DISTILL_SIZES)
+def test_distill(C, n, K, rest):
+    rng = np.random.default_rng(C + n + K)
+    for j, dtype in enumerate(TYPES):
+        temperature, weight = ((1.0, 1.0), (2.0, 0.5), (0.7, 0.25))[j]
+        z = (rng.standard_normal((C, n)) * 2).astype(np.float32)
+        classes, t, full = D.teacher(rng, C, n, K, repeated=j == 1)
+        t = rounded(t, dtype)
+        lse = np.log(np.exp(full.astype(np.float64) / temperature).sum(1)).astype(np.float32) if rest else None
+        labels = rng.integers(0, C, n).astype(np.float32)
+        labels[::5] = np.array([-1, C, 0.5, np.nan, np.inf], np.float32)[np.arange(len(labels[::5])) % 5]
+        want = O.distill(z, classes, t, labels, lse, temperature, weight)
+        g = dict(classes=torch.from_numpy(classes).cuda(), teacher=torch.from_numpy(t).to(dtype).cuda(), temperature=temperature, weight=weight,
+                 teacher_lse=None if lse is None else torch.from_numpy(lse).cuda(), labels=torch.from_numpy(labels).cuda())
+        x = place(z, "class", pad=j, shift=j)
+        check_distill(S.distill(x, **g), want)
+        loss, none = S.distill(x, gradient=False, **g)
+        assert none is None
+        check_distill((loss, None), want)
+
+
+def test_distill_is_the_objective_without_a_teacher():
+    """weight 0: the gradient pairs of multi:softmax."""
+    rng = np.random.default_rng(2)
+    C, n = 8, 500
+    z = (rng.standard_normal((C, n)) * 3).astype(np.float32)
+    y = rng.integers(0, C, n).astype(np.float32)
+    classes = torch.full((n, 1), -1, dtype=torch.int32, device="cuda")
+    loss, pairs = S.distill(place(z, "class"), classes, torch.zeros(n, 1, device="cuda"), labels=torch.from_numpy(y).cuda(), weight=0.0)
+    p = np.exp(O.log_softmax(z.astype(np.float64)))
+    g = p - (np.arange(C)[:, None] == y)
+    # (the room of an exponential, a sum of eight and their quotient; 1 - p as well)
+    np.testing.assert_allclose(pairs[..., 0].cpu().numpy(), g, rtol=0, atol=2.0**-24 * 60)
+    np.testing.assert_allclose(pairs[..., 1].cpu().numpy(), np.maximum(2 * p * (1 - p), 1e-16), rtol=0, atol=2.0**-24 * 60)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_gradient_is_the_loss_s(rest):
+    """The gradient against differences of the loss, in 64 bits in the restatement, and the kernel's against that one."""
+    rng = np.random.default_rng(12)
+    C, n, K = 6, 9, 3
+    z = rng.standard_normal((C, n))
+    classes, t, full = D.teacher(rng, C, n, K, repeated=True)
+    lse = np.log(np.exp(full.astype(np.float64) / 2).sum(1)).astype(np.float32) if rest else None
+    y = rng.integers(0, C, n).astype(np.float32)
+    args = (classes, t, y, lse, 2.0, 0.75)
+    step = 1e-5
+    loss, pairs, *_ = O.distill(z, *args)
+    for c in range(C):
+        up, down = z.copy(), z.copy()
+        up[c] += step
+        down[c] -= step
+        slope = (O.distill(up, *args)[0] - O.distill(down, *args)[0]) / (2 * step)
+        # (a third derivative of at most about T^-1 = 0.5 times step^2 / 6, and 2^-52 of the loss over the step)
+        np.testing.assert_allclose(pairs[c, :, 0], slope, rtol=0, atol=1e-9)
+    z32 = z.astype(np.float32)
+    check_distill(S.distill(place(z32, "class"), torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda(), labels=torch.from_numpy(y).cuda(),
+                            teacher_lse=None if lse is None else torch.from_numpy(lse).cuda(), temperature=2.0, weight=0.75), O.distill(z32, *args))
+
+
+@pytest.mark.parametrize("C,n", [(5, 6), (2000, 6), (40_000, 6)])
+def test_distill_far_scores(C, n):
+    """The student is far from the teacher: p of the others far below what 32 bits hold, every class named, scores of -inf, NaN."""
+    rng = np.random.default_rng(C)
+    K = min(C, 5)
+    z = (rng.standard_normal((C, n))).astype(np.float32)
+    classes = np.tile(np.arange(K, dtype=np.int32), (n, 1))
+    t = rng.standard_normal((n, K)).astype(np.float32)
+    lse = (np.log(np.exp(t.astype(np.float64)).sum(1)) + 0.3).astype(np.float32)
+    z[K:, 0] -= 500        # the others' part is exp(-500)
+    z[:K, 1] -= 500        # the named ones'
+    z[:, 2] *= 100
+    z[K - 1, 3] = -np.inf  # a named class that the student rules out: the loss is infinite
+    z[:, 4] = -np.inf      # every class ruled out
+    for rest in (None, lse):
+        want = O.distill(z, classes, t, None, rest)
+        got = S.distill(place(z, "class"), torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda(),
+                        teacher_lse=None if rest is None else torch.from_numpy(rest).cuda())
+        check_distill(got, want)
+        bad = z.copy()
+        bad[C // 2, 1] = np.nan
+        bad[0, 2] = np.inf
+        loss, pairs = S.distill(place(bad, "class"), torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda())
+        assert torch.isnan(loss).tolist() == [False, True, True, False, False, False]
+        assert torch.isnan(pairs).all(2).all(0).tolist() == [False, True, True, False, False, False]
+        assert torch.isfinite(pairs).all(2).all(0).tolist() == [True, False, False, True, True, True]
+
+
+def test_distill_teacher_s_odd_scores():
+    """A NaN or an infinite score of the teacher's makes the row NaN, wherever the entry's class is one; the others keep theirs."""
+    rng = np.random.default_rng(6)
+    for C, n, K in ((6, 5, 3), (40_000, 5, 3)):
+        z = rng.standard_normal((C, n)).astype(np.float32)
+        classes = np.tile(np.arange(K, dtype=np.int32), (n, 1))
+        t = rng.standard_normal((n, K)).astype(np.float32)
+        t[0, 1], t[1, 0], t[2, 2], t[3, 0] = np.nan, np.inf, np.nan, -np.inf
+        classes[2, 2] = C  # (left out)
+        for lse in (None, torch.full((n,), 3.0, device="cuda")):
+            loss, pairs = S.distill(place(z, "class"), torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda(), teacher_lse=lse)
+            assert torch.isnan(loss).tolist() == [True, True, False, False, False]
+            assert torch.isnan(pairs).all(2).all(0).tolist() == [True, True, False, False, False]
+            fine = np.arange(2, 5)
+            want = O.distill(z[:, fine], classes[fine], t[fine], None, None if lse is None else np.full(3, 3.0))
+            check_distill((loss[2:], pairs[:, 2:]), want)
+
+
+def test_distill_same_answer_twice():
+    rng = np.random.default_rng(3)
+    for C, n, K in ((8, 1000, 5), (1000, 100, 32), (40_000, 9, 64)):
+        z = place(D.scores(rng, C, n), "class")
+        classes, t, _ = D.teacher(rng, C, n, K, repeated=True)
+        args = (z, torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda())
+        a, b = S.distill(*args), S.distill(*args)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_distill_refuses():
+    x = torch.zeros(8, 10, device="cuda")
+    c, t = torch.zeros(10, 3, dtype=torch.int32, device="cuda"), torch.zeros(10, 3, device="cuda")
+    for more, msg in (
+        (dict(scores=torch.zeros(10, 8, device="cuda").t()), "side by side"),
+        (dict(scores=x.half()), "float32"),
+        (dict(classes=c.long()), "classes"),
+        (dict(classes=c[:9]), "classes"),
+        (dict(teacher=t.double()), "teacher"),
+        (dict(teacher=t[:, :0]), "teacher"),
+        (dict(teacher=torch.zeros(10, 129, device="cuda"), classes=torch.zeros(10, 129, dtype=torch.int32, device="cuda")), "128"),
+        (dict(teacher=torch.zeros(3, 10, device="cuda").t()), "contiguous"),
+        (dict(teacher_lse=torch.zeros(9, device="cuda")), "teacher_lse"),
+        (dict(temperature=0.0), "temperature"),
+        (dict(weight=1.5), "weight"),
+        (dict(weight=float("nan")), "weight"),
+        (dict(weight=0.5), "labels"),
+        (dict(labels=torch.zeros(10, dtype=torch.int64, device="cuda"), weight=0.5), "labels"),
+    ):
+        with pytest.raises(ValueError, match=msg):
+            S.distill(**dict(dict(scores=x, classes=c, teacher=t), **more))
+    loss, pairs = S.distill(torch.zeros(5, 0, device="cuda"), c[:0], t[:0])
+    assert loss.shape == (0,) and pairs.shape == (5, 0, 2)
+
+
+def test_distill_in_a_graph():
+    rng = np.random.default_rng(4)
+    for C, n, K in ((30, 200, 6), (30_000, 4, 20)):
+        z = place(rng.standard_normal((C, n)).astype(np.float32), "class")
+        classes, t, _ = D.teacher(rng, C, n, K)
+        c, s = torch.from_numpy(classes).cuda(), torch.from_numpy(t).cuda()
+        S.distill(z, c, s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = S.distill(z, c, s)
+        for _ in range(3):
+            z2 = rng.standard_normal((C, n)).astype(np.float32)
+            z.copy_(torch.from_numpy(z2))
+            graph.replay()
+            eager = S.distill(z, c, s)
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+            check_distill(got, O.distill(z2, classes, t))
+
+
+def test_from_a_teacher_s_scores_to_pairs():
+    """A teacher's scores, adjusted and listed, and a student held against them: the calls one behind the other."""
+    rng = np.random.default_rng(5)
+    C, n, k, temperature = 400, 150, 12, 2.0
+    full = rounded(D.scores(rng, C, n), torch.bfloat16)
+    r = D.rules(rng, C, n, sets="one")
+    x = O.adjusted(full, **r)
+    values, classes, lse = S.top(place(full, "row", torch.bfloat16), k, temperature=temperature, **on_gpu(r))
+    check_top((values, classes, lse), x, k, temperature)
+    after = S.adjust(place(full, "row", torch.float32), **on_gpu(r))
+    check_top(S.top(after, k, temperature=temperature), x, k, temperature)
+    z = rng.standard_normal((C, n)).astype(np.float32)
+    got = S.distill(place(z, "class"), classes, values, teacher_lse=lse, temperature=temperature)
+    check_distill(got, O.distill(z, classes.cpu().numpy(), values.cpu().numpy(), None, lse.cpu().numpy(), temperature))

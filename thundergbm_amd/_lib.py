@@ -57,6 +57,8 @@ SIGNATURES = {
     "tgbm_release_memory": (None, []),
     "tgbm_cut_points": (C.c_int, [C.c_int, C.c_int, _P, _P, _P, C.c_int, _P, _P, _P, _P]),
     "tgbm_scores_adjust": (C.c_int, [_P, _P, _P, _P]),
+    "tgbm_scores_distill_workspace": (C.c_size_t, [_P, C.c_int]),
+    "tgbm_scores_distill": (C.c_int, [_P, _P, _P, C.c_float, C.c_float, _P, _P, C.c_longlong, _P, C.c_size_t, _P]),
     "tgbm_scores_top_workspace": (C.c_size_t, [_P, C.c_int]),
     "tgbm_scores_top": (C.c_int, [_P, _P, C.c_int, C.c_float, _P, _P, _P, _P, C.c_size_t, _P]),
 }

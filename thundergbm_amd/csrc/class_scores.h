@@ -22,4 +22,9 @@ size_t scores_top_workspace(bool columns, int classes, int rows, int k);
 void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
                        void *workspace);
 
+// row_of (may be null): the teacher's row, and the loss's, of every row of the scores, the labels and the pairs.
+size_t scores_distill_workspace(int classes, int rows, int entries);
+void launch_scores_distill(hipStream_t s, const tgbm_scores &in, const tgbm_teacher &teacher, const float *labels, float temperature, float weight,
+                           float *loss, void *pairs, long pair_stride, const int *row_of, void *workspace);
+
 }  // namespace tgbm

@@ -105,3 +105,31 @@ extern "C" int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *ru
     launch_scores_top(static_cast<hipStream_t>(stream), *in, *rules, k, temperature, values, classes, lse, workspace);
     return launched(entry);
 }
+
+extern "C" size_t tgbm_scores_distill_workspace(const tgbm_scores *in, int entries) {
+    if (check_scores("tgbm_scores_distill_workspace", "in", in) != 0 || entries < 1 || entries > kTeacherMost || in->rows == 0) return 0;
+    return scores_distill_workspace(in->classes, in->rows, entries);
+}
+
+extern "C" int tgbm_scores_distill(const tgbm_scores *in, const tgbm_teacher *teacher, const float *labels, float temperature, float weight, float *loss,
+                                   float *pairs, long long pair_stride, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *entry = "tgbm_scores_distill";
+    if (const int rc = check_scores(entry, "in", in)) return rc;
+    if (in->type != TGBM_F32) return refused(entry, "in: float scores are wanted");
+    if (in->rows > 1 && in->row_stride != 1) return refused(entry, "in: the rows of a class lie side by side");
+    if (teacher == nullptr) return refused(entry, "teacher is null");
+    if (teacher->type != TGBM_F32 && teacher->type != TGBM_F16 && teacher->type != TGBM_BF16) return refused(entry, "teacher: unknown type %d", teacher->type);
+    if (teacher->entries < 1 || teacher->entries > kTeacherMost)
+        return refused(entry, "teacher: %d entries: 1 to %d are wanted", teacher->entries, kTeacherMost);
+    if (!(temperature >= 1e-3f && temperature <= 1e3f)) return refused(entry, "temperature is %g: 1e-3 to 1e3 is wanted", temperature);
+    if (!(weight >= 0.f && weight <= 1.f)) return refused(entry, "weight is %g: 0 to 1 is wanted", weight);
+    if (labels == nullptr && weight != 1.f && in->rows > 0) return refused(entry, "weight is %g, and there are no labels", weight);
+    if (pairs != nullptr && in->classes > 1 && pair_stride < in->rows) return refused(entry, "pair_stride is %lld for %d rows", pair_stride, in->rows);
+    if (in->rows == 0) return 0;
+    if (teacher->classes == nullptr || teacher->scores == nullptr) return refused(entry, "teacher: null entries");
+    if (loss == nullptr && pairs == nullptr) return refused(entry, "there is no output");
+    const size_t needed = scores_distill_workspace(in->classes, in->rows, teacher->entries);
+    if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
+    launch_scores_distill(static_cast<hipStream_t>(stream), *in, *teacher, labels, temperature, weight, loss, pairs, pair_stride, nullptr, workspace);
+    return launched(entry);
+}

@@ -1,5 +1,6 @@
 """Operators on class scores that lie on the GPU, as torch tensors (tgbm_scores_*): what is known besides the model is put on
-the scores (`adjust`), the best classes of every row are listed (`top`). torch is imported by the caller, never here.
+the scores (`adjust`), the best classes of every row are listed (`top`), and they
+are held against a teacher's best scores (`distill`). torch is imported by the caller, never here.
 
 Scores are [classes, rows], float32, float16 or bfloat16, in either order: the rows of a class side by side, as trainers and
 predictors hold them, or the classes of a row side by side (`x.t()` of a [rows, classes] tensor). Everything is launched on
@@ -22,6 +23,10 @@ class _Rules(C.Structure):
     _fields_ = [("bias", C.c_void_p), ("allowed", C.c_void_p), ("allowed_set", C.c_void_p), ("shown", C.c_void_p),
                 ("shown_begin", C.c_void_p), ("n_shown", C.c_longlong), ("allowed_sets", C.c_int), ("repetition", C.c_float),
                 ("frequency", C.c_float), ("presence", C.c_float)]
+
+
+class _Teacher(C.Structure):
+    _fields_ = [("classes", C.c_void_p), ("scores", C.c_void_p), ("lse", C.c_void_p), ("type", C.c_int), ("entries", C.c_int)]
 
 
 _types = None
@@ -201,6 +206,54 @@ def top(scores, k, bias=None, allowed=None, allowed_set=None, shown=None, shown_
         _call(torch, scores, "tgbm_scores_top", C.byref(s), C.byref(r), k, temperature, values.data_ptr(), classes.data_ptr(), lse.data_ptr(),
               room.data_ptr() if size else None, size)
     return values, classes, lse
+
+
+def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature=1.0, weight=1.0, gradient=True):
+    """The loss of class scores z against a teacher's best scores, float32 [rows], and the gradient pairs for the trees of the
+    next boosting round, float32 [classes, rows, 2] (None where `gradient` is false).
+
+    scores: float32, the rows of a class side by side.
+    classes, teacher: int32 and a floating type, [rows, entries] with 1 to 128 entries in any order, as `top` lists them.
+      Entries whose class is negative or no class of the student, or whose score is -inf, are left out; entries that name
+      the same class add up.
+    teacher_lse: float32 [rows], the teacher's log of the sum of exp(score / temperature) over all its classes, as `top` gives it for
+      the same temperature. With it q = exp(teacher / T - teacher_lse), and what is left, r = 1 - sum(q), belongs to the classes
+      that are not named, taken together; without it the entries' q add up to 1.
+    labels: float32 [rows], class numbers; a row whose label is none has no part in the second term.
+
+    With p = softmax(z / T) and R its part on the classes that are not named:
+      loss = weight * T^2 * (sum(q * (log q - log p)) + r * (log r - log R)) + (1 - weight) * -log softmax(z)[label]
+      gradient = weight * T * (p - q) + (1 - weight) * (softmax(z) - [label]); q of a class that is not named is r * p / R
+      hessian = max(2 * (weight * p * (1 - p) + (1 - weight) * s * (1 - s)), 1e-16), s = softmax(z), like multi:softmax's."""
+    torch = _torch()
+    s = _scores(torch, "scores", scores)
+    if s.type != 0 or (s.row_stride != 1 and s.rows > 1):
+        raise ValueError("scores: float32 with the rows of a class side by side is wanted")
+    n, C_ = s.rows, s.classes
+    _on_gpu(torch, "teacher", teacher)
+    kind = _types.get(teacher.dtype)
+    if kind is None:
+        raise ValueError("teacher: float32, float16 or bfloat16 is wanted, got %s" % teacher.dtype)
+    if teacher.dim() != 2 or not 1 <= teacher.shape[1] <= 128:
+        raise ValueError("teacher: [rows, entries] with 1 to 128 entries is wanted, got %s" % (tuple(teacher.shape),))
+    entries = teacher.shape[1]
+    t = _Teacher(_plain(torch, "classes", classes, scores, torch.int32, (n, entries)), _plain(torch, "teacher", teacher, scores, teacher.dtype, (n, entries)),
+                 None if teacher_lse is None else _plain(torch, "teacher_lse", teacher_lse, scores, torch.float32, (n,)), kind, entries)
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError("temperature is %r: 1e-3 to 1e3 is wanted" % (temperature,))
+    if not 0 <= weight <= 1:
+        raise ValueError("weight is %r: 0 to 1 is wanted" % (weight,))
+    if labels is None and weight != 1:
+        raise ValueError("weight is %r, and there are no labels" % (weight,))
+    y = None if labels is None else _plain(torch, "labels", labels, scores, torch.float32, (n,))
+    loss = torch.empty(n, dtype=torch.float32, device=scores.device)
+    pairs = torch.empty((C_, n, 2), dtype=torch.float32, device=scores.device) if gradient else None
+    if n:
+        size = _lib.load().tgbm_scores_distill_workspace(C.byref(s), entries)
+        room = torch.empty(size, dtype=torch.uint8, device=scores.device) if size else None
+        _call(torch, scores, "tgbm_scores_distill", C.byref(s), C.byref(t), y, temperature, weight, loss.data_ptr(),
+              pairs.data_ptr() if gradient else None, n, room.data_ptr() if size else None, size)
+    return loss, pairs
 
 
 def _apart(s, o, size):
