@@ -306,6 +306,24 @@ size_t tgbm_scores_distill_workspace(const tgbm_scores *in, int entries);
 int tgbm_scores_distill(const tgbm_scores *in, const tgbm_teacher *teacher, const float *labels, float temperature, float weight,
                         float *loss, float *pairs, long long pair_stride, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The boosting rounds of a session (Part 2) with a multi:softmax or multi:softprob objective from here on train on that loss:
+ * tgbm_trainer_boost and tgbm_trainer_gradient take their gradient pairs from it, with the session's labels. Here the teacher's arrays are
+ * host arrays, in the order of the session's rows, classes being numbers of the session's ascending distinct labels; they
+ * are copied. NULL: on the labels alone again. Metrics stay those of the labels. Wrong arguments abort the process, as in Part 2. */
+void tgbm_trainer_set_teacher(tgbm_trainer *t, const tgbm_teacher *teacher, float temperature, float weight);
+/* The mean of that loss over the rows with the current predictions. */
+double tgbm_trainer_teacher_loss(tgbm_trainer *t);
+
+/* The scores of a model with one tree per class and round (tgbm_predict_raw with a base score of 0), as the rules leave them, and
+ * the best classes by them. Here every pointer, those in the rules among them, is a host pointer, rows are CSR as in
+ * sparse_predict_scikit, and calls block until the results are there. adjusted: [trees_per_iter][row_size]; the
+ * other outputs as tgbm_scores_top writes them. Wrong arguments abort the process, as in Part 1. */
+void tgbm_predict_adjusted(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees,
+                           int trees_per_iter, float learning_rate, const tgbm_score_rules *rules, float *adjusted);
+void tgbm_predict_top(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees,
+                      int trees_per_iter, float learning_rate, const tgbm_score_rules *rules, int k, float temperature, float *values,
+                      int *classes, float *lse);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@
 #include <thread>
 
 #include "../../include/thundergbm.h"
+#include "class_scores.h"
 #include "model_handle.h"
 #include "trainer.h"
 
@@ -130,6 +131,63 @@ int count_distinct(const float *v, int n) {
         }
     }
     return (int)held + (zero_seen ? 1 : 0);
+}
+
+// Host rules on the device, for the time of a call.
+class DeviceRules {
+  public:
+    DeviceRules(hipStream_t s, const tgbm_score_rules &host, int classes, int rows) : rules_(host) {
+        up(s, rules_.bias, (size_t)classes);
+        up(s, rules_.allowed, (size_t)host.allowed_sets * ((classes + 31) / 32));
+        up(s, rules_.allowed_set, (size_t)rows);
+        if (host.n_shown == 0) rules_.shown = nullptr;
+        up(s, rules_.shown, (size_t)host.n_shown);
+        if (rules_.shown == nullptr) rules_.shown_begin = nullptr;
+        up(s, rules_.shown_begin, (size_t)rows + 1);
+    }
+    ~DeviceRules() {
+        for (void *p : blocks_) device_free(p);
+    }
+    const tgbm_score_rules &get() const { return rules_; }
+
+  private:
+    template <typename T>
+    void up(hipStream_t s, const T *&p, size_t count) {
+        if (p == nullptr) return;
+        void *to = device_alloc(std::max<size_t>(1, count) * sizeof(T));
+        blocks_.push_back(to);
+        upload_large(s, to, p, count * sizeof(T));
+        p = static_cast<const T *>(to);
+    }
+    tgbm_score_rules rules_;
+    std::vector<void *> blocks_;
+};
+
+// What tgbm_predict_adjusted and tgbm_predict_top do alike: the scores on the device and the rules beside them.
+template <typename Use>
+void with_scores(const char *entry, int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees, int trees_per_iter,
+                 float learning_rate, const tgbm_score_rules *rules, Use use) {
+    TGBM_CHECK(model != nullptr, "model is null!");
+    const tgbm_scores shape{model, (long long)std::max(row_size, 1), 1, TGBM_F32, trees_per_iter, row_size};  // (the address stands for the scores' own)
+    TGBM_CHECK(scores_ok(entry, "scores", &shape) && rules_ok(entry, rules, row_size), "%s: wrong arguments", entry);
+    GBMParam p;
+    p.learning_rate = learning_rate;
+    p.base_score = 0;
+    DataSet ds;
+    GBMParam load_param = p;
+    const int saved = g_verbose;
+    g_verbose = 0;
+    ds.load_from_sparse(row_size, val, row_ptr, col_ptr, nullptr, nullptr, 0, load_param, false);
+    g_verbose = saved;
+    if (row_size == 0) return;
+    score_on_device(p, *model, n_trees, trees_per_iter, ds, [&](hipStream_t s, const float *d_scores) {
+        DeviceRules on_device(s, *rules, trees_per_iter, row_size);
+        tgbm_scores scores = shape;
+        scores.data = d_scores;
+        use(s, scores, on_device.get());
+        HIP_CHECK_LAUNCHES(entry);
+        HIP_CHECK(hipStreamSynchronize(s));
+    });
 }
 
 }  // namespace
@@ -379,6 +437,10 @@ tgbm_trainer *tgbm_trainer_create_grouped(int row_size, const float *val, const 
 void tgbm_trainer_destroy(tgbm_trainer *t) { delete t; }
 
 void tgbm_trainer_set_option(tgbm_trainer *t, const char *key, double value) { t->impl->set_option(key, value); }
+void tgbm_trainer_set_teacher(tgbm_trainer *t, const tgbm_teacher *teacher, float temperature, float weight) {
+    t->impl->set_teacher(teacher != nullptr ? *teacher : tgbm_teacher{}, temperature, weight);
+}
+double tgbm_trainer_teacher_loss(tgbm_trainer *t) { return t->impl->teacher_loss(); }
 void tgbm_trainer_sample_columns(tgbm_trainer *t) { t->impl->sample_columns(); }
 
 void tgbm_trainer_boost(tgbm_trainer *t, int rounds) {
@@ -441,6 +503,41 @@ void tgbm_predict_raw(int row_size, const float *val, const int *row_ptr, const 
     g_verbose = saved;
     TGBM_CHECK(model != nullptr, "model is null!");
     score(p, *model, n_trees, trees_per_iter, ds, false, false, out);
+}
+
+void tgbm_predict_adjusted(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees,
+                           int trees_per_iter, float learning_rate, const tgbm_score_rules *rules, float *adjusted) {
+    std::lock_guard<std::mutex> lock(g_call_mutex);
+    with_scores("tgbm_predict_adjusted", row_size, val, row_ptr, col_ptr, model, n_trees, trees_per_iter, learning_rate, rules,
+                [&](hipStream_t s, const tgbm_scores &scores, const tgbm_score_rules &r) {
+                    launch_scores_adjust(s, scores, r, scores);
+                    hipStream_t down = stream_acquire();
+                    download_large(s, down, adjusted, scores.data, sizeof(float) * (size_t)row_size * trees_per_iter);
+                    HIP_CHECK(hipStreamSynchronize(down));
+                    stream_release(down);
+                });
+}
+
+void tgbm_predict_top(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees, int trees_per_iter,
+                      float learning_rate, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes, float *lse) {
+    std::lock_guard<std::mutex> lock(g_call_mutex);
+    TGBM_CHECK(k >= 1 && k <= kTopMost, "tgbm_predict_top: k is %d: 1 to %d is wanted", k, kTopMost);
+    TGBM_CHECK(temperature >= 1e-6f && temperature <= 1e6f, "tgbm_predict_top: temperature is %g: 1e-6 to 1e6 is wanted", temperature);
+    with_scores("tgbm_predict_top", row_size, val, row_ptr, col_ptr, model, n_trees, trees_per_iter, learning_rate, rules,
+                [&](hipStream_t s, const tgbm_scores &scores, const tgbm_score_rules &r) {
+                    const size_t n = (size_t)row_size, room = scores_top_workspace(true, trees_per_iter, row_size, k);
+                    float *d_values = static_cast<float *>(device_alloc(sizeof(float) * n * (2 * (size_t)k + 1)));
+                    int *d_classes = reinterpret_cast<int *>(d_values + n * k);
+                    float *d_lse = d_values + 2 * n * k;
+                    void *workspace = room > 0 ? device_alloc(room) : nullptr;
+                    launch_scores_top(s, scores, r, k, temperature, d_values, d_classes, d_lse, workspace);
+                    HIP_CHECK(hipMemcpyAsync(values, d_values, sizeof(float) * n * k, hipMemcpyDeviceToHost, s));
+                    HIP_CHECK(hipMemcpyAsync(classes, d_classes, sizeof(int) * n * k, hipMemcpyDeviceToHost, s));
+                    HIP_CHECK(hipMemcpyAsync(lse, d_lse, sizeof(float) * n, hipMemcpyDeviceToHost, s));
+                    HIP_CHECK(hipStreamSynchronize(s));
+                    device_free(d_values);
+                    device_free(workspace);
+                });
 }
 
 int tgbm_cut_points(int row_size, int n_features, const float *val, const int *row_ptr, const int *col_ptr,

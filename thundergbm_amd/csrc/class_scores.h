@@ -14,6 +14,10 @@ namespace tgbm {
 constexpr int kTopMost = 128;      // classes that top lists
 constexpr int kTeacherMost = 128;  // entries of a teacher's row
 
+// Whether the arguments of an entry point can be worked on; if not, why not is said on stderr (scores_api.hip).
+bool scores_ok(const char *entry, const char *what, const tgbm_scores *s);
+bool rules_ok(const char *entry, const tgbm_score_rules *rules, int rows);
+
 inline bool rows_side_by_side(const tgbm_scores &s) { return !(s.class_stride == 1 && (s.rows == 1 || s.row_stride != 1)); }
 
 void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out);

@@ -2,9 +2,12 @@
 // class trees of an iteration next to each other. Opaque to callers; shared by the translation units that
 // implement entry points taking a handle. The trees never change once the handle exists.
 #pragma once
+#include <functional>
 #include <memory>
 #include <mutex>
 #include <vector>
+
+#include <hip/hip_runtime.h>
 
 #include "host.h"
 
@@ -26,5 +29,9 @@ namespace tgbm {
 // handle. out: class-major raw scores (n rows x n_class floats), or with `transform` the objective's predictions.
 void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds, bool transform,
            bool log_metric, float *out);
+// The same up to the raw scores, which `use` gets where they are: on the device, class-major, complete on the stream when what
+// it launches there runs. They are gone when it returns, so it waits for what it has launched.
+void score_on_device(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds,
+                     const std::function<void(hipStream_t, const float *)> &use);
 
 }  // namespace tgbm

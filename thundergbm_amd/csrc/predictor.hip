@@ -288,10 +288,8 @@ bool score_small(hipStream_t s, const GBMParam &param, const ScoreModel &m, cons
     return launched;
 }
 
-}  // namespace
-
-void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds, bool transform,
-           bool log_metric, float *out) {
+void score_any(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds, bool transform,
+               bool log_metric, float *out, const std::function<void(hipStream_t, const float *)> *use) {
     int n_dev = 0;
     hipError_t e = hipGetDeviceCount(&n_dev);
     TGBM_CHECK(e == hipSuccess && n_dev >= 1, "no HIP device available: this library has no CPU path");
@@ -316,7 +314,7 @@ void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, co
     std::shared_ptr<const DeviceModel> dm;
     if (want_records) dm = device_model(s, model, n_iter, n_class);
     const bool usable = dm != nullptr && dm->usable;
-    if (usable && n > 0 && !log_metric && score_small(s, param, dm->m, ds, transform, out)) {
+    if (usable && n > 0 && !log_metric && use == nullptr && score_small(s, param, dm->m, ds, transform, out)) {
         lap("rows in pinned memory");
         stream_release(s);
         return;
@@ -435,7 +433,12 @@ void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, co
         n_ret = transform_scores(s, param, ds, n, n_class, d_out, d_label);
     }
     HIP_CHECK_LAUNCHES("predict (metric, transform)");
-    download_large(s, s_up, out, d_out, sizeof(float) * n_ret);
+    if (use != nullptr) {
+        (*use)(s, d_out);
+        HIP_CHECK(hipStreamSynchronize(s));
+    } else {
+        download_large(s, s_up, out, d_out, sizeof(float) * n_ret);
+    }
     HIP_CHECK(hipStreamSynchronize(s_up));
     HIP_CHECK(hipEventDestroy(up));
     lap("traversal, transform and download");
@@ -445,6 +448,18 @@ void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, co
     stream_release(s_up);
     stream_release(s);
     lap("release");
+}
+
+}  // namespace
+
+void score(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds, bool transform,
+           bool log_metric, float *out) {
+    score_any(param, model, n_iter, n_class, ds, transform, log_metric, out, nullptr);
+}
+
+void score_on_device(const GBMParam &param, tgbm_model &model, int n_iter, int n_class, const DataSet &ds,
+                     const std::function<void(hipStream_t, const float *)> &use) {
+    score_any(param, model, n_iter, n_class, ds, false, false, nullptr, &use);
 }
 
 // (callers that hold the trees as the parser returns them: the CLI and the R interface)

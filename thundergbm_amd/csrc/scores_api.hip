@@ -71,6 +71,11 @@ int check_temperature(const char *entry, float t) {
 
 }  // namespace
 
+namespace tgbm {
+bool scores_ok(const char *entry, const char *what, const tgbm_scores *s) { return check_scores(entry, what, s) == 0; }
+bool rules_ok(const char *entry, const tgbm_score_rules *rules, int rows) { return check_rules(entry, rules, rows) == 0; }
+}  // namespace tgbm
+
 extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream) {
     const char *entry = "tgbm_scores_adjust";
     int rc = check_scores(entry, "in", in);

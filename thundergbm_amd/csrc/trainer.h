@@ -7,6 +7,7 @@
 #include <string>
 #include <vector>
 
+#include "class_scores.h"
 #include "device_api.h"
 #include "host.h"
 #include "rank.h"
@@ -56,6 +57,10 @@ class Trainer {
     // "column_sampling_rate", "bagging", "reorder_first", "reorder_burst", "reorder_every", "reorder_min_rows"
     void set_option(const std::string &key, double value);
     void compute_gradient();
+    // Softmax objectives: the rounds from here on train on the loss against a teacher's best scores (launch_scores_distill) instead
+    // of the labels alone. Host arrays [rows][entries] in the caller's row order; classes == nullptr: on the labels again.
+    void set_teacher(const tgbm_teacher &host, float temperature, float weight);
+    double teacher_loss();  // of the current predictions, the mean over the rows
     void tree_init(int k);
     void find_split(int level);  // histogram, merge/subtract, split search, update_tree
     void partition(int level);   // update_ins2node_id + next level's row lists
@@ -128,6 +133,14 @@ class Trainer {
     float *d_yp_ = nullptr;
     long n_yp_ = 0;
     GHPair *d_gh_ = nullptr;
+    struct {
+        tgbm_teacher of{};  // device arrays; of.classes == nullptr: there is none
+        float temperature = 1.f, weight = 1.f;
+        void *workspace = nullptr;
+    } teacher_;
+    void release_teacher();
+    void launch_teacher(float *loss, GHPair *gh);
+    void objective_gradient();  // of the predictions as they are, into d_gh_ (all but the ranking objectives)
     DeviceCuts cuts_;
     std::vector<int> h_cut_row_ptr_;
     std::vector<int> h_col_bin_begin_;  // dense layout: first global bin of every column of the matrix (+ the bin count)

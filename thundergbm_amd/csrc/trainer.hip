@@ -769,6 +769,7 @@ Trainer::~Trainer() {
     for (auto &m : marks_) (void)hipEventDestroy(m.ev);
     reorder_sorter_.release();
     for (void *p : allocs_) device_free(p);
+    release_teacher();
     if (stream_) stream_release(stream_);
 }
 
@@ -784,6 +785,66 @@ void Trainer::mark(int phase, int level) {
     marks_.push_back(m);
 }
 
+void Trainer::release_teacher() {
+    for (void *p : {(void *)teacher_.of.classes, (void *)teacher_.of.scores, (void *)teacher_.of.lse, teacher_.workspace}) device_free(p);
+    teacher_.of = tgbm_teacher{};
+    teacher_.workspace = nullptr;
+}
+
+void Trainer::set_teacher(const tgbm_teacher &host, float temperature, float weight) {
+    TGBM_CHECK(objective_ == OBJ_SOFTMAX, "a teacher's class scores need a multi:softmax or multi:softprob objective");
+    ensure_gh_array();
+    sync();  // (the arrays of the teacher before are freed)
+    release_teacher();
+    next_round_ready_ = false;
+    if (host.classes == nullptr) return;
+    TGBM_CHECK(host.scores != nullptr, "teacher: null scores");
+    TGBM_CHECK(host.type == TGBM_F32 || host.type == TGBM_F16 || host.type == TGBM_BF16, "teacher: unknown type %d", host.type);
+    TGBM_CHECK(host.entries >= 1 && host.entries <= kTeacherMost, "teacher: %d entries: 1 to %d are wanted", host.entries, kTeacherMost);
+    TGBM_CHECK(temperature >= 1e-3f && temperature <= 1e3f, "teacher: temperature is %g: 1e-3 to 1e3 is wanted", temperature);
+    TGBM_CHECK(weight >= 0.f && weight <= 1.f, "teacher: weight is %g: 0 to 1 is wanted", weight);
+    const size_t count = (size_t)n_ * host.entries, score_bytes = host.type == TGBM_F32 ? 4 : 2;
+    auto up = [&](const void *from, size_t bytes) {
+        void *to = device_alloc(std::max<size_t>(bytes, 4));
+        upload_large(stream_, to, from, bytes);
+        return to;
+    };
+    teacher_.of.classes = static_cast<const int *>(up(host.classes, count * sizeof(int)));
+    teacher_.of.scores = up(host.scores, count * score_bytes);
+    if (host.lse != nullptr) teacher_.of.lse = static_cast<const float *>(up(host.lse, sizeof(float) * (size_t)n_));
+    teacher_.of.type = host.type;
+    teacher_.of.entries = host.entries;
+    teacher_.temperature = temperature;
+    teacher_.weight = weight;
+    const size_t room = scores_distill_workspace(param_.num_class, n_, host.entries);
+    if (room > 0) teacher_.workspace = device_alloc(room);
+    sync();
+}
+
+void Trainer::launch_teacher(float *loss, GHPair *gh) {
+    const tgbm_scores z{d_yp_, (long long)n_, 1, TGBM_F32, param_.num_class, n_};
+    launch_scores_distill(stream_, z, teacher_.of, d_y_, teacher_.temperature, teacher_.weight, loss, gh, n_, d_perm_, teacher_.workspace);
+}
+
+double Trainer::teacher_loss() {
+    TGBM_CHECK(teacher_.of.classes != nullptr, "teacher_loss: there is no teacher");
+    std::vector<float> host((size_t)n_);
+    float *loss = static_cast<float *>(device_alloc(sizeof(float) * (size_t)std::max(n_, 1)));
+    launch_teacher(loss, nullptr);
+    HIP_CHECK_LAUNCHES("teacher_loss");
+    HIP_CHECK(hipMemcpyAsync(host.data(), loss, sizeof(float) * (size_t)n_, hipMemcpyDeviceToHost, stream_));
+    sync();
+    device_free(loss);
+    double sum = 0;
+    for (float v : host) sum += v;
+    return sum / std::max(n_, 1);
+}
+
+void Trainer::objective_gradient() {
+    if (teacher_.of.classes != nullptr) launch_teacher(nullptr, d_gh_);
+    else launch_gradient(stream_, objective_, n_, param_.num_class, d_y_, d_yp_, d_gh_, nullptr, 0);
+}
+
 // The first two steps of Booster::boost (include/thundergbm/booster.h:80-84): the objective's gradients, then
 // bagging when it is switched on.
 void Trainer::compute_gradient() {
@@ -795,7 +856,7 @@ void Trainer::compute_gradient() {
         rank_->gradient(d_yp_, d_gh_, (unsigned)std::rand(), rank_order_fresh_);
         rank_order_fresh_ = false;
     } else {
-        launch_gradient(stream_, objective_, n_, param_.num_class, d_y_, d_yp_, d_gh_, nullptr, 0);
+        objective_gradient();
     }
     gh_words_fresh_ = gh_records_fresh_ = false;
     if (d_gh_words_ != nullptr && !param_.bagging) {  // (bagging multiplies the pairs by draw counts)
@@ -897,7 +958,7 @@ void Trainer::begin_tree(const TreeBuffers &tb, const GHPair *gh, bool stats_rea
 
 void Trainer::ensure_gh_array() {
     if (!gh_array_stale_) return;
-    launch_gradient(stream_, objective_, n_, param_.num_class, d_y_, d_yp_, d_gh_, nullptr, 0);
+    objective_gradient();
     gh_array_stale_ = false;
 }
 
@@ -1514,7 +1575,7 @@ void Trainer::reorder_rows() {
     next_round_ready_ = false;
     gh_words_fresh_ = gh_records_fresh_ = false;
     gh_array_stale_ = false;  // (recomputed here)
-    launch_gradient(stream_, objective_, n_, param_.num_class, d_y_, d_yp_, d_gh_, nullptr, 0);
+    objective_gradient();
     ++reorders_done_;
 }
 

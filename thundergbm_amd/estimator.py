@@ -9,6 +9,8 @@ import scipy.sparse as sp
 from sklearn.base import BaseEstimator, ClassifierMixin, RegressorMixin
 
 from . import _lib
+from .scores import _Rules
+from .session import Session, teacher_arrays
 
 _PARAMS = ("depth", "n_trees", "n_gpus", "min_child_weight", "lambda_tgbm", "gamma", "max_num_bin", "verbose",
            "column_sampling_rate", "bagging", "n_parallel_trees", "learning_rate", "objective", "num_class",
@@ -67,6 +69,23 @@ def _stored_label_count(model_path):
     return n_label
 
 
+class Teacher:
+    """What a classifier is trained against besides its labels: for every training row a teacher's best classes (labels as they are
+    in y; None, NaN or a label that does not occur in y: an entry that is left out) and their scores, both [rows, entries] with up to
+    128 entries. lse: the teacher's log of the sum of exp(score / temperature) over all its classes, for what it does not name.
+    weight: the part of the teacher in the loss, the rest is the labels' (scores.distill has the formula)."""
+
+    def __init__(self, labels, scores, lse=None, temperature=1.0, weight=1.0):
+        self.labels, self.scores, self.lse, self.temperature, self.weight = labels, scores, lse, temperature, weight
+
+    def class_numbers(self, known):
+        """The entries' places among the ascending labels `known`, -1 for those that are none."""
+        labels = np.asarray(self.labels, dtype=np.float32)
+        at = np.searchsorted(known, labels)
+        at = np.minimum(at, len(known) - 1)
+        return np.where(known[at] == labels, at, -1).astype(np.int32)
+
+
 class TGBMModel(BaseEstimator):
     def __init__(self, depth=6, n_trees=40, n_gpus=1, min_child_weight=1.0, lambda_tgbm=1.0, gamma=1.0,
                  max_num_bin=255, verbose=1, column_sampling_rate=1.0, bagging=0, n_parallel_trees=1,
@@ -85,7 +104,10 @@ class TGBMModel(BaseEstimator):
             _lib.load().model_free(C.byref(self.model))
             self.model = None
 
-    def fit(self, X, y, groups=None):
+    def fit(self, X, y, groups=None, teacher=None):
+        """teacher: a Teacher, for the objectives multi:softmax and multi:softprob."""
+        if teacher is not None:
+            return self._fit_teacher(X, y, teacher)
         lib = _lib.load()
         self._release()
         dense = _dense(X)
@@ -138,6 +160,109 @@ class TGBMModel(BaseEstimator):
         if not self.model:
             raise RuntimeError("The model returned is empty!")
         return self
+
+    def _fit_teacher(self, X, y, teacher):
+        if self.objective not in ("multi:softmax", "multi:softprob"):
+            raise ValueError("a teacher's class scores need the objective multi:softmax or multi:softprob")
+        if self.tree_method not in ("auto", "hist"):
+            raise ValueError("tree_method %s is not part of this build (hist only)" % self.tree_method)
+        X = _csr(X)
+        y = np.ascontiguousarray(y, dtype=np.float32)
+        if X.shape[0] != len(y):
+            raise ValueError("X and y have different numbers of rows")
+        known = np.unique(y)
+        if len(known) < 3:
+            raise ValueError("a teacher's class scores need three classes or more")
+        numbers = teacher.class_numbers(known)
+        # (everything that is wrong with the teacher is said before the training begins)
+        teacher_arrays(len(y), numbers, teacher.scores, teacher.lse, teacher.temperature, teacher.weight)
+        s = Session(X.data, X.indptr, X.indices, y, depth=self.depth, n_trees=self.n_trees, min_child_weight=self.min_child_weight,
+                    lambda_=self.lambda_tgbm, gamma=self.gamma, max_num_bin=self.max_num_bin, learning_rate=self.learning_rate,
+                    objective=self.objective, num_class=self.num_class, verbose=self.verbose)
+        try:
+            s.set_option("column_sampling_rate", self.column_sampling_rate)
+            s.set_option("bagging", int(self.bagging))
+            s.set_teacher(numbers, teacher.scores, teacher.lse, teacher.temperature, teacher.weight)
+            s.boost(self.n_trees)
+            self._release()
+            self.model = C.c_void_p(s.export_model())
+            self.tree_per_iter = s.tree_per_rounds
+            self.num_class = len(known)
+            self.group_label = s.labels().tolist()
+        finally:
+            s.close()
+        return self
+
+    def _class_rules(self, n, bias, allowed, shown, repetition, frequency, presence):
+        """The checked rules of a prediction of n rows on the host, and the struct that points to them."""
+        if not self.model:
+            raise ValueError("Please train the model first or load model from file!")
+        if self.objective not in ("multi:softmax", "multi:softprob"):
+            raise ValueError("class scores need a model with the objective multi:softmax or multi:softprob")
+        classes, known = self.tree_per_iter, np.asarray(self.group_label, dtype=np.float32)
+        r, keep = _Rules(repetition=1.0), []
+        if bias is not None:
+            bias = np.ascontiguousarray(bias, dtype=np.float32)
+            if bias.shape != (classes,):
+                raise ValueError("bias: a number for each of %d classes is wanted, got the shape %s" % (classes, bias.shape))
+            r.bias = bias.ctypes.data
+            keep.append(bias)
+        if allowed is not None:
+            allowed = np.atleast_2d(np.asarray(allowed, dtype=bool))
+            if allowed.shape not in ((1, classes), (n, classes)):
+                raise ValueError("allowed: [classes] or [rows, classes] is wanted, got %s" % (allowed.shape,))
+            padded = np.zeros((len(allowed), (classes + 31) // 32 * 32), dtype=bool)
+            padded[:, :classes] = allowed
+            words = np.packbits(padded, axis=1, bitorder="little")
+            r.allowed, r.allowed_sets = words.ctypes.data, len(allowed)
+            keep.append(words)
+        if shown is not None:
+            if len(shown) != n:
+                raise ValueError("shown: a list of labels for each of %d rows is wanted, got %d" % (n, len(shown)))
+            begin = np.zeros(n + 1, dtype=np.int64)
+            begin[1:] = np.cumsum([len(labels) for labels in shown])
+            labels = np.concatenate([np.asarray(labels, dtype=np.float32) for labels in shown]) if n else np.zeros(0, np.float32)
+            at = np.minimum(np.searchsorted(known, labels), classes - 1)
+            lists = np.where(known[at] == labels, at, -1).astype(np.int32)
+            if not (repetition > 0 and np.isfinite(repetition) and np.isfinite(frequency) and np.isfinite(presence)):
+                raise ValueError("repetition %r, frequency %r, presence %r: numbers are wanted, the first above 0" % (repetition, frequency, presence))
+            if len(lists):
+                r.shown, r.shown_begin, r.n_shown = lists.ctypes.data, begin.ctypes.data, len(lists)
+            r.repetition, r.frequency, r.presence = repetition, frequency, presence
+            keep += [lists, begin]
+        return r, keep
+
+    def class_scores(self, X, bias=None, allowed=None, shown=None, repetition=1.0, frequency=0.0, presence=0.0):
+        """The scores of the classes (in the order of group_label) with what is known besides the model, float32 [classes, rows]:
+        bias [classes] is added; classes that a row was shown before (shown: a sequence of labels for each row) are held back as
+        scores.adjust says; classes that are not allowed (truth values, [classes] or [rows, classes]) get -inf."""
+        X = _csr(X)
+        n = X.shape[0]
+        r, keep = self._class_rules(n, bias, allowed, shown, repetition, frequency, presence)
+        indptr, indices = np.ascontiguousarray(X.indptr, dtype=np.int32), np.ascontiguousarray(X.indices, dtype=np.int32)
+        out = np.empty((self.tree_per_iter, n), dtype=np.float32)
+        _lib.load().tgbm_predict_adjusted(n, _ptr(X.data), _ptr(indptr), _ptr(indices), self.model, self.n_trees, self.tree_per_iter,
+                                          self.learning_rate, C.byref(r), _ptr(out))
+        return out
+
+    def top_classes(self, X, k=1, bias=None, allowed=None, shown=None, repetition=1.0, frequency=0.0, presence=0.0, temperature=1.0):
+        """The labels of the k best classes of every row by `class_scores`, [rows, k], and their probabilities (softmax of the scores over the
+        temperature). Where fewer are allowed a list ends with NaN and probability 0."""
+        X = _csr(X)
+        n = X.shape[0]
+        r, keep = self._class_rules(n, bias, allowed, shown, repetition, frequency, presence)
+        if not 1 <= k <= 128:
+            raise ValueError("k is %r: 1 to 128 is wanted" % (k,))
+        if not 1e-6 <= temperature <= 1e6:
+            raise ValueError("temperature is %r: 1e-6 to 1e6 is wanted" % (temperature,))
+        indptr, indices = np.ascontiguousarray(X.indptr, dtype=np.int32), np.ascontiguousarray(X.indices, dtype=np.int32)
+        values, classes, lse = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+        _lib.load().tgbm_predict_top(n, _ptr(X.data), _ptr(indptr), _ptr(indices), self.model, self.n_trees, self.tree_per_iter,
+                                     self.learning_rate, C.byref(r), k, temperature, _ptr(values), _ptr(classes), _ptr(lse))
+        known = np.asarray(self.group_label, dtype=np.float32)
+        labels = np.where(classes >= 0, known[np.maximum(classes, 0)], np.float32(np.nan))
+        lse = np.where(np.isneginf(lse), np.float32(0), lse)  # (nothing is allowed: no probability anywhere)
+        return labels, np.exp(values / np.float32(temperature) - lse[:, None])
 
     def predict(self, X, groups=None):
         if not self.model:

@@ -4,6 +4,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
+from .scores import _Teacher
 
 NODE_DTYPE = np.dtype(
     [
@@ -28,6 +29,30 @@ CTL_DTYPE = np.dtype([("hchunk", "<i4"), ("n_hitems", "<i4"), ("n_pitems", "<i4"
 
 def _p(a):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def teacher_arrays(n, classes, scores, lse, temperature, weight):
+    """The checked arrays of a teacher on the host, and the struct that points to them."""
+    classes = np.ascontiguousarray(classes, dtype=np.int32)
+    scores = np.asarray(scores)
+    scores = np.ascontiguousarray(scores, dtype=np.float16 if scores.dtype == np.float16 else np.float32)
+    if classes.ndim != 2 or classes.shape != scores.shape or len(classes) != n:
+        raise ValueError("teacher: classes and scores of %d rows are wanted, got %s and %s" % (n, classes.shape, scores.shape))
+    if not 1 <= classes.shape[1] <= 128:
+        raise ValueError("teacher: 1 to 128 entries are wanted, got %d" % classes.shape[1])
+    if np.isnan(scores).any() or np.isposinf(scores).any():
+        raise ValueError("teacher: a score is NaN or infinite")
+    if lse is not None:
+        lse = np.ascontiguousarray(lse, dtype=np.float32)
+        if lse.shape != (n,) or not np.isfinite(lse).all():
+            raise ValueError("teacher: lse of %d rows, all finite, is wanted" % n)
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError("teacher: temperature is %r: 1e-3 to 1e3 is wanted" % (temperature,))
+    if not 0 <= weight <= 1:
+        raise ValueError("teacher: weight is %r: 0 to 1 is wanted" % (weight,))
+    t = _Teacher(classes.ctypes.data, scores.ctypes.data, None if lse is None else lse.ctypes.data, 1 if scores.dtype == np.float16 else 0,
+                 classes.shape[1])
+    return (classes, scores, lse), t
 
 
 class Session:
@@ -72,6 +97,19 @@ class Session:
 
     def set_option(self, key, value):
         self.L.tgbm_trainer_set_option(self.h, key.encode(), float(value))
+
+    def set_teacher(self, classes, scores=None, lse=None, temperature=1.0, weight=1.0):
+        """The rounds from here on train on the loss against a teacher's best scores (scores.distill), with the session's labels:
+        classes [rows, entries] are numbers of its ascending distinct labels, scores are float32 or float16 (others become
+        float32). None: on the labels alone again."""
+        if classes is None:
+            self.L.tgbm_trainer_set_teacher(self.h, None, 1.0, 1.0)
+            return
+        arrays, t = teacher_arrays(self.n, classes, scores, lse, temperature, weight)
+        self.L.tgbm_trainer_set_teacher(self.h, C.byref(t), temperature, weight)
+
+    def teacher_loss(self):
+        return self.L.tgbm_trainer_teacher_loss(self.h)
 
     def sample_columns(self):
         self.L.tgbm_trainer_sample_columns(self.h)
