@@ -34,16 +34,27 @@ __device__ __forceinline__ void group_sync() {
     else __syncthreads();
 }
 
+// What a group of W wavefronts shares. The list of candidates is elsewhere (Places).
 template <int W>
-struct TopList {
-    static constexpr int kRoom = W == 1 ? 256 : 1024;
-    unsigned long long entry[kRoom];  // ordered score, then the complement of the place: larger is better
+struct TopShared {
     unsigned best[W == 1 ? 1 : W * 64];
     int first[W == 1 ? 1 : W * 64];
     float part_max[W], part_sum[W];
     int part[W];
     int count, exact, at_most;
     unsigned bound;
+};
+
+// The list: candidate e is the ordered score base[2 * e * stride] and the complement of its place behind it; larger is better.
+struct Places {
+    unsigned *base;
+    int stride, room;
+    __device__ __forceinline__ void put(int e, unsigned score, int place) const {
+        base[(size_t)(2 * e) * stride] = score;
+        base[(size_t)(2 * e + 1) * stride] = (unsigned)~place;
+    }
+    __device__ __forceinline__ unsigned score(int e) const { return base[(size_t)(2 * e) * stride]; }
+    __device__ __forceinline__ unsigned place(int e) const { return base[(size_t)(2 * e + 1) * stride]; }
 };
 
 template <int M>
@@ -66,8 +77,16 @@ __device__ __forceinline__ int count_up_to(const int (&f)[M], int most) {
 template <int M>
 __device__ __forceinline__ unsigned find_bound(const unsigned (&b)[M], int k, int limit, int *exact) {
     *exact = 0;
-    unsigned lo = kLeast, hi = 0xff800001u;  // (one past infinity)
-    if (count_from(b, lo) <= limit) return lo;
+    if (count_from(b, kLeast) <= limit) return kLeast;
+    // bisection between the least and the largest of them
+    float most = kNothing, least = -kNothing;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+        most = fmaxf(most, from_ordered(b[j]));
+        least = fminf(least, b[j] >= kLeast ? from_ordered(b[j]) : -kNothing);
+    }
+    unsigned lo = ordered(-wave_max_f(-least)), hi = ordered(wave_max_f(most)) + 1;
+    if (count_from(b, hi - 1) > limit) lo = hi - 1;  // (many are the largest)
     while (hi - lo > 1) {
         const unsigned mid = lo + (hi - lo) / 2;
         const int n = count_from(b, mid);
@@ -94,9 +113,9 @@ __device__ __forceinline__ int find_place(const int (&f)[M], int need) {
     return hi;
 }
 
-// The same over all scores of the group.
+// Over all threads of the group.
 template <int W>
-__device__ __forceinline__ int group_sum(int n, TopList<W> &sh) {
+__device__ __forceinline__ int group_sum(int n, TopShared<W> &sh) {
     n = wave_sum_i(n);
     if constexpr (W == 1) return n;
     __syncthreads();
@@ -107,17 +126,66 @@ __device__ __forceinline__ int group_sum(int n, TopList<W> &sh) {
     return all;
 }
 
-// The candidates of the group's k best: sh.entry, as many as are returned, the same in all threads. at(i): the place of v[i],
-// which ascends with i. Every thread of the group comes here.
-template <int W, int E, typename At>
-__device__ __forceinline__ int list_candidates(const float (&v)[E], At at, int k, TopList<W> &sh) {
-    const int lane = lane_id(), t = W == 1 ? lane : (int)threadIdx.x;
+// Where the scores of a thread lie: v[i] at base + i / V * step + i % V, the last of N at `extra` where it is apart from them.
+template <int N, int V, bool EXTRA>
+struct Layout {
+    int base, step, extra;
+    __device__ __forceinline__ int at(int i) const { return EXTRA && i == N - 1 ? extra : base + i / V * step + i % V; }
+    // (with a constant i: at(i) <= most without a register for every at(i))
+    __device__ __forceinline__ bool up_to(int i, int most) const { return EXTRA && i == N - 1 ? extra <= most : base <= most - (i / V * step + i % V); }
+};
+
+// Keeps the compiler from working out all of a loop's conditions or addresses ahead of it, in registers that it does not have.
+__device__ __forceinline__ unsigned one_by_one(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+__device__ __forceinline__ float one_by_one(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+template <int E>
+__device__ __forceinline__ float best_of(const float (&v)[E]) {
     float best = kNothing;
 #pragma unroll
     for (int i = 0; i < E; ++i) best = fmaxf(best, v[i]);
+    return best;
+}
+
+// Writes the scores that `mine` marks (bit i: v[i]) behind those of the threads before, and returns how many the group has, the
+// list's room being there or not.
+template <int W, int E, typename At>
+__device__ __forceinline__ int put_marked(const float (&v)[E], unsigned mine, At at, TopShared<W> &sh, const Places &list) {
+    const int scan = wave_scan_i(__popc(mine));
+    int total = __shfl(scan, 63), to = scan - __popc(mine);
+    if constexpr (W > 1) {
+        int base = 0;
+        if (lane_id() == 0) base = atomicAdd(&sh.count, total);
+        to += __shfl(base, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        mine = one_by_one(mine);
+        if (mine >> i & 1u) {
+            if (to < list.room) list.put(to, ordered(one_by_one(v[i])), at.at(i));
+            ++to;
+        }
+    }
+    group_sync<W>();
+    if constexpr (W > 1) total = sh.count;
+    return total;
+}
+
+// The candidates of the group's k best, as many as are returned, the same in all threads. at: a Layout, whose places
+// ascend with i; best: the thread's largest. Every thread of the group comes here. The list holds at least k.
+template <int W, int E, typename At>
+__device__ __forceinline__ int list_candidates(const float (&v)[E], float best, At at, int k, TopShared<W> &sh, const Places &list) {
+    const int lane = lane_id(), t = W == 1 ? lane : (int)threadIdx.x;
     const int limit = k + max(4, k / 4);
     unsigned bound;
-    int exact, at_most = INT_MAX;
+    int exact;
     if constexpr (W == 1) {
         const unsigned b[1] = {ordered(best)};
         bound = find_bound(b, k, limit, &exact);
@@ -140,12 +208,16 @@ __device__ __forceinline__ int list_candidates(const float (&v)[E], At at, int k
         bound = sh.bound;
         exact = sh.exact;
     }
-    if (exact) {  // (the same in all threads)
-        const float equal = from_ordered(bound);
-        int first = INT_MAX;
+    const float least = from_ordered(bound);
+    unsigned mine = 0;
+    if (!exact) {  // (the same in all threads)
 #pragma unroll
-        for (int i = E - 1; i >= 0; --i) first = v[i] == equal ? at(i) : first;
-        if (best != equal) first = INT_MAX;
+        for (int i = 0; i < E; ++i) mine |= (v[i] >= least ? 1u : 0u) << i;
+    } else {
+        int first = INT_MAX, at_most;
+#pragma unroll
+        for (int i = E - 1; i >= 0; --i) first = v[i] == least ? i : first;
+        first = best == least ? at.at(first) : INT_MAX;
         if constexpr (W == 1) {
             const unsigned b[1] = {ordered(best)};
             const int f[1] = {first};
@@ -167,75 +239,46 @@ __device__ __forceinline__ int list_candidates(const float (&v)[E], At at, int k
             __syncthreads();
             at_most = sh.at_most;
         }
-    }
-    const float least = from_ordered(bound);
-    unsigned mine = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) mine |= (v[i] >= least && (v[i] > least || at(i) <= at_most) ? 1u : 0u) << i;
-    int scan = wave_scan_i(__popc(mine));
-    int total = __shfl(scan, 63), begin = scan - __popc(mine);
-    if constexpr (W > 1) {
-        int base = 0;
-        if (lane == 0) base = atomicAdd(&sh.count, total);
-        begin += __shfl(base, 0);
+        for (int i = 0; i < E; ++i) mine |= (v[i] > least || (v[i] == least && at.up_to(i, at_most)) ? 1u : 0u) << i;
     }
-    auto put = [&] {
-        int to = begin;
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (mine >> i & 1u) {
-                if (to < TopList<W>::kRoom) sh.entry[to] = (unsigned long long)ordered(v[i]) << 32 | (unsigned)~at(i);
-                ++to;
-            }
-    };
-    put();
-    group_sync<W>();
-    if constexpr (W > 1) total = sh.count;
-    if (total <= TopList<W>::kRoom) return total;
+    const int total = put_marked<W>(v, mine, at, sh, list);
+    if (total <= list.room) return total;
     // The best scores lie together in few threads: the exact k-th one by bisection over all of them.
-    unsigned lo = bound, hi = 0xff800001u;
-    auto count = [&](unsigned from) {
-        const float f = from_ordered(from);
+    unsigned lo = bound, hi = 0xff800001u;  // (one past infinity)
+    while (hi - lo > 1) {
+        const unsigned mid = lo + (hi - lo) / 2;
+        const float f = from_ordered(mid);
         int n = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) n += v[i] >= f ? 1 : 0;
-        return group_sum<W>(n, sh);
-    };
-    while (hi - lo > 1) {
-        const unsigned mid = lo + (hi - lo) / 2;
-        if (count(mid) >= k) lo = mid;
+        if (group_sum<W>(n, sh) >= k) lo = mid;
         else hi = mid;
     }
-    const int need = k - (lo == 0xff800000u ? 0 : count(lo + 1));
     const float equal = from_ordered(lo);
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) above += v[i] > equal ? 1 : 0;
+    const int need = k - group_sum<W>(above, sh);
     int p_lo = -1, p_hi = INT_MAX - 1;
     while (p_hi - p_lo > 1) {
         const int mid = p_lo + (p_hi - p_lo) / 2;
+        const float now = one_by_one(equal);
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) n += v[i] == equal && at(i) <= mid ? 1 : 0;
+        for (int i = 0; i < E; ++i) n += v[i] == now && at.up_to(i, mid) ? 1 : 0;
         if (group_sum<W>(n, sh) >= need) p_hi = mid;
         else p_lo = mid;
     }
     mine = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) mine |= (v[i] > equal || (v[i] == equal && at(i) <= p_hi) ? 1u : 0u) << i;
-    scan = wave_scan_i(__popc(mine));
-    begin = scan - __popc(mine);
-    total = __shfl(scan, 63);
+    for (int i = 0; i < E; ++i) mine |= (v[i] > equal || (v[i] == equal && at.up_to(i, p_hi)) ? 1u : 0u) << i;
     if constexpr (W > 1) {
         __syncthreads();
-        sh.part[wave_id()] = total;
+        if (t == 0) sh.count = 0;
         __syncthreads();
-        total = 0;
-        for (int w = 0; w < W; ++w) {
-            if (w < wave_id()) begin += sh.part[w];
-            total += sh.part[w];
-        }
     }
-    put();
-    group_sync<W>();
-    return total;
+    return put_marked<W>(v, mine, at, sh, list);
 }
 
 // Where a row's (or a chunk's) best classes go.
@@ -247,15 +290,18 @@ struct TopOut {
 
 // The candidates in order. class_at(place): the class.
 template <int W, typename Class>
-__device__ __forceinline__ void write_best(const TopList<W> &sh, int found, int k, size_t slot, const TopOut &out, Class class_at) {
+__device__ __forceinline__ void write_best(const Places &list, int found, int k, size_t slot, const TopOut &out, Class class_at) {
     const int t = W == 1 ? lane_id() : (int)threadIdx.x;
     for (int j = t; j < found; j += 64 * W) {
-        const unsigned long long e = sh.entry[j];
+        const unsigned score = list.score(j), place = list.place(j);
         int better = 0;
-        for (int o = 0; o < found; ++o) better += sh.entry[o] > e ? 1 : 0;
+        for (int o = 0; o < found; ++o) {
+            const unsigned s = list.score(o);
+            better += s > score || (s == score && list.place(o) > place) ? 1 : 0;
+        }
         if (better < k) {
-            out.values[slot * k + better] = from_ordered((unsigned)(e >> 32));
-            out.classes[slot * k + better] = class_at((int)~(unsigned)e);
+            out.values[slot * k + better] = from_ordered(score);
+            out.classes[slot * k + better] = class_at((int)~place);
         }
     }
     for (int j = found + t; j < k; j += 64 * W) {
@@ -264,8 +310,6 @@ __device__ __forceinline__ void write_best(const TopList<W> &sh, int found, int 
     }
 }
 
-// The largest of the group's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
-// NaN, an infinity makes it infinite.
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float reference_of(float m) { return fabsf(m) <= FLT_MAX ? m : 0.f; }
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -275,15 +319,25 @@ __device__ __forceinline__ float rescaled(float sum, float from, float to, float
     return sum <= FLT_MAX ? sum * exp2_of((from - to) * by) : sum;
 }
 
+// The largest of the group's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
+// NaN, an infinity makes it infinite. best: the thread's largest.
 template <int W, int E>
-__device__ __forceinline__ void sum_exponentials(const float (&v)[E], float by, TopList<W> &sh, float *reference, float *sum) {
-    float m = kNothing;
+__device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best, float by, TopShared<W> &sh, float *reference, float *sum) {
+    float m = reference_of(wave_max_f(best));
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    if (fabsf(m) < 1e30f) {
+        // one multiply-add for the argument; what the product m * by was rounded by is put right in the sum
+        const float shift = m * by, off = __builtin_fmaf(m, by, -shift);
 #pragma unroll
-    for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
-    m = reference_of(wave_max_f(m));
-    float s = 0.f;
+        for (int i = 0; i < E; ++i) part[i % 4] += exp2_of(__builtin_fmaf(v[i], by, -shift));
+        const float s = (part[0] + part[1]) + (part[2] + part[3]);
+        part[0] = s <= FLT_MAX ? __builtin_fmaf(s, -off * kLn2, s) : s;
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += exp2_of((v[i] - m) * by);
+        for (int i = 0; i < E; ++i) part[i % 4] += exp2_of((v[i] - m) * by);
+        part[0] = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    float s = part[0];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     if constexpr (W > 1) {
@@ -307,70 +361,127 @@ __device__ __forceinline__ float log_sum(float m, float s, float temperature) {
     return s > 0.f || s != s ? m / temperature + __builtin_amdgcn_logf(s) * kLn2 : kNothing;
 }
 
-// Classes side by side: E scores of a thread, by vectors of 16 bytes.
+// Classes side by side: E scores of a thread, by vectors of 16 bytes, which need not lie on such an address.
 template <typename T>
 struct Vector {
     static constexpr int kOf = 16 / (int)sizeof(T);
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
+typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// A group of W wavefronts takes chunk `tile % chunks` of a row; with W = 1 there are four groups to a workgroup. LDS behind the
-// lists: how often the classes of the chunk were shown, where there are lists.
-template <typename T, int W, int E>
-__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
+// LDS of a group's lists of shown classes: a bit for each class of the chunk, and how often where the bit is set.
+template <int W>
+__device__ __forceinline__ void count_shown(const tgbm_score_rules &rules, long long b, long long e, int c0, int c1, int chunk, unsigned *bits, unsigned *times) {
+    const int t = W == 1 ? lane_id() : (int)threadIdx.x;
+    for (int w = t; w < chunk / 32; w += 64 * W) bits[w] = 0;
+    group_sync<W>();
+    for (long long i = b + t; i < e; i += 64 * W) {
+        const int c = rules.shown[i];
+        if (c < c0 || c >= c1) continue;
+        times[c - c0] = 0;
+        atomicOr(&bits[(c - c0) / 32], 1u << ((c - c0) % 32));
+    }
+    group_sync<W>();
+    for (long long i = b + t; i < e; i += 64 * W) {
+        const int c = rules.shown[i];
+        if (c >= c0 && c < c1) atomicAdd(&times[c - c0], 1u);
+    }
+    group_sync<W>();
+}
+
+// A group of W wavefronts takes chunk `tile % chunks` (a multiple of 32 classes) of a row; with W = 1 there are four groups to a
+// workgroup. A thread has E scores in whole vectors, and one of what is left behind the last vector. RULES: there may be any. LDS: the lists of candidates,
+// then, where classes were shown, bits and times.
+template <typename T, int W, int E, bool RULES>
+__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
                                                                           int chunks, int chunk, long tiles, bool whole) {
-    constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
-    __shared__ TopList<W> lists[kGroups];
-    extern __shared__ unsigned shown_times[];
-    constexpr int V = Vector<T>::kOf;
+    constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1, kRoom = W == 1 ? 256 : 1024;
+    __shared__ TopShared<W> shared[kGroups];
+    __shared__ unsigned candidates[kGroups][2 * kRoom];
+    extern __shared__ unsigned shown_lds[];
+    constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
-    TopList<W> &sh = lists[group];
-    unsigned *times = shown_times + (size_t)group * chunk;
+    TopShared<W> &sh = shared[group];
+    const Places list{candidates[group], 1, kRoom};
+    unsigned *bits = shown_lds + (size_t)group * (chunk + chunk / 32), *times = bits + chunk / 32;
     const float by = kLog2e / temperature;
     for (long tile = (long)blockIdx.x * kGroups + group; tile < tiles; tile += (long)gridDim.x * kGroups) {
         const long row = tile / chunks;
-        const int c0 = (int)(tile % chunks) * chunk, c1 = min(in.classes, c0 + chunk);
-        bool counted = false;
-        if (rules.shown != nullptr) {
-            long long b, e;
-            shown_range(rules, row, &b, &e);
-            counted = b < e;  // (the same for the group)
-            if (counted) {
-                for (int c = t; c < chunk; c += 64 * W) times[c] = 0;
-                group_sync<W>();
-                for (long long i = b + t; i < e; i += 64 * W) {
-                    const int c = rules.shown[i];
-                    if (c >= c0 && c < c1) atomicAdd(&times[c - c0], 1u);
+        const int c0 = (int)(tile % chunks) * chunk, size = min(in.classes - c0, chunk), whole_size = size / V * V;
+        // (a thread's places are worked out where they are used, not kept over the tiles)
+        const Layout<N, V, true> at{(int)one_by_one((unsigned)t * V), kStep, (int)one_by_one((unsigned)(whole_size + t))};
+        const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride + c0;
+        float v[N];
+        {
+            typename Vector<T>::type x[E / V];
+#pragma unroll
+            for (int g = 0; g < E / V; ++g) {
+                x[g] = (T)kNothing;
+                if (at.base < whole_size - g * kStep) x[g] = *reinterpret_cast<const typename Vector<T>::type *>(src + at.base + g * kStep);
+            }
+            v[E] = t < size - whole_size ? score_to_float(src[at.extra]) : kNothing;
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = score_to_float(x[i / V][i % V]);
+        }
+        if constexpr (RULES) {
+            if (rules.bias != nullptr) {
+                const float *bias = rules.bias + c0;
+#pragma unroll
+                for (int g = 0; g < E / V; ++g)
+                    if (at.base < whole_size - g * kStep) {
+#pragma unroll
+                        for (int j = 0; j < V; j += 4) {
+                            const Float4 b = *reinterpret_cast<const Float4 *>(bias + at.base + g * kStep + j);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) v[g * V + j + q] += b[q];
+                        }
+                    }
+                if (t < size - whole_size) v[E] += bias[at.extra];
+            }
+            bool none;
+            const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+            if (rules.shown != nullptr) {
+                long long b, e;
+                shown_range(rules, row, &b, &e);
+                if (b < e) {  // (the same for the group)
+                    count_shown<W>(rules, b, e, c0, c0 + size, chunk, bits, times);
+                    unsigned held = 0;
+#pragma unroll
+                    for (int g = 0; g < E / V; ++g) {
+                        const int c = at.base + g * kStep;
+                        if (c < whole_size) held |= (bits[c / 32] >> (c % 32) & ((1u << V) - 1u)) << (g * V);
+                    }
+                    if (t < size - whole_size) held |= (bits[at.extra / 32] >> (at.extra % 32) & 1u) << E;
+                    // few of a thread's scores are: one at a time, from the start (its register has no number that a loop can use)
+                    while (__any(held != 0)) {
+                        const bool now = held != 0;
+                        const int i = now ? __ffs((int)held) - 1 : 0;
+                        float s = 0.f;
+                        if (now) {
+                            const int c = at.at(i);
+                            s = adjusted(score_to_float(src[c]), rules.bias != nullptr ? rules.bias[c0 + c] : 0.f, times[c], true, rules);
+                        }
+                        held &= held - 1;
+#pragma unroll
+                        for (int j = 0; j < N; ++j) v[j] = now && j == i ? s : v[j];
+                    }
                 }
-                group_sync<W>();
+            }
+            if (words != nullptr || none) {
+#pragma unroll
+                for (int g = 0; g < E / V; ++g) {
+                    const int c = at.base + g * kStep;
+                    const unsigned ok = words != nullptr && c < whole_size ? words[(c0 + c) / 32] >> (c % 32) : 0u;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[g * V + j] = ok >> j & 1u ? v[g * V + j] : kNothing;
+                }
+                const bool ok = words != nullptr && t < size - whole_size && (words[(c0 + at.extra) / 32] >> (at.extra % 32) & 1u);
+                v[E] = ok ? v[E] : kNothing;
             }
         }
-        bool none;
-        const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-        const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
-        float v[E];
-#pragma unroll
-        for (int g = 0; g < E / V; ++g) {
-            const int c = c0 + (g * 64 * W + t) * V;
-            typename Vector<T>::type x;
-            if (c + V <= c1) {
-                x = *reinterpret_cast<const typename Vector<T>::type *>(src + c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = c + j < c1 ? src[c + j] : (T)kNothing;
-            }
-            unsigned ok = none ? 0u : ~0u;
-            if (words != nullptr && c < c1) ok = words[c / 32] >> (c % 32);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float s = score_to_float(x[j]);
-                if (c + j < c1)
-                    s = adjusted(s, rules.bias != nullptr ? rules.bias[c + j] : 0.f, counted ? times[c + j - c0] : 0u, ok >> j & 1u, rules);
-                v[g * V + j] = s;
-            }
-        }
+        const float best = best_of(v);
         float m, s;
-        sum_exponentials<W>(v, by, sh, &m, &s);
+        sum_exponentials<W>(v, best, by, sh, &m, &s);
         if (t == 0) {
             if (whole) {
                 out.lse[row] = log_sum(m, s, temperature);
@@ -379,60 +490,94 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_rows(tgbm_s
                 out.lse[tile * 2 + 1] = s;
             }
         }
-        const int found = list_candidates<W>(v, [&](int i) { return c0 + ((i / V) * 64 * W + t) * V + i % V; }, k, sh);
-        write_best(sh, found, k, (size_t)tile, out, [](int place) { return place; });
+        const int found = list_candidates<W>(v, best, at, k, sh, list);
+        write_best<W>(list, found, k, (size_t)tile, out, [&](int p) { return c0 + p; });
         group_sync<W>();
     }
 }
 
-// Rows side by side: a workgroup brings `rows` rows of a chunk of at most 64 * E classes into LDS, class by class, and its
-// wavefronts take a row each.
-constexpr int kColumnBlock = 512;
-template <typename T, int E>
-__global__ __launch_bounds__(kColumnBlock) void k_top_columns(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out, int chunks,
-                                                              int chunk, int row_bits, long tiles, bool whole) {
-    __shared__ TopList<1> lists[kColumnBlock / 64];
-    extern __shared__ unsigned cell[];  // [chunk][rows + 1]
+// Rows side by side: a workgroup brings `rows` rows of a chunk (a multiple of 32, at most 64 * E classes) into LDS, class by class, eight
+// classes of a row to a thread at a time, and its wavefronts take a row each. A row's column is its list of candidates once
+// its scores are in registers. LDS: [tile_classes][rows + 1] scores, then, where classes were shown, [rows][chunk / 32] bits.
+constexpr int kColumnBlock = 1024;
+template <typename T, int E, bool RULES>
+__global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out, int chunks,
+                                                                 int chunk, int row_bits, int tile_classes, long tiles, bool whole) {
+    __shared__ TopShared<1> sh;  // (nothing of it is used by one wavefront)
+    extern __shared__ unsigned cell[];
     const int rows = 1 << row_bits, pitch = rows + 1;
+    unsigned *const bits = cell + (size_t)tile_classes * pitch;
     const float by = kLog2e / temperature;
     const int r = threadIdx.x & (rows - 1), slot = threadIdx.x >> row_bits, slots = kColumnBlock >> row_bits;
+    const T *src = static_cast<const T *>(in.data);
     for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const long row0 = tile / chunks * rows, row = row0 + r;
         const int c0 = (int)(tile % chunks) * chunk, c1 = min(in.classes, c0 + chunk);
-        if (rules.shown != nullptr) {
-            for (int i = threadIdx.x; i < chunk * pitch; i += kColumnBlock) cell[i] = 0;
-            __syncthreads();
-            long long b = 0, e = 0;
-            if (row < in.rows) shown_range(rules, row, &b, &e);
-            for (long long i = b + slot; i < e; i += slots) {
-                const int c = rules.shown[i];
-                if (c >= c0 && c < c1) atomicAdd(&cell[(c - c0) * pitch + r], 1u);
+        unsigned *const my_bits = bits + r * (chunk / 32);
+        bool counted = false;
+        if constexpr (RULES) {
+            counted = rules.shown != nullptr;
+            if (counted) {
+                for (int i = threadIdx.x; i < rows * (chunk / 32); i += kColumnBlock) bits[i] = 0;
+                __syncthreads();
+                long long b = 0, e = 0;
+                if (row < in.rows) shown_range(rules, row, &b, &e);
+                for (long long i = b + slot; i < e; i += slots) {
+                    const int c = rules.shown[i] - c0;
+                    if (c < 0 || c >= c1 - c0) continue;
+                    cell[c * pitch + r] = 0;
+                    atomicOr(&my_bits[c / 32], 1u << (c % 32));
+                }
+                __syncthreads();
+                for (long long i = b + slot; i < e; i += slots) {
+                    const int c = rules.shown[i] - c0;
+                    if (c >= 0 && c < c1 - c0) atomicAdd(&cell[c * pitch + r], 1u);
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (row < in.rows) {
-            bool none;
-            const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-            const T *src = static_cast<const T *>(in.data);
-            for (int c = c0 + slot; c < c1; c += slots) {
-                const float z = score_to_float(src[(size_t)c * in.class_stride + row]);
-                unsigned *at = cell + (c - c0) * pitch + r;
-                const bool ok = !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u));
-                *at = __float_as_uint(adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, rules.shown != nullptr ? *at : 0u, ok, rules));
+            bool none = false;
+            const unsigned *words = RULES ? allowed_words(rules, row, (in.classes + 31) / 32, &none) : nullptr;
+            for (int c = slot * 8; c < c1 - c0; c += slots * 8) {
+                const T *from = src + (size_t)(c0 + c) * in.class_stride + row;
+                unsigned *to = cell + c * pitch + r;
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = c + j < c1 - c0 ? score_to_float(from[(size_t)j * in.class_stride]) : kNothing;
+                if constexpr (!RULES) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c + j < c1 - c0) to[j * pitch] = __float_as_uint(z[j]);
+                } else {
+                    unsigned ok = none ? 0u : words != nullptr ? words[(c0 + c) / 32] >> ((c0 + c) % 32) : ~0u;
+                    unsigned held = counted ? my_bits[c / 32] >> (c % 32) & 0xffu : 0u;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c + j < c1 - c0) {
+                            const float s = rules.bias != nullptr ? z[j] + rules.bias[c0 + c + j] : z[j];
+                            if (!(held >> j & 1u)) to[j * pitch] = __float_as_uint(ok >> j & 1u ? s : kNothing);
+                        }
+                    while (held != 0) {
+                        const int j = __ffs((int)held) - 1;
+                        held &= held - 1;
+                        to[j * pitch] = __float_as_uint(adjusted(score_to_float(from[(size_t)j * in.class_stride]), rules.bias != nullptr ? rules.bias[c0 + c + j] : 0.f,
+                                                                 to[j * pitch], ok >> j & 1u, rules));
+                    }
+                }
             }
         }
         __syncthreads();
-        TopList<1> &sh = lists[wave_id()];
         for (int q = wave_id(); q < rows && row0 + q < in.rows; q += kColumnBlock / 64) {
+            const int lane = (int)one_by_one((unsigned)lane_id());  // (places are worked out where they are used)
+            const unsigned *from = cell + lane * pitch + q;
             float v[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const int c = i * 64 + lane_id();
-                v[i] = c < c1 - c0 ? __uint_as_float(cell[c * pitch + q]) : kNothing;
-            }
+            for (int i = 0; i < E; ++i) v[i] = lane < c1 - c0 - i * 64 ? __uint_as_float(from[i * 64 * pitch]) : kNothing;
             const size_t out_at = (size_t)(row0 + q) * chunks + tile % chunks;
+            const float best = best_of(v);
             float m, s;
-            sum_exponentials<1>(v, by, sh, &m, &s);
+            sum_exponentials<1>(v, best, by, sh, &m, &s);
             if (lane_id() == 0) {
                 if (whole) {
                     out.lse[row0 + q] = log_sum(m, s, temperature);
@@ -441,9 +586,10 @@ __global__ __launch_bounds__(kColumnBlock) void k_top_columns(tgbm_scores in, tg
                     out.lse[out_at * 2 + 1] = s;
                 }
             }
-            const int found = list_candidates<1>(v, [&](int i) { return c0 + i * 64 + lane_id(); }, k, sh);
-            write_best(sh, found, k, out_at, out, [](int place) { return place; });
             wave_fence();
+            const Places list{cell + q, pitch, tile_classes / 2};
+            const int found = list_candidates<1>(v, best, Layout<E, 1, false>{lane, 64, 0}, k, sh, list);
+            write_best<1>(list, found, k, out_at, out, [&](int p) { return c0 + p; });
         }
         __syncthreads();
     }
@@ -510,9 +656,12 @@ template <int W, int E>
 __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int parts, int per_join, int joins, long tiles, int k, float temperature, TopOut in,
                                                                           TopOut out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
-    __shared__ TopList<W> lists[kGroups];
+    constexpr int kRoom = W == 1 ? 256 : 1024;
+    __shared__ TopShared<W> shared[kGroups];
+    __shared__ unsigned candidates[kGroups][2 * kRoom];
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
-    TopList<W> &sh = lists[group];
+    TopShared<W> &sh = shared[group];
+    const Places list{candidates[group], 1, kRoom};
     const float by = kLog2e / temperature;
     for (long tile = (long)blockIdx.x * kGroups + group; tile < tiles; tile += (long)gridDim.x * kGroups) {
         const int first = (int)(tile % joins) * per_join, mine = min(parts - first, per_join), count = mine * k;
@@ -545,8 +694,8 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
                 out.lse[tile * 2 + 1] = s;
             }
         }
-        const int found = list_candidates<W>(v, [&](int i) { return i * 64 * W + t; }, k, sh);
-        write_best(sh, found, k, (size_t)tile, out, [&](int place) { return classes[place]; });
+        const int found = list_candidates<W>(v, best_of(v), Layout<E, 1, false>{(int)one_by_one((unsigned)t), 64 * W, 0}, k, sh, list);
+        write_best<W>(list, found, k, (size_t)tile, out, [&](int p) { return classes[p]; });
         group_sync<W>();
     }
 }
@@ -559,9 +708,11 @@ struct TopPlan {
     int chunks, chunk;
     int waves;     // classes side by side: wavefronts of a group
     int row_bits;  // rows side by side
+    int tile_classes;
     int per_thread;
 };
 constexpr int kFewClasses = 32;
+constexpr int kRowScores = 24;  // classes side by side: the most that a thread has in whole vectors
 constexpr int kJoinMost = 16384;  // scores that a join takes
 constexpr int kGroupsWanted = 512;
 
@@ -572,7 +723,7 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
     p.chunks = 1;
     p.chunk = classes;
     if (p.few) return p;
-    const int most = columns ? 1024 : 16384, least = columns ? 1024 : 2048;
+    const int most = columns ? 1024 : 8 * 64 * kRowScores, least = columns ? 1024 : 64 * kRowScores;
     long tiles = columns ? (rows + 15) / 16 : rows;
     long chunks = (classes - 1) / most + 1;
     chunks = std::max(chunks, std::min<long>((classes - 1) / least + 1, kGroupsWanted / std::max(1l, tiles)));
@@ -582,38 +733,40 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
     if (columns) {
         p.per_thread = 1;
         while (p.per_thread * 64 < p.chunk) p.per_thread *= 2;
+        p.tile_classes = std::max(p.chunk, 2 * kTopMost);  // (a list's room)
         p.row_bits = 4;
-        while (p.row_bits < 7 && (64l * p.per_thread << (p.row_bits + 1)) <= 16384) ++p.row_bits;
+        while (p.row_bits < 6 && (p.tile_classes << (p.row_bits + 1)) <= 16384) ++p.row_bits;
     } else {
-        p.waves = p.chunk <= 2048 ? 1 : p.chunk <= 8192 ? 4 : 8;
-        p.per_thread = p.waves > 1 ? 32 : p.chunk <= 512 ? 8 : p.chunk <= 1024 ? 16 : 32;
+        p.waves = p.chunk <= 64 * kRowScores ? 1 : p.chunk <= 256 * kRowScores ? 4 : 8;
+        p.per_thread = p.waves > 1 ? kRowScores : p.chunk <= 512 ? 8 : p.chunk <= 1024 ? 16 : kRowScores;
     }
     return p;
 }
 
-template <typename T, int W, int E>
+template <typename T, int W, int E, bool RULES>
 void top_rows(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     const long tiles = (long)in.rows * p.chunks;
-    const size_t lds = rules.shown != nullptr ? sizeof(unsigned) * (size_t)p.chunk * kGroups : 0;
+    const size_t lds = rules.shown != nullptr ? sizeof(unsigned) * (size_t)(p.chunk + p.chunk / 32) * kGroups : 0;
     if (lds > 32 * 1024) {
         static LdsOptIn opt_in;
-        opt_in({reinterpret_cast<const void *>(&k_top_rows<T, W, E>)});
+        opt_in({reinterpret_cast<const void *>(&k_top_rows<T, W, E, RULES>)});
     }
-    k_top_rows<T, W, E><<<blocks_of((tiles - 1) / kGroups + 1), W == 1 ? kTopBlock : 64 * W, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, tiles,
-                                                                                                    p.chunks == 1);
+    k_top_rows<T, W, E, RULES><<<blocks_of((tiles - 1) / kGroups + 1), W == 1 ? kTopBlock : 64 * W, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk,
+                                                                                                           tiles, p.chunks == 1);
 }
 
-template <typename T, int E>
+template <typename T, int E, bool RULES>
 void top_columns(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
     const long tiles = ((long)((in.rows - 1) >> p.row_bits) + 1) * p.chunks;
-    const size_t lds = sizeof(unsigned) * (size_t)p.chunk * ((1 << p.row_bits) + 1);
+    const size_t lds = sizeof(unsigned) * ((size_t)p.tile_classes * ((1 << p.row_bits) + 1) + (rules.shown != nullptr ? (size_t)p.chunk / 32 << p.row_bits : 0));
     static LdsOptIn opt_in;
-    opt_in({reinterpret_cast<const void *>(&k_top_columns<T, E>)});
-    k_top_columns<T, E><<<blocks_of(tiles), kColumnBlock, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.row_bits, tiles, p.chunks == 1);
+    opt_in({reinterpret_cast<const void *>(&k_top_columns<T, E, RULES>)});
+    k_top_columns<T, E, RULES><<<blocks_of(tiles), kColumnBlock, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.row_bits, p.tile_classes, tiles,
+                                                                      p.chunks == 1);
 }
 
-template <typename T>
+template <typename T, bool RULES>
 void top(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
     if (p.few) {
         const int blocks = blocks_of(((long)in.rows - 1) / kTopBlock + 1);
@@ -621,22 +774,28 @@ void top(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_scor
         else if (in.classes <= 16) k_top_few<T, 16><<<blocks, kTopBlock, 0, s>>>(in, rules, k, temperature, out);
         else k_top_few<T, 32><<<blocks, kTopBlock, 0, s>>>(in, rules, k, temperature, out);
     } else if (p.columns) {
-        if (p.per_thread <= 1) top_columns<T, 1>(s, p, in, rules, k, temperature, out);
-        else if (p.per_thread == 2) top_columns<T, 2>(s, p, in, rules, k, temperature, out);
-        else if (p.per_thread == 4) top_columns<T, 4>(s, p, in, rules, k, temperature, out);
-        else if (p.per_thread == 8) top_columns<T, 8>(s, p, in, rules, k, temperature, out);
-        else top_columns<T, 16>(s, p, in, rules, k, temperature, out);
+        constexpr bool kRules = RULES || sizeof(T) != 4;
+        if (p.per_thread <= 2) top_columns<T, 2, kRules>(s, p, in, rules, k, temperature, out);
+        else if (p.per_thread == 4) top_columns<T, 4, kRules>(s, p, in, rules, k, temperature, out);
+        else if (p.per_thread == 8) top_columns<T, 8, kRules>(s, p, in, rules, k, temperature, out);
+        else top_columns<T, 16, kRules>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 8) {
-        top_rows<T, 8, 32>(s, p, in, rules, k, temperature, out);
+        top_rows<T, 8, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 4) {
-        top_rows<T, 4, 32>(s, p, in, rules, k, temperature, out);
-    } else if (p.per_thread == 32) {
-        top_rows<T, 1, 32>(s, p, in, rules, k, temperature, out);
+        top_rows<T, 4, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
+    } else if (p.per_thread == kRowScores) {
+        top_rows<T, 1, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.per_thread == 16) {
-        top_rows<T, 1, 16>(s, p, in, rules, k, temperature, out);
+        top_rows<T, 1, 16, RULES>(s, p, in, rules, k, temperature, out);
     } else {
-        top_rows<T, 1, 8>(s, p, in, rules, k, temperature, out);
+        top_rows<T, 1, 8, RULES>(s, p, in, rules, k, temperature, out);
     }
+}
+
+template <typename T>
+void top_any(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
+    if (rules.bias != nullptr || rules.allowed != nullptr || rules.shown != nullptr) top<T, true>(s, p, in, rules, k, temperature, out);
+    else top<T, false>(s, p, in, rules, k, temperature, out);
 }
 
 template <int W, int E>
@@ -677,9 +836,9 @@ void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_ru
         return o;
     };
     TopOut now = next(p.chunks);
-    if (in.type == TGBM_F32) top<float>(s, p, in, rules, k, temperature, now);
-    else if (in.type == TGBM_F16) top<_Float16>(s, p, in, rules, k, temperature, now);
-    else top<__bf16>(s, p, in, rules, k, temperature, now);
+    if (in.type == TGBM_F32) top_any<float>(s, p, in, rules, k, temperature, now);
+    else if (in.type == TGBM_F16) top_any<_Float16>(s, p, in, rules, k, temperature, now);
+    else top_any<__bf16>(s, p, in, rules, k, temperature, now);
     for (int parts = p.chunks; parts > 1;) {
         const int per_join = std::min(parts, parts_of_a_join(k)), joins = (parts - 1) / per_join + 1, count = per_join * k;
         const TopOut to = next(joins);
