@@ -6,11 +6,15 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/thundergbm.h"
 #include "common.h"
 
 namespace tgbm {
 
+constexpr int kClassesMost = 1 << 26;
+constexpr int kSliceRows = 1 << 22;  // rows of a launch
 constexpr int kTopMost = 128;      // classes that top lists
 constexpr int kTeacherMost = 128;  // entries of a teacher's row
 
@@ -19,6 +23,20 @@ bool scores_ok(const char *entry, const char *what, const tgbm_scores *s);
 bool rules_ok(const char *entry, const tgbm_score_rules *rules, int rows);
 
 inline bool rows_side_by_side(const tgbm_scores &s) { return !(s.class_stride == 1 && (s.rows == 1 || s.row_stride != 1)); }
+
+// Rows [first, first + rows) of the scores, and the rules for them.
+inline void take_rows(tgbm_scores &s, tgbm_score_rules &rules, int first, int rows) {
+    const size_t size = s.type == TGBM_F32 ? 4 : 2;
+    s.data = static_cast<const char *>(s.data) + size * (size_t)first * (size_t)s.row_stride;
+    // (a set for each row: the later rows' sets)
+    if (rules.allowed != nullptr && rules.allowed_set == nullptr && rules.allowed_sets > 1) {
+        rules.allowed += (size_t)first * ((s.classes + 31) / 32);
+        rules.allowed_sets = std::max(2, rules.allowed_sets - first);  // (one would be everybody's)
+    }
+    if (rules.allowed_set != nullptr) rules.allowed_set += first;
+    if (rules.shown_begin != nullptr) rules.shown_begin += first;
+    s.rows = rows;
+}
 
 void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out);
 

@@ -33,7 +33,7 @@ int launched(const char *entry) {
 int check_scores(const char *entry, const char *what, const tgbm_scores *s) {
     if (s == nullptr) return refused(entry, "%s is null", what);
     if (s->type != TGBM_F32 && s->type != TGBM_F16 && s->type != TGBM_BF16) return refused(entry, "%s: unknown type %d", what, s->type);
-    if (s->classes < 1 || s->classes > 1 << 30) return refused(entry, "%s: %d classes", what, s->classes);
+    if (s->classes < 1 || s->classes > kClassesMost) return refused(entry, "%s: %d classes", what, s->classes);
     if (s->rows < 0) return refused(entry, "%s: %d rows", what, s->rows);
     if (s->rows > 0 && s->data == nullptr) return refused(entry, "%s: null data", what);
     const bool columns = s->row_stride == 1 && (s->classes == 1 || s->class_stride >= s->rows);

@@ -2,10 +2,11 @@
 //
 // A group of wavefronts holds a row, or a chunk of it, in registers. The k-th largest of the threads' own maxima is a lower
 // bound of the k-th largest score: the k threads above it hold one such score each. Any bound that between k and a few more
-// maxima reach will do, so it is found by bisection over the maxima (ballots, no memory), and what reaches it - about as many
-// scores, a thread rarely holds two of the best - goes to a short list in LDS, which is put in order by counting. Equal scores
-// are told apart by their class, so that the list stays short where many are equal. Rows that go by chunks leave k scores of
-// each, and a launch of its own makes the same choice among those.
+// maxima reach will do, so it is found by bisection over the maxima (ballots, no memory). Only the threads whose maximum reaches it, about k of
+// them, can hold a score that does: they lay theirs out in LDS, where all threads look through them side by side, and what reaches the bound -
+// a thread rarely holds two of the best - is put in order by counting. Equal scores are told apart by their class, so that no more
+// than k threads are left where many are equal. Rows that go by chunks leave k scores of each, and a launch of its own makes
+// the same choice among those.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -34,28 +35,19 @@ __device__ __forceinline__ void group_sync() {
     else __syncthreads();
 }
 
-// What a group of W wavefronts shares. The list of candidates is elsewhere (Places).
+// What a group of W wavefronts shares.
 template <int W>
 struct TopShared {
     unsigned best[W == 1 ? 1 : W * 64];
     int first[W == 1 ? 1 : W * 64];
     float part_max[W], part_sum[W];
     int part[W];
-    int count, exact, at_most;
+    int threads, listed, exact, at_most;
     unsigned bound;
 };
-
-// The list: candidate e is the ordered score base[2 * e * stride] and the complement of its place behind it; larger is better.
-struct Places {
-    unsigned *base;
-    int stride, room;
-    __device__ __forceinline__ void put(int e, unsigned score, int place) const {
-        base[(size_t)(2 * e) * stride] = score;
-        base[(size_t)(2 * e + 1) * stride] = (unsigned)~place;
-    }
-    __device__ __forceinline__ unsigned score(int e) const { return base[(size_t)(2 * e) * stride]; }
-    __device__ __forceinline__ unsigned place(int e) const { return base[(size_t)(2 * e + 1) * stride]; }
-};
+constexpr int kListRoom = 192;                            // candidates: more than kTopMost
+constexpr int kMostThreads = kTopMost + kTopMost / 4;       // that lay their scores out
+constexpr int candidates_wanted(int k) { return k + (k / 4 > 4 ? k / 4 : 4); }
 
 template <int M>
 __device__ __forceinline__ int count_from(const unsigned (&b)[M], unsigned least) {
@@ -126,22 +118,22 @@ __device__ __forceinline__ int group_sum(int n, TopShared<W> &sh) {
     return all;
 }
 
-// Where the scores of a thread lie: v[i] at base + i / V * step + i % V, the last of N at `extra` where it is apart from them.
-template <int N, int V, bool EXTRA>
+// Where the scores of thread t lie: score i at t * V + i / V * step + i % V, the last of N at extra + t where it is apart from them.
+template <int N_, int V, bool EXTRA>
 struct Layout {
-    int base, step, extra;
-    __device__ __forceinline__ int at(int i) const { return EXTRA && i == N - 1 ? extra : base + i / V * step + i % V; }
-    // (with a constant i: at(i) <= most without a register for every at(i))
-    __device__ __forceinline__ bool up_to(int i, int most) const { return EXTRA && i == N - 1 ? extra <= most : base <= most - (i / V * step + i % V); }
+    static constexpr int N = N_;
+    int step, extra;
+    __device__ __forceinline__ int at(int t, int i) const { return EXTRA && i == N - 1 ? extra + t : t * V + i / V * step + i % V; }
+};
+// One wavefront, whose lanes count as several threads each, thread t = lane + 64 * part: lane + 64 * (part * N + i).
+template <int N_>
+struct LaneParts {
+    static constexpr int N = N_;
+    __device__ __forceinline__ int at(int t, int i) const { return (t & 63) + ((t >> 6) * N + i) * 64; }
 };
 
 // Keeps the compiler from working out all of a loop's conditions or addresses ahead of it, in registers that it does not have.
 __device__ __forceinline__ unsigned one_by_one(unsigned v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
-__device__ __forceinline__ float one_by_one(float v) {
     asm volatile("" : "+v"(v));
     return v;
 }
@@ -154,51 +146,96 @@ __device__ __forceinline__ float best_of(const float (&v)[E]) {
     return best;
 }
 
-// Writes the scores that `mine` marks (bit i: v[i]) behind those of the threads before, and returns how many the group has, the
-// list's room being there or not.
-template <int W, int E, typename At>
-__device__ __forceinline__ int put_marked(const float (&v)[E], unsigned mine, At at, TopShared<W> &sh, const Places &list) {
-    const int scan = wave_scan_i(__popc(mine));
-    int total = __shfl(scan, 63), to = scan - __popc(mine);
-    if constexpr (W > 1) {
-        int base = 0;
-        if (lane_id() == 0) base = atomicAdd(&sh.count, total);
-        to += __shfl(base, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        mine = one_by_one(mine);
-        if (mine >> i & 1u) {
-            if (to < list.room) list.put(to, ordered(one_by_one(v[i])), at.at(i));
-            ++to;
-        }
-    }
-    group_sync<W>();
-    if constexpr (W > 1) total = sh.count;
-    return total;
-}
+// Where a row's (or a chunk's) best classes go.
+struct TopOut {
+    float *values;  // [][k]
+    int *classes;
+    float *lse;     // [] of rows, or the largest score and the sum of chunks
+};
 
-// The candidates of the group's k best, as many as are returned, the same in all threads. at: a Layout, whose places
-// ascend with i; best: the thread's largest. Every thread of the group comes here. The list holds at least k.
-template <int W, int E, typename At>
-__device__ __forceinline__ int list_candidates(const float (&v)[E], float best, At at, int k, TopShared<W> &sh, const Places &list) {
+// LDS of a group: the scores of the threads that reach the bound, score i of the q-th of them at q * N + i, and who they are; then
+// what reaches the bound of those, and how many of these are better.
+template <int W, int N>
+struct LaidOut {
+    static constexpr int kRoom = kListRoom;
+    static constexpr int kThreads = W == 1 ? 64 : kMostThreads;
+    float score[kThreads * N];
+    unsigned short owner[kThreads];
+    float list_score[kListRoom];
+    int list_place[kListRoom];
+    int better[W == 1 ? 1 : kListRoom];
+
+    __device__ __forceinline__ void put(int q, int t, const float *v) {
+        owner[q] = (unsigned short)t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) score[q * N + i] = v[i];
+    }
+    template <typename At>
+    __device__ __forceinline__ float get(int q, int i, const At &, int *) const { return score[q * N + i]; }
+    template <typename At>
+    __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(owner[q], i); }
+    __device__ __forceinline__ void list(int to, float s, int p) {
+        list_score[to] = s;
+        list_place[to] = p;
+        if constexpr (W > 1) better[to] = 0;
+    }
+    __device__ __forceinline__ void listed(int j, float *s, int *p) const {
+        *s = list_score[j];
+        *p = list_place[j];
+    }
+};
+// A row's column of a tile holds the scores already, by their places.
+struct ColumnLists {
+    static constexpr int kRoom = 160;
+    unsigned char owner[kMostThreads];
+    unsigned short entry[kRoom];
+};
+struct Column {
+    static constexpr int kRoom = ColumnLists::kRoom;
+    const unsigned *column;
+    int pitch, lines;
+    ColumnLists &lists;
+    __device__ __forceinline__ float at_line(int p) const { return __uint_as_float(column[p * pitch]); }
+    __device__ __forceinline__ void put(int q, int t, const float *) { lists.owner[q] = (unsigned char)t; }
+    template <typename At>
+    __device__ __forceinline__ float get(int q, int i, const At &at, int *) const {
+        const int p = at.at(lists.owner[q], i);
+        return p < lines ? at_line(p) : kNothing;
+    }
+    template <typename At>
+    __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(lists.owner[q], i); }
+    __device__ __forceinline__ void list(int to, float, int p) { lists.entry[to] = (unsigned short)p; }
+    __device__ __forceinline__ void listed(int j, float *s, int *p) const {
+        *p = lists.entry[j];
+        *s = at_line(*p);
+    }
+};
+
+// The k best of the group's scores go to `slot` of the output, in order. v: M times N scores, each N of them a thread's to the
+// choice (M is 1 but for one wavefront); best: the largest of each; at: where they lie, ascending with i; room: LDS of the group; class_at(place): the class. Every
+// thread of the group comes here.
+template <int W, int M, int N, typename At, typename Room, typename Class>
+__device__ __forceinline__ void write_top(const float (&v)[M * N], const float (&best)[M], const At &at, int k, TopShared<W> &sh, Room &room, size_t slot,
+                                          const TopOut &out, Class class_at) {
+    static_assert(M == 1 || W == 1);
     const int lane = lane_id(), t = W == 1 ? lane : (int)threadIdx.x;
-    const int limit = k + max(4, k / 4);
     unsigned bound;
-    int exact;
+    int exact, at_most = INT_MAX;
     if constexpr (W == 1) {
-        const unsigned b[1] = {ordered(best)};
-        bound = find_bound(b, k, limit, &exact);
+        unsigned b[M];
+#pragma unroll
+        for (int j = 0; j < M; ++j) b[j] = ordered(best[j]);
+        bound = find_bound(b, k, candidates_wanted(k), &exact);
     } else {
-        sh.best[t] = ordered(best);
-        if (t == 0) sh.count = 0;
+        sh.best[t] = ordered(best[0]);
+        if (t == 0) sh.threads = sh.listed = 0;
         __syncthreads();
         if (wave_id() == 0) {
             unsigned b[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) b[j] = sh.best[j * 64 + lane];
             int e;
-            const unsigned found = find_bound(b, k, limit, &e);
+            const unsigned found = find_bound(b, k, candidates_wanted(k), &e);
             if (lane == 0) {
                 sh.bound = found;
                 sh.exact = e;
@@ -209,21 +246,23 @@ __device__ __forceinline__ int list_candidates(const float (&v)[E], float best, 
         exact = sh.exact;
     }
     const float least = from_ordered(bound);
-    unsigned mine = 0;
-    if (!exact) {  // (the same in all threads)
+    int first[M];
 #pragma unroll
-        for (int i = 0; i < E; ++i) mine |= (v[i] >= least ? 1u : 0u) << i;
-    } else {
-        int first = INT_MAX, at_most;
+    for (int j = 0; j < M; ++j) first[j] = INT_MAX;
+    if (exact) {  // (the same in all threads)
 #pragma unroll
-        for (int i = E - 1; i >= 0; --i) first = v[i] == least ? i : first;
-        first = best == least ? at.at(first) : INT_MAX;
+        for (int j = 0; j < M; ++j) {
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i) first[j] = v[j * N + i] == least ? i : first[j];
+            first[j] = best[j] == least ? at.at(t + 64 * j, first[j]) : INT_MAX;
+        }
         if constexpr (W == 1) {
-            const unsigned b[1] = {ordered(best)};
-            const int f[1] = {first};
-            at_most = find_place(f, k - count_from(b, bound + 1));
+            unsigned b[M];
+#pragma unroll
+            for (int j = 0; j < M; ++j) b[j] = ordered(best[j]);
+            at_most = find_place(first, k - count_from(b, bound + 1));
         } else {
-            sh.first[t] = first;
+            sh.first[t] = first[0];
             __syncthreads();
             if (wave_id() == 0) {
                 unsigned b[W];
@@ -239,75 +278,152 @@ __device__ __forceinline__ int list_candidates(const float (&v)[E], float best, 
             __syncthreads();
             at_most = sh.at_most;
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i) mine |= (v[i] > least || (v[i] == least && at.up_to(i, at_most)) ? 1u : 0u) << i;
     }
-    const int total = put_marked<W>(v, mine, at, sh, list);
-    if (total <= list.room) return total;
-    // The best scores lie together in few threads: the exact k-th one by bisection over all of them.
-    unsigned lo = bound, hi = 0xff800001u;  // (one past infinity)
-    while (hi - lo > 1) {
-        const unsigned mid = lo + (hi - lo) / 2;
-        const float f = from_ordered(mid);
-        int n = 0;
+    // the threads: at most candidates_wanted(k), or k where the bound is exact
+    int threads = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) n += v[i] >= f ? 1 : 0;
-        if (group_sum<W>(n, sh) >= k) lo = mid;
-        else hi = mid;
+    for (int j = 0; j < M; ++j) {
+        const bool reaches = best[j] > least || (best[j] == least && (!exact || first[j] <= at_most));
+        const unsigned long long who = __ballot(reaches);
+        int q = threads + lanes_below(who);
+        threads += __popcll(who);
+        if constexpr (W > 1) {
+            int base = 0;
+            if (lane == 0 && threads > 0) base = atomicAdd(&sh.threads, threads);
+            q += __shfl(base, 0);
+        }
+        if (reaches) room.put(q, t + 64 * j, v + j * N);
     }
-    const float equal = from_ordered(lo);
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) above += v[i] > equal ? 1 : 0;
-    const int need = k - group_sum<W>(above, sh);
-    int p_lo = -1, p_hi = INT_MAX - 1;
-    while (p_hi - p_lo > 1) {
-        const int mid = p_lo + (p_hi - p_lo) / 2;
-        const float now = one_by_one(equal);
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) n += v[i] == now && at.up_to(i, mid) ? 1 : 0;
-        if (group_sum<W>(n, sh) >= need) p_hi = mid;
-        else p_lo = mid;
+    group_sync<W>();
+    if constexpr (W > 1) threads = sh.threads;
+    // their scores
+    const int entries = threads * N;
+    int listed = 0;
+    auto value = [&](int e) { return room.get(e / N, e % N, at, (int *)nullptr); };
+    auto place = [&](int e) { return room.place(e / N, e % N, at); };
+    auto list = [&](float from, int last) {
+        for (int e0 = 0; e0 < entries; e0 += 64 * W) {
+            const int e = e0 + t;
+            float x = kNothing;
+            bool is = false;
+            if (e < entries) {
+                x = value(e);
+                is = x > from || (x == from && (last == INT_MAX || place(e) <= last));
+            }
+            const unsigned long long which = __ballot(is);
+            if (which == 0) continue;
+            int to;
+            if constexpr (W == 1) {
+                to = listed;
+                listed += __popcll(which);
+            } else {
+                to = 0;
+                if (lane == 0) to = atomicAdd(&sh.listed, __popcll(which));
+                to = __shfl(to, 0);
+            }
+            to += lanes_below(which);
+            if (is && to < Room::kRoom) room.list(to, x, place(e));
+        }
+        group_sync<W>();
+        if constexpr (W > 1) listed = sh.listed;
+    };
+    list(least, at_most);
+    if (listed > Room::kRoom) {  // (the same in all threads)
+        // The best scores lie together in few threads: the exact k-th one by bisection over all that were laid out.
+        auto count = [&](auto is) {
+            int n = 0;
+            for (int e = t; e < entries; e += 64 * W) n += is(e) ? 1 : 0;
+            return group_sum<W>(n, sh);
+        };
+        unsigned lo = bound, hi = 0xff800001u;  // (one past infinity)
+        while (hi - lo > 1) {
+            const unsigned mid = lo + (hi - lo) / 2;
+            const float f = from_ordered(mid);
+            if (count([&](int e) { return value(e) >= f; }) >= k) lo = mid;
+            else hi = mid;
+        }
+        const float equal = from_ordered(lo);
+        const int need = k - count([&](int e) { return value(e) > equal; });
+        int p_lo = -1, p_hi = INT_MAX - 1;
+        while (p_hi - p_lo > 1) {
+            const int mid = p_lo + (p_hi - p_lo) / 2;
+            if (count([&](int e) { return value(e) == equal && place(e) <= mid; }) >= need) p_hi = mid;
+            else p_lo = mid;
+        }
+        if constexpr (W > 1) {
+            __syncthreads();
+            if (t == 0) sh.listed = 0;
+            __syncthreads();
+        }
+        listed = 0;
+        list(equal, p_hi);
     }
-    mine = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) mine |= (v[i] > equal || (v[i] == equal && at.up_to(i, p_hi)) ? 1u : 0u) << i;
-    if constexpr (W > 1) {
+    float *const values = out.values + slot * k;
+    int *const classes = out.classes + slot * k;
+    auto write = [&](float score, int at_place, int rank) {
+        if (rank < k) {
+            values[rank] = score + 0.f;
+            classes[rank] = class_at(at_place);
+        }
+    };
+    auto is_better = [](float a, int pa, float b, int pb) { return a > b || (a == b && pa < pb) ? 1 : 0; };
+    if constexpr (W == 1) {
+        for (int j0 = 0; j0 < listed; j0 += 64) {
+            float mine;
+            int my_place, rank = 0;
+            room.listed(min(j0 + lane, listed - 1), &mine, &my_place);
+            if (listed <= 64) {
+                for (int o = 0; o < listed; ++o) rank += is_better(read_lane(mine, o), read_lane(my_place, o), mine, my_place);
+            } else {
+                for (int o = 0; o < listed; ++o) {
+                    float s;
+                    int p;
+                    room.listed(o, &s, &p);
+                    rank += is_better(s, p, mine, my_place);
+                }
+            }
+            if (j0 + lane < listed) write(mine, my_place, rank);
+        }
+    } else {
+        // the threads beyond the candidates compare as well
+        const int lines = max((listed + 63) / 64, 1), parts = W / lines;
+        const int j = t - t / (64 * lines) * (64 * lines), part = t / (64 * lines);
+        if (j < listed && part < parts) {
+            float mine;
+            int my_place, rank = 0;
+            room.listed(j, &mine, &my_place);
+            for (int o = part; o < listed; o += parts) {
+                float s;
+                int p;
+                room.listed(o, &s, &p);
+                rank += is_better(s, p, mine, my_place);
+            }
+            atomicAdd(&room.better[j], rank);
+        }
         __syncthreads();
-        if (t == 0) sh.count = 0;
-        __syncthreads();
+        if (t < listed) {
+            float mine;
+            int my_place;
+            room.listed(t, &mine, &my_place);
+            write(mine, my_place, room.better[t]);
+        }
     }
-    return put_marked<W>(v, mine, at, sh, list);
+    for (int j = listed + t; j < k; j += 64 * W) {
+        values[j] = kNothing;
+        classes[j] = -1;
+    }
 }
 
-// Where a row's (or a chunk's) best classes go.
-struct TopOut {
-    float *values;  // [][k]
-    int *classes;
-    float *lse;     // [] of rows, or the largest score and the sum of chunks
+// Over a wavefront, the same in every lane.
+struct WaveSumF {
+    float v;
+    template <int CTRL, int ROWS>
+    __device__ __forceinline__ void at() { v += __int_as_float(dpp_i<CTRL, ROWS>(0, __float_as_int(v))); }
 };
-
-// The candidates in order. class_at(place): the class.
-template <int W, typename Class>
-__device__ __forceinline__ void write_best(const Places &list, int found, int k, size_t slot, const TopOut &out, Class class_at) {
-    const int t = W == 1 ? lane_id() : (int)threadIdx.x;
-    for (int j = t; j < found; j += 64 * W) {
-        const unsigned score = list.score(j), place = list.place(j);
-        int better = 0;
-        for (int o = 0; o < found; ++o) {
-            const unsigned s = list.score(o);
-            better += s > score || (s == score && list.place(o) > place) ? 1 : 0;
-        }
-        if (better < k) {
-            out.values[slot * k + better] = from_ordered(score);
-            out.classes[slot * k + better] = class_at((int)~place);
-        }
-    }
-    for (int j = found + t; j < k; j += 64 * W) {
-        out.values[slot * k + j] = kNothing;
-        out.classes[slot * k + j] = -1;
-    }
+__device__ __forceinline__ float wave_sum_f(float v) {
+    WaveSumF s{v};
+    wave_scan_steps(s);
+    return read_lane(s.v, 63);
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -337,9 +453,7 @@ __device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best
         for (int i = 0; i < E; ++i) part[i % 4] += exp2_of((v[i] - m) * by);
         part[0] = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    float s = part[0];
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    float s = wave_sum_f(part[0]);
     if constexpr (W > 1) {
         if (lane_id() == 0) {
             sh.part_max[wave_id()] = s > 0.f || s != s ? m : kNothing;
@@ -389,27 +503,29 @@ __device__ __forceinline__ void count_shown(const tgbm_score_rules &rules, long 
     group_sync<W>();
 }
 
-// A group of W wavefronts takes chunk `tile % chunks` (a multiple of 32 classes) of a row; with W = 1 there are four groups to a
+// A group of W wavefronts takes a chunk (a multiple of 32 classes) of a row; with W = 1 there are four groups to a
 // workgroup. A thread has E scores in whole vectors, and one of what is left behind the last vector. RULES: there may be any. LDS: the lists of candidates,
 // then, where classes were shown, bits and times.
 template <typename T, int W, int E, bool RULES>
-__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
-                                                                          int chunks, int chunk, long tiles, bool whole) {
-    constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1, kRoom = W == 1 ? 256 : 1024;
-    __shared__ TopShared<W> shared[kGroups];
-    __shared__ unsigned candidates[kGroups][2 * kRoom];
-    extern __shared__ unsigned shown_lds[];
+__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, W == 1 ? 5 : 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
+                                                                          int chunks, int chunk, bool whole) {
+    constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
+    __shared__ TopShared<W> shared[kGroups];
+    __shared__ LaidOut<W, N> rooms[kGroups];
+    extern __shared__ unsigned shown_lds[];
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
     TopShared<W> &sh = shared[group];
-    const Places list{candidates[group], 1, kRoom};
     unsigned *bits = shown_lds + (size_t)group * (chunk + chunk / 32), *times = bits + chunk / 32;
     const float by = kLog2e / temperature;
-    for (long tile = (long)blockIdx.x * kGroups + group; tile < tiles; tile += (long)gridDim.x * kGroups) {
-        const long row = tile / chunks;
-        const int c0 = (int)(tile % chunks) * chunk, size = min(in.classes - c0, chunk), whole_size = size / V * V;
-        // (a thread's places are worked out where they are used, not kept over the tiles)
-        const Layout<N, V, true> at{(int)one_by_one((unsigned)t * V), kStep, (int)one_by_one((unsigned)(whole_size + t))};
+    const int part = blockIdx.y;
+    const long row = (long)blockIdx.x * kGroups + group;
+    if (W == 1 && row >= in.rows) return;
+    {
+        const size_t out_at = (size_t)row * chunks + part;
+        const int c0 = part * chunk, size = min(in.classes - c0, chunk), whole_size = size / V * V;
+        const Layout<N, V, true> at{kStep, whole_size};
+        const int base = (int)one_by_one((unsigned)t * V);  // (places are worked out where they are used, not kept over the tiles)
         const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride + c0;
         float v[N];
         {
@@ -417,9 +533,9 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgb
 #pragma unroll
             for (int g = 0; g < E / V; ++g) {
                 x[g] = (T)kNothing;
-                if (at.base < whole_size - g * kStep) x[g] = *reinterpret_cast<const typename Vector<T>::type *>(src + at.base + g * kStep);
+                if (base < whole_size - g * kStep) x[g] = *reinterpret_cast<const typename Vector<T>::type *>(src + base + g * kStep);
             }
-            v[E] = t < size - whole_size ? score_to_float(src[at.extra]) : kNothing;
+            v[E] = t < size - whole_size ? score_to_float(src[whole_size + t]) : kNothing;
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] = score_to_float(x[i / V][i % V]);
         }
@@ -428,15 +544,15 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgb
                 const float *bias = rules.bias + c0;
 #pragma unroll
                 for (int g = 0; g < E / V; ++g)
-                    if (at.base < whole_size - g * kStep) {
+                    if (base < whole_size - g * kStep) {
 #pragma unroll
                         for (int j = 0; j < V; j += 4) {
-                            const Float4 b = *reinterpret_cast<const Float4 *>(bias + at.base + g * kStep + j);
+                            const Float4 b = *reinterpret_cast<const Float4 *>(bias + base + g * kStep + j);
 #pragma unroll
                             for (int q = 0; q < 4; ++q) v[g * V + j + q] += b[q];
                         }
                     }
-                if (t < size - whole_size) v[E] += bias[at.extra];
+                if (t < size - whole_size) v[E] += bias[whole_size + t];
             }
             bool none;
             const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
@@ -448,17 +564,17 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgb
                     unsigned held = 0;
 #pragma unroll
                     for (int g = 0; g < E / V; ++g) {
-                        const int c = at.base + g * kStep;
+                        const int c = base + g * kStep;
                         if (c < whole_size) held |= (bits[c / 32] >> (c % 32) & ((1u << V) - 1u)) << (g * V);
                     }
-                    if (t < size - whole_size) held |= (bits[at.extra / 32] >> (at.extra % 32) & 1u) << E;
+                    if (t < size - whole_size) held |= (bits[(whole_size + t) / 32] >> ((whole_size + t) % 32) & 1u) << E;
                     // few of a thread's scores are: one at a time, from the start (its register has no number that a loop can use)
                     while (__any(held != 0)) {
                         const bool now = held != 0;
                         const int i = now ? __ffs((int)held) - 1 : 0;
                         float s = 0.f;
                         if (now) {
-                            const int c = at.at(i);
+                            const int c = at.at(t, i);
                             s = adjusted(score_to_float(src[c]), rules.bias != nullptr ? rules.bias[c0 + c] : 0.f, times[c], true, rules);
                         }
                         held &= held - 1;
@@ -470,100 +586,115 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, 6) void k_top_rows(tgb
             if (words != nullptr || none) {
 #pragma unroll
                 for (int g = 0; g < E / V; ++g) {
-                    const int c = at.base + g * kStep;
+                    const int c = base + g * kStep;
                     const unsigned ok = words != nullptr && c < whole_size ? words[(c0 + c) / 32] >> (c % 32) : 0u;
 #pragma unroll
                     for (int j = 0; j < V; ++j) v[g * V + j] = ok >> j & 1u ? v[g * V + j] : kNothing;
                 }
-                const bool ok = words != nullptr && t < size - whole_size && (words[(c0 + at.extra) / 32] >> (at.extra % 32) & 1u);
+                const bool ok = words != nullptr && t < size - whole_size && (words[(c0 + whole_size + t) / 32] >> ((whole_size + t) % 32) & 1u);
                 v[E] = ok ? v[E] : kNothing;
             }
         }
-        const float best = best_of(v);
+        const float best[1] = {best_of(v)};
         float m, s;
-        sum_exponentials<W>(v, best, by, sh, &m, &s);
+        sum_exponentials<W>(v, best[0], by, sh, &m, &s);
         if (t == 0) {
             if (whole) {
                 out.lse[row] = log_sum(m, s, temperature);
             } else {
-                out.lse[tile * 2] = m;
-                out.lse[tile * 2 + 1] = s;
+                out.lse[out_at * 2] = m;
+                out.lse[out_at * 2 + 1] = s;
             }
         }
-        const int found = list_candidates<W>(v, best, at, k, sh, list);
-        write_best<W>(list, found, k, (size_t)tile, out, [&](int p) { return c0 + p; });
-        group_sync<W>();
+        write_top<W, 1, N>(v, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; });
     }
 }
 
 // Rows side by side: a workgroup brings `rows` rows of a chunk (a multiple of 32, at most 64 * E classes) into LDS, class by class, eight
-// classes of a row to a thread at a time, and its wavefronts take a row each. A row's column is its list of candidates once
-// its scores are in registers. LDS: [tile_classes][rows + 1] scores, then, where classes were shown, [rows][chunk / 32] bits.
+// classes of a row to a thread at a time, and its wavefronts take a row each. M: parts of a lane's scores that count as threads, so that
+// there are more of them than best classes. LDS: [chunk][rows + 1] scores, then, where classes were shown, [rows][chunk / 32] bits: such a
+// class's cell holds how often first; whoever takes its bit away puts the score there.
 constexpr int kColumnBlock = 1024;
-template <typename T, int E, bool RULES>
+template <typename T, int E, int M, bool RULES>
 __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out, int chunks,
-                                                                 int chunk, int row_bits, int tile_classes, long tiles, bool whole) {
+                                                                 int chunk, int row_bits, bool whole) {
     __shared__ TopShared<1> sh;  // (nothing of it is used by one wavefront)
+    __shared__ ColumnLists lists[kColumnBlock / 64];
     extern __shared__ unsigned cell[];
     const int rows = 1 << row_bits, pitch = rows + 1;
-    unsigned *const bits = cell + (size_t)tile_classes * pitch;
+    unsigned *const bits = cell + (size_t)chunk * pitch;
     const float by = kLog2e / temperature;
     const int r = threadIdx.x & (rows - 1), slot = threadIdx.x >> row_bits, slots = kColumnBlock >> row_bits;
-    const T *src = static_cast<const T *>(in.data);
-    for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const long row0 = tile / chunks * rows, row = row0 + r;
-        const int c0 = (int)(tile % chunks) * chunk, c1 = min(in.classes, c0 + chunk);
+    const long row_tiles = ((in.rows - 1) >> row_bits) + 1;
+    const int part = blockIdx.y;
+    // (blocks go to the eight dies in turn: two tiles that share cache lines go to the same one)
+    const long tile = ((long)blockIdx.x & ~15l) + (blockIdx.x & 7) * 2 + (blockIdx.x >> 3 & 1);
+    if (tile >= row_tiles) return;
+    {
+        const long row0 = tile << row_bits, row = row0 + r;
+        const int c0 = part * chunk, size = min(in.classes - c0, chunk);
+        const T *src = static_cast<const T *>(in.data) + (size_t)c0 * in.class_stride + row;
         unsigned *const my_bits = bits + r * (chunk / 32);
-        bool counted = false;
+        bool none = false;
+        const unsigned *words = nullptr;
+        const float *bias = rules.bias != nullptr ? rules.bias + c0 : nullptr;
+        long long b = 0, e = 0;
         if constexpr (RULES) {
-            counted = rules.shown != nullptr;
-            if (counted) {
+            if (row < in.rows) words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+            if (words != nullptr) words += c0 / 32;
+            if (rules.shown != nullptr) {
                 for (int i = threadIdx.x; i < rows * (chunk / 32); i += kColumnBlock) bits[i] = 0;
                 __syncthreads();
-                long long b = 0, e = 0;
                 if (row < in.rows) shown_range(rules, row, &b, &e);
                 for (long long i = b + slot; i < e; i += slots) {
                     const int c = rules.shown[i] - c0;
-                    if (c < 0 || c >= c1 - c0) continue;
+                    if (c < 0 || c >= size) continue;
                     cell[c * pitch + r] = 0;
                     atomicOr(&my_bits[c / 32], 1u << (c % 32));
                 }
                 __syncthreads();
                 for (long long i = b + slot; i < e; i += slots) {
                     const int c = rules.shown[i] - c0;
-                    if (c >= 0 && c < c1 - c0) atomicAdd(&cell[c * pitch + r], 1u);
+                    if (c >= 0 && c < size) atomicAdd(&cell[c * pitch + r], 1u);
                 }
-                __syncthreads();
             }
         }
         if (row < in.rows) {
-            bool none = false;
-            const unsigned *words = RULES ? allowed_words(rules, row, (in.classes + 31) / 32, &none) : nullptr;
-            for (int c = slot * 8; c < c1 - c0; c += slots * 8) {
-                const T *from = src + (size_t)(c0 + c) * in.class_stride + row;
+            for (int c = slot * 8; c < size; c += slots * 8) {
+                const T *from = src + (size_t)c * in.class_stride;
                 unsigned *to = cell + c * pitch + r;
                 float z[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z[j] = c + j < c1 - c0 ? score_to_float(from[(size_t)j * in.class_stride]) : kNothing;
-                if constexpr (!RULES) {
+                for (int j = 0; j < 8; ++j) {
+                    z[j] = c + j < size ? score_to_float(*from) : kNothing;
+                    from += in.class_stride;
+                }
+                unsigned held = 0, ok = ~0u;
+                if constexpr (RULES) {
+                    ok = none ? 0u : words != nullptr ? words[c / 32] >> (c % 32) : ~0u;
+                    held = rules.shown != nullptr ? my_bits[c / 32] >> (c % 32) & 0xffu : 0u;
+                    if (bias != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (c + j < c1 - c0) to[j * pitch] = __float_as_uint(z[j]);
-                } else {
-                    unsigned ok = none ? 0u : words != nullptr ? words[(c0 + c) / 32] >> ((c0 + c) % 32) : ~0u;
-                    unsigned held = counted ? my_bits[c / 32] >> (c % 32) & 0xffu : 0u;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (c + j < c1 - c0) {
-                            const float s = rules.bias != nullptr ? z[j] + rules.bias[c0 + c + j] : z[j];
-                            if (!(held >> j & 1u)) to[j * pitch] = __float_as_uint(ok >> j & 1u ? s : kNothing);
-                        }
-                    while (held != 0) {
-                        const int j = __ffs((int)held) - 1;
-                        held &= held - 1;
-                        to[j * pitch] = __float_as_uint(adjusted(score_to_float(from[(size_t)j * in.class_stride]), rules.bias != nullptr ? rules.bias[c0 + c + j] : 0.f,
-                                                                 to[j * pitch], ok >> j & 1u, rules));
+                        for (int j = 0; j < 8; ++j)
+                            if (c + j < size) z[j] += bias[c + j];
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < size && !(held >> j & 1u)) to[j * pitch] = __float_as_uint(ok >> j & 1u ? z[j] : kNothing);
+            }
+        }
+        if constexpr (RULES) {
+            if (rules.shown != nullptr) {
+                __syncthreads();
+                for (long long i = b + slot; i < e; i += slots) {
+                    const int c = rules.shown[i] - c0;
+                    if (c < 0 || c >= size) continue;
+                    const unsigned bit = 1u << (c % 32);
+                    if (!(atomicAnd(&my_bits[c / 32], ~bit) & bit)) continue;  // (another mention of the class has come first)
+                    const bool ok = !none && (words == nullptr || words[c / 32] & bit);
+                    unsigned *to = cell + c * pitch + r;
+                    *to = __float_as_uint(adjusted(score_to_float(src[(size_t)c * in.class_stride]), bias != nullptr ? bias[c] : 0.f, *to, ok, rules));
                 }
             }
         }
@@ -571,13 +702,20 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
         for (int q = wave_id(); q < rows && row0 + q < in.rows; q += kColumnBlock / 64) {
             const int lane = (int)one_by_one((unsigned)lane_id());  // (places are worked out where they are used)
             const unsigned *from = cell + lane * pitch + q;
-            float v[E];
+            float v[E], best[M];
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = lane < c1 - c0 - i * 64 ? __uint_as_float(from[i * 64 * pitch]) : kNothing;
-            const size_t out_at = (size_t)(row0 + q) * chunks + tile % chunks;
-            const float best = best_of(v);
+            for (int i = 0; i < E; ++i) v[i] = lane < size - i * 64 ? __uint_as_float(from[i * 64 * pitch]) : kNothing;
+            float largest = kNothing;
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                best[j] = kNothing;
+#pragma unroll
+                for (int i = 0; i < E / M; ++i) best[j] = fmaxf(best[j], v[j * (E / M) + i]);
+                largest = fmaxf(largest, best[j]);
+            }
+            const size_t out_at = (size_t)(row0 + q) * chunks + part;
             float m, s;
-            sum_exponentials<1>(v, best, by, sh, &m, &s);
+            sum_exponentials<1>(v, largest, by, sh, &m, &s);
             if (lane_id() == 0) {
                 if (whole) {
                     out.lse[row0 + q] = log_sum(m, s, temperature);
@@ -586,12 +724,10 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
                     out.lse[out_at * 2 + 1] = s;
                 }
             }
+            Column column{cell + q, pitch, size, lists[wave_id()]};
+            write_top<1, M, E / M>(v, best, LaneParts<E / M>{}, k, sh, column, out_at, out, [&](int p) { return c0 + p; });
             wave_fence();
-            const Places list{cell + q, pitch, tile_classes / 2};
-            const int found = list_candidates<1>(v, best, Layout<E, 1, false>{lane, 64, 0}, k, sh, list);
-            write_best<1>(list, found, k, out_at, out, [&](int p) { return c0 + p; });
         }
-        __syncthreads();
     }
 }
 
@@ -599,7 +735,8 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
 template <typename T, int E>
 __global__ __launch_bounds__(kTopBlock) void k_top_few(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out) {
     const float by = kLog2e / temperature;
-    for (long row = (long)blockIdx.x * kTopBlock + threadIdx.x; row < in.rows; row += (long)gridDim.x * kTopBlock) {
+    const long row = (long)blockIdx.x * kTopBlock + threadIdx.x;
+    if (row < in.rows) {
         const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
         float v[E];
 #pragma unroll
@@ -653,19 +790,20 @@ __global__ __launch_bounds__(kTopBlock) void k_top_few(tgbm_scores in, tgbm_scor
 
 // `per_join` parts of a row become one: places among them ascend with the class wherever scores are equal.
 template <int W, int E>
-__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int parts, int per_join, int joins, long tiles, int k, float temperature, TopOut in,
+__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int parts, int per_join, int joins, int rows, int k, float temperature, TopOut in,
                                                                           TopOut out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
-    constexpr int kRoom = W == 1 ? 256 : 1024;
     __shared__ TopShared<W> shared[kGroups];
-    __shared__ unsigned candidates[kGroups][2 * kRoom];
+    __shared__ LaidOut<W, E> rooms[kGroups];
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
     TopShared<W> &sh = shared[group];
-    const Places list{candidates[group], 1, kRoom};
     const float by = kLog2e / temperature;
-    for (long tile = (long)blockIdx.x * kGroups + group; tile < tiles; tile += (long)gridDim.x * kGroups) {
-        const int first = (int)(tile % joins) * per_join, mine = min(parts - first, per_join), count = mine * k;
-        const size_t from = (size_t)(tile / joins) * parts + first;
+    const int part = blockIdx.y;
+    const long row = (long)blockIdx.x * kGroups + group;
+    if (W == 1 && row >= rows) return;
+    {
+        const int first = part * per_join, mine = min(parts - first, per_join), count = mine * k;
+        const size_t from = (size_t)row * parts + first, tile = (size_t)row * joins + part;
         const float *values = in.values + from * k;
         const int *classes = in.classes + from * k;
         float v[E];
@@ -681,26 +819,22 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
         m = reference_of(wave_max_f(m));
         float s = 0.f;
         for (int c = lane_id(); c < mine; c += 64) {
-            const float part = sums[c * 2 + 1];
-            if (part != 0.f) s += rescaled(part, sums[c * 2], m, by);
+            const float its = sums[c * 2 + 1];
+            if (its != 0.f) s += rescaled(its, sums[c * 2], m, by);
         }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        s = wave_sum_f(s);
         if (t == 0) {
             if (joins == 1) {
-                out.lse[tile] = log_sum(m, s, temperature);
+                out.lse[row] = log_sum(m, s, temperature);
             } else {
                 out.lse[tile * 2] = m;
                 out.lse[tile * 2 + 1] = s;
             }
         }
-        const int found = list_candidates<W>(v, best_of(v), Layout<E, 1, false>{(int)one_by_one((unsigned)t), 64 * W, 0}, k, sh, list);
-        write_best<W>(list, found, k, (size_t)tile, out, [&](int p) { return classes[p]; });
-        group_sync<W>();
+        const float best[1] = {best_of(v)};
+        write_top<W, 1, E>(v, best, Layout<E, 1, false>{64 * W, 0}, k, sh, rooms[group], tile, out, [&](int p) { return classes[p]; });
     }
 }
-
-int blocks_of(long groups) { return (int)std::max(1l, std::min(groups, 1l << 20)); }
 
 // How a call goes: chunks of a row, and the classes of one.
 struct TopPlan {
@@ -708,10 +842,12 @@ struct TopPlan {
     int chunks, chunk;
     int waves;     // classes side by side: wavefronts of a group
     int row_bits;  // rows side by side
-    int tile_classes;
     int per_thread;
+    int parts;  // of a lane's scores, rows side by side
 };
 constexpr int kFewClasses = 32;
+// With up to so many best classes the maxima of 64 lanes give a bound that few scores reach: with all of them the lists overflow.
+constexpr int kFewBest = 32;
 constexpr int kRowScores = 24;  // classes side by side: the most that a thread has in whole vectors
 constexpr int kJoinMost = 16384;  // scores that a join takes
 constexpr int kGroupsWanted = 512;
@@ -733,43 +869,51 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
     if (columns) {
         p.per_thread = 1;
         while (p.per_thread * 64 < p.chunk) p.per_thread *= 2;
-        p.tile_classes = std::max(p.chunk, 2 * kTopMost);  // (a list's room)
+        p.per_thread = std::max(p.per_thread, 2);
         p.row_bits = 4;
-        while (p.row_bits < 6 && (p.tile_classes << (p.row_bits + 1)) <= 16384) ++p.row_bits;
+        while (p.row_bits < 6 && (p.chunk << (p.row_bits + 1)) <= 16384) ++p.row_bits;
+    } else if (k > kFewBest && p.chunk <= 64 * kRowScores) {
+        p.waves = 4;
+        p.per_thread = 8;
     } else {
         p.waves = p.chunk <= 64 * kRowScores ? 1 : p.chunk <= 256 * kRowScores ? 4 : 8;
         p.per_thread = p.waves > 1 ? kRowScores : p.chunk <= 512 ? 8 : p.chunk <= 1024 ? 16 : kRowScores;
     }
+    p.parts = columns && k > kFewBest ? std::min(4, p.per_thread) : 1;
     return p;
 }
 
 template <typename T, int W, int E, bool RULES>
 void top_rows(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
-    const long tiles = (long)in.rows * p.chunks;
     const size_t lds = rules.shown != nullptr ? sizeof(unsigned) * (size_t)(p.chunk + p.chunk / 32) * kGroups : 0;
     if (lds > 32 * 1024) {
         static LdsOptIn opt_in;
         opt_in({reinterpret_cast<const void *>(&k_top_rows<T, W, E, RULES>)});
     }
-    k_top_rows<T, W, E, RULES><<<blocks_of((tiles - 1) / kGroups + 1), W == 1 ? kTopBlock : 64 * W, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk,
-                                                                                                           tiles, p.chunks == 1);
+    const dim3 grid((unsigned)((in.rows - 1) / kGroups + 1), (unsigned)p.chunks);
+    k_top_rows<T, W, E, RULES><<<grid, W == 1 ? kTopBlock : 64 * W, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.chunks == 1);
 }
 
+template <typename T, int E, int M, bool RULES>
+void top_columns(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
+    const long tiles = (((long)((in.rows - 1) >> p.row_bits) + 1) + 15) / 16 * 16;
+    const size_t lds = sizeof(unsigned) * ((size_t)p.chunk * ((1 << p.row_bits) + 1) + (rules.shown != nullptr ? (size_t)p.chunk / 32 << p.row_bits : 0));
+    static LdsOptIn opt_in;
+    opt_in({reinterpret_cast<const void *>(&k_top_columns<T, E, M, RULES>)});
+    const dim3 grid((unsigned)tiles, (unsigned)p.chunks);
+    k_top_columns<T, E, M, RULES><<<grid, kColumnBlock, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.row_bits, p.chunks == 1);
+}
 template <typename T, int E, bool RULES>
 void top_columns(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
-    const long tiles = ((long)((in.rows - 1) >> p.row_bits) + 1) * p.chunks;
-    const size_t lds = sizeof(unsigned) * ((size_t)p.tile_classes * ((1 << p.row_bits) + 1) + (rules.shown != nullptr ? (size_t)p.chunk / 32 << p.row_bits : 0));
-    static LdsOptIn opt_in;
-    opt_in({reinterpret_cast<const void *>(&k_top_columns<T, E, RULES>)});
-    k_top_columns<T, E, RULES><<<blocks_of(tiles), kColumnBlock, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.row_bits, p.tile_classes, tiles,
-                                                                      p.chunks == 1);
+    if (p.parts == 1) top_columns<T, E, 1, RULES>(s, p, in, rules, k, temperature, out);
+    else top_columns<T, E, E < 4 ? E : 4, RULES>(s, p, in, rules, k, temperature, out);
 }
 
 template <typename T, bool RULES>
 void top(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
     if (p.few) {
-        const int blocks = blocks_of(((long)in.rows - 1) / kTopBlock + 1);
+        const unsigned blocks = (unsigned)((in.rows - 1) / kTopBlock + 1);
         if (in.classes <= 8) k_top_few<T, 8><<<blocks, kTopBlock, 0, s>>>(in, rules, k, temperature, out);
         else if (in.classes <= 16) k_top_few<T, 16><<<blocks, kTopBlock, 0, s>>>(in, rules, k, temperature, out);
         else k_top_few<T, 32><<<blocks, kTopBlock, 0, s>>>(in, rules, k, temperature, out);
@@ -781,6 +925,8 @@ void top(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_scor
         else top_columns<T, 16, kRules>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 8) {
         top_rows<T, 8, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
+    } else if (p.waves == 4 && p.per_thread == 8) {
+        top_rows<T, 4, 8, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 4) {
         top_rows<T, 4, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.per_thread == kRowScores) {
@@ -801,8 +947,8 @@ void top_any(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_
 template <int W, int E>
 void join(hipStream_t s, int parts, int per_join, int joins, int rows, int k, float temperature, const TopOut &in, const TopOut &out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
-    const long tiles = (long)rows * joins;
-    k_top_join<W, E><<<blocks_of((tiles - 1) / kGroups + 1), W == 1 ? kTopBlock : 64 * W, 0, s>>>(parts, per_join, joins, tiles, k, temperature, in, out);
+    const dim3 grid((unsigned)((rows - 1) / kGroups + 1), (unsigned)joins);
+    k_top_join<W, E><<<grid, W == 1 ? kTopBlock : 64 * W, 0, s>>>(parts, per_join, joins, rows, k, temperature, in, out);
 }
 
 size_t part_bytes(size_t parts, int k) { return sizeof(float) * parts * (2 * (size_t)k + 2); }
@@ -818,14 +964,15 @@ int parts_of_a_join(int k) { return std::max(2, kJoinMost / k); }
 }  // namespace
 
 size_t scores_top_workspace(bool columns, int classes, int rows, int k) {
+    rows = std::min(rows, kSliceRows);
     const TopPlan p = plan_top(columns, classes, rows, k);
     size_t bytes = 0;
     for (int parts = p.chunks; parts > 1; parts = (parts - 1) / parts_of_a_join(k) + 1) bytes += part_bytes((size_t)rows * parts, k);
     return bytes;
 }
 
-void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
-                       void *workspace) {
+static void launch_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
+                         void *workspace) {
     const TopPlan p = plan_top(rows_side_by_side(in), in.classes, in.rows, k);
     const TopOut out{values, classes, lse};
     char *room = static_cast<char *>(workspace);
@@ -842,12 +989,24 @@ void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_ru
     for (int parts = p.chunks; parts > 1;) {
         const int per_join = std::min(parts, parts_of_a_join(k)), joins = (parts - 1) / per_join + 1, count = per_join * k;
         const TopOut to = next(joins);
-        if (count <= 256) join<1, 4>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
+        if (k > kFewBest && count <= 1024) join<4, 4>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
+        else if (count <= 256) join<1, 4>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
         else if (count <= 1024) join<1, 16>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
         else if (count <= 4096) join<4, 16>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
         else join<8, 32>(s, parts, per_join, joins, in.rows, k, temperature, now, to);
         now = to;
         parts = joins;
+    }
+}
+
+// (a launch has fewer than 2^32 threads in a direction: very many rows go by slices, which share the workspace one after the other)
+void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
+                       void *workspace) {
+    for (int row = 0; row < in.rows; row += std::min(kSliceRows, in.rows - row)) {
+        tgbm_scores part = in;
+        tgbm_score_rules r = rules;
+        take_rows(part, r, row, std::min(kSliceRows, in.rows - row));
+        launch_slice(s, part, r, k, temperature, values + (size_t)row * k, classes + (size_t)row * k, lse + row, workspace);
     }
 }
 
