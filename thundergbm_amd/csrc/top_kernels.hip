@@ -153,16 +153,16 @@ struct TopOut {
     float *lse;     // [] of rows, or the largest score and the sum of chunks
 };
 
-// LDS of a group: the scores of the threads that reach the bound, score i of the q-th of them at q * N + i, and who they are; then
-// what reaches the bound of those, and how many of these are better.
+// LDS of a group: the candidates, ordered score in front of the complement of the place (larger is better), and how many of them are
+// better; and, where the candidates are too many for that, the scores of the threads that reach the bound, score i of the q-th of them at
+// q * N + i, and who they are.
 template <int W, int N>
 struct LaidOut {
     static constexpr int kRoom = kListRoom;
     static constexpr int kThreads = W == 1 ? 64 : kMostThreads;
     float score[kThreads * N];
     unsigned short owner[kThreads];
-    float list_score[kListRoom];
-    int list_place[kListRoom];
+    unsigned long long key[kListRoom];
     int better[W == 1 ? 1 : kListRoom];
 
     __device__ __forceinline__ void put(int q, int t, const float *v) {
@@ -171,18 +171,14 @@ struct LaidOut {
         for (int i = 0; i < N; ++i) score[q * N + i] = v[i];
     }
     template <typename At>
-    __device__ __forceinline__ float get(int q, int i, const At &, int *) const { return score[q * N + i]; }
+    __device__ __forceinline__ float get(int q, int i, const At &) const { return score[q * N + i]; }
     template <typename At>
     __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(owner[q], i); }
     __device__ __forceinline__ void list(int to, float s, int p) {
-        list_score[to] = s;
-        list_place[to] = p;
+        key[to] = (unsigned long long)ordered(s) << 32 | (unsigned)~p;
         if constexpr (W > 1) better[to] = 0;
     }
-    __device__ __forceinline__ void listed(int j, float *s, int *p) const {
-        *s = list_score[j];
-        *p = list_place[j];
-    }
+    __device__ __forceinline__ unsigned long long listed(int j) const { return key[j]; }
 };
 // A row's column of a tile holds the scores already, by their places.
 struct ColumnLists {
@@ -198,25 +194,25 @@ struct Column {
     __device__ __forceinline__ float at_line(int p) const { return __uint_as_float(column[p * pitch]); }
     __device__ __forceinline__ void put(int q, int t, const float *) { lists.owner[q] = (unsigned char)t; }
     template <typename At>
-    __device__ __forceinline__ float get(int q, int i, const At &at, int *) const {
+    __device__ __forceinline__ float get(int q, int i, const At &at) const {
         const int p = at.at(lists.owner[q], i);
         return p < lines ? at_line(p) : kNothing;
     }
     template <typename At>
     __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(lists.owner[q], i); }
     __device__ __forceinline__ void list(int to, float, int p) { lists.entry[to] = (unsigned short)p; }
-    __device__ __forceinline__ void listed(int j, float *s, int *p) const {
-        *p = lists.entry[j];
-        *s = at_line(*p);
+    __device__ __forceinline__ unsigned long long listed(int j) const {
+        const int p = lists.entry[j];
+        return (unsigned long long)ordered(at_line(p)) << 32 | (unsigned)~p;
     }
 };
 
 // The k best of the group's scores go to `slot` of the output, in order. v: M times N scores, each N of them a thread's to the
-// choice (M is 1 but for one wavefront); best: the largest of each; at: where they lie, ascending with i; room: LDS of the group; class_at(place): the class. Every
-// thread of the group comes here.
-template <int W, int M, int N, typename At, typename Room, typename Class>
+// choice (M is 1 but for one wavefront); best: the largest of each; at: where they lie, ascending with i; room: LDS of the group; class_at(place): the class; meanwhile():
+// what the last of several wavefronts does while the first one looks for the bound, behind a barrier. Every thread of the group comes here.
+template <int W, int M, int N, typename At, typename Room, typename Class, typename Meanwhile>
 __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (&best)[M], const At &at, int k, TopShared<W> &sh, Room &room, size_t slot,
-                                          const TopOut &out, Class class_at) {
+                                          const TopOut &out, Class class_at, Meanwhile meanwhile) {
     static_assert(M == 1 || W == 1);
     const int lane = lane_id(), t = W == 1 ? lane : (int)threadIdx.x;
     unsigned bound;
@@ -241,6 +237,7 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
                 sh.exact = e;
             }
         }
+        if (wave_id() == W - 1) meanwhile();
         __syncthreads();
         bound = sh.bound;
         exact = sh.exact;
@@ -279,57 +276,74 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
             at_most = sh.at_most;
         }
     }
-    // the threads: at most candidates_wanted(k), or k where the bound is exact
-    int threads = 0;
+    // the candidates: a bit for each score that reaches the bound
+    constexpr int kWords = (M * N + 31) / 32;
+    unsigned mine[kWords];
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
-        const bool reaches = best[j] > least || (best[j] == least && (!exact || first[j] <= at_most));
-        const unsigned long long who = __ballot(reaches);
-        int q = threads + lanes_below(who);
-        threads += __popcll(who);
-        if constexpr (W > 1) {
-            int base = 0;
-            if (lane == 0 && threads > 0) base = atomicAdd(&sh.threads, threads);
-            q += __shfl(base, 0);
+    for (int w = 0; w < kWords; ++w) mine[w] = 0;
+    if (!exact) {
+#pragma unroll
+        for (int i = M * N - 1; i >= 0; --i) mine[i / 32] = mine[i / 32] + mine[i / 32] + (v[i] >= least ? 1u : 0u);
+    } else {
+#pragma unroll
+        for (int i = M * N - 1; i >= 0; --i)
+            mine[i / 32] = mine[i / 32] + mine[i / 32] + (v[i] > least || (v[i] == least && at.at(t + 64 * (i / N), i % N) <= at_most) ? 1u : 0u);
+    }
+    int listed = 0;
+    auto slot_of = [&](unsigned long long which) {  // the lanes that have one more for the list: where it goes
+        int to = listed;
+        if constexpr (W == 1) {
+            listed += __popcll(which);
+        } else {
+            if (lane == 0) to = atomicAdd(&sh.listed, __popcll(which));
+            to = __shfl(to, 0);
         }
-        if (reaches) room.put(q, t + 64 * j, v + j * N);
+        return to + lanes_below(which);
+    };
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+        bool largest_first = true;
+        while (true) {
+            const unsigned long long which = __ballot(mine[w] != 0);
+            if (which == 0) break;
+            const int to = slot_of(which), i = mine[w] != 0 ? __ffs((int)mine[w]) - 1 + w * 32 : 0;
+            // (nearly always a thread has the one that is its largest)
+            float s = kNothing;
+            if (M == 1 && kWords == 1 && largest_first && __ballot((mine[w] & (mine[w] - 1)) != 0) == 0) {
+                s = best[0];
+            } else {
+#pragma unroll
+                for (int j = w * 32; j < (w * 32 + 32 < M * N ? w * 32 + 32 : M * N); ++j) s = j == i ? v[j] : s;
+            }
+            largest_first = false;
+            if (mine[w] != 0 && to < Room::kRoom) room.list(to, s, at.at(t + 64 * (i / N), i % N));
+            mine[w] &= mine[w] - 1;
+        }
     }
     group_sync<W>();
-    if constexpr (W > 1) threads = sh.threads;
-    // their scores
-    const int entries = threads * N;
-    int listed = 0;
-    auto value = [&](int e) { return room.get(e / N, e % N, at, (int *)nullptr); };
-    auto place = [&](int e) { return room.place(e / N, e % N, at); };
-    auto list = [&](float from, int last) {
-        for (int e0 = 0; e0 < entries; e0 += 64 * W) {
-            const int e = e0 + t;
-            float x = kNothing;
-            bool is = false;
-            if (e < entries) {
-                x = value(e);
-                is = x > from || (x == from && (last == INT_MAX || place(e) <= last));
+    if constexpr (W > 1) listed = sh.listed;
+    if (listed > Room::kRoom) {  // (the same in all threads)
+        // The best scores lie together in few threads, at most candidates_wanted(k), or k where the bound is exact: these lay theirs out,
+        // and the exact k-th one is found by bisection over all of them.
+        int threads = 0;
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const bool reaches = best[j] > least || (best[j] == least && (!exact || first[j] <= at_most));
+            const unsigned long long who = __ballot(reaches);
+            int q = threads + lanes_below(who);
+            threads += __popcll(who);
+            if constexpr (W > 1) {
+                int base = 0;
+                if (lane == 0 && threads > 0) base = atomicAdd(&sh.threads, threads);
+                q += __shfl(base, 0);
             }
-            const unsigned long long which = __ballot(is);
-            if (which == 0) continue;
-            int to;
-            if constexpr (W == 1) {
-                to = listed;
-                listed += __popcll(which);
-            } else {
-                to = 0;
-                if (lane == 0) to = atomicAdd(&sh.listed, __popcll(which));
-                to = __shfl(to, 0);
-            }
-            to += lanes_below(which);
-            if (is && to < Room::kRoom) room.list(to, x, place(e));
+            if (reaches) room.put(q, t + 64 * j, v + j * N);
         }
         group_sync<W>();
-        if constexpr (W > 1) listed = sh.listed;
-    };
-    list(least, at_most);
-    if (listed > Room::kRoom) {  // (the same in all threads)
-        // The best scores lie together in few threads: the exact k-th one by bisection over all that were laid out.
+        if constexpr (W > 1) threads = sh.threads;
+        const int entries = threads * N;
+        auto value = [&](int e) { return room.get(e / N, e % N, at); };
+        auto place = [&](int e) { return room.place(e / N, e % N, at); };
         auto count = [&](auto is) {
             int n = 0;
             for (int e = t; e < entries; e += 64 * W) n += is(e) ? 1 : 0;
@@ -356,57 +370,52 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
             __syncthreads();
         }
         listed = 0;
-        list(equal, p_hi);
+        for (int e0 = 0; e0 < entries; e0 += 64 * W) {
+            const int e = e0 + t;
+            float x = kNothing;
+            bool is = false;
+            if (e < entries) {
+                x = value(e);
+                is = x > equal || (x == equal && place(e) <= p_hi);
+            }
+            const unsigned long long which = __ballot(is);
+            if (which == 0) continue;
+            const int to = slot_of(which);
+            if (is && to < Room::kRoom) room.list(to, x, place(e));
+        }
+        group_sync<W>();
+        if constexpr (W > 1) listed = sh.listed;
     }
     float *const values = out.values + slot * k;
     int *const classes = out.classes + slot * k;
-    auto write = [&](float score, int at_place, int rank) {
+    auto write = [&](unsigned long long key, int rank) {
         if (rank < k) {
-            values[rank] = score + 0.f;
-            classes[rank] = class_at(at_place);
+            values[rank] = from_ordered((unsigned)(key >> 32));
+            classes[rank] = class_at((int)~(unsigned)key);
         }
     };
-    auto is_better = [](float a, int pa, float b, int pb) { return a > b || (a == b && pa < pb) ? 1 : 0; };
     if constexpr (W == 1) {
         for (int j0 = 0; j0 < listed; j0 += 64) {
-            float mine;
-            int my_place, rank = 0;
-            room.listed(min(j0 + lane, listed - 1), &mine, &my_place);
+            const unsigned long long mine_key = room.listed(min(j0 + lane, listed - 1));
+            int rank = 0;
             if (listed <= 64) {
-                for (int o = 0; o < listed; ++o) rank += is_better(read_lane(mine, o), read_lane(my_place, o), mine, my_place);
+                for (int o = 0; o < listed; ++o) rank += (unsigned long long)read_lane_ll((long long)mine_key, o) > mine_key ? 1 : 0;
             } else {
-                for (int o = 0; o < listed; ++o) {
-                    float s;
-                    int p;
-                    room.listed(o, &s, &p);
-                    rank += is_better(s, p, mine, my_place);
-                }
+                for (int o = 0; o < listed; ++o) rank += room.listed(o) > mine_key ? 1 : 0;
             }
-            if (j0 + lane < listed) write(mine, my_place, rank);
+            if (j0 + lane < listed) write(mine_key, rank);
         }
     } else {
         // the threads beyond the candidates compare as well
-        const int lines = max((listed + 63) / 64, 1), parts = W / lines;
-        const int j = t - t / (64 * lines) * (64 * lines), part = t / (64 * lines);
+        const int lines = max((listed + 63) / 64, 1), parts = W / lines, part = wave_id() / lines, j = (wave_id() - part * lines) * 64 + lane;
         if (j < listed && part < parts) {
-            float mine;
-            int my_place, rank = 0;
-            room.listed(j, &mine, &my_place);
-            for (int o = part; o < listed; o += parts) {
-                float s;
-                int p;
-                room.listed(o, &s, &p);
-                rank += is_better(s, p, mine, my_place);
-            }
+            const unsigned long long mine_key = room.listed(j);
+            int rank = 0;
+            for (int o = part; o < listed; o += parts) rank += room.listed(o) > mine_key ? 1 : 0;
             atomicAdd(&room.better[j], rank);
         }
         __syncthreads();
-        if (t < listed) {
-            float mine;
-            int my_place;
-            room.listed(t, &mine, &my_place);
-            write(mine, my_place, room.better[t]);
-        }
+        if (t < listed) write(room.listed(t), room.better[t]);
     }
     for (int j = listed + t; j < k; j += 64 * W) {
         values[j] = kNothing;
@@ -435,10 +444,10 @@ __device__ __forceinline__ float rescaled(float sum, float from, float to, float
     return sum <= FLT_MAX ? sum * exp2_of((from - to) * by) : sum;
 }
 
-// The largest of the group's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
+// The largest of a wavefront's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
 // NaN, an infinity makes it infinite. best: the thread's largest.
-template <int W, int E>
-__device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best, float by, TopShared<W> &sh, float *reference, float *sum) {
+template <int E>
+__device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best, float by, float *reference, float *sum) {
     float m = reference_of(wave_max_f(best));
     float part[4] = {0.f, 0.f, 0.f, 0.f};
     if (fabsf(m) < 1e30f) {
@@ -453,22 +462,8 @@ __device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best
         for (int i = 0; i < E; ++i) part[i % 4] += exp2_of((v[i] - m) * by);
         part[0] = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    float s = wave_sum_f(part[0]);
-    if constexpr (W > 1) {
-        if (lane_id() == 0) {
-            sh.part_max[wave_id()] = s > 0.f || s != s ? m : kNothing;
-            sh.part_sum[wave_id()] = s;
-        }
-        __syncthreads();
-        m = kNothing;
-        for (int w = 0; w < W; ++w) m = fmaxf(m, sh.part_max[w]);
-        m = reference_of(m);
-        s = 0.f;
-        for (int w = 0; w < W; ++w)
-            if (sh.part_max[w] > kNothing) s += rescaled(sh.part_sum[w], sh.part_max[w], m, by);
-    }
     *reference = m;
-    *sum = s;
+    *sum = wave_sum_f(part[0]);
 }
 // (a sum that nothing adds to has no reference: log(0) + 0)
 __device__ __forceinline__ float log_sum(float m, float s, float temperature) {
@@ -597,16 +592,30 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, W == 1 ? 5 : 6) void k
         }
         const float best[1] = {best_of(v)};
         float m, s;
-        sum_exponentials<W>(v, best[0], by, sh, &m, &s);
-        if (t == 0) {
+        sum_exponentials(v, best[0], by, &m, &s);
+        auto leave = [&](float reference, float sum) {
             if (whole) {
-                out.lse[row] = log_sum(m, s, temperature);
+                out.lse[row] = log_sum(reference, sum, temperature);
             } else {
-                out.lse[out_at * 2] = m;
-                out.lse[out_at * 2 + 1] = s;
+                out.lse[out_at * 2] = reference;
+                out.lse[out_at * 2 + 1] = sum;
+            }
+        };
+        if (lane_id() == 0) {
+            if constexpr (W == 1) {
+                leave(m, s);
+            } else {
+                sh.part_max[wave_id()] = m;
+                sh.part_sum[wave_id()] = s;
             }
         }
-        write_top<W, 1, N>(v, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; });
+        write_top<W, 1, N>(v, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; }, [&] {
+            const bool in = lane_id() < W;
+            const float its_max = in ? sh.part_max[lane_id()] : 0.f, its_sum = in ? sh.part_sum[lane_id()] : 0.f;
+            const float all = reference_of(wave_max_f(its_sum > 0.f ? its_max : kNothing));
+            const float sum = wave_sum_f(its_sum != 0.f ? rescaled(its_sum, its_max, all, by) : 0.f);
+            if (lane_id() == 0) leave(all, sum);
+        });
     }
 }
 
@@ -663,25 +672,45 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
             for (int c = slot * 8; c < size; c += slots * 8) {
                 const T *from = src + (size_t)c * in.class_stride;
                 unsigned *to = cell + c * pitch + r;
-                float z[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    z[j] = c + j < size ? score_to_float(*from) : kNothing;
-                    from += in.class_stride;
-                }
                 unsigned held = 0, ok = ~0u;
                 if constexpr (RULES) {
                     ok = none ? 0u : words != nullptr ? words[c / 32] >> (c % 32) : ~0u;
                     held = rules.shown != nullptr ? my_bits[c / 32] >> (c % 32) & 0xffu : 0u;
-                    if (bias != nullptr) {
+                }
+                if (c + 8 <= size) {
+                    float z[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (c + j < size) z[j] += bias[c + j];
+                    for (int j = 0; j < 8; ++j) z[j] = score_to_float(from[(size_t)j * in.class_stride]);
+                    if constexpr (RULES) {
+                        if (bias != nullptr) {
+#pragma unroll
+                            for (int j = 0; j < 8; j += 4) {
+                                const Float4 more = *reinterpret_cast<const Float4 *>(bias + c + j);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) z[j + q] += more[q];
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) z[j] = ok >> j & 1u ? z[j] : kNothing;
+                        if (held == 0) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) to[j * pitch] = __float_as_uint(z[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (!(held >> j & 1u)) to[j * pitch] = __float_as_uint(z[j]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) to[j * pitch] = __float_as_uint(z[j]);
+                    }
+                } else {
+                    for (int j = 0; c + j < size; ++j) {
+                        float z = score_to_float(from[(size_t)j * in.class_stride]);
+                        if (bias != nullptr) z += bias[c + j];
+                        if (!(held >> j & 1u)) to[j * pitch] = __float_as_uint(ok >> j & 1u ? z : kNothing);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < size && !(held >> j & 1u)) to[j * pitch] = __float_as_uint(ok >> j & 1u ? z[j] : kNothing);
             }
         }
         if constexpr (RULES) {
@@ -715,7 +744,7 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
             }
             const size_t out_at = (size_t)(row0 + q) * chunks + part;
             float m, s;
-            sum_exponentials<1>(v, largest, by, sh, &m, &s);
+            sum_exponentials(v, largest, by, &m, &s);
             if (lane_id() == 0) {
                 if (whole) {
                     out.lse[row0 + q] = log_sum(m, s, temperature);
@@ -725,7 +754,7 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
                 }
             }
             Column column{cell + q, pitch, size, lists[wave_id()]};
-            write_top<1, M, E / M>(v, best, LaneParts<E / M>{}, k, sh, column, out_at, out, [&](int p) { return c0 + p; });
+            write_top<1, M, E / M>(v, best, LaneParts<E / M>{}, k, sh, column, out_at, out, [&](int p) { return c0 + p; }, [] {});
             wave_fence();
         }
     }
@@ -812,27 +841,29 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
             const int at = i * 64 * W + t;
             v[i] = at < count ? values[at] : kNothing;
         }
-        // (every wavefront for itself: a part has one sum)
-        const float *sums = in.lse + from * 2;
-        float m = kNothing;
-        for (int c = lane_id(); c < mine; c += 64) m = fmaxf(m, sums[c * 2 + 1] > 0.f ? sums[c * 2] : kNothing);
-        m = reference_of(wave_max_f(m));
-        float s = 0.f;
-        for (int c = lane_id(); c < mine; c += 64) {
-            const float its = sums[c * 2 + 1];
-            if (its != 0.f) s += rescaled(its, sums[c * 2], m, by);
-        }
-        s = wave_sum_f(s);
-        if (t == 0) {
-            if (joins == 1) {
-                out.lse[row] = log_sum(m, s, temperature);
-            } else {
-                out.lse[tile * 2] = m;
-                out.lse[tile * 2 + 1] = s;
+        auto join_sums = [&] {  // (by one wavefront)
+            const float *sums = in.lse + from * 2;
+            float m = kNothing;
+            for (int c = lane_id(); c < mine; c += 64) m = fmaxf(m, sums[c * 2 + 1] > 0.f ? sums[c * 2] : kNothing);
+            m = reference_of(wave_max_f(m));
+            float s = 0.f;
+            for (int c = lane_id(); c < mine; c += 64) {
+                const float its = sums[c * 2 + 1];
+                if (its != 0.f) s += rescaled(its, sums[c * 2], m, by);
             }
-        }
+            s = wave_sum_f(s);
+            if (lane_id() == 0) {
+                if (joins == 1) {
+                    out.lse[row] = log_sum(m, s, temperature);
+                } else {
+                    out.lse[tile * 2] = m;
+                    out.lse[tile * 2 + 1] = s;
+                }
+            }
+        };
+        if constexpr (W == 1) join_sums();
         const float best[1] = {best_of(v)};
-        write_top<W, 1, E>(v, best, Layout<E, 1, false>{64 * W, 0}, k, sh, rooms[group], tile, out, [&](int p) { return classes[p]; });
+        write_top<W, 1, E>(v, best, Layout<E, 1, false>{64 * W, 0}, k, sh, rooms[group], tile, out, [&](int p) { return classes[p]; }, join_sums);
     }
 }
 
