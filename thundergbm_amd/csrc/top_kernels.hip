@@ -154,8 +154,7 @@ struct TopOut {
 };
 
 // LDS of a group: the candidates, ordered score in front of the complement of the place (larger is better), and how many of them are
-// better; and, where the candidates are too many for that, the scores of the threads that reach the bound, score i of the q-th of them at
-// q * N + i, and who they are.
+// better; the scores of the threads that reach the bound, score i of the q-th of them at q * N + i, and who they are.
 template <int W, int N>
 struct LaidOut {
     static constexpr int kRoom = kListRoom;
@@ -174,6 +173,7 @@ struct LaidOut {
     __device__ __forceinline__ float get(int q, int i, const At &) const { return score[q * N + i]; }
     template <typename At>
     __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(owner[q], i); }
+    __device__ __forceinline__ float laid_out(int q, int i, int) const { return score[q * N + i]; }
     __device__ __forceinline__ void list(int to, float s, int p) {
         key[to] = (unsigned long long)ordered(s) << 32 | (unsigned)~p;
         if constexpr (W > 1) better[to] = 0;
@@ -200,6 +200,7 @@ struct Column {
     }
     template <typename At>
     __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(lists.owner[q], i); }
+    __device__ __forceinline__ float laid_out(int, int, int p) const { return at_line(p); }
     __device__ __forceinline__ void list(int to, float, int p) { lists.entry[to] = (unsigned short)p; }
     __device__ __forceinline__ unsigned long long listed(int j) const {
         const int p = lists.entry[j];
@@ -289,58 +290,54 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
         for (int i = M * N - 1; i >= 0; --i)
             mine[i / 32] = mine[i / 32] + mine[i / 32] + (v[i] > least || (v[i] == least && at.at(t + 64 * (i / N), i % N) <= at_most) ? 1u : 0u);
     }
-    int listed = 0;
-    auto slot_of = [&](unsigned long long which) {  // the lanes that have one more for the list: where it goes
-        int to = listed;
-        if constexpr (W == 1) {
-            listed += __popcll(which);
-        } else {
-            if (lane == 0) to = atomicAdd(&sh.listed, __popcll(which));
-            to = __shfl(to, 0);
+    // their threads - at most candidates_wanted(k), or k where the bound is exact - lay their scores out and list what reaches it
+    int listed = 0, threads = 0;
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+        unsigned bits[(N + 31) / 32];
+        int count = 0;
+#pragma unroll
+        for (int w = 0; w < (N + 31) / 32; ++w) {
+            if constexpr (M == 1) bits[w] = mine[w];
+            else bits[w] = mine[j * N / 32] >> (j * N % 32) & ((1u << N) - 1u);  // (M is 1 where N does not divide 32)
+            count += __popc(bits[w]);
         }
-        return to + lanes_below(which);
-    };
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-        bool largest_first = true;
-        while (true) {
-            const unsigned long long which = __ballot(mine[w] != 0);
-            if (which == 0) break;
-            const int to = slot_of(which), i = mine[w] != 0 ? __ffs((int)mine[w]) - 1 + w * 32 : 0;
-            // (nearly always a thread has the one that is its largest)
-            float s = kNothing;
-            if (M == 1 && kWords == 1 && largest_first && __ballot((mine[w] & (mine[w] - 1)) != 0) == 0) {
-                s = best[0];
-            } else {
-#pragma unroll
-                for (int j = w * 32; j < (w * 32 + 32 < M * N ? w * 32 + 32 : M * N); ++j) s = j == i ? v[j] : s;
+        const unsigned long long who = __ballot(count != 0);
+        if (who == 0) continue;
+        const int scan = wave_scan_i(count), total = read_lane(scan, 63);
+        int q = threads + lanes_below(who), to = listed + scan - count;
+        if constexpr (W == 1) {
+            threads += __popcll(who);
+            listed += total;
+        } else {
+            int q0 = 0, to0 = 0;
+            if (lane == 0) {
+                q0 = atomicAdd(&sh.threads, __popcll(who));
+                to0 = atomicAdd(&sh.listed, total);
             }
-            largest_first = false;
-            if (mine[w] != 0 && to < Room::kRoom) room.list(to, s, at.at(t + 64 * (i / N), i % N));
-            mine[w] &= mine[w] - 1;
+            q += __shfl(q0, 0);
+            to += __shfl(to0, 0);
+        }
+        if (count != 0) {
+            room.put(q, t + 64 * j, v + j * N);
+            wave_fence();
+#pragma unroll
+            for (int w = 0; w < (N + 31) / 32; ++w)
+                while (bits[w] != 0) {
+                    const int i = __ffs((int)bits[w]) - 1 + w * 32, p = at.at(t + 64 * j, i);
+                    bits[w] &= bits[w] - 1;
+                    if (to < Room::kRoom) room.list(to, room.laid_out(q, i, p), p);
+                    ++to;
+                }
         }
     }
     group_sync<W>();
-    if constexpr (W > 1) listed = sh.listed;
+    if constexpr (W > 1) {
+        listed = sh.listed;
+        threads = sh.threads;
+    }
     if (listed > Room::kRoom) {  // (the same in all threads)
-        // The best scores lie together in few threads, at most candidates_wanted(k), or k where the bound is exact: these lay theirs out,
-        // and the exact k-th one is found by bisection over all of them.
-        int threads = 0;
-#pragma unroll
-        for (int j = 0; j < M; ++j) {
-            const bool reaches = best[j] > least || (best[j] == least && (!exact || first[j] <= at_most));
-            const unsigned long long who = __ballot(reaches);
-            int q = threads + lanes_below(who);
-            threads += __popcll(who);
-            if constexpr (W > 1) {
-                int base = 0;
-                if (lane == 0 && threads > 0) base = atomicAdd(&sh.threads, threads);
-                q += __shfl(base, 0);
-            }
-            if (reaches) room.put(q, t + 64 * j, v + j * N);
-        }
-        group_sync<W>();
-        if constexpr (W > 1) threads = sh.threads;
+        // The best scores lie together in few threads: the exact k-th one by bisection over all that were laid out.
         const int entries = threads * N;
         auto value = [&](int e) { return room.get(e / N, e % N, at); };
         auto place = [&](int e) { return room.place(e / N, e % N, at); };
@@ -380,7 +377,14 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
             }
             const unsigned long long which = __ballot(is);
             if (which == 0) continue;
-            const int to = slot_of(which);
+            int to = listed;
+            if constexpr (W == 1) {
+                listed += __popcll(which);
+            } else {
+                if (lane == 0) to = atomicAdd(&sh.listed, __popcll(which));
+                to = __shfl(to, 0);
+            }
+            to += lanes_below(which);
             if (is && to < Room::kRoom) room.list(to, x, place(e));
         }
         group_sync<W>();
@@ -502,7 +506,7 @@ __device__ __forceinline__ void count_shown(const tgbm_score_rules &rules, long 
 // workgroup. A thread has E scores in whole vectors, and one of what is left behind the last vector. RULES: there may be any. LDS: the lists of candidates,
 // then, where classes were shown, bits and times.
 template <typename T, int W, int E, bool RULES>
-__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, W == 1 ? 5 : 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
+__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 5 : 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
                                                                           int chunks, int chunk, bool whole) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
@@ -556,25 +560,28 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, W == 1 ? 5 : 6) void k
                 shown_range(rules, row, &b, &e);
                 if (b < e) {  // (the same for the group)
                     count_shown<W>(rules, b, e, c0, c0 + size, chunk, bits, times);
-                    unsigned held = 0;
-#pragma unroll
-                    for (int g = 0; g < E / V; ++g) {
-                        const int c = base + g * kStep;
-                        if (c < whole_size) held |= (bits[c / 32] >> (c % 32) & ((1u << V) - 1u)) << (g * V);
-                    }
-                    if (t < size - whole_size) held |= (bits[(whole_size + t) / 32] >> ((whole_size + t) % 32) & 1u) << E;
                     // few of a thread's scores are: one at a time, from the start (its register has no number that a loop can use)
-                    while (__any(held != 0)) {
-                        const bool now = held != 0;
-                        const int i = now ? __ffs((int)held) - 1 : 0;
-                        float s = 0.f;
-                        if (now) {
-                            const int c = at.at(t, i);
-                            s = adjusted(score_to_float(src[c]), rules.bias != nullptr ? rules.bias[c0 + c] : 0.f, times[c], true, rules);
-                        }
-                        held &= held - 1;
 #pragma unroll
-                        for (int j = 0; j < N; ++j) v[j] = now && j == i ? s : v[j];
+                    for (int w = 0; w < (N + 23) / 24; ++w) {  // (24 scores are whole vectors)
+                        unsigned held = 0;
+#pragma unroll
+                        for (int i = w * 24; i < (w * 24 + 24 < E ? w * 24 + 24 : E); i += V) {
+                            const int c = base + i / V * kStep;
+                            if (c < whole_size) held |= (bits[c / 32] >> (c % 32) & ((1u << V) - 1u)) << (i - w * 24);
+                        }
+                        if (w == E / 24 && t < size - whole_size) held |= (bits[(whole_size + t) / 32] >> ((whole_size + t) % 32) & 1u) << (E - w * 24);
+                        while (__any(held != 0)) {
+                            const bool now = held != 0;
+                            const int i = now ? __ffs((int)held) - 1 + w * 24 : 0;
+                            float s = 0.f;
+                            if (now) {
+                                const int c = at.at(t, i);
+                                s = adjusted(score_to_float(src[c]), rules.bias != nullptr ? rules.bias[c0 + c] : 0.f, times[c], true, rules);
+                            }
+                            held &= held - 1;
+#pragma unroll
+                            for (int j = w * 24; j < (w * 24 + 24 < N ? w * 24 + 24 : N); ++j) v[j] = now && j == i ? s : v[j];
+                        }
                     }
                 }
             }
@@ -879,7 +886,9 @@ struct TopPlan {
 constexpr int kFewClasses = 32;
 // With up to so many best classes the maxima of 64 lanes give a bound that few scores reach: with all of them the lists overflow.
 constexpr int kFewBest = 32;
-constexpr int kRowScores = 24;  // classes side by side: the most that a thread has in whole vectors
+// Classes side by side: the most scores that a thread has in whole vectors. Looking for the bound, the list and its order cost about as much as
+// the scores of 24, so rows that fill them go by 48.
+constexpr int kRowScores = 24, kRowScoresWide = 48;
 constexpr int kJoinMost = 16384;  // scores that a join takes
 constexpr int kGroupsWanted = 512;
 
@@ -890,7 +899,7 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
     p.chunks = 1;
     p.chunk = classes;
     if (p.few) return p;
-    const int most = columns ? 1024 : 8 * 64 * kRowScores, least = columns ? 1024 : 64 * kRowScores;
+    const int most = columns ? 1024 : 8 * 64 * kRowScoresWide, least = columns ? 1024 : 64 * kRowScores;
     long tiles = columns ? (rows + 15) / 16 : rows;
     long chunks = (classes - 1) / most + 1;
     chunks = std::max(chunks, std::min<long>((classes - 1) / least + 1, kGroupsWanted / std::max(1l, tiles)));
@@ -908,7 +917,7 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
         p.per_thread = 8;
     } else {
         p.waves = p.chunk <= 64 * kRowScores ? 1 : p.chunk <= 256 * kRowScores ? 4 : 8;
-        p.per_thread = p.waves > 1 ? kRowScores : p.chunk <= 512 ? 8 : p.chunk <= 1024 ? 16 : kRowScores;
+        p.per_thread = p.chunk > 512 * kRowScores ? kRowScoresWide : p.waves > 1 ? kRowScores : p.chunk <= 512 ? 8 : p.chunk <= 1024 ? 16 : kRowScores;
     }
     p.parts = columns && k > kFewBest ? std::min(4, p.per_thread) : 1;
     return p;
@@ -954,6 +963,8 @@ void top(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_scor
         else if (p.per_thread == 4) top_columns<T, 4, kRules>(s, p, in, rules, k, temperature, out);
         else if (p.per_thread == 8) top_columns<T, 8, kRules>(s, p, in, rules, k, temperature, out);
         else top_columns<T, 16, kRules>(s, p, in, rules, k, temperature, out);
+    } else if (p.waves == 8 && p.per_thread == kRowScoresWide) {
+        top_rows<T, 8, kRowScoresWide, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 8) {
         top_rows<T, 8, kRowScores, RULES>(s, p, in, rules, k, temperature, out);
     } else if (p.waves == 4 && p.per_thread == 8) {
