@@ -5,7 +5,8 @@
 // of their own so that it keeps its precision when it is tiny), so a tile of [classes][rows] scores in LDS is enough: the
 // named ones are replaced by marks there, what belongs to them stands in a list of [entries][rows], and one pass over the tile
 // gives the sums, a second one the pairs. Scores are read once, pairs written once. Classes beyond a tile go by chunks: one
-// launch leaves each chunk's sums, a second one adds them up and writes the pairs, which reads the scores a second time.
+// launch leaves each chunk's sums, a second one adds them up and writes the pairs, which reads the scores a second time. Up to 32
+// classes a thread holds its whole row.
 #include <algorithm>
 #include <cfloat>
 
@@ -15,13 +16,12 @@
 namespace tgbm {
 namespace {
 
-constexpr int kDistillBlock = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kNone = -__builtin_inff();
 
 // Marks in the tile: NaNs that no score is left as (a score that is NaN becomes the one of the hardware).
 constexpr unsigned kNaN = 0x7fc00000u, kMark = 0xffc00000u;
-__device__ __forceinline__ bool is_mark(unsigned v) { return v >= kMark && v < kMark + kTeacherMost; }
+__device__ __forceinline__ bool is_mark(unsigned v) { return v - kMark < (unsigned)kTeacherMost; }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * kLn2; }
@@ -31,353 +31,525 @@ __device__ __forceinline__ float reference_of(float m) { return fabsf(m) <= FLT_
 // such a score, and the whole row becomes NaN.
 __device__ __forceinline__ float inverse_of(float sum) { return sum == 0.f ? 0.f : sum <= FLT_MAX ? 1.f / sum : __builtin_nanf(""); }
 
-// What a chunk leaves of a row.
-struct ChunkSums {
-    float other_max, other_sum, other_sum1;  // of the classes that are not named: largest score, sums of exp((z - it) / T) and exp(z - it)
+// What the classes of a row, or of a chunk of it, add up to. Sums are those of exp((z - max) / T), and with 1 of exp(z - max).
+struct RowSums {
+    float other_max, other_sum, other_sum1;  // of the classes that are not named
     float named_max, named_sum, named_sum1;
-    float cross, mass;  // sum of q (log q - (z - named_max) / T) and of q over the chunk's named classes
-    float label;        // z - max(other_max, named_max) of the label, if it is one of the chunk's (else 0)
-    float has_label;
+    float cross, mass;  // sum of q (log q - (z - named_max) / T), and of q, over the named classes
+    float label;        // the label's score, where it is one of the classes
 };
 
-enum DistillPart { DISTILL_WHOLE, DISTILL_SUMS, DISTILL_PAIRS };
+// What the call is about.
+struct DistillCall {
+    tgbm_scores in;
+    tgbm_teacher teacher;
+    const float *labels;  // nullptr: the teacher alone
+    float temperature, weight;
+    float *loss;
+    GHPair *pairs;
+    long pair_stride;
+    const int *row_of;  // rows may lie in another order than the teacher's
+};
 
 __device__ __forceinline__ float teacher_at(const tgbm_teacher &t, size_t at) {
     if (t.type == TGBM_F32) return static_cast<const float *>(t.scores)[at];
     if (t.type == TGBM_F16) return (float)static_cast<const _Float16 *>(t.scores)[at];
     return (float)static_cast<const __bf16 *>(t.scores)[at];
 }
-
-// Sum, or largest, over the threads of a row (thread = slot * R + row): over the lanes of each wavefront, then over the wavefronts.
-template <int R, bool MAX>
-__device__ __forceinline__ float over_slots(float v, float *room) {
-    if constexpr (R == kDistillBlock) return v;
-    constexpr int kRows = R < 64 ? R : 64;  // of a wavefront
-    for (int d = kRows; d < 64; d <<= 1) {
-        const float o = __shfl_xor(v, d);
-        v = MAX ? fmaxf(v, o) : v + o;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) < kRows) room[(threadIdx.x >> 6) * 64 + (threadIdx.x & (kRows - 1))] = v;
-    __syncthreads();
-    constexpr int kStep = R > 64 ? R / 64 : 1;  // wavefronts that hold the same rows
-    const int first = R > 64 ? (threadIdx.x >> 6) % kStep : 0;
-    float all = room[first * 64 + (threadIdx.x & (kRows - 1))];
-#pragma unroll
-    for (int w = first + kStep; w < kDistillBlock / 64; w += kStep) {
-        const float o = room[w * 64 + (threadIdx.x & (kRows - 1))];
-        all = MAX ? fmaxf(all, o) : all + o;
-    }
-    return all;
+__device__ __forceinline__ int label_of(const DistillCall &call, long row) {  // -1: none
+    if (call.labels == nullptr) return -1;
+    const float y = call.labels[row];
+    return y >= 0.f && y < (float)call.in.classes && y == floorf(y) ? (int)y : -1;
 }
 
-// R rows of a workgroup, kDistillBlock / R threads for each. tile: chunk classes; LDS: [chunk][R] scores, [entries][R] pairs of q and z.
-template <int R, DistillPart PART>
-__global__ __launch_bounds__(kDistillBlock) void k_distill(tgbm_scores in, tgbm_teacher teacher, const float *__restrict__ labels, float temperature, float weight,
-                                                           float *__restrict__ loss, GHPair *__restrict__ pairs, long pair_stride,
-                                                           const int *__restrict__ row_of, ChunkSums *__restrict__ sums, int chunks, int chunk,
-                                                           long tiles) {
-    extern __shared__ unsigned cell[];  // [chunk][R]
-    __shared__ float room[kDistillBlock];
-    constexpr int kSlots = kDistillBlock / R;
-    const int K = teacher.entries;
-    float *const q_of = reinterpret_cast<float *>(cell + (size_t)chunk * R);  // [K][R]
-    float *const z_of = q_of + (size_t)K * R;
-    const int r = threadIdx.x % R, slot = threadIdx.x / R;
-    const float by1 = kLog2e, by = kLog2e / temperature;
-    const bool hard = labels != nullptr;
-    for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        if (PART == DISTILL_PAIRS && pairs == nullptr && tile % chunks != 0) continue;  // (the loss alone)
-        const long row = tile / chunks * R + r;
-        const bool on = row < in.rows;
-        const int c0 = (int)(tile % chunks) * chunk, c1 = min(in.classes, c0 + chunk);
-        const float *z = static_cast<const float *>(in.data) + row;
-        // rows may lie in another order than the teacher's
-        const size_t given = on ? (size_t)(row_of != nullptr ? row_of[row] : row) : 0;
-        if (on)
-            for (int c = c0 + slot; c < c1; c += kSlots) {
-                const float v = z[(size_t)c * in.class_stride];
-                cell[(c - c0) * R + r] = v == v ? __float_as_uint(v) : kNaN;
-            }
-        // the teacher's entries: q
-        const int *named = teacher.classes + given * K;
-        auto entry = [&](int j, int *c) {  // its score over the temperature; -inf: left out
-            *c = on ? named[j] : -1;
-            const float t = on ? teacher_at(teacher, given * K + j) / temperature : kNone;
-            return (unsigned)*c < (unsigned)in.classes ? t : kNone;
-        };
-        float top = kNone, any = 0.f;
-        int c;
-        for (int j = slot; j < K; j += kSlots) {
-            const float t = entry(j, &c);
+// What turns a row's scores into pairs. Every probability is an exponential to one of the two references times a factor: with
+// e = exp((z - max) / T), e1 = exp(z - max): p = e * p_by, the gradient is e * g_by + e1 * g1_by, less b at the label; a named
+// class's has aT * q less.
+struct RowFactors {
+    float other_max, other_p, other_p1, other_g;
+    float named_max, named_p, named_p1;
+    float a, b, aT;
+};
+
+// sum: of all classes; any: the teacher names a class; given: the sum of all entries' q; label < 0: none. Returns the loss as well.
+__device__ __forceinline__ RowFactors factors_of(const RowSums &sum, bool any, float given, bool has_rest, int label, float temperature, float weight, float *loss) {
+    const float by = kLog2e / temperature;
+    const bool others = sum.other_sum != 0.f, named = sum.named_sum != 0.f;
+    const float higher = reference_of(fmaxf(others ? sum.other_max : kNone, named ? sum.named_max : kNone));
+    const float other_up = others ? exp2_of((sum.other_max - higher) * by) : 0.f, named_up = named ? exp2_of((sum.named_max - higher) * by) : 0.f;
+    const float Z = sum.other_sum * other_up + sum.named_sum * named_up, inv = inverse_of(Z);
+    RowFactors f;
+    f.a = !any ? 0.f : given <= FLT_MAX ? weight : __builtin_nanf("");
+    f.b = label >= 0 ? 1.f - weight : 0.f;
+    f.aT = f.a * temperature;
+    const float rest = has_rest && others && any ? fmaxf(0.f, 1.f - given) : 0.f;  // the teacher's mass on the other classes
+    f.other_max = sum.other_max;
+    f.named_max = sum.named_max;
+    f.other_p = other_up * inv;
+    f.named_p = named_up * inv;
+    f.other_g = f.aT * (f.other_p - (rest != 0.f ? rest / sum.other_sum : 0.f));
+    f.other_p1 = f.named_p1 = 0.f;
+    float log_Z1 = 0.f;
+    if (label >= 0) {
+        const float other_up1 = others ? exp2_of((sum.other_max - higher) * kLog2e) : 0.f, named_up1 = named ? exp2_of((sum.named_max - higher) * kLog2e) : 0.f;
+        const float Z1 = sum.other_sum1 * other_up1 + sum.named_sum1 * named_up1, inv1 = inverse_of(Z1);
+        f.other_p1 = other_up1 * inv1;
+        f.named_p1 = named_up1 * inv1;
+        log_Z1 = Z1 != 0.f ? log_of(Z1) : 0.f;
+    }
+    float value = 0.f;
+    if (f.a != 0.f) {  // (or NaN)
+        const float log_Z = Z != 0.f ? log_of(Z) : 0.f;
+        // log p of a named class is (z - named_max) / T less log Z + (higher - named_max) / T
+        float soft = sum.mass != 0.f ? sum.cross + sum.mass * (log_Z + (higher - sum.named_max) / temperature) : 0.f;
+        if (rest != 0.f) soft += rest * (log_of(rest) - (log_of(sum.other_sum) + (sum.other_max - higher) / temperature - log_Z));
+        value = f.a * temperature * temperature * soft;
+    }
+    if (f.b != 0.f) value += f.b * (log_Z1 - (sum.label - higher));
+    *loss = value;
+    return f;
+}
+
+// g and h from p, p1 and the gradient before the label's part.
+__device__ __forceinline__ GHPair pair_of(const RowFactors &f, float p, float p1, float g, bool is_label) {
+    const float h = 2.f * (f.a * (p * (1.f - p)) + f.b * (p1 * (1.f - p1)));
+    return GHPair{g + f.b * (p1 - (is_label ? 1.f : 0.f)), h < 1e-16f ? 1e-16f : h};  // (NaN stays)
+}
+
+// ------------------------------------------------------------------------------------------------------ few classes
+constexpr int kFewBlock = 256;
+template <int C>
+__global__ __launch_bounds__(kFewBlock) void k_distill_few(DistillCall call) {
+    const long row = (long)blockIdx.x * kFewBlock + threadIdx.x;
+    if (row >= call.in.rows) return;
+    const int classes = call.in.classes, K = call.teacher.entries;
+    const size_t given_row = (size_t)(call.row_of != nullptr ? call.row_of[row] : row);
+    const float by = kLog2e / call.temperature;
+    const bool hard = call.labels != nullptr;
+    const float *from = static_cast<const float *>(call.in.data) + row;
+    float z[C], q[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) z[c] = c < classes ? from[(size_t)c * call.in.class_stride] : kNone;
+    // the teacher: what the entries of a class add up to
+    const int *named = call.teacher.classes + given_row * K;
+    float top = kNone;
+    unsigned there = 0;  // (bit c: class c is named)
+    for (int j = 0; j < K; ++j) {
+        const int c = named[j];
+        const float t = teacher_at(call.teacher, given_row * K + j);
+        if ((unsigned)c < (unsigned)classes && t != kNone) {
             top = fmaxf(top, t);
-            any = t != kNone ? 1.f : any;  // (NaN is an entry)
+            there |= 1u << c;
         }
-        any = over_slots<R, true>(any, room);
-        float norm;  // log of what the exponentials are divided by
-        if (teacher.lse != nullptr) {
-            norm = on ? teacher.lse[given] : 0.f;
-        } else {
-            top = reference_of(over_slots<R, true>(top, room));
-            float s = 0.f;
-            for (int j = slot; j < K; j += kSlots) s += exp2_of((entry(j, &c) - top) * kLog2e);
-            norm = top + log_of(over_slots<R, false>(s, room));
+    }
+    top = reference_of(top);
+#pragma unroll
+    for (int c = 0; c < C; ++c) q[c] = 0.f;
+    float sum_q = 0.f;
+    for (int j = 0; j < K; ++j) {
+        const int c = named[j];
+        const float t = teacher_at(call.teacher, given_row * K + j);
+        const float e = (unsigned)c < (unsigned)classes && t != kNone ? exp2_of((t - top) * by) : 0.f;
+        sum_q += e;
+#pragma unroll
+        for (int o = 0; o < C; ++o) q[o] += o == c ? e : 0.f;
+    }
+    const bool rest = call.teacher.lse != nullptr, any = there != 0;
+    const float scale = rest ? exp2_of((top / call.temperature - call.teacher.lse[given_row]) * kLog2e) : any ? 1.f / sum_q : 0.f;
+    RowSums s{};
+    const int label = label_of(call, row);
+    float mo = kNone, mn = kNone;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        q[c] *= scale;
+        if (there >> c & 1u) mn = fmaxf(mn, z[c]);
+        else mo = fmaxf(mo, z[c]);
+        s.label = c == label ? z[c] : s.label;
+    }
+    s.other_max = reference_of(mo);
+    s.named_max = reference_of(mn);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const bool is_named = there >> c & 1u;
+        const float d = z[c] - (is_named ? s.named_max : s.other_max), e = exp2_of(d * by), e1 = hard ? exp2_of(d * kLog2e) : 0.f;
+        s.named_sum += is_named ? e : 0.f;
+        s.other_sum += is_named || c >= classes ? 0.f : e;
+        s.named_sum1 += is_named ? e1 : 0.f;
+        s.other_sum1 += is_named || c >= classes ? 0.f : e1;
+        if (is_named && q[c] != 0.f) {
+            s.cross += q[c] * (log_of(q[c]) - d / call.temperature);
+            s.mass += q[c];
         }
-        float mass = 0.f;
-        bool twice = false;
+    }
+    float value;
+    const RowFactors f = factors_of(s, any, any ? sum_q * scale : 0.f, rest, label, call.temperature, call.weight, &value);
+    if (call.loss != nullptr) call.loss[given_row] = value;
+    if (call.pairs == nullptr) return;
+    GHPair *to = call.pairs + row;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const bool is_named = there >> c & 1u;
+        const float d = z[c] - (is_named ? f.named_max : f.other_max), e = exp2_of(d * by), e1 = hard ? exp2_of(d * kLog2e) : 0.f;
+        const float p = e * (is_named ? f.named_p : f.other_p), p1 = e1 * (is_named ? f.named_p1 : f.other_p1);
+        if (c < classes) *to = pair_of(f, p, p1, is_named ? f.aT * (p - q[c]) : e * f.other_g, c == label);
+        to += call.pair_stride;
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------- more classes
+enum DistillPart { DISTILL_WHOLE, DISTILL_SUMS, DISTILL_PAIRS };
+
+// R rows of a workgroup of B threads, thread = slot * R + row.
+template <int R, int B>
+struct Rows {
+    static constexpr int kSlots = B / R, kWaves = B / 64, kLanes = R < 64 ? R : 64;  // kLanes: rows of a wavefront
+    static_assert(R <= 64);
+    static constexpr int kMostValues = 6;
+    float part[kMostValues][kWaves][kLanes], all[kMostValues][kLanes];
+
+    // Sums over a row's threads (largest of the first MAXIMA), the same in all of them: over lanes, then over wavefronts.
+    template <int N, int MAXIMA>
+    __device__ __forceinline__ void reduce(float (&v)[N]) {
+        static_assert(N <= kMostValues && N * kLanes <= B);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int d = kLanes; d < 64; d <<= 1) {
+                const float o = __shfl_xor(v[k], d);
+                v[k] = k < MAXIMA ? fmaxf(v[k], o) : v[k] + o;
+            }
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = threadIdx.x & (kLanes - 1);
+        if (lane < kLanes) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) part[k][wave][lane] = v[k];
+        }
+        __syncthreads();
+        if (threadIdx.x < N * kLanes) {
+            const int k = threadIdx.x / kLanes;
+            float x = part[k][0][r];
+            for (int w = 1; w < kWaves; ++w) x = k < MAXIMA ? fmaxf(x, part[k][w][r]) : x + part[k][w][r];
+            all[k][r] = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = all[k][r];
+    }
+};
+
+// LDS: [chunk][R] scores; then of the entries [K][R + 1]: their classes, q, and scores.
+template <int R, int B, DistillPart PART>
+__global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__restrict__ sums, int chunks, int chunk) {
+    using Group = Rows<R, B>;
+    constexpr int kSlots = Group::kSlots, kPitch = R + 1;
+    __shared__ Group group;
+    __shared__ RowFactors factors[R];
+    __shared__ float label_score[R];
+    extern __shared__ unsigned cell[];
+    const int K = call.teacher.entries;
+    int *const class_of = reinterpret_cast<int *>(cell + (size_t)chunk * R);
+    float *const q_of = reinterpret_cast<float *>(class_of + K * kPitch), *const z_of = q_of + K * kPitch;
+    const int r = threadIdx.x % R, slot = threadIdx.x / R;
+    // (workgroups go to the eight dies in turn: two tiles that share cache lines go to the same one)
+    const long tile = R * 4 < 128 ? ((long)blockIdx.x & ~15l) + (blockIdx.x & 7) * 2 + (blockIdx.x >> 3 & 1) : blockIdx.x;
+    const long row0 = tile * R, row = row0 + r;
+    if (row0 >= call.in.rows) return;
+    const bool on = row < call.in.rows, hard = call.labels != nullptr;
+    const int c0 = blockIdx.y * chunk, size = min(call.in.classes - c0, chunk);
+    const float by = kLog2e / call.temperature;
+    const float *from = static_cast<const float *>(call.in.data) + (size_t)c0 * call.in.class_stride + row;
+    const auto given_of = [&](long i) { return (size_t)(call.row_of != nullptr ? call.row_of[i] : i); };
+
+    if (on) {
+        for (int c = slot; c < size; c += 8 * kSlots) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c + j * kSlots < size ? from[(size_t)(c + j * kSlots) * call.in.class_stride] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j * kSlots < size) cell[(c + j * kSlots) * R + r] = v[j] == v[j] ? __float_as_uint(v[j]) : kNaN;
+        }
+    }
+    // the entries: their scores over the temperature for now, -1 for the class of one that is left out
+    for (int i = threadIdx.x; i < R * K; i += B) {
+        const int of = i / K, j = i - of * K;
+        int c = -1;
+        float t = kNone;
+        if (row0 + of < call.in.rows) {
+            const size_t at = given_of(row0 + of) * K + j;
+            c = call.teacher.classes[at];
+            t = teacher_at(call.teacher, at) / call.temperature;
+        }
+        class_of[j * kPitch + of] = (unsigned)c < (unsigned)call.in.classes && t != kNone ? c : -1;
+        q_of[j * kPitch + of] = t;
+    }
+    if (threadIdx.x < R) label_score[threadIdx.x] = 0.f;
+    __syncthreads();
+    float first[2] = {kNone, kNone};  // the largest, and whether there is one (NaN is an entry)
+    for (int j = slot; j < K; j += kSlots)
+        if (class_of[j * kPitch + r] >= 0) {
+            first[0] = fmaxf(first[0], q_of[j * kPitch + r]);
+            first[1] = 1.f;
+        }
+    group.template reduce<2, 2>(first);
+    const bool any = first[1] == 1.f;
+    float norm;  // log of what the exponentials are divided by
+    if (call.teacher.lse != nullptr) {
+        norm = on ? call.teacher.lse[given_of(row)] : 0.f;
+    } else {
+        const float top = reference_of(first[0]);
+        float s[1] = {0.f};
+        for (int j = slot; j < K; j += kSlots)
+            if (class_of[j * kPitch + r] >= 0) s[0] += exp2_of((q_of[j * kPitch + r] - top) * kLog2e);
+        group.template reduce<1, 0>(s);
+        norm = top + log_of(s[0]);
+    }
+    float given = 0.f;
+    for (int j = slot; j < K; j += kSlots) {
+        const int c = class_of[j * kPitch + r] - c0;
+        if (c + c0 < 0) continue;
+        const float q = exp2_of((q_of[j * kPitch + r] - norm) * kLog2e);
+        given += q;
+        q_of[j * kPitch + r] = q;
+        if (c >= 0 && c < size) z_of[j * kPitch + r] = __uint_as_float(cell[c * R + r]);
+        else class_of[j * kPitch + r] = -1;  // (another chunk's)
+    }
+    __syncthreads();
+    for (int j = slot; j < K; j += kSlots) {
+        const int c = class_of[j * kPitch + r] - c0;
+        if (c >= 0) cell[c * R + r] = kMark + j;
+    }
+    __syncthreads();
+    bool twice = false;
+    for (int j = slot; j < K; j += kSlots) {
+        const int c = class_of[j * kPitch + r] - c0;
+        twice |= c >= 0 && cell[c * R + r] != kMark + j;
+    }
+    if (__syncthreads_or(twice)) {  // a class that several entries name belongs to the first of them
         for (int j = slot; j < K; j += kSlots) {
-            const float t = entry(j, &c);
-            const bool there = t != kNone;
-            const float q = there ? exp2_of((t - norm) * kLog2e) : 0.f;
-            mass += q;
-            const bool mine = there && c >= c0 && c < c1;
-            q_of[j * R + r] = q;
-            z_of[j * R + r] = mine ? __uint_as_float(cell[(c - c0) * R + r]) : kNone;
-        }
-        mass = over_slots<R, false>(mass, room);  // (and all entries have read their scores)
-        for (int j = slot; j < K; j += kSlots) {
-            const bool mine = entry(j, &c) != kNone && c >= c0 && c < c1;
-            if (mine) cell[(c - c0) * R + r] = kMark + j;
+            const int c = class_of[j * kPitch + r] - c0;
+            if (c >= 0) atomicMin(&cell[c * R + r], kMark + j);
         }
         __syncthreads();
         for (int j = slot; j < K; j += kSlots) {
-            const bool mine = entry(j, &c) != kNone && c >= c0 && c < c1;
-            if (mine && cell[(c - c0) * R + r] != kMark + j) twice = true;
+            const int c = class_of[j * kPitch + r] - c0;
+            if (c < 0 || cell[c * R + r] != kMark + j) continue;
+            float q = q_of[j * kPitch + r];
+            for (int o = j + 1; o < K; ++o)
+                if (class_of[o * kPitch + r] == c + c0) q += q_of[o * kPitch + r];
+            q_of[j * kPitch + r] = q;  // (nobody else reads it: the others' sums are of other classes)
         }
-        if (__syncthreads_or(twice)) {  // a class that several entries name belongs to the first of them
-            for (int j = slot; j < K; j += kSlots) {
-                const bool mine = entry(j, &c) != kNone && c >= c0 && c < c1;
-                if (mine) atomicMin(&cell[(c - c0) * R + r], kMark + j);
-            }
-            __syncthreads();
-            for (int j = slot; j < K; j += kSlots) {
-                const bool mine = entry(j, &c) != kNone && c >= c0 && c < c1;
-                if (!mine || cell[(c - c0) * R + r] != kMark + j) continue;
-                float q = q_of[j * R + r];
-                for (int o = j + 1; o < K; ++o) {
-                    int co;
-                    if (entry(o, &co) != kNone && co == c) q += q_of[o * R + r];
-                }
-                q_of[j * R + r] = q;  // (read by nobody else: the others' sums take entries behind their own of other classes)
-            }
-            __syncthreads();
-        }
-        // the sums
-        ChunkSums sum{};
-        float m = kNone;
-        if (on)
-            for (int i = slot; i < c1 - c0; i += kSlots) {
-                const unsigned v = cell[i * R + r];
-                if (!is_mark(v)) m = fmaxf(m, __uint_as_float(v));
-            }
-        sum.other_max = reference_of(over_slots<R, true>(m, room));
-        float s = 0.f, s1 = 0.f;
-        if (on)
-            for (int i = slot; i < c1 - c0; i += kSlots) {
-                const unsigned v = cell[i * R + r];
-                if (is_mark(v)) continue;
-                const float d = __uint_as_float(v) - sum.other_max;
-                s += exp2_of(d * by);
-                if (hard) s1 += exp2_of(d * by1);
-            }
-        sum.other_sum = over_slots<R, false>(s, room);
-        if (hard) sum.other_sum1 = over_slots<R, false>(s1, room);
-        // (the first of a class's entries stands for it)
-        auto owner = [&](int j, int *c) { return entry(j, c) != kNone && *c >= c0 && *c < c1 && cell[(*c - c0) * R + r] == kMark + j; };
-        m = kNone;
-        for (int j = slot; j < K; j += kSlots)
-            if (owner(j, &c)) m = fmaxf(m, z_of[j * R + r]);
-        sum.named_max = reference_of(over_slots<R, true>(m, room));
-        s = s1 = 0.f;
-        float cross = 0.f, part = 0.f;
+        __syncthreads();
         for (int j = slot; j < K; j += kSlots) {
-            if (!owner(j, &c)) continue;
-            const float d = z_of[j * R + r] - sum.named_max, q = q_of[j * R + r];
-            s += exp2_of(d * by);
-            if (hard) s1 += exp2_of(d * by1);
-            if (q != 0.f) {
-                cross += q * (log_of(q) - d / temperature);
-                part += q;
+            const int c = class_of[j * kPitch + r] - c0;
+            if (c >= 0 && cell[c * R + r] != kMark + j) class_of[j * kPitch + r] = -1;
+        }
+    }
+    // the sums
+    float most[3] = {kNone, kNone, given};
+    if (on) {
+#pragma unroll 4
+        for (int i = slot; i < size; i += kSlots) {
+            const unsigned v = cell[i * R + r];
+            most[0] = fmaxf(most[0], is_mark(v) ? kNone : __uint_as_float(v));
+        }
+    }
+    for (int j = slot; j < K; j += kSlots)
+        if (class_of[j * kPitch + r] >= 0) most[1] = fmaxf(most[1], z_of[j * kPitch + r]);
+    group.template reduce<3, 2>(most);
+    given = most[2];
+    RowSums sum{};
+    sum.other_max = reference_of(most[0]);
+    sum.named_max = reference_of(most[1]);
+    float s[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (on) {
+#pragma unroll 4
+        for (int i = slot; i < size; i += kSlots) {
+            const unsigned v = cell[i * R + r];
+            const float d = is_mark(v) ? kNone : __uint_as_float(v) - sum.other_max;
+            s[0] += exp2_of(d * by);
+            if (hard) s[1] += exp2_of(d * kLog2e);
+        }
+    }
+    const int label = on ? label_of(call, row) : -1;
+    for (int j = slot; j < K; j += kSlots) {
+        const int c = class_of[j * kPitch + r];
+        if (c < 0) continue;
+        const float z = z_of[j * kPitch + r], d = z - sum.named_max, q = q_of[j * kPitch + r];
+        s[2] += exp2_of(d * by);
+        if (hard) s[3] += exp2_of(d * kLog2e);
+        if (q != 0.f) {
+            s[4] += q * (log_of(q) - d / call.temperature);
+            s[5] += q;
+        }
+        if (c == label) label_score[r] = z;
+    }
+    if (slot == 0 && label >= c0 && label < c0 + size && !is_mark(cell[(label - c0) * R + r])) label_score[r] = __uint_as_float(cell[(label - c0) * R + r]);
+    group.template reduce<6, 0>(s);
+    sum.other_sum = s[0];
+    sum.other_sum1 = s[1];
+    sum.named_sum = s[2];
+    sum.named_sum1 = s[3];
+    sum.cross = s[4];
+    sum.mass = s[5];
+    sum.label = label_score[r];
+    if constexpr (PART == DISTILL_SUMS) {
+        if (on && slot == 0) sums[row * chunks + blockIdx.y] = sum;
+        return;
+    }
+    if constexpr (PART == DISTILL_PAIRS) {
+        // all chunks' sums: a row's threads share them out
+        const RowSums *its = sums + row * chunks;
+        float m[2] = {kNone, kNone};
+        if (on)
+            for (int p = slot; p < chunks; p += kSlots) {
+                if (its[p].other_sum != 0.f) m[0] = fmaxf(m[0], its[p].other_max);
+                if (its[p].named_sum != 0.f) m[1] = fmaxf(m[1], its[p].named_max);
             }
-        }
-        sum.named_sum = over_slots<R, false>(s, room);
-        if (hard) sum.named_sum1 = over_slots<R, false>(s1, room);
-        sum.cross = over_slots<R, false>(cross, room);
-        sum.mass = over_slots<R, false>(part, room);
-        const float y = hard && on ? labels[row] : -1.f;
-        const int label = y >= 0.f && y < (float)in.classes && y == floorf(y) ? (int)y : -1;
-        if (label >= c0 && label < c1) {
-            const unsigned v = cell[(label - c0) * R + r];
-            sum.has_label = 1.f;
-            const float higher = fmaxf(sum.other_sum > 0.f ? sum.other_max : kNone, sum.named_sum > 0.f ? sum.named_max : kNone);
-            sum.label = (is_mark(v) ? z_of[(v - kMark) * R + r] : __uint_as_float(v)) - reference_of(higher);
-        }
-        if constexpr (PART == DISTILL_SUMS) {
-            if (on && slot == 0) sums[row * chunks + tile % chunks] = sum;
-            __syncthreads();
-            continue;
-        }
-        // all chunks' sums
-        ChunkSums all = sum;
-        if constexpr (PART == DISTILL_PAIRS) {
-            all = ChunkSums{};
-            float mo = kNone, mn = kNone;
-            if (on)
-                for (int p = 0; p < chunks; ++p) {
-                    const ChunkSums &a = sums[row * chunks + p];
-                    if (a.other_sum != 0.f) mo = fmaxf(mo, a.other_max);
-                    if (a.named_sum != 0.f) mn = fmaxf(mn, a.named_max);
+        group.template reduce<2, 2>(m);
+        sum.other_max = reference_of(m[0]);
+        sum.named_max = reference_of(m[1]);
+        float a[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l[1] = {0.f};
+        if (on)
+            for (int p = slot; p < chunks; p += kSlots) {
+                const RowSums c = its[p];
+                if (c.other_sum != 0.f) {
+                    a[0] += c.other_sum * exp2_of((c.other_max - sum.other_max) * by);
+                    a[1] += c.other_sum1 * exp2_of((c.other_max - sum.other_max) * kLog2e);
                 }
-            all.other_max = reference_of(mo);
-            all.named_max = reference_of(mn);
-            const float higher = reference_of(fmaxf(mo, mn));
-            if (on)
-                for (int p = 0; p < chunks; ++p) {
-                    const ChunkSums &a = sums[row * chunks + p];
-                    if (a.other_sum != 0.f) {
-                        all.other_sum += a.other_sum * exp2_of((a.other_max - all.other_max) * by);
-                        all.other_sum1 += a.other_sum1 * exp2_of((a.other_max - all.other_max) * by1);
-                    }
-                    if (a.named_sum != 0.f) {
-                        const float d = a.named_max - all.named_max;
-                        all.named_sum += a.named_sum * exp2_of(d * by);
-                        all.named_sum1 += a.named_sum1 * exp2_of(d * by1);
-                    }
-                    if (a.mass != 0.f) {
-                        all.cross += a.cross - a.mass * ((a.named_max - all.named_max) / temperature);
-                        all.mass += a.mass;
-                    }
-                    if (a.has_label != 0.f) {
-                        const float own = fmaxf(a.other_sum > 0.f ? a.other_max : kNone, a.named_sum > 0.f ? a.named_max : kNone);
-                        all.has_label = 1.f;
-                        all.label = a.label + (reference_of(own) - higher);
-                    }
+                if (c.named_sum != 0.f) {
+                    const float d = c.named_max - sum.named_max;
+                    a[2] += c.named_sum * exp2_of(d * by);
+                    a[3] += c.named_sum1 * exp2_of(d * kLog2e);
                 }
-        }
-        // the row: every probability is an exponential to one of the two references times a factor
-        const float no_other = all.other_sum == 0.f ? 1.f : 0.f, no_named = all.named_sum == 0.f ? 1.f : 0.f;
-        const float higher = reference_of(fmaxf(no_other != 0.f ? kNone : all.other_max, no_named != 0.f ? kNone : all.named_max));
-        const float other_up = no_other != 0.f ? 0.f : exp2_of((all.other_max - higher) * by), named_up = no_named != 0.f ? 0.f : exp2_of((all.named_max - higher) * by);
-        const float Z = all.other_sum * other_up + all.named_sum * named_up;
-        const float invZ = inverse_of(Z);
-        const float a = any == 0.f ? 0.f : mass <= FLT_MAX ? weight : __builtin_nanf(""), b = label >= 0 ? 1.f - weight : 0.f;
-        float rest = 0.f;  // the teacher's mass on the other classes
-        if (teacher.lse != nullptr && no_other == 0.f && any != 0.f) rest = fmaxf(0.f, 1.f - mass);
-        const float named_factor = named_up * invZ;                               // p = exp((z - named_max) / T) * it
-        const float other_factor = other_up * invZ;                               // p = exp((z - other_max) / T) * it
-        const float target_factor = rest != 0.f ? rest / all.other_sum : 0.f;       // the teacher's share, likewise
-        float named_factor1 = 0.f, other_factor1 = 0.f, log_Z1 = 0.f;
-        if (hard) {
-            const float other_up1 = no_other != 0.f ? 0.f : exp2_of((all.other_max - higher) * by1);
-            const float named_up1 = no_named != 0.f ? 0.f : exp2_of((all.named_max - higher) * by1);
-            const float Z1 = all.other_sum1 * other_up1 + all.named_sum1 * named_up1;
-            const float invZ1 = inverse_of(Z1);
-            named_factor1 = named_up1 * invZ1;
-            other_factor1 = other_up1 * invZ1;
-            log_Z1 = Z1 != 0.f ? log_of(Z1) : 0.f;
-        }
-        if (loss != nullptr && on && slot == 0 && tile % chunks == 0) {
-            float value = 0.f;
-            if (a != 0.f) {  // (or NaN)
-                const float log_Z = Z != 0.f ? log_of(Z) : 0.f;
-                // log p of a named class = (z - named_max) / T - [log Z + (higher - named_max) / T]
-                float soft = all.mass != 0.f ? all.cross + all.mass * (log_Z + (higher - all.named_max) / temperature) : 0.f;
-                if (rest > 0.f || rest != rest)
-                    soft += rest * (log_of(rest) - (log_of(all.other_sum) + (all.other_max - higher) / temperature - log_Z));
-                value = a * temperature * temperature * soft;
+                if (c.mass != 0.f) {
+                    a[4] += c.cross - c.mass * ((c.named_max - sum.named_max) / call.temperature);
+                    a[5] += c.mass;
+                }
+                if (label >= p * chunk && label < (p + 1) * chunk) l[0] = c.label;
             }
-            if (b != 0.f && all.has_label != 0.f) value += b * (log_Z1 - all.label);
-            loss[given] = value;
+        group.template reduce<6, 0>(a);
+        group.template reduce<1, 0>(l);
+        sum.other_sum = a[0];
+        sum.other_sum1 = a[1];
+        sum.named_sum = a[2];
+        sum.named_sum1 = a[3];
+        sum.cross = a[4];
+        sum.mass = a[5];
+        sum.label = l[0];
+    }
+    if (slot == 0) {
+        float value;
+        factors[r] = factors_of(sum, any, given, call.teacher.lse != nullptr, label, call.temperature, call.weight, &value);
+        if (call.loss != nullptr && on && blockIdx.y == 0) call.loss[given_of(row)] = value;
+    }
+    if (call.pairs == nullptr) return;
+    __syncthreads();
+    if (!on) return;
+    const RowFactors f = factors[r];
+    GHPair *const to = call.pairs + (size_t)c0 * call.pair_stride + row;
+#pragma unroll 2
+    for (int i = slot; i < size; i += kSlots) {
+        const unsigned v = cell[i * R + r];
+        const bool named = is_mark(v);
+        float z = __uint_as_float(v), q = 0.f;
+        if (named) {
+            z = z_of[(v - kMark) * kPitch + r];
+            q = q_of[(v - kMark) * kPitch + r];
         }
-        if (pairs != nullptr) {
-            const float aT = a * temperature;
-            auto put = [&](int c, float p, float target, float p1) {
-                const float g = aT * (p - target) + b * (p1 - (c == label ? 1.f : 0.f));
-                const float h = a * (p * (1.f - p)) + b * (p1 * (1.f - p1));
-                pairs[(size_t)c * pair_stride + row] = GHPair{g, 2.f * h < 1e-16f ? 1e-16f : 2.f * h};  // (NaN stays)
-            };
-            if (on)
-                for (int i = slot; i < c1 - c0; i += kSlots) {
-                    const unsigned v = cell[i * R + r];
-                    if (is_mark(v)) {
-                        const int j = (int)(v - kMark);
-                        const float d = z_of[j * R + r] - all.named_max;
-                        put(c0 + i, exp2_of(d * by) * named_factor, q_of[j * R + r], hard ? exp2_of(d * by1) * named_factor1 : 0.f);
-                    } else {
-                        const float d = __uint_as_float(v) - all.other_max, e = exp2_of(d * by);
-                        put(c0 + i, e * other_factor, e * target_factor, hard ? exp2_of(d * by1) * other_factor1 : 0.f);
-                    }
-                }
-        }
-        __syncthreads();  // (the tile is the next one's)
+        const float d = z - (named ? f.named_max : f.other_max), e = exp2_of(d * by), e1 = hard ? exp2_of(d * kLog2e) : 0.f;
+        const float p = e * (named ? f.named_p : f.other_p), p1 = e1 * (named ? f.named_p1 : f.other_p1);
+        to[(size_t)i * call.pair_stride] = pair_of(f, p, p1, named ? f.aT * (p - q) : e * f.other_g, c0 + i == label);
     }
 }
 
 // How a call goes: rows of a workgroup, chunks of the classes.
 struct DistillPlan {
-    int rows, chunks, chunk;
+    int rows, chunks, chunk;  // rows 0: few classes
     size_t lds;
 };
-constexpr size_t kTileBytes = 76 * 1024;  // two workgroups a CU
+constexpr int kFewClasses = 32;
+constexpr size_t kTileBytes = 72 * 1024;   // two workgroups a CU,
+constexpr size_t kMostBytes = 144 * 1024;  // or one
 
 DistillPlan plan_distill(int classes, int rows, int entries) {
-    auto bytes = [&](int chunk, int r) { return sizeof(float) * (size_t)r * ((size_t)chunk + 2 * (size_t)entries); };
     DistillPlan p{};
-    p.rows = 1;
-    for (int kind : {4, 16})
-        if (kind / 2 < rows) p.rows = kind;
-    for (int kind : {64, 256})
-        if (kind / 2 < rows && bytes(classes, kind) <= kTileBytes) p.rows = kind;
-    const long fit = (long)(kTileBytes / sizeof(float) / p.rows) - 2 * entries;
+    p.chunks = 1;
+    p.chunk = classes;
+    if (classes <= kFewClasses) return p;
+    auto bytes = [&](int chunk, int r) { return sizeof(float) * ((size_t)r * chunk + 3 * (size_t)entries * (r + 1)); };
+    p.rows = rows <= 2 ? 1 : rows <= 8 ? 4 : 16;
+    if (rows > 32 && bytes(classes, 64) <= kTileBytes / 2) p.rows = 64;
     const long row_tiles = ((long)rows - 1) / p.rows + 1;
-    long chunks = bytes(classes, p.rows) <= kTileBytes ? 1 : (classes - 1) / fit + 1;
-    if (row_tiles < 256 && classes > 4096) chunks = std::max(chunks, std::min<long>(512 / row_tiles, (classes - 1) / 1024 + 1));
+    long chunks = 1;
+    if (bytes(classes, p.rows) > kMostBytes) chunks = (classes - 1) / (long)((kTileBytes / sizeof(float) - 3 * (size_t)entries * (p.rows + 1)) / p.rows) + 1;
+    // few rows: their classes are shared out over the chip, 512 at least to a workgroup
+    if (row_tiles < 128 && classes > 2048) chunks = std::max(chunks, std::min<long>(512 / row_tiles, (classes - 1) / 512 + 1));
     p.chunk = (int)((classes - 1) / chunks + 1);
     p.chunks = (classes - 1) / p.chunk + 1;
     p.lds = bytes(p.chunk, p.rows);
     return p;
 }
 
-template <int R, DistillPart PART>
-void distill(hipStream_t s, const DistillPlan &p, const tgbm_scores &in, const tgbm_teacher &teacher, const float *labels, float temperature, float weight,
-             float *loss, GHPair *pairs, long pair_stride, const int *row_of, ChunkSums *sums) {
+template <int R, int B, DistillPart PART>
+void distill_part(hipStream_t s, const DistillPlan &p, const DistillCall &call, RowSums *sums) {
     static LdsOptIn opt_in;
-    opt_in({reinterpret_cast<const void *>(&k_distill<R, PART>)});
-    const long tiles = (((long)in.rows - 1) / R + 1) * p.chunks;
-    k_distill<R, PART><<<(unsigned)std::min(tiles, 1l << 20), kDistillBlock, p.lds, s>>>(in, teacher, labels, temperature, weight, loss, pairs, pair_stride, row_of,
-                                                                                       sums, p.chunks, p.chunk, tiles);
+    opt_in({reinterpret_cast<const void *>(&k_distill<R, B, PART>)});
+    const unsigned tiles = (unsigned)((call.in.rows - 1) / R + 1);
+    // (the loss alone needs one chunk's workgroup to add up)
+    const dim3 grid(R * 4 < 128 ? (tiles + 15) / 16 * 16 : tiles, PART == DISTILL_PAIRS && call.pairs == nullptr ? 1 : p.chunks);
+    k_distill<R, B, PART><<<grid, B, p.lds, s>>>(call, sums, p.chunks, p.chunk);
 }
 
-template <int R>
-void distill_rows(hipStream_t s, const DistillPlan &p, const tgbm_scores &in, const tgbm_teacher &teacher, const float *labels, float temperature, float weight,
-                  float *loss, GHPair *pairs, long pair_stride, const int *row_of, ChunkSums *sums) {
+template <int R, int B>
+void distill_rows(hipStream_t s, const DistillPlan &p, const DistillCall &call, RowSums *sums) {
     if (p.chunks == 1) {
-        distill<R, DISTILL_WHOLE>(s, p, in, teacher, labels, temperature, weight, loss, pairs, pair_stride, row_of, nullptr);
+        distill_part<R, B, DISTILL_WHOLE>(s, p, call, nullptr);
     } else {
-        distill<R, DISTILL_SUMS>(s, p, in, teacher, labels, temperature, weight, nullptr, nullptr, 0, row_of, sums);
-        distill<R, DISTILL_PAIRS>(s, p, in, teacher, labels, temperature, weight, loss, pairs, pair_stride, row_of, sums);
+        distill_part<R, B, DISTILL_SUMS>(s, p, call, sums);
+        distill_part<R, B, DISTILL_PAIRS>(s, p, call, sums);
     }
 }
 
 }  // namespace
 
 size_t scores_distill_workspace(int classes, int rows, int entries) {
+    rows = std::min(rows, kSliceRows);
     const DistillPlan p = plan_distill(classes, rows, entries);
-    return p.chunks == 1 ? 0 : sizeof(ChunkSums) * (size_t)rows * p.chunks;
+    return p.chunks == 1 ? 0 : sizeof(RowSums) * (size_t)rows * p.chunks;
 }
 
 void launch_scores_distill(hipStream_t s, const tgbm_scores &in, const tgbm_teacher &teacher, const float *labels, float temperature, float weight,
                            float *loss, void *pairs, long pair_stride, const int *row_of, void *workspace) {
-    const DistillPlan p = plan_distill(in.classes, in.rows, teacher.entries);
-    if (weight == 1.f) labels = nullptr;
-    GHPair *gh = static_cast<GHPair *>(pairs);
-    ChunkSums *sums = static_cast<ChunkSums *>(workspace);
-    switch (p.rows) {
-        case 1: distill_rows<1>(s, p, in, teacher, labels, temperature, weight, loss, gh, pair_stride, row_of, sums); break;
-        case 4: distill_rows<4>(s, p, in, teacher, labels, temperature, weight, loss, gh, pair_stride, row_of, sums); break;
-        case 16: distill_rows<16>(s, p, in, teacher, labels, temperature, weight, loss, gh, pair_stride, row_of, sums); break;
-        case 64: distill_rows<64>(s, p, in, teacher, labels, temperature, weight, loss, gh, pair_stride, row_of, sums); break;
-        default: distill_rows<256>(s, p, in, teacher, labels, temperature, weight, loss, gh, pair_stride, row_of, sums); break;
+    RowSums *sums = static_cast<RowSums *>(workspace);
+    const size_t score = teacher.type == TGBM_F32 ? 4 : 2;
+    for (int row = 0; row < in.rows; row += std::min(kSliceRows, in.rows - row)) {
+        DistillCall call{in, teacher, weight == 1.f ? nullptr : labels, temperature, weight, loss, static_cast<GHPair *>(pairs), pair_stride, row_of};
+        call.in.data = static_cast<const float *>(in.data) + row;
+        call.in.rows = std::min(kSliceRows, in.rows - row);
+        if (call.labels != nullptr) call.labels += row;
+        if (call.pairs != nullptr) call.pairs += row;
+        if (row_of != nullptr) {
+            call.row_of += row;
+        } else {
+            const size_t first = (size_t)row * teacher.entries;
+            call.teacher.classes += first;
+            call.teacher.scores = static_cast<const char *>(teacher.scores) + first * score;
+            if (teacher.lse != nullptr) call.teacher.lse += row;
+            if (loss != nullptr) call.loss += row;
+        }
+        const DistillPlan p = plan_distill(in.classes, call.in.rows, teacher.entries);
+        const unsigned few = (unsigned)((call.in.rows - 1) / kFewBlock + 1);
+        switch (p.rows) {
+            case 0:
+                if (in.classes <= 8) k_distill_few<8><<<few, kFewBlock, 0, s>>>(call);
+                else if (in.classes <= 16) k_distill_few<16><<<few, kFewBlock, 0, s>>>(call);
+                else k_distill_few<32><<<few, kFewBlock, 0, s>>>(call);
+                break;
+            case 1: distill_rows<1, 1024>(s, p, call, sums); break;
+            case 4: distill_rows<4, 1024>(s, p, call, sums); break;
+            case 16: distill_rows<16, 1024>(s, p, call, sums); break;
+            default: distill_rows<64, 512>(s, p, call, sums); break;
+        }
     }
 }
 
