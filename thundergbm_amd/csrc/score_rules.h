@@ -11,6 +11,14 @@
 namespace tgbm {
 namespace {
 
+// Tiles of less than a cache line of rows: workgroups go to the eight dies in turn, so the two tiles that share their lines go to
+// workgroups that are eight apart, and are read into one L2 (where there are enough of them to fill the dies that way).
+constexpr unsigned kPairedTiles = 256;
+inline unsigned blocks_of_tiles(unsigned tiles) { return tiles < kPairedTiles ? tiles : (tiles + 15) / 16 * 16; }
+__device__ __forceinline__ long tile_of_block(unsigned block, unsigned blocks) {
+    return blocks < kPairedTiles ? block : (block & ~15u) + (block & 7) * 2 + (block >> 3 & 1);
+}
+
 template <typename T>
 __device__ __forceinline__ float score_to_float(T v);
 template <>

@@ -643,8 +643,7 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
     const int r = threadIdx.x & (rows - 1), slot = threadIdx.x >> row_bits, slots = kColumnBlock >> row_bits;
     const long row_tiles = ((in.rows - 1) >> row_bits) + 1;
     const int part = blockIdx.y;
-    // (blocks go to the eight dies in turn: two tiles that share cache lines go to the same one)
-    const long tile = ((long)blockIdx.x & ~15l) + (blockIdx.x & 7) * 2 + (blockIdx.x >> 3 & 1);
+    const long tile = tile_of_block(blockIdx.x, gridDim.x);
     if (tile >= row_tiles) return;
     {
         const long row0 = tile << row_bits, row = row0 + r;
@@ -937,11 +936,10 @@ void top_rows(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm
 
 template <typename T, int E, int M, bool RULES>
 void top_columns(hipStream_t s, const TopPlan &p, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, const TopOut &out) {
-    const long tiles = (((long)((in.rows - 1) >> p.row_bits) + 1) + 15) / 16 * 16;
     const size_t lds = sizeof(unsigned) * ((size_t)p.chunk * ((1 << p.row_bits) + 1) + (rules.shown != nullptr ? (size_t)p.chunk / 32 << p.row_bits : 0));
     static LdsOptIn opt_in;
     opt_in({reinterpret_cast<const void *>(&k_top_columns<T, E, M, RULES>)});
-    const dim3 grid((unsigned)tiles, (unsigned)p.chunks);
+    const dim3 grid(blocks_of_tiles((unsigned)((in.rows - 1) >> p.row_bits) + 1), (unsigned)p.chunks);
     k_top_columns<T, E, M, RULES><<<grid, kColumnBlock, lds, s>>>(in, rules, k, temperature, out, p.chunks, p.chunk, p.row_bits, p.chunks == 1);
 }
 template <typename T, int E, bool RULES>
