@@ -239,7 +239,7 @@ int tgbm_cut_points(int row_size, int n_features, const float *val, const int *r
 
 /* The score of class c in row i is data[c * class_stride + i * row_stride]; one of the strides is 1: row_stride where the
  * rows of a class lie side by side, as trainers and predictors hold them, class_stride where the classes of a row do. 1 to
- * 2^26 classes. */
+ * 2^22 classes. */
 typedef struct tgbm_scores {
     const void *data;
     long long class_stride, row_stride;

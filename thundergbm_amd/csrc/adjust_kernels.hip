@@ -1,5 +1,8 @@
-// tgbm_scores_adjust. One read and one write of every score; the lists of shown classes are counted in LDS, a tile of
-// classes at a time, with integer additions (their order does not change a count).
+// tgbm_scores_adjust. One read and one write of every score, by 16 bytes of a thread: bias and allowed sets. Classes that a row was
+// shown are few, so a second launch goes through the lists: for every class that is in a row's list it counts how often, by integers, and
+// stores the score as computed from its beginning over what the first launch has stored. Where `out` is `in` that beginning is gone by
+// then: there the lists are counted in LDS, tile by tile, in the one launch that goes over the scores (100003 x 500 float32, 64 sets and 20
+// shown classes a row: 274 us that way).
 #include <algorithm>
 
 #include "device_api.h"
@@ -9,101 +12,290 @@ namespace tgbm {
 namespace {
 
 constexpr int kAdjustBlock = 256;
-constexpr int kTileRows = 64;     // rows side by side: a wavefront's lanes are rows,
-constexpr int kTileClasses = 128;  // and a workgroup takes so many classes
-constexpr int kRowClasses = 8192;  // classes side by side: classes of a row that a workgroup takes
 
-// Rows side by side. Tiles are row tiles * class tiles, and a workgroup takes every gridDim.x-th one.
+template <typename T, int N>
+struct ScoreVector {  // side by side, on any address of a score
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ bool is_in_set(const unsigned *words, bool none, int c) { return !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u)); }
+
+// ---------------------------------------------------------------------------------------------- bias and allowed sets
+// Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side.
+// ALONG: out is in the same order.
+template <typename T, bool ALONG>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int quad_bits) {
+    using V = typename ScoreVector<T, 4>::type;
+    const int lane = threadIdx.x & 63, step = 64 >> quad_bits;
+    const int g = ((int)blockIdx.y * (kAdjustBlock / 64) + (int)(threadIdx.x >> 6)) * 32, end = std::min(g + 32, in.classes);
+    const long row = (((long)blockIdx.x << quad_bits) + (lane & ((1 << quad_bits) - 1))) * 4;
+    const int live = (int)std::min(4l, in.rows - row);
+    if (g >= in.classes || live <= 0) return;
+    unsigned ok[4] = {~0u, ~0u, ~0u, ~0u};
+    if (rules.allowed != nullptr) {
+        const int set_words = (in.classes + 31) / 32;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bool none;
+            const unsigned *words = allowed_words(rules, std::min(row + j, (long)in.rows - 1), set_words, &none);
+            ok[j] = none ? 0u : words != nullptr ? words[g / 32] : ~0u;
+        }
+    }
+    int c = g + (lane >> quad_bits);
+    const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
+    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
+    if (ALONG && live == 4) {
+        constexpr int kAtOnce = 8;
+        for (; c < end; c += kAtOnce * step) {
+            V x[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (c + u * step < end) x[u] = *reinterpret_cast<const V *>(from);
+                from += (size_t)step * in.class_stride;
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (c + u * step < end) {
+                    const float bias = rules.bias != nullptr ? rules.bias[c + u * step] : 0.f;
+                    V v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (c + u * step - g) & 1u ? score_to_float(x[u][j]) + bias : -__builtin_inff());
+                    *reinterpret_cast<V *>(to) = v;
+                }
+                to += (size_t)step * out.class_stride;
+            }
+        }
+    } else {
+        for (; c < end; c += step) {
+            const float bias = rules.bias != nullptr ? rules.bias[c] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < live) to[(size_t)j * out.row_stride] = (T)(ok[j] >> (c - g) & 1u ? score_to_float(from[j]) + bias : -__builtin_inff());
+            from += (size_t)step * in.class_stride;
+            to += (size_t)step * out.class_stride;
+        }
+    }
+}
+
+// Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them.
+constexpr int kRowVectors = 4;
+template <typename T, bool ALONG>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int row_bits) {
+    constexpr int kOf = 16 / (int)sizeof(T);
+    using V = typename ScoreVector<T, kOf>::type;
+    const int per_row = 1 << row_bits, at = threadIdx.x & (per_row - 1), step = per_row * kOf;
+    const long row = (long)blockIdx.x * (kAdjustBlock >> row_bits) + (threadIdx.x >> row_bits);
+    if (row >= in.rows) return;
+    const int c0 = (int)blockIdx.y * kRowVectors * step, c1 = std::min(in.classes, c0 + kRowVectors * step), whole = c0 + (c1 - c0) / kOf * kOf;
+    const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
+    T *dst = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    const int c = c0 + at * kOf;
+    V x[kRowVectors];
+    if constexpr (ALONG) {
+#pragma unroll
+        for (int u = 0; u < kRowVectors; ++u)
+            if (c + u * step < whole) x[u] = *reinterpret_cast<const V *>(src + c + u * step);
+#pragma unroll
+        for (int u = 0; u < kRowVectors; ++u) {
+            const int cu = c + u * step;
+            if (cu >= whole) break;
+            const unsigned ok = none ? 0u : words != nullptr ? words[cu / 32] >> (cu % 32) : ~0u;
+            V v;
+#pragma unroll
+            for (int j = 0; j < kOf; j += 4) {
+                Float4 bias = {0.f, 0.f, 0.f, 0.f};
+                if (rules.bias != nullptr) bias = *reinterpret_cast<const Float4 *>(rules.bias + cu + j);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[j + q] = (T)(ok >> (j + q) & 1u ? score_to_float(x[u][j + q]) + bias[q] : -__builtin_inff());
+            }
+            *reinterpret_cast<V *>(dst + cu) = v;
+        }
+    }
+    for (int o = (ALONG ? whole : c0) + at; o < c1; o += per_row) {
+        const float z = score_to_float(src[o]) + (rules.bias != nullptr ? rules.bias[o] : 0.f);
+        dst[(size_t)o * out.class_stride] = (T)(is_in_set(words, none, o) ? z : -__builtin_inff());
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- shown classes
+// The score of class c of a row that was shown it `times` times, from its beginning.
 template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int class_tiles, long tiles) {
+__device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row, int c, unsigned times) {
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    const float z = score_to_float(static_cast<const T *>(in.data)[(size_t)c * in.class_stride + (size_t)row * in.row_stride]);
+    static_cast<T *>(const_cast<void *>(out.data))[(size_t)c * out.class_stride + (size_t)row * out.row_stride] =
+        (T)adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, times, is_in_set(words, none, c), rules);
+}
+
+// Short lists: a thread takes an entry of the lists of 64 rows and looks through the entry's list for others of its class. The first one stores.
+constexpr int kListRows = 64;
+template <typename T>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
+    __shared__ long long begin[kListRows];
+    __shared__ long long before[kListRows + 1];  // entries of the rows before
+    const long row0 = (long)blockIdx.x * kListRows;
+    if (threadIdx.x < 64) {
+        long long b = 0, e = 0;
+        if (row0 + threadIdx.x < in.rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
+        long long sum = e - b;
+        begin[threadIdx.x] = b;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long o = __shfl_up(sum, d);
+            if ((int)threadIdx.x >= d) sum += o;
+        }
+        before[threadIdx.x + 1] = sum;
+        if (threadIdx.x == 0) before[0] = 0;
+    }
+    __syncthreads();
+    for (long long i = threadIdx.x; i < before[kListRows]; i += kAdjustBlock) {
+        int r = 0;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            if (before[r + d] <= i) r += d;
+        const int *list = rules.shown + begin[r];
+        const long long mine = i - before[r], length = before[r + 1] - before[r];
+        const int c = list[mine];
+        if (c < 0 || c >= in.classes) continue;
+        unsigned times = 0;
+        bool first = true;
+        for (long long o = 0; o < length; ++o) {
+            const bool same = list[o] == c;
+            times += same ? 1u : 0u;
+            first = first && !(same && o < mine);
+        }
+        if (first) store_held_back<T>(in, rules, out, row0 + r, c, times);
+    }
+}
+
+// Long lists: a workgroup takes a row and kTableClasses classes, counts them in LDS, and whoever takes a count away stores.
+constexpr int kTableClasses = 8192;
+template <typename T>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_long_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
+    __shared__ unsigned times[kTableClasses];
+    const long row = blockIdx.x;
+    const int c0 = (int)blockIdx.y * kTableClasses, size = std::min(in.classes - c0, kTableClasses);
+    long long b, e;
+    shown_range(rules, row, &b, &e);
+    if (b >= e) return;
+    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
+        const int c = rules.shown[i] - c0;
+        if ((unsigned)c < (unsigned)size) times[c] = 0;
+    }
+    __syncthreads();
+    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
+        const int c = rules.shown[i] - c0;
+        if ((unsigned)c < (unsigned)size) atomicAdd(&times[c], 1u);
+    }
+    __syncthreads();
+    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
+        const int c = rules.shown[i] - c0;
+        if ((unsigned)c >= (unsigned)size) continue;
+        const unsigned n = atomicExch(&times[c], 0u);
+        if (n != 0) store_held_back<T>(in, rules, out, row, c0 + c, n);
+    }
+}
+
+// In place: a workgroup takes 64 rows and 128 classes (rows side by side), or 2^row_bits threads a row and up to kTableClasses classes of it.
+constexpr int kTileRows = 64, kTileClasses = 128;
+template <typename T>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns_in_place(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
     __shared__ unsigned times[kTileClasses * kTileRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const long row = tile / class_tiles * kTileRows + lane;
-        const int c0 = (int)(tile % class_tiles) * kTileClasses;
-        const int c1 = row < in.rows ? min(in.classes, c0 + kTileClasses) : c0;
-        if (rules.shown != nullptr) {
-            for (int i = threadIdx.x; i < kTileClasses * kTileRows; i += kAdjustBlock) times[i] = 0;
-            __syncthreads();
-            // four threads a row
-            long long b = 0, e = 0;
-            if (row < in.rows) shown_range(rules, row, &b, &e);
-            for (long long i = b + wave; i < e; i += kAdjustBlock / 64) {
-                const int c = rules.shown[i];
-                if (c >= c0 && c < c1) atomicAdd(&times[(c - c0) * kTileRows + lane], 1u);
-            }
-            __syncthreads();
-        }
-        if (row < in.rows) {
-            bool none;
-            const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-            const T *src = static_cast<const T *>(in.data);
-            T *dst = static_cast<T *>(const_cast<void *>(out.data));
-            for (int c = c0 + wave; c < c1; c += kAdjustBlock / 64) {
-                const float z = score_to_float(src[(size_t)c * in.class_stride + row]);
-                const bool ok = !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u));
-                const float v = adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f,
-                                         rules.shown != nullptr ? times[(c - c0) * kTileRows + lane] : 0u, ok, rules);
-                dst[(size_t)c * out.class_stride + (size_t)row * out.row_stride] = (T)v;
-            }
-        }
-        __syncthreads();  // (the counts are cleared for the next tile)
+    const long row = (long)blockIdx.x * kTileRows + lane;
+    const int c0 = (int)blockIdx.y * kTileClasses, c1 = row < in.rows ? std::min(in.classes, c0 + kTileClasses) : c0;
+    for (int i = threadIdx.x; i < kTileClasses * kTileRows; i += kAdjustBlock) times[i] = 0;
+    __syncthreads();
+    long long b = 0, e = 0;
+    if (row < in.rows) shown_range(rules, row, &b, &e);
+    for (long long i = b + wave; i < e; i += kAdjustBlock / 64) {
+        const int c = rules.shown[i];
+        if (c >= c0 && c < c1) atomicAdd(&times[(c - c0) * kTileRows + lane], 1u);
+    }
+    __syncthreads();
+    if (row >= in.rows) return;
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    T *at = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
+    for (int c = c0 + wave; c < c1; c += kAdjustBlock / 64) {
+        T *z = at + (size_t)c * out.class_stride;
+        *z = (T)adjusted(score_to_float(*z), rules.bias != nullptr ? rules.bias[c] : 0.f, times[(c - c0) * kTileRows + lane], is_in_set(words, none, c), rules);
     }
 }
-
-// Classes side by side. Short rows share a workgroup: 2^row_bits threads each, up to eight classes a thread. Tiles are
-// row groups * chunks, and a workgroup takes every gridDim.x-th one.
 template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int row_bits, int chunks,
-                                                              long tiles) {
-    __shared__ unsigned times_of[kRowClasses];
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows_in_place(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int row_bits) {
+    __shared__ unsigned times_of[kTableClasses];
     const int per_row = 1 << row_bits, at = threadIdx.x & (per_row - 1), slot = threadIdx.x >> row_bits;
-    unsigned *times = times_of + (size_t)slot * min(in.classes, kRowClasses);
-    for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const long row = tile / chunks * (kAdjustBlock >> row_bits) + slot;
-        const int c0 = (int)(tile % chunks) * kRowClasses;
-        const int c1 = row < in.rows ? min(in.classes, c0 + kRowClasses) : c0;
-        if (rules.shown != nullptr) {
-            long long b = 0, e = 0;
-            if (row < in.rows) shown_range(rules, row, &b, &e);
-            for (int c = c0 + at; c < c1; c += per_row) times[c - c0] = 0;
-            __syncthreads();
-            for (long long i = b + at; i < e; i += per_row) {
-                const int c = rules.shown[i];
-                if (c >= c0 && c < c1) atomicAdd(&times[c - c0], 1u);
-            }
-            __syncthreads();
-        }
-        if (row < in.rows) {
-            bool none;
-            const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-            const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
-            T *dst = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
-            for (int c = c0 + at; c < c1; c += per_row) {
-                const float z = score_to_float(src[c]);
-                const bool ok = !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u));
-                const float v = adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, rules.shown != nullptr ? times[c - c0] : 0u, ok, rules);
-                dst[(size_t)c * out.class_stride] = (T)v;
-            }
-        }
-        __syncthreads();  // (the counts are cleared for the next tile)
+    unsigned *times = times_of + (size_t)slot * std::min(in.classes, kTableClasses);
+    const long row = (long)blockIdx.x * (kAdjustBlock >> row_bits) + slot;
+    const int c0 = (int)blockIdx.y * kTableClasses, c1 = row < in.rows ? std::min(in.classes, c0 + kTableClasses) : c0;
+    long long b = 0, e = 0;
+    if (row < in.rows) shown_range(rules, row, &b, &e);
+    for (int c = c0 + at; c < c1; c += per_row) times[c - c0] = 0;
+    __syncthreads();
+    for (long long i = b + at; i < e; i += per_row) {
+        const int c = rules.shown[i];
+        if (c >= c0 && c < c1) atomicAdd(&times[c - c0], 1u);
     }
+    __syncthreads();
+    if (row >= in.rows) return;
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
+    for (int c = c0 + at; c < c1; c += per_row)
+        to[c] = (T)adjusted(score_to_float(to[c]), rules.bias != nullptr ? rules.bias[c] : 0.f, times[c - c0], is_in_set(words, none, c), rules);
 }
 
-unsigned grid_of(long tiles) { return (unsigned)std::min(tiles, 1l << 20); }
+template <typename T, bool ALONG>
+void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out) {
+    const bool columns = rows_side_by_side(in);
+    if (rules.shown != nullptr && in.data == out.data) {
+        if (columns) {
+            const dim3 grid((in.rows - 1) / kTileRows + 1, (in.classes - 1) / kTileClasses + 1);
+            k_adjust_columns_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
+        } else {
+            int row_bits = 3;
+            while (row_bits < 8 && (8 << row_bits) < in.classes) ++row_bits;
+            const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / kTableClasses + 1);
+            k_adjust_rows_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
+        }
+        return;
+    }
+    if (columns) {
+        const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 ? 4 : 6;
+        const dim3 grid((in.rows - 1) / (4 << quad_bits) + 1, (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
+        k_adjust_columns<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
+    } else {
+        constexpr int kOf = 16 / (int)sizeof(T);
+        int row_bits = 2;
+        while (row_bits < 8 && (kRowVectors * kOf << row_bits) < in.classes) ++row_bits;
+        const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / (kRowVectors * kOf << row_bits) + 1);
+        k_adjust_rows<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
+    }
+    if (rules.shown == nullptr) return;
+    // an entry is compared with its whole list below, which costs as much as a table for some
+    constexpr int kShort = 96;
+    if (rules.n_shown <= (long long)kShort * in.rows) {
+        k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
+    } else {
+        k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
+    }
+}
 
 template <typename T>
 void adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out) {
-    if (rows_side_by_side(in)) {
-        const int class_tiles = (in.classes - 1) / kTileClasses + 1;
-        const long tiles = (long)class_tiles * ((in.rows - 1) / kTileRows + 1);
-        k_adjust_columns<T><<<grid_of(tiles), kAdjustBlock, 0, s>>>(in, rules, out, class_tiles, tiles);
-    } else {
-        int row_bits = 3;
-        while (row_bits < 8 && (8 << row_bits) < in.classes) ++row_bits;
-        const int chunks = (in.classes - 1) / kRowClasses + 1;
-        const long tiles = (long)chunks * ((in.rows - 1) / (kAdjustBlock >> row_bits) + 1);
-        k_adjust_rows<T><<<grid_of(tiles), kAdjustBlock, 0, s>>>(in, rules, out, row_bits, chunks, tiles);
+    const bool along = rows_side_by_side(in) ? out.row_stride == 1 : out.class_stride == 1;
+    for (int row = 0; row < in.rows; row += std::min(kSliceRows, in.rows - row)) {
+        tgbm_scores from = in, to = out;
+        tgbm_score_rules r = rules, unused = tgbm_score_rules{};
+        take_rows(from, r, row, std::min(kSliceRows, in.rows - row));
+        take_rows(to, unused, row, from.rows);
+        if (along) adjust_slice<T, true>(s, from, r, to);
+        else adjust_slice<T, false>(s, from, r, to);
     }
 }
 

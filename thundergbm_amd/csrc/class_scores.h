@@ -13,7 +13,7 @@
 
 namespace tgbm {
 
-constexpr int kClassesMost = 1 << 26;
+constexpr int kClassesMost = 1 << 22;  // (the tiles of a row are one direction of a launch: at most 65 535)
 constexpr int kSliceRows = 1 << 22;  // rows of a launch
 constexpr int kTopMost = 128;      // classes that top lists
 constexpr int kTeacherMost = 128;  // entries of a teacher's row

@@ -66,7 +66,7 @@ def _scores(torch, name, x):
         raise ValueError("%s: [classes, rows] is wanted, got %d dimensions" % (name, x.dim()))
     classes, rows = x.shape
     by_class, by_row = x.stride()
-    if classes < 1 or classes > 1 << 26 or rows >= 1 << 31:
+    if classes < 1 or classes > 1 << 22 or rows >= 1 << 31:
         raise ValueError("%s: %d classes, %d rows" % (name, classes, rows))
     if classes == 1:  # (the stride along a single class says nothing)
         by_class = max(by_class, rows, 1) if by_row == 1 else 1
