@@ -131,49 +131,83 @@ __device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgb
         (T)adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, times, is_in_set(words, none, c), rules);
 }
 
-// Short lists: a thread takes an entry of the lists of 64 rows and looks through the entry's list for others of its class. The first one stores.
-constexpr int kListRows = 64;
+// Short lists: a thread takes an entry of the lists of kListRows rows, brought into LDS where they fit, and looks through the entry's list for
+// others of its class. The first one stores.
+constexpr int kListRows = 16, kStaged = 4096;
 template <typename T>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
     __shared__ long long begin[kListRows];
     __shared__ long long before[kListRows + 1];  // entries of the rows before
+    __shared__ int staged[kStaged + 4];
     const long row0 = (long)blockIdx.x * kListRows;
     if (threadIdx.x < 64) {
         long long b = 0, e = 0;
-        if (row0 + threadIdx.x < in.rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
+        if (threadIdx.x < kListRows && row0 + threadIdx.x < in.rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
         long long sum = e - b;
-        begin[threadIdx.x] = b;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
+        for (int d = 1; d < kListRows; d <<= 1) {
             const long long o = __shfl_up(sum, d);
             if ((int)threadIdx.x >= d) sum += o;
         }
-        before[threadIdx.x + 1] = sum;
+        if (threadIdx.x < kListRows) {
+            begin[threadIdx.x] = b;
+            before[threadIdx.x + 1] = sum;
+        }
         if (threadIdx.x == 0) before[0] = 0;
     }
     __syncthreads();
-    for (long long i = threadIdx.x; i < before[kListRows]; i += kAdjustBlock) {
+    const long long total = before[kListRows];
+    auto row_of = [&](long long i) {
         int r = 0;
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1)
+        for (int d = kListRows / 2; d > 0; d >>= 1)
             if (before[r + d] <= i) r += d;
+        return r;
+    };
+    if (total <= kStaged) {
+        const int n = (int)total;
+        for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
+            const int r = row_of(i);
+            staged[i] = rules.shown[begin[r] + (i - (int)before[r])];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
+            const int r = row_of(i), first = (int)before[r], last = (int)before[r + 1], c = staged[i];
+            if (c < 0 || c >= in.classes) continue;
+            unsigned times = 0;
+            bool earlier = false;
+            for (int o = first; o < last; o += 4) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {  // (up to three places behind the list may be looked at, and do not count)
+                    const bool same = staged[o + u] == c && o + u < last;
+                    times += same ? 1u : 0u;
+                    earlier |= same && o + u < i;
+                }
+            }
+            if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
+        }
+        return;
+    }
+    for (long long i = threadIdx.x; i < total; i += kAdjustBlock) {
+        const int r = row_of(i);
         const int *list = rules.shown + begin[r];
         const long long mine = i - before[r], length = before[r + 1] - before[r];
         const int c = list[mine];
         if (c < 0 || c >= in.classes) continue;
         unsigned times = 0;
-        bool first = true;
+        bool earlier = false;
         for (long long o = 0; o < length; ++o) {
             const bool same = list[o] == c;
             times += same ? 1u : 0u;
-            first = first && !(same && o < mine);
+            earlier |= same && o < mine;
         }
-        if (first) store_held_back<T>(in, rules, out, row0 + r, c, times);
+        if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
     }
 }
 
-// Long lists: a workgroup takes a row and kTableClasses classes, counts them in LDS, and whoever takes a count away stores.
-constexpr int kTableClasses = 8192;
+// Long lists: a workgroup takes a row and kTableClasses classes, counts them in LDS, and whoever takes a count away stores. A thread keeps its
+// first entries: the list is gone through three times, and every load is waited for.
+constexpr int kTableClasses = 8192, kKept = 8;
 template <typename T>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_long_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
     __shared__ unsigned times[kTableClasses];
@@ -182,22 +216,30 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_long_lists(tgbm_scores 
     long long b, e;
     shown_range(rules, row, &b, &e);
     if (b >= e) return;
-    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
-        const int c = rules.shown[i] - c0;
-        if ((unsigned)c < (unsigned)size) times[c] = 0;
+    int kept[kKept];  // (-1: none of this workgroup's)
+#pragma unroll
+    for (int u = 0; u < kKept; ++u) {
+        const long long i = b + threadIdx.x + u * kAdjustBlock;
+        const int c = i < e ? rules.shown[i] - c0 : -1;
+        kept[u] = (unsigned)c < (unsigned)size ? c : -1;
     }
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < kKept; ++u)
+            if (kept[u] >= 0) f(kept[u]);
+        for (long long i = b + threadIdx.x + kKept * kAdjustBlock; i < e; i += kAdjustBlock) {
+            const int c = rules.shown[i] - c0;
+            if ((unsigned)c < (unsigned)size) f(c);
+        }
+    };
+    each([&](int c) { times[c] = 0; });
     __syncthreads();
-    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
-        const int c = rules.shown[i] - c0;
-        if ((unsigned)c < (unsigned)size) atomicAdd(&times[c], 1u);
-    }
+    each([&](int c) { atomicAdd(&times[c], 1u); });
     __syncthreads();
-    for (long long i = b + threadIdx.x; i < e; i += kAdjustBlock) {
-        const int c = rules.shown[i] - c0;
-        if ((unsigned)c >= (unsigned)size) continue;
+    each([&](int c) {
         const unsigned n = atomicExch(&times[c], 0u);
         if (n != 0) store_held_back<T>(in, rules, out, row, c0 + c, n);
-    }
+    });
 }
 
 // In place: a workgroup takes 64 rows and 128 classes (rows side by side), or 2^row_bits threads a row and up to kTableClasses classes of it.
