@@ -4,6 +4,7 @@
 // then: there the lists are counted in LDS, tile by tile, in the one launch that goes over the scores (100003 x 500 float32, 64 sets and 20
 // shown classes a row: 274 us that way).
 #include <algorithm>
+#include <type_traits>
 
 #include "device_api.h"
 #include "score_rules.h"
@@ -21,60 +22,176 @@ typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ bool is_in_set(const unsigned *words, bool none, int c) { return !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u)); }
 
-// ---------------------------------------------------------------------------------------------- bias and allowed sets
-// Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side.
-// ALONG: out is in the same order.
-template <typename T, bool ALONG>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int quad_bits) {
-    using V = typename ScoreVector<T, 4>::type;
-    const int lane = threadIdx.x & 63, step = 64 >> quad_bits;
-    const int g = ((int)blockIdx.y * (kAdjustBlock / 64) + (int)(threadIdx.x >> 6)) * 32, end = std::min(g + 32, in.classes);
-    const long row = (((long)blockIdx.x << quad_bits) + (lane & ((1 << quad_bits) - 1))) * 4;
-    const int live = (int)std::min(4l, in.rows - row);
-    if (g >= in.classes || live <= 0) return;
-    unsigned ok[4] = {~0u, ~0u, ~0u, ~0u};
-    if (rules.allowed != nullptr) {
-        const int set_words = (in.classes + 31) / 32;
+// ------------------------------------------------------------------------------------------------------- shown classes
+// The score of class c of a row that was shown it `times` times, from its beginning.
+template <typename T>
+__device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row, int c, unsigned times) {
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    const float z = score_to_float(static_cast<const T *>(in.data)[(size_t)c * in.class_stride + (size_t)row * in.row_stride]);
+    static_cast<T *>(const_cast<void *>(out.data))[(size_t)c * out.class_stride + (size_t)row * out.row_stride] =
+        (T)adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, times, is_in_set(words, none, c), rules);
+}
+
+// The lists of ROWS rows, one behind the other, in LDS where they fit. A thread takes an entry and looks through the entry's list for others of its
+// class; the first one stores. All threads of the workgroup come to stage(), and to a barrier before store().
+constexpr int kStaged = 4096;
+template <int ROWS>
+struct ShortLists {
+    static_assert(ROWS <= 64);
+    long long begin[ROWS];
+    long long before[ROWS + 1];  // entries of the rows before
+    int staged[kStaged + 4];
+
+    __device__ __forceinline__ int row_of(long long i) const {
+        int r = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            bool none;
-            const unsigned *words = allowed_words(rules, std::min(row + j, (long)in.rows - 1), set_words, &none);
-            ok[j] = none ? 0u : words != nullptr ? words[g / 32] : ~0u;
+        for (int d = ROWS / 2; d > 0; d >>= 1)
+            if (before[r + d] <= i) r += d;
+        return r;
+    }
+    __device__ __forceinline__ void stage(const tgbm_score_rules &rules, long row0, int rows) {
+        if (threadIdx.x < 64) {
+            long long b = 0, e = 0;
+            if (threadIdx.x < ROWS && row0 + threadIdx.x < rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
+            long long sum = e - b;
+#pragma unroll
+            for (int d = 1; d < ROWS; d <<= 1) {
+                const long long o = __shfl_up(sum, d);
+                if ((int)threadIdx.x >= d) sum += o;
+            }
+            if (threadIdx.x < ROWS) {
+                begin[threadIdx.x] = b;
+                before[threadIdx.x + 1] = sum;
+            }
+            if (threadIdx.x == 0) before[0] = 0;
+        }
+        __syncthreads();
+        if (before[ROWS] <= kStaged)
+            for (int i = threadIdx.x; i < (int)before[ROWS]; i += kAdjustBlock) {
+                const int r = row_of(i);
+                staged[i] = rules.shown[begin[r] + (i - (int)before[r])];
+            }
+    }
+    // of the classes [c0, c1)
+    template <typename T>
+    __device__ __forceinline__ void store(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) const {
+        const long long total = before[ROWS];
+        if (total <= kStaged) {
+            const int n = (int)total;
+            for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
+                const int c = staged[i];
+                if (c < c0 || c >= c1) continue;
+                const int r = row_of(i), first = (int)before[r], last = (int)before[r + 1];
+                unsigned times = 0;
+                bool earlier = false;
+                for (int o = first; o < last; o += 4) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {  // (up to three places behind the list may be looked at, and do not count)
+                        const bool same = staged[o + u] == c && o + u < last;
+                        times += same ? 1u : 0u;
+                        earlier |= same && o + u < i;
+                    }
+                }
+                if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
+            }
+            return;
+        }
+        for (long long i = threadIdx.x; i < total; i += kAdjustBlock) {
+            const int r = row_of(i);
+            const int *list = rules.shown + begin[r];
+            const long long mine = i - before[r], length = before[r + 1] - before[r];
+            const int c = list[mine];
+            if (c < c0 || c >= c1) continue;
+            unsigned times = 0;
+            bool earlier = false;
+            for (long long o = 0; o < length; ++o) {
+                const bool same = list[o] == c;
+                times += same ? 1u : 0u;
+                earlier |= same && o < mine;
+            }
+            if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
         }
     }
-    int c = g + (lane >> quad_bits);
-    const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
-    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
-    if (ALONG && live == 4) {
-        constexpr int kAtOnce = 8;
-        for (; c < end; c += kAtOnce * step) {
-            V x[kAtOnce];
+};
+
+constexpr int kListRows = 16;
+template <typename T>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
+    __shared__ ShortLists<kListRows> lists;
+    const long row0 = (long)blockIdx.x * kListRows;
+    lists.stage(rules, row0, in.rows);
+    __syncthreads();
+    lists.store<T>(in, rules, out, row0, 0, in.classes);
+}
+
+// ---------------------------------------------------------------------------------------------- bias and allowed sets
+// Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side.
+// ALONG: out is in the same order. LISTS (quad_bits is 4): the workgroup's part of short lists is stored behind it, while the lines that it touches are in
+// the L2: read and written again by a launch of its own, 20 entries a row of 500 classes took 72 us, with 108 for the scores.
+template <typename T, bool ALONG, bool LISTS>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int quad_bits) {
+    using V = typename ScoreVector<T, 4>::type;
+    __shared__ typename std::conditional<LISTS, ShortLists<64>, char>::type lists;
+    const long tile = tile_of_block(blockIdx.x, gridDim.x);
+    if constexpr (LISTS) {
+        quad_bits = 4;
+        lists.stage(rules, tile * 64, in.rows);
+    }
+    const int lane = threadIdx.x & 63, step = 64 >> quad_bits;
+    const int g = ((int)blockIdx.y * (kAdjustBlock / 64) + (int)(threadIdx.x >> 6)) * 32, end = std::min(g + 32, in.classes);
+    const long row = ((tile << quad_bits) + (lane & ((1 << quad_bits) - 1))) * 4;
+    const int live = (int)std::min(4l, in.rows - row);
+    if (g < in.classes && live > 0) {
+        unsigned ok[4] = {~0u, ~0u, ~0u, ~0u};
+        if (rules.allowed != nullptr) {
+            const int set_words = (in.classes + 31) / 32;
 #pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                if (c + u * step < end) x[u] = *reinterpret_cast<const V *>(from);
-                from += (size_t)step * in.class_stride;
+            for (int j = 0; j < 4; ++j) {
+                bool none;
+                const unsigned *words = allowed_words(rules, std::min(row + j, (long)in.rows - 1), set_words, &none);
+                ok[j] = none ? 0u : words != nullptr ? words[g / 32] : ~0u;
             }
+        }
+        int c = g + (lane >> quad_bits);
+        const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
+        T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
+        if (ALONG && live == 4) {
+            constexpr int kAtOnce = 8;
+            for (; c < end; c += kAtOnce * step) {
+                V x[kAtOnce];
 #pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-                if (c + u * step < end) {
-                    const float bias = rules.bias != nullptr ? rules.bias[c + u * step] : 0.f;
-                    V v;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (c + u * step - g) & 1u ? score_to_float(x[u][j]) + bias : -__builtin_inff());
-                    *reinterpret_cast<V *>(to) = v;
+                for (int u = 0; u < kAtOnce; ++u) {
+                    if (c + u * step < end) x[u] = *reinterpret_cast<const V *>(from);
+                    from += (size_t)step * in.class_stride;
                 }
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    if (c + u * step < end) {
+                        const float bias = rules.bias != nullptr ? rules.bias[c + u * step] : 0.f;
+                        V v;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (c + u * step - g) & 1u ? score_to_float(x[u][j]) + bias : -__builtin_inff());
+                        *reinterpret_cast<V *>(to) = v;
+                    }
+                    to += (size_t)step * out.class_stride;
+                }
+            }
+        } else {
+            for (; c < end; c += step) {
+                const float bias = rules.bias != nullptr ? rules.bias[c] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < live) to[(size_t)j * out.row_stride] = (T)(ok[j] >> (c - g) & 1u ? score_to_float(from[j]) + bias : -__builtin_inff());
+                from += (size_t)step * in.class_stride;
                 to += (size_t)step * out.class_stride;
             }
         }
-    } else {
-        for (; c < end; c += step) {
-            const float bias = rules.bias != nullptr ? rules.bias[c] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < live) to[(size_t)j * out.row_stride] = (T)(ok[j] >> (c - g) & 1u ? score_to_float(from[j]) + bias : -__builtin_inff());
-            from += (size_t)step * in.class_stride;
-            to += (size_t)step * out.class_stride;
-        }
+    }
+    if constexpr (LISTS) {
+        __syncthreads();
+        const int c0 = (int)blockIdx.y * (kAdjustBlock / 64 * 32);
+        lists.template store<T>(in, rules, out, tile * 64, c0, std::min(in.classes, c0 + kAdjustBlock / 64 * 32));
     }
 }
 
@@ -117,91 +234,6 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows(tgbm_scores in, tg
     for (int o = (ALONG ? whole : c0) + at; o < c1; o += per_row) {
         const float z = score_to_float(src[o]) + (rules.bias != nullptr ? rules.bias[o] : 0.f);
         dst[(size_t)o * out.class_stride] = (T)(is_in_set(words, none, o) ? z : -__builtin_inff());
-    }
-}
-
-// ------------------------------------------------------------------------------------------------------- shown classes
-// The score of class c of a row that was shown it `times` times, from its beginning.
-template <typename T>
-__device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row, int c, unsigned times) {
-    bool none;
-    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-    const float z = score_to_float(static_cast<const T *>(in.data)[(size_t)c * in.class_stride + (size_t)row * in.row_stride]);
-    static_cast<T *>(const_cast<void *>(out.data))[(size_t)c * out.class_stride + (size_t)row * out.row_stride] =
-        (T)adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, times, is_in_set(words, none, c), rules);
-}
-
-// Short lists: a thread takes an entry of the lists of kListRows rows, brought into LDS where they fit, and looks through the entry's list for
-// others of its class. The first one stores.
-constexpr int kListRows = 16, kStaged = 4096;
-template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
-    __shared__ long long begin[kListRows];
-    __shared__ long long before[kListRows + 1];  // entries of the rows before
-    __shared__ int staged[kStaged + 4];
-    const long row0 = (long)blockIdx.x * kListRows;
-    if (threadIdx.x < 64) {
-        long long b = 0, e = 0;
-        if (threadIdx.x < kListRows && row0 + threadIdx.x < in.rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
-        long long sum = e - b;
-#pragma unroll
-        for (int d = 1; d < kListRows; d <<= 1) {
-            const long long o = __shfl_up(sum, d);
-            if ((int)threadIdx.x >= d) sum += o;
-        }
-        if (threadIdx.x < kListRows) {
-            begin[threadIdx.x] = b;
-            before[threadIdx.x + 1] = sum;
-        }
-        if (threadIdx.x == 0) before[0] = 0;
-    }
-    __syncthreads();
-    const long long total = before[kListRows];
-    auto row_of = [&](long long i) {
-        int r = 0;
-#pragma unroll
-        for (int d = kListRows / 2; d > 0; d >>= 1)
-            if (before[r + d] <= i) r += d;
-        return r;
-    };
-    if (total <= kStaged) {
-        const int n = (int)total;
-        for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
-            const int r = row_of(i);
-            staged[i] = rules.shown[begin[r] + (i - (int)before[r])];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
-            const int r = row_of(i), first = (int)before[r], last = (int)before[r + 1], c = staged[i];
-            if (c < 0 || c >= in.classes) continue;
-            unsigned times = 0;
-            bool earlier = false;
-            for (int o = first; o < last; o += 4) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {  // (up to three places behind the list may be looked at, and do not count)
-                    const bool same = staged[o + u] == c && o + u < last;
-                    times += same ? 1u : 0u;
-                    earlier |= same && o + u < i;
-                }
-            }
-            if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
-        }
-        return;
-    }
-    for (long long i = threadIdx.x; i < total; i += kAdjustBlock) {
-        const int r = row_of(i);
-        const int *list = rules.shown + begin[r];
-        const long long mine = i - before[r], length = before[r + 1] - before[r];
-        const int c = list[mine];
-        if (c < 0 || c >= in.classes) continue;
-        unsigned times = 0;
-        bool earlier = false;
-        for (long long o = 0; o < length; ++o) {
-            const bool same = list[o] == c;
-            times += same ? 1u : 0u;
-            earlier |= same && o < mine;
-        }
-        if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
     }
 }
 
@@ -307,10 +339,17 @@ void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &
         }
         return;
     }
+    // an entry is compared with its whole list where lists are short, which costs as much as a table for some
+    constexpr int kShort = 96;
+    const bool lists = rules.shown != nullptr, short_ones = lists && rules.n_shown <= (long long)kShort * in.rows;
+    // (and every tile of 128 classes goes through its rows' lists: that pays while there are few)
+    constexpr int kTogether = 2048;
+    const bool together = columns && short_ones && in.classes <= kTogether;
     if (columns) {
-        const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 ? 4 : 6;
-        const dim3 grid((in.rows - 1) / (4 << quad_bits) + 1, (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
-        k_adjust_columns<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
+        const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 || together ? 4 : 6;
+        const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << (together ? 4 : quad_bits)) + 1), (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
+        if (together) k_adjust_columns<T, ALONG, true><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, 4);
+        else k_adjust_columns<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
     } else {
         constexpr int kOf = 16 / (int)sizeof(T);
         int row_bits = 2;
@@ -318,14 +357,9 @@ void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &
         const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / (kRowVectors * kOf << row_bits) + 1);
         k_adjust_rows<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
     }
-    if (rules.shown == nullptr) return;
-    // an entry is compared with its whole list below, which costs as much as a table for some
-    constexpr int kShort = 96;
-    if (rules.n_shown <= (long long)kShort * in.rows) {
-        k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
-    } else {
-        k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
-    }
+    if (!lists || together) return;
+    if (short_ones) k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
+    else k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
 }
 
 template <typename T>

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
     int *const class_of = reinterpret_cast<int *>(cell + (size_t)chunk * R);
     float *const q_of = reinterpret_cast<float *>(class_of + K * kPitch), *const z_of = q_of + K * kPitch;
     const int r = threadIdx.x % R, slot = threadIdx.x / R;
-    const long tile = R * 4 < 128 ? tile_of_block(blockIdx.x, gridDim.x) : blockIdx.x;
+    const long tile = tile_of_block(blockIdx.x, gridDim.x);
     const long row0 = tile * R, row = row0 + r;
     if (row0 >= call.in.rows) return;
     const bool on = row < call.in.rows, hard = call.labels != nullptr;
@@ -495,7 +495,7 @@ void distill_part(hipStream_t s, const DistillPlan &p, const DistillCall &call, 
     opt_in({reinterpret_cast<const void *>(&k_distill<R, B, PART>)});
     const unsigned tiles = (unsigned)((call.in.rows - 1) / R + 1);
     // (the loss alone needs one chunk's workgroup to add up)
-    const dim3 grid(R * 4 < 128 ? blocks_of_tiles(tiles) : tiles, PART == DISTILL_PAIRS && call.pairs == nullptr ? 1 : p.chunks);
+    const dim3 grid(blocks_of_tiles(tiles), PART == DISTILL_PAIRS && call.pairs == nullptr ? 1 : p.chunks);
     k_distill<R, B, PART><<<grid, B, p.lds, s>>>(call, sums, p.chunks, p.chunk);
 }
 

@@ -11,12 +11,12 @@
 namespace tgbm {
 namespace {
 
-// Tiles of less than a cache line of rows: workgroups go to the eight dies in turn, so the two tiles that share their lines go to
-// workgroups that are eight apart, and are read into one L2 (where there are enough of them to fill the dies that way).
-constexpr unsigned kPairedTiles = 256;
-inline unsigned blocks_of_tiles(unsigned tiles) { return tiles < kPairedTiles ? tiles : (tiles + 15) / 16 * 16; }
+// Tiles of rows whose neighbours share cache lines with them. Workgroups go to the eight dies in turn; here a die gets tiles that follow one another, so
+// that the shared lines are read into, and put together in, one L2 (where there are enough tiles to fill the dies that way).
+constexpr unsigned kDies = 8, kTilesForDies = 256;
+inline unsigned blocks_of_tiles(unsigned tiles) { return tiles < kTilesForDies ? tiles : (tiles + kDies - 1) / kDies * kDies; }
 __device__ __forceinline__ long tile_of_block(unsigned block, unsigned blocks) {
-    return blocks < kPairedTiles ? block : (block & ~15u) + (block & 7) * 2 + (block >> 3 & 1);
+    return blocks < kTilesForDies ? block : (block % kDies) * (blocks / kDies) + block / kDies;
 }
 
 template <typename T>
