@@ -6,7 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "device_api.h"
+#include "kernel_common.h"
 #include "score_rules.h"
 
 namespace tgbm {
@@ -115,6 +115,90 @@ struct ShortLists {
     }
 };
 
+// The lists of the 64 rows of a tile of kTileClasses classes that begin at c0, with counts in LDS of 8 bits: [classes][rows]. Whoever counts a class
+// first puts it on a list, and that list, a part of all entries without any class twice, is what is stored in the end.
+constexpr int kTileRows = 64, kTileClasses = 128;
+struct TileLists {
+    static constexpr int kEntries = 4096, kKept = 8;
+    long long begin[kTileRows];
+    int before[kTileRows + 1];  // entries of the rows before
+    int fits, held;
+    unsigned counts[kTileRows * kTileClasses / 4];
+    unsigned short cell_of[kEntries];
+
+    __device__ __forceinline__ void count(const tgbm_score_rules &rules, long row0, int rows, int c0, int c1) {
+        const uint4 zero = {0, 0, 0, 0};
+        for (int i = threadIdx.x; i < kTileRows * kTileClasses / 16; i += kAdjustBlock) reinterpret_cast<uint4 *>(counts)[i] = zero;
+        if (threadIdx.x < 64) {
+            long long b = 0, e = 0;
+            if (row0 + threadIdx.x < rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
+            const bool all_short = __all(e - b <= 255);
+            const int sum = wave_scan_i(all_short ? (int)(e - b) : 0);
+            begin[threadIdx.x] = b;
+            before[threadIdx.x + 1] = sum;
+            if (threadIdx.x == 0) before[0] = held = 0;
+            if (threadIdx.x == 63) fits = all_short && sum <= kEntries ? 1 : 0;
+        }
+        __syncthreads();
+        if (!fits) return;
+        const int n = before[kTileRows];
+        auto entry = [&](int i, int *r) {
+            *r = 0;
+#pragma unroll
+            for (int d = kTileRows / 2; d > 0; d >>= 1)
+                if (before[*r + d] <= i) *r += d;
+            return rules.shown[begin[*r] + (i - before[*r])] - c0;
+        };
+        auto add = [&](int c, int r) {
+            if ((unsigned)c >= (unsigned)(c1 - c0)) return;
+            const int cell = c * kTileRows + r, shift = cell % 4 * 8;
+            if ((atomicAdd(&counts[cell / 4], 1u << shift) >> shift & 0xffu) == 0) cell_of[atomicAdd(&held, 1)] = (unsigned short)cell;
+        };
+        int c[kKept], r[kKept];
+#pragma unroll
+        for (int u = 0; u < kKept; ++u) {
+            c[u] = -1;
+            if ((int)threadIdx.x + u * kAdjustBlock < n) c[u] = entry(threadIdx.x + u * kAdjustBlock, &r[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kKept; ++u)
+            if ((int)threadIdx.x + u * kAdjustBlock < n) add(c[u], r[u]);
+        for (int i = threadIdx.x + kKept * kAdjustBlock; i < n; i += kAdjustBlock) {
+            int of;
+            const int cls = entry(i, &of);
+            add(cls, of);
+        }
+    }
+    // (behind a barrier)
+    template <typename T>
+    __device__ __forceinline__ void store(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) const {
+        if (fits) {
+            for (int j = threadIdx.x; j < held; j += kAdjustBlock) {
+                const int cell = cell_of[j];
+                store_held_back<T>(in, rules, out, row0 + cell % kTileRows, c0 + cell / kTileRows, counts[cell / 4] >> (cell % 4 * 8) & 0xffu);
+            }
+            return;
+        }
+        // a long list among them: every entry is compared with its list, four threads to a row
+        const long row = row0 + threadIdx.x % kTileRows;
+        if (row >= in.rows) return;
+        long long b, e;
+        shown_range(rules, row, &b, &e);
+        for (long long i = b + threadIdx.x / kTileRows; i < e; i += kAdjustBlock / kTileRows) {
+            const int c = rules.shown[i];
+            if (c < c0 || c >= c1) continue;
+            unsigned times = 0;
+            bool earlier = false;
+            for (long long o = b; o < e; ++o) {
+                const bool same = rules.shown[o] == c;
+                times += same ? 1u : 0u;
+                earlier |= same && o < i;
+            }
+            if (!earlier) store_held_back<T>(in, rules, out, row, c, times);
+        }
+    }
+};
+
 constexpr int kListRows = 16;
 template <typename T>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
@@ -128,15 +212,17 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores
 // ---------------------------------------------------------------------------------------------- bias and allowed sets
 // Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side.
 // ALONG: out is in the same order. LISTS (quad_bits is 4): the workgroup's part of short lists is stored behind it, while the lines that it touches are in
-// the L2: read and written again by a launch of its own, 20 entries a row of 500 classes took 72 us, with 108 for the scores.
+// the L2.
 template <typename T, bool ALONG, bool LISTS>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int quad_bits) {
     using V = typename ScoreVector<T, 4>::type;
-    __shared__ typename std::conditional<LISTS, ShortLists<64>, char>::type lists;
+    static_assert(kAdjustBlock / 64 * 32 == kTileClasses);
+    __shared__ __align__(16) typename std::conditional<LISTS, TileLists, char>::type lists;
     const long tile = tile_of_block(blockIdx.x, gridDim.x);
     if constexpr (LISTS) {
         quad_bits = 4;
-        lists.stage(rules, tile * 64, in.rows);
+        const int first = (int)blockIdx.y * kTileClasses;
+        lists.count(rules, tile * kTileRows, in.rows, first, std::min(in.classes, first + kTileClasses));
     }
     const int lane = threadIdx.x & 63, step = 64 >> quad_bits;
     const int g = ((int)blockIdx.y * (kAdjustBlock / 64) + (int)(threadIdx.x >> 6)) * 32, end = std::min(g + 32, in.classes);
@@ -190,8 +276,8 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in,
     }
     if constexpr (LISTS) {
         __syncthreads();
-        const int c0 = (int)blockIdx.y * (kAdjustBlock / 64 * 32);
-        lists.template store<T>(in, rules, out, tile * 64, c0, std::min(in.classes, c0 + kAdjustBlock / 64 * 32));
+        const int first = (int)blockIdx.y * kTileClasses;
+        lists.template store<T>(in, rules, out, tile * kTileRows, first, std::min(in.classes, first + kTileClasses));
     }
 }
 
@@ -275,7 +361,6 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_long_lists(tgbm_scores 
 }
 
 // In place: a workgroup takes 64 rows and 128 classes (rows side by side), or 2^row_bits threads a row and up to kTableClasses classes of it.
-constexpr int kTileRows = 64, kTileClasses = 128;
 template <typename T>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns_in_place(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
     __shared__ unsigned times[kTileClasses * kTileRows];
