@@ -8,6 +8,7 @@ torch's current stream of the tensors' device; nothing waits, and calls can be c
 raise ValueError before anything is launched. The calls take no part in autograd: a tensor that requires a gradient is refused.
 """
 import ctypes as C
+import functools
 import math
 import sys
 
@@ -43,11 +44,6 @@ def _torch():
     return torch
 
 
-def _is(condition, *what):
-    if not condition:
-        raise ValueError(what[0] % what[1:] if len(what) > 1 else what[0])
-
-
 def _on_gpu(torch, name, x):
     if not isinstance(x, torch.Tensor):
         raise ValueError("%s: a torch tensor is wanted, got %s" % (name, type(x).__name__))
@@ -79,7 +75,10 @@ def _scores(torch, name, x):
 
 
 def _plain(torch, name, x, like, dtype, shape):
-    """A contiguous tensor of one type, on the scores' device."""
+    """The address of a contiguous tensor of one type, on the scores' device."""
+    if (isinstance(x, torch.Tensor) and x.dtype is dtype and x.shape == shape and x.is_cuda and x.get_device() == like.get_device()
+            and x.is_contiguous() and not x.requires_grad):
+        return x.data_ptr()
     _on_gpu(torch, name, x)
     if x.dtype != dtype:
         raise ValueError("%s: %s is wanted, got %s" % (name, dtype, x.dtype))
@@ -87,14 +86,12 @@ def _plain(torch, name, x, like, dtype, shape):
         raise ValueError("%s is on %s, the scores are on %s" % (name, x.device, like.device))
     if tuple(x.shape) != shape:
         raise ValueError("%s: the shape %s is wanted, got %s" % (name, shape, tuple(x.shape)))
-    if not x.is_contiguous():
-        raise ValueError("%s: a contiguous tensor is wanted" % name)
-    return x.data_ptr()
+    raise ValueError("%s: a contiguous tensor is wanted" % name)
 
 
 def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence):
     classes, rows = scores.shape
-    r = _Rules(repetition=1.0)
+    r = _Rules()
     if bias is not None:
         r.bias = _plain(torch, "bias", bias, scores, torch.float32, (classes,))
     if allowed is not None:
@@ -129,17 +126,38 @@ def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repeti
     return r
 
 
+_functions = {}
+
+
 def _call(torch, scores, name, *args):
     """One call of the library on the current stream of the scores' device."""
-    fn = getattr(_lib.load(), name)
-    device = scores.device.index
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.load(), name)
+    device = scores.get_device()
     if device == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        rc = fn(*args, _stream(torch, device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _stream(torch, device))
     if rc:
         raise (ValueError if rc == 1 else RuntimeError)("%s failed; it has said why on stderr" % name)
+
+
+def _stream(torch, device):
+    """The number of the current stream (3 us through torch's stream objects, as much as a launch)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+@functools.lru_cache(maxsize=256)
+def _top_workspace(by_class, by_row, classes, rows, k):
+    return _lib.load().tgbm_scores_top_workspace(C.byref(_Scores(1, by_class, by_row, 0, classes, rows)), k)
+
+
+@functools.lru_cache(maxsize=256)
+def _distill_workspace(classes, rows, entries):
+    return _lib.load().tgbm_scores_distill_workspace(C.byref(_Scores(1, max(rows, 1), 1, 0, classes, rows)), entries)
 
 
 def adjust(scores, bias=None, allowed=None, allowed_set=None, shown=None, shown_begin=None, repetition=1.0, frequency=0.0,
@@ -161,9 +179,14 @@ def adjust(scores, bias=None, allowed=None, allowed_set=None, shown=None, shown_
         # (in the scores' order, without the gaps that a part of a larger array has)
         if s.class_stride == 1 and s.rows > 1:
             out = torch.empty((s.rows, s.classes), dtype=scores.dtype, device=scores.device).t()
+            o = _Scores(out.data_ptr(), 1, s.classes, s.type, s.classes, s.rows)
         else:
             out = torch.empty((s.classes, s.rows), dtype=scores.dtype, device=scores.device)
-    elif not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != scores.device:
+            o = _Scores(out.data_ptr(), max(s.rows, 1), 1, s.type, s.classes, s.rows)
+        if s.rows:
+            _call(torch, scores, "tgbm_scores_adjust", C.byref(s), C.byref(r), C.byref(o))
+        return out
+    if not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != scores.device:
         raise ValueError("out: a tensor of the scores' type, shape and device is wanted")
     o = _scores(torch, "out", out)
     if s.rows:
@@ -200,7 +223,7 @@ def top(scores, k, bias=None, allowed=None, allowed_set=None, shown=None, shown_
     classes = torch.empty((n, k), dtype=torch.int32, device=device)
     lse = torch.empty(n, dtype=torch.float32, device=device)
     if n:
-        size = _lib.load().tgbm_scores_top_workspace(C.byref(s), k)
+        size = _top_workspace(s.class_stride, s.row_stride, s.classes, n, k)
         # (torch keeps it until the stream's work that uses it is done, and a captured graph has its own)
         room = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _call(torch, scores, "tgbm_scores_top", C.byref(s), C.byref(r), k, temperature, values.data_ptr(), classes.data_ptr(), lse.data_ptr(),
@@ -249,7 +272,7 @@ def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature
     loss = torch.empty(n, dtype=torch.float32, device=scores.device)
     pairs = torch.empty((C_, n, 2), dtype=torch.float32, device=scores.device) if gradient else None
     if n:
-        size = _lib.load().tgbm_scores_distill_workspace(C.byref(s), entries)
+        size = _distill_workspace(C_, n, entries)
         room = torch.empty(size, dtype=torch.uint8, device=scores.device) if size else None
         _call(torch, scores, "tgbm_scores_distill", C.byref(s), C.byref(t), y, temperature, weight, loss.data_ptr(),
               pairs.data_ptr() if gradient else None, n, room.data_ptr() if size else None, size)
