@@ -136,6 +136,20 @@ def test_top_workspace(lib, by_class):
                 assert lib.tgbm_scores_top_workspace(C.byref(a), 0) == lib.tgbm_scores_top_workspace(C.byref(a), 129) == 0
 
 
+@pytest.mark.parametrize("last", [1, 2, 7, 40, 1000])
+@pytest.mark.parametrize("classes", [33, 700, 1600, 2100, 5000, 40_000])
+def test_workspace_of_rows_beyond_a_launch(lib, classes, last):
+    """Rows go by slices of 2^22: the few of the last one are shared out over the chip, and their parts have room too."""
+    rows = (1 << 22) + last
+    for class_stride, row_stride in ((rows, 1), (1, classes)):
+        many, few = (array(class_stride=class_stride, row_stride=row_stride, classes=classes, rows=n) for n in (rows, last))
+        for k in (1, 20, 128):
+            assert lib.tgbm_scores_top_workspace(C.byref(many), k) >= lib.tgbm_scores_top_workspace(C.byref(few), k)
+    many, few = (array(class_stride=rows, classes=classes, rows=n) for n in (rows, last))
+    for entries in (1, 32, 128):
+        assert lib.tgbm_scores_distill_workspace(C.byref(many), entries) >= lib.tgbm_scores_distill_workspace(C.byref(few), entries)
+
+
 def test_distill_refuses(lib, capfd):
     def call(a=array(), teacher=True, classes=ADDRESS, scores=ADDRESS, kind=0, entries=3, labels=ADDRESS, temperature=1.0, weight=0.5, loss=ADDRESS, pairs=ADDRESS,
              stride=10, room=ADDRESS, size=1 << 20):

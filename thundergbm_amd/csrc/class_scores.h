@@ -38,6 +38,14 @@ inline void take_rows(tgbm_scores &s, tgbm_score_rules &rules, int first, int ro
     s.rows = rows;
 }
 
+// The workspace of a call that goes by slices of rows: what of(rows) says for a whole slice, or for the last one, which may be split over
+// the chip in another way.
+template <typename Of>
+size_t workspace_of_slices(int rows, Of of) {
+    const int last = rows % kSliceRows;
+    return std::max(of(std::min(rows, kSliceRows)), rows > kSliceRows && last > 0 ? of(last) : (size_t)0);
+}
+
 void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out);
 
 size_t scores_top_workspace(bool columns, int classes, int rows, int k);

@@ -512,9 +512,10 @@ void distill_rows(hipStream_t s, const DistillPlan &p, const DistillCall &call, 
 }  // namespace
 
 size_t scores_distill_workspace(int classes, int rows, int entries) {
-    rows = std::min(rows, kSliceRows);
-    const DistillPlan p = plan_distill(classes, rows, entries);
-    return p.chunks == 1 ? 0 : sizeof(RowSums) * (size_t)rows * p.chunks;
+    return workspace_of_slices(rows, [&](int slice) {
+        const DistillPlan p = plan_distill(classes, slice, entries);
+        return p.chunks == 1 ? 0 : sizeof(RowSums) * (size_t)slice * p.chunks;
+    });
 }
 
 void launch_scores_distill(hipStream_t s, const tgbm_scores &in, const tgbm_teacher &teacher, const float *labels, float temperature, float weight,

@@ -1004,11 +1004,12 @@ int parts_of_a_join(int k) { return std::max(2, kJoinMost / k); }
 }  // namespace
 
 size_t scores_top_workspace(bool columns, int classes, int rows, int k) {
-    rows = std::min(rows, kSliceRows);
-    const TopPlan p = plan_top(columns, classes, rows, k);
-    size_t bytes = 0;
-    for (int parts = p.chunks; parts > 1; parts = (parts - 1) / parts_of_a_join(k) + 1) bytes += part_bytes((size_t)rows * parts, k);
-    return bytes;
+    return workspace_of_slices(rows, [&](int slice) {
+        const TopPlan p = plan_top(columns, classes, slice, k);
+        size_t bytes = 0;
+        for (int parts = p.chunks; parts > 1; parts = (parts - 1) / parts_of_a_join(k) + 1) bytes += part_bytes((size_t)slice * parts, k);
+        return bytes;
+    });
 }
 
 static void launch_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
