@@ -266,7 +266,7 @@ typedef struct tgbm_score_rules {
 } tgbm_score_rules;
 
 /* out = the scores as the rules leave them, rounded once to their type. out: another array of the same type, classes and
- * rows, in either order, or `in` itself. */
+ * rows, in either order, that shares no element with `in`, or `in` itself. */
 int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream);
 
 /* The k (1 to 128) best classes of every row by the scores as the rules leave them, and the logarithm of the sum of

@@ -79,6 +79,17 @@ def test_adjust_refuses_pairs_and_nulls(lib, capfd):
         assert capfd.readouterr().err.startswith("tgbm_scores_adjust: ")
 
 
+@pytest.mark.parametrize("away,out", [
+    (4, dict()), (36, dict()), (-36, dict()), (156, dict()), (156, dict(class_stride=1, row_stride=4)),
+    (4 * 9, dict(class_stride=20)), (4 * 15, dict(class_stride=20)), (4 * 20 - 4, dict(class_stride=20)), (2, dict(kind=1)),
+    (4, dict(classes=1, class_stride=0)), (4, dict(rows=1, class_stride=1, row_stride=0)), (8, dict(rows=1, class_stride=2)),
+])
+def test_adjust_refuses_overlaps(lib, capfd, away, out):
+    of_in = {k: v for k, v in out.items() if k in ("kind", "classes", "rows") or out.get("class_stride") in (0, 2, 20) or "rows" in out}
+    assert lib.tgbm_scores_adjust(C.byref(array(**of_in)), C.byref(rules()), C.byref(array(data=ADDRESS + away, **out)), None) == 1
+    assert "out overlaps in" in capfd.readouterr().err
+
+
 def test_no_rows_are_no_work(lib):
     assert lib.tgbm_scores_adjust(C.byref(array(rows=0, data=None)), C.byref(rules()), C.byref(array(rows=0, data=None)), None) == 0
 

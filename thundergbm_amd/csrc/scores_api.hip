@@ -45,6 +45,20 @@ int check_scores(const char *entry, const char *what, const tgbm_scores *s) {
     return 0;
 }
 
+// Whether two arrays of one type and the same sizes share an element. Parts of one larger array may lie between each other's lines: they have its strides.
+bool overlap(const tgbm_scores &a, const tgbm_scores &b) {
+    const long long size = a.type == TGBM_F32 ? 4 : 2;
+    const auto bytes = [&](const tgbm_scores &s) { return ((s.classes - 1) * s.class_stride + (s.rows - 1) * s.row_stride + 1) * size; };
+    const char *first = static_cast<const char *>(a.data), *second = static_cast<const char *>(b.data);
+    if (first + bytes(a) <= second || second + bytes(b) <= first) return false;
+    if (a.class_stride != b.class_stride || a.row_stride != b.row_stride) return true;
+    const bool columns = rows_side_by_side(a);
+    if ((columns ? a.classes : a.rows) == 1) return true;  // (one line, whose pitch says nothing)
+    const long long pitch = columns ? a.class_stride : a.row_stride, width = columns ? a.rows : a.classes;
+    const long long apart = (first < second ? second - first : first - second) % (pitch * size);
+    return apart < width * size || apart > (pitch - width) * size;
+}
+
 int check_rules(const char *entry, const tgbm_score_rules *r, int rows) {
     if (r == nullptr) return refused(entry, "rules is null");
     if (r->allowed != nullptr) {
@@ -86,6 +100,7 @@ extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules 
     if (in->data == out->data && (in->class_stride != out->class_stride || in->row_stride != out->row_stride))
         return refused(entry, "out is in's memory with other strides");
     if (in->rows == 0) return 0;
+    if (in->data != out->data && overlap(*in, *out)) return refused(entry, "out overlaps in");
     launch_scores_adjust(static_cast<hipStream_t>(stream), *in, *rules, *out);
     return launched(entry);
 }
