@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "kernel_common.h"
 #include "score_rules.h"
@@ -138,11 +139,35 @@ __device__ __forceinline__ unsigned one_by_one(unsigned v) {
     return v;
 }
 
-template <int E>
-__device__ __forceinline__ float best_of(const float (&v)[E]) {
+// A thread's scores: as they are worked out,
+template <int N>
+struct Held {
+    float v[N];
+    __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+    __device__ __forceinline__ void look_again() {}
+};
+// or as they were read, two of 16 bits to a register, and unpacked wherever they are looked at.
+template <typename T, int E>
+struct HeldPairs {
+    unsigned pair[E / 2];
+    float last;
+    __device__ __forceinline__ float operator[](int i) const {
+        if (i == E) return last;
+        if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(i % 2 ? pair[i / 2] & 0xffff0000u : pair[i / 2] << 16);
+        else return (float)__builtin_bit_cast(_Float16, (unsigned short)(pair[i / 2] >> (i % 2 * 16)));
+    }
+    // (the compiler is not to keep what it has unpacked so far)
+    __device__ __forceinline__ void look_again() {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) asm volatile("" : "+v"(pair[i]));
+    }
+};
+
+template <int N, typename Scores>
+__device__ __forceinline__ float best_of(const Scores &v) {
     float best = kNothing;
 #pragma unroll
-    for (int i = 0; i < E; ++i) best = fmaxf(best, v[i]);
+    for (int i = 0; i < N; ++i) best = fmaxf(best, v[i]);
     return best;
 }
 
@@ -164,10 +189,11 @@ struct LaidOut {
     unsigned long long key[kListRoom];
     int better[W == 1 ? 1 : kListRoom];
 
-    __device__ __forceinline__ void put(int q, int t, const float *v) {
+    template <typename Scores>
+    __device__ __forceinline__ void put(int q, int t, const Scores &v, int first) {
         owner[q] = (unsigned short)t;
 #pragma unroll
-        for (int i = 0; i < N; ++i) score[q * N + i] = v[i];
+        for (int i = 0; i < N; ++i) score[q * N + i] = v[first + i];
     }
     template <typename At>
     __device__ __forceinline__ float get(int q, int i, const At &) const { return score[q * N + i]; }
@@ -192,7 +218,8 @@ struct Column {
     int pitch, lines;
     ColumnLists &lists;
     __device__ __forceinline__ float at_line(int p) const { return __uint_as_float(column[p * pitch]); }
-    __device__ __forceinline__ void put(int q, int t, const float *) { lists.owner[q] = (unsigned char)t; }
+    template <typename Scores>
+    __device__ __forceinline__ void put(int q, int t, const Scores &, int) { lists.owner[q] = (unsigned char)t; }
     template <typename At>
     __device__ __forceinline__ float get(int q, int i, const At &at) const {
         const int p = at.at(lists.owner[q], i);
@@ -211,8 +238,8 @@ struct Column {
 // The k best of the group's scores go to `slot` of the output, in order. v: M times N scores, each N of them a thread's to the
 // choice (M is 1 but for one wavefront); best: the largest of each; at: where they lie, ascending with i; room: LDS of the group; class_at(place): the class; meanwhile():
 // what the last of several wavefronts does while the first one looks for the bound, behind a barrier. Every thread of the group comes here.
-template <int W, int M, int N, typename At, typename Room, typename Class, typename Meanwhile>
-__device__ __forceinline__ void write_top(const float (&v)[M * N], const float (&best)[M], const At &at, int k, TopShared<W> &sh, Room &room, size_t slot,
+template <int W, int M, int N, typename Scores, typename At, typename Room, typename Class, typename Meanwhile>
+__device__ __forceinline__ void write_top(Scores &v, const float (&best)[M], const At &at, int k, TopShared<W> &sh, Room &room, size_t slot,
                                           const TopOut &out, Class class_at, Meanwhile meanwhile) {
     static_assert(M == 1 || W == 1);
     const int lane = lane_id(), t = W == 1 ? lane : (int)threadIdx.x;
@@ -248,6 +275,7 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
 #pragma unroll
     for (int j = 0; j < M; ++j) first[j] = INT_MAX;
     if (exact) {  // (the same in all threads)
+        v.look_again();
 #pragma unroll
         for (int j = 0; j < M; ++j) {
 #pragma unroll
@@ -278,6 +306,7 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
         }
     }
     // the candidates: a bit for each score that reaches the bound
+    v.look_again();
     constexpr int kWords = (M * N + 31) / 32;
     unsigned mine[kWords];
 #pragma unroll
@@ -319,7 +348,8 @@ __device__ __forceinline__ void write_top(const float (&v)[M * N], const float (
             to += __shfl(to0, 0);
         }
         if (count != 0) {
-            room.put(q, t + 64 * j, v + j * N);
+            v.look_again();
+            room.put(q, t + 64 * j, v, j * N);
             wave_fence();
 #pragma unroll
             for (int w = 0; w < (N + 31) / 32; ++w)
@@ -450,8 +480,8 @@ __device__ __forceinline__ float rescaled(float sum, float from, float to, float
 
 // The largest of a wavefront's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
 // NaN, an infinity makes it infinite. best: the thread's largest.
-template <int E>
-__device__ __forceinline__ void sum_exponentials(const float (&v)[E], float best, float by, float *reference, float *sum) {
+template <int E, typename Scores>
+__device__ __forceinline__ void sum_exponentials(const Scores &v, float best, float by, float *reference, float *sum) {
     float m = reference_of(wave_max_f(best));
     float part[4] = {0.f, 0.f, 0.f, 0.f};
     if (fabsf(m) < 1e30f) {
@@ -505,11 +535,16 @@ __device__ __forceinline__ void count_shown(const tgbm_score_rules &rules, long 
 // A group of W wavefronts takes a chunk (a multiple of 32 classes) of a row; with W = 1 there are four groups to a
 // workgroup. A thread has E scores in whole vectors, and one of what is left behind the last vector. RULES: there may be any. LDS: the lists of candidates,
 // then, where classes were shown, bits and times.
+template <typename T, int E, bool RULES>
+constexpr bool held_in_pairs() { return sizeof(T) == 2 && !RULES && E > 24; }
 template <typename T, int W, int E, bool RULES>
-__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 5 : 6) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
+constexpr int waves_of_top_rows() { return held_in_pairs<T, E, RULES>() ? 6 : E > 24 ? 4 : W == 1 ? 5 : 6; }
+template <typename T, int W, int E, bool RULES>
+__global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, W, E, RULES>())) void k_top_rows(tgbm_scores in, tgbm_score_rules rules, int k, float temperature, TopOut out,
                                                                           int chunks, int chunk, bool whole) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
+    constexpr bool kPairs = held_in_pairs<T, E, RULES>();
     __shared__ TopShared<W> shared[kGroups];
     __shared__ LaidOut<W, N> rooms[kGroups];
     extern __shared__ unsigned shown_lds[];
@@ -526,7 +561,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 
         const Layout<N, V, true> at{kStep, whole_size};
         const int base = (int)one_by_one((unsigned)t * V);  // (places are worked out where they are used, not kept over the tiles)
         const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride + c0;
-        float v[N];
+        typename std::conditional<kPairs, HeldPairs<T, E>, Held<N>>::type held_scores;
         {
             typename Vector<T>::type x[E / V];
 #pragma unroll
@@ -534,11 +569,20 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 
                 x[g] = (T)kNothing;
                 if (base < whole_size - g * kStep) x[g] = *reinterpret_cast<const typename Vector<T>::type *>(src + base + g * kStep);
             }
-            v[E] = t < size - whole_size ? score_to_float(src[whole_size + t]) : kNothing;
+            const float last = t < size - whole_size ? score_to_float(src[whole_size + t]) : kNothing;
+            if constexpr (kPairs) {
+                held_scores.last = last;
+                typedef unsigned Words __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = score_to_float(x[i / V][i % V]);
+                for (int i = 0; i < E / 2; ++i) held_scores.pair[i] = __builtin_bit_cast(Words, x[i / 4])[i % 4];
+            } else {
+                held_scores.v[E] = last;
+#pragma unroll
+                for (int i = 0; i < E; ++i) held_scores.v[i] = score_to_float(x[i / V][i % V]);
+            }
         }
         if constexpr (RULES) {
+            auto &v = held_scores.v;
             if (rules.bias != nullptr) {
                 const float *bias = rules.bias + c0;
 #pragma unroll
@@ -597,9 +641,10 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 
                 v[E] = ok ? v[E] : kNothing;
             }
         }
-        const float best[1] = {best_of(v)};
+        const float best[1] = {best_of<N>(held_scores)};
         float m, s;
-        sum_exponentials(v, best[0], by, &m, &s);
+        held_scores.look_again();
+        sum_exponentials<N>(held_scores, best[0], by, &m, &s);
         auto leave = [&](float reference, float sum) {
             if (whole) {
                 out.lse[row] = log_sum(reference, sum, temperature);
@@ -616,7 +661,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, E > 24 ? 4 : W == 1 ? 
                 sh.part_sum[wave_id()] = s;
             }
         }
-        write_top<W, 1, N>(v, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; }, [&] {
+        write_top<W, 1, N>(held_scores, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; }, [&] {
             const bool in = lane_id() < W;
             const float its_max = in ? sh.part_max[lane_id()] : 0.f, its_sum = in ? sh.part_sum[lane_id()] : 0.f;
             const float all = reference_of(wave_max_f(its_sum > 0.f ? its_max : kNothing));
@@ -737,9 +782,10 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
         for (int q = wave_id(); q < rows && row0 + q < in.rows; q += kColumnBlock / 64) {
             const int lane = (int)one_by_one((unsigned)lane_id());  // (places are worked out where they are used)
             const unsigned *from = cell + lane * pitch + q;
-            float v[E], best[M];
+            Held<E> v;
+            float best[M];
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = lane < size - i * 64 ? __uint_as_float(from[i * 64 * pitch]) : kNothing;
+            for (int i = 0; i < E; ++i) v.v[i] = lane < size - i * 64 ? __uint_as_float(from[i * 64 * pitch]) : kNothing;
             float largest = kNothing;
 #pragma unroll
             for (int j = 0; j < M; ++j) {
@@ -750,7 +796,7 @@ __global__ __launch_bounds__(kColumnBlock, 8) void k_top_columns(tgbm_scores in,
             }
             const size_t out_at = (size_t)(row0 + q) * chunks + part;
             float m, s;
-            sum_exponentials(v, largest, by, &m, &s);
+            sum_exponentials<E>(v, largest, by, &m, &s);
             if (lane_id() == 0) {
                 if (whole) {
                     out.lse[row0 + q] = log_sum(m, s, temperature);
@@ -841,11 +887,11 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
         const size_t from = (size_t)row * parts + first, tile = (size_t)row * joins + part;
         const float *values = in.values + from * k;
         const int *classes = in.classes + from * k;
-        float v[E];
+        Held<E> v;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const int at = i * 64 * W + t;
-            v[i] = at < count ? values[at] : kNothing;
+            v.v[i] = at < count ? values[at] : kNothing;
         }
         auto join_sums = [&] {  // (by one wavefront)
             const float *sums = in.lse + from * 2;
@@ -868,7 +914,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
             }
         };
         if constexpr (W == 1) join_sums();
-        const float best[1] = {best_of(v)};
+        const float best[1] = {best_of<E>(v)};
         write_top<W, 1, E>(v, best, Layout<E, 1, false>{64 * W, 0}, k, sh, rooms[group], tile, out, [&](int p) { return classes[p]; }, join_sums);
     }
 }
