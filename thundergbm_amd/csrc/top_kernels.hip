@@ -145,17 +145,24 @@ struct Held {
     float v[N];
     __device__ __forceinline__ float operator[](int i) const { return v[i]; }
     __device__ __forceinline__ void look_again() {}
+    // N words of 32 bits, and a score of those
+    static constexpr int kWords = N;
+    __device__ __forceinline__ unsigned word(int i) const { return __float_as_uint(v[i]); }
+    static __device__ __forceinline__ float score_of(const unsigned *words, int i) { return __uint_as_float(words[i]); }
 };
 // or as they were read, two of 16 bits to a register, and unpacked wherever they are looked at.
 template <typename T, int E>
 struct HeldPairs {
     unsigned pair[E / 2];
     float last;
-    __device__ __forceinline__ float operator[](int i) const {
-        if (i == E) return last;
-        if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(i % 2 ? pair[i / 2] & 0xffff0000u : pair[i / 2] << 16);
-        else return (float)__builtin_bit_cast(_Float16, (unsigned short)(pair[i / 2] >> (i % 2 * 16)));
+    static constexpr int kWords = E / 2 + 1;
+    static __device__ __forceinline__ float half(unsigned pair, int i) {
+        if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(i % 2 ? pair & 0xffff0000u : pair << 16);
+        else return (float)__builtin_bit_cast(_Float16, (unsigned short)(pair >> (i % 2 * 16)));
     }
+    __device__ __forceinline__ float operator[](int i) const { return i == E ? last : half(pair[i / 2], i); }
+    __device__ __forceinline__ unsigned word(int i) const { return i == E / 2 ? __float_as_uint(last) : pair[i]; }
+    static __device__ __forceinline__ float score_of(const unsigned *words, int i) { return i == E ? __uint_as_float(words[E / 2]) : half(words[i / 2], i); }
     // (the compiler is not to keep what it has unpacked so far)
     __device__ __forceinline__ void look_again() {
 #pragma unroll
@@ -179,27 +186,26 @@ struct TopOut {
 };
 
 // LDS of a group: the candidates, ordered score in front of the complement of the place (larger is better), and how many of them are
-// better; the scores of the threads that reach the bound, score i of the q-th of them at q * N + i, and who they are.
-template <int W, int N>
+// better; the scores of the threads that reach the bound, the words of the q-th of them from q * kWords on, and who they are.
+template <int W, typename Scores>
 struct LaidOut {
-    static constexpr int kRoom = kListRoom;
+    static constexpr int kRoom = kListRoom, kWords = Scores::kWords;
     static constexpr int kThreads = W == 1 ? 64 : kMostThreads;
-    float score[kThreads * N];
+    unsigned word[kThreads * kWords];
     unsigned short owner[kThreads];
     unsigned long long key[kListRoom];
     int better[W == 1 ? 1 : kListRoom];
 
-    template <typename Scores>
-    __device__ __forceinline__ void put(int q, int t, const Scores &v, int first) {
+    __device__ __forceinline__ void put(int q, int t, const Scores &v, int) {
         owner[q] = (unsigned short)t;
 #pragma unroll
-        for (int i = 0; i < N; ++i) score[q * N + i] = v[first + i];
+        for (int i = 0; i < kWords; ++i) word[q * kWords + i] = v.word(i);
     }
     template <typename At>
-    __device__ __forceinline__ float get(int q, int i, const At &) const { return score[q * N + i]; }
+    __device__ __forceinline__ float get(int q, int i, const At &) const { return Scores::score_of(word + q * kWords, i); }
     template <typename At>
     __device__ __forceinline__ int place(int q, int i, const At &at) const { return at.at(owner[q], i); }
-    __device__ __forceinline__ float laid_out(int q, int i, int) const { return score[q * N + i]; }
+    __device__ __forceinline__ float laid_out(int q, int i, int) const { return Scores::score_of(word + q * kWords, i); }
     __device__ __forceinline__ void list(int to, float s, int p) {
         key[to] = (unsigned long long)ordered(s) << 32 | (unsigned)~p;
         if constexpr (W > 1) better[to] = 0;
@@ -348,7 +354,6 @@ __device__ __forceinline__ void write_top(Scores &v, const float (&best)[M], con
             to += __shfl(to0, 0);
         }
         if (count != 0) {
-            v.look_again();
             room.put(q, t + 64 * j, v, j * N);
             wave_fence();
 #pragma unroll
@@ -546,7 +551,8 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
     constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
     constexpr bool kPairs = held_in_pairs<T, E, RULES>();
     __shared__ TopShared<W> shared[kGroups];
-    __shared__ LaidOut<W, N> rooms[kGroups];
+    using Scores = typename std::conditional<held_in_pairs<T, E, RULES>(), HeldPairs<T, E>, Held<N>>::type;
+    __shared__ LaidOut<W, Scores> rooms[kGroups];
     extern __shared__ unsigned shown_lds[];
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
     TopShared<W> &sh = shared[group];
@@ -561,7 +567,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
         const Layout<N, V, true> at{kStep, whole_size};
         const int base = (int)one_by_one((unsigned)t * V);  // (places are worked out where they are used, not kept over the tiles)
         const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride + c0;
-        typename std::conditional<kPairs, HeldPairs<T, E>, Held<N>>::type held_scores;
+        Scores held_scores;
         {
             typename Vector<T>::type x[E / V];
 #pragma unroll
@@ -875,7 +881,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W) void k_top_join(int pa
                                                                           TopOut out) {
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     __shared__ TopShared<W> shared[kGroups];
-    __shared__ LaidOut<W, E> rooms[kGroups];
+    __shared__ LaidOut<W, Held<E>> rooms[kGroups];
     const int t = W == 1 ? lane_id() : (int)threadIdx.x, group = W == 1 ? wave_id() : 0;
     TopShared<W> &sh = shared[group];
     const float by = kLog2e / temperature;
