@@ -281,45 +281,109 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in,
     }
 }
 
-// Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them.
+// Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them. LISTS: a bit in LDS says that a class was shown, and
+// a word how often; the row's threads go through its list meanwhile the scores are on their way.
 constexpr int kRowVectors = 4;
-template <typename T, bool ALONG>
+template <int CELLS>
+struct ShownTimes {
+    static constexpr int kKept = 8;
+    unsigned bits[CELLS / 32];
+    unsigned times[CELLS];
+
+    // of classes [c0, c0 + size) of a row whose cells begin at `first`, by its per_row threads. All threads of the workgroup come here.
+    __device__ __forceinline__ void count(const tgbm_score_rules &rules, long row, bool on, int c0, int size, int first, int at, int per_row) {
+#pragma unroll
+        for (int i = 0; i < CELLS / 32; i += kAdjustBlock)
+            if (i + (int)threadIdx.x < CELLS / 32) bits[i + threadIdx.x] = 0;
+        long long b = 0, e = 0;
+        if (on) shown_range(rules, row, &b, &e);
+        int kept[kKept];  // (-1: none of these classes; a list is gone through twice, and every load is waited for)
+#pragma unroll
+        for (int u = 0; u < kKept; ++u) {
+            const long long i = b + at + u * per_row;
+            const int c = i < e ? rules.shown[i] - c0 : -1;
+            kept[u] = (unsigned)c < (unsigned)size ? first + c : -1;
+        }
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int u = 0; u < kKept; ++u)
+                if (kept[u] >= 0) f(kept[u]);
+            for (long long i = b + at + kKept * per_row; i < e; i += per_row) {
+                const int c = rules.shown[i] - c0;
+                if ((unsigned)c < (unsigned)size) f(first + c);
+            }
+        };
+        __syncthreads();
+        each([&](int cell) {
+            times[cell] = 0;
+            atomicOr(&bits[cell / 32], 1u << cell % 32);
+        });
+        __syncthreads();
+        each([&](int cell) { atomicAdd(&times[cell], 1u); });
+        __syncthreads();
+    }
+};
+
+template <typename T, bool ALONG, bool LISTS>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int row_bits) {
     constexpr int kOf = 16 / (int)sizeof(T);
     using V = typename ScoreVector<T, kOf>::type;
-    const int per_row = 1 << row_bits, at = threadIdx.x & (per_row - 1), step = per_row * kOf;
-    const long row = (long)blockIdx.x * (kAdjustBlock >> row_bits) + (threadIdx.x >> row_bits);
-    if (row >= in.rows) return;
-    const int c0 = (int)blockIdx.y * kRowVectors * step, c1 = std::min(in.classes, c0 + kRowVectors * step), whole = c0 + (c1 - c0) / kOf * kOf;
+    __shared__ typename std::conditional<LISTS, ShownTimes<kRowVectors * kOf * kAdjustBlock>, char>::type shown;
+    const int per_row = 1 << row_bits, at = threadIdx.x & (per_row - 1), step = per_row * kOf, group = threadIdx.x >> row_bits;
+    const long row = (long)blockIdx.x * (kAdjustBlock >> row_bits) + group;
+    const bool on = row < in.rows;
+    const int c0 = (int)blockIdx.y * kRowVectors * step, c1 = on ? std::min(in.classes, c0 + kRowVectors * step) : c0, whole = c0 + (c1 - c0) / kOf * kOf;
     const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
     T *dst = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
-    bool none;
-    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-    const int c = c0 + at * kOf;
+    const int c = c0 + at * kOf, first = group * kRowVectors * step - c0;  // (first + a class: its cell)
     V x[kRowVectors];
     if constexpr (ALONG) {
 #pragma unroll
         for (int u = 0; u < kRowVectors; ++u)
             if (c + u * step < whole) x[u] = *reinterpret_cast<const V *>(src + c + u * step);
+    }
+    if constexpr (LISTS) shown.count(rules, row, on, c0, c1 - c0, first + c0, at, per_row);
+    if (!on) return;
+    bool none;
+    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
+    if constexpr (ALONG) {
 #pragma unroll
         for (int u = 0; u < kRowVectors; ++u) {
             const int cu = c + u * step;
             if (cu >= whole) break;
             const unsigned ok = none ? 0u : words != nullptr ? words[cu / 32] >> (cu % 32) : ~0u;
-            V v;
+            float s[kOf];
 #pragma unroll
             for (int j = 0; j < kOf; j += 4) {
                 Float4 bias = {0.f, 0.f, 0.f, 0.f};
                 if (rules.bias != nullptr) bias = *reinterpret_cast<const Float4 *>(rules.bias + cu + j);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) v[j + q] = (T)(ok >> (j + q) & 1u ? score_to_float(x[u][j + q]) + bias[q] : -__builtin_inff());
+                for (int q = 0; q < 4; ++q) s[j + q] = score_to_float(x[u][j + q]) + bias[q];
             }
+            if constexpr (LISTS) {
+                // few are: one at a time (a register has no number that a loop can use)
+                unsigned held = shown.bits[(first + cu) / 32] >> ((first + cu) % 32) & ((1u << kOf) - 1u);
+                while (held != 0) {
+                    const int i = __ffs((int)held) - 1;
+                    held &= held - 1;
+                    float its = s[0];
+#pragma unroll
+                    for (int j = 1; j < kOf; ++j) its = i == j ? s[j] : its;
+                    its = held_back(its, shown.times[first + cu + i], rules);
+#pragma unroll
+                    for (int j = 0; j < kOf; ++j) s[j] = i == j ? its : s[j];
+                }
+            }
+            V v;
+#pragma unroll
+            for (int j = 0; j < kOf; ++j) v[j] = (T)(ok >> j & 1u ? s[j] : -__builtin_inff());
             *reinterpret_cast<V *>(dst + cu) = v;
         }
     }
     for (int o = (ALONG ? whole : c0) + at; o < c1; o += per_row) {
-        const float z = score_to_float(src[o]) + (rules.bias != nullptr ? rules.bias[o] : 0.f);
-        dst[(size_t)o * out.class_stride] = (T)(is_in_set(words, none, o) ? z : -__builtin_inff());
+        unsigned times = 0;
+        if constexpr (LISTS) times = shown.bits[(first + o) / 32] >> ((first + o) % 32) & 1u ? shown.times[first + o] : 0u;
+        dst[(size_t)o * out.class_stride] = (T)adjusted(score_to_float(src[o]), rules.bias != nullptr ? rules.bias[o] : 0.f, times, is_in_set(words, none, o), rules);
     }
 }
 
@@ -385,43 +449,21 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns_in_place(tgbm_s
         *z = (T)adjusted(score_to_float(*z), rules.bias != nullptr ? rules.bias[c] : 0.f, times[(c - c0) * kTileRows + lane], is_in_set(words, none, c), rules);
     }
 }
-template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_rows_in_place(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int row_bits) {
-    __shared__ unsigned times_of[kTableClasses];
-    const int per_row = 1 << row_bits, at = threadIdx.x & (per_row - 1), slot = threadIdx.x >> row_bits;
-    unsigned *times = times_of + (size_t)slot * std::min(in.classes, kTableClasses);
-    const long row = (long)blockIdx.x * (kAdjustBlock >> row_bits) + slot;
-    const int c0 = (int)blockIdx.y * kTableClasses, c1 = row < in.rows ? std::min(in.classes, c0 + kTableClasses) : c0;
-    long long b = 0, e = 0;
-    if (row < in.rows) shown_range(rules, row, &b, &e);
-    for (int c = c0 + at; c < c1; c += per_row) times[c - c0] = 0;
-    __syncthreads();
-    for (long long i = b + at; i < e; i += per_row) {
-        const int c = rules.shown[i];
-        if (c >= c0 && c < c1) atomicAdd(&times[c - c0], 1u);
-    }
-    __syncthreads();
-    if (row >= in.rows) return;
-    bool none;
-    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
-    for (int c = c0 + at; c < c1; c += per_row)
-        to[c] = (T)adjusted(score_to_float(to[c]), rules.bias != nullptr ? rules.bias[c] : 0.f, times[c - c0], is_in_set(words, none, c), rules);
-}
-
 template <typename T, bool ALONG>
 void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out) {
     const bool columns = rows_side_by_side(in);
+    if (!columns) {
+        constexpr int kOf = 16 / (int)sizeof(T);
+        int row_bits = 2;
+        while (row_bits < 8 && (kRowVectors * kOf << row_bits) < in.classes) ++row_bits;
+        const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / (kRowVectors * kOf << row_bits) + 1);
+        if (rules.shown != nullptr) k_adjust_rows<T, ALONG, true><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
+        else k_adjust_rows<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
+        return;
+    }
     if (rules.shown != nullptr && in.data == out.data) {
-        if (columns) {
-            const dim3 grid((in.rows - 1) / kTileRows + 1, (in.classes - 1) / kTileClasses + 1);
-            k_adjust_columns_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
-        } else {
-            int row_bits = 3;
-            while (row_bits < 8 && (8 << row_bits) < in.classes) ++row_bits;
-            const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / kTableClasses + 1);
-            k_adjust_rows_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
-        }
+        const dim3 grid((in.rows - 1) / kTileRows + 1, (in.classes - 1) / kTileClasses + 1);
+        k_adjust_columns_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
         return;
     }
     // an entry is compared with its whole list where lists are short, which costs as much as a table for some
@@ -429,19 +471,11 @@ void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &
     const bool lists = rules.shown != nullptr, short_ones = lists && rules.n_shown <= (long long)kShort * in.rows;
     // (and every tile of 128 classes goes through its rows' lists: that pays while there are few)
     constexpr int kTogether = 2048;
-    const bool together = columns && short_ones && in.classes <= kTogether;
-    if (columns) {
-        const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 || together ? 4 : 6;
-        const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << (together ? 4 : quad_bits)) + 1), (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
-        if (together) k_adjust_columns<T, ALONG, true><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, 4);
-        else k_adjust_columns<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
-    } else {
-        constexpr int kOf = 16 / (int)sizeof(T);
-        int row_bits = 2;
-        while (row_bits < 8 && (kRowVectors * kOf << row_bits) < in.classes) ++row_bits;
-        const dim3 grid((in.rows - 1) / (kAdjustBlock >> row_bits) + 1, (in.classes - 1) / (kRowVectors * kOf << row_bits) + 1);
-        k_adjust_rows<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
-    }
+    const bool together = short_ones && in.classes <= kTogether;
+    const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 || together ? 4 : 6;
+    const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << (together ? 4 : quad_bits)) + 1), (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
+    if (together) k_adjust_columns<T, ALONG, true><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, 4);
+    else k_adjust_columns<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
     if (!lists || together) return;
     if (short_ones) k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
     else k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
