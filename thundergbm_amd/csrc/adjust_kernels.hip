@@ -115,33 +115,34 @@ struct ShortLists {
     }
 };
 
-// The lists of the 64 rows of a tile of kTileClasses classes that begin at c0, with counts in LDS of 8 bits: [classes][rows]. Whoever counts a class
-// first puts it on a list, and that list, a part of all entries without any class twice, is what is stored in the end.
+// The lists of the 64 rows of a tile of kTileClasses classes that begin at c0, as counts in LDS of 8 bits: [classes][rows], those of a class and four rows
+// are one word.
 constexpr int kTileRows = 64, kTileClasses = 128;
 struct TileLists {
-    static constexpr int kEntries = 4096, kKept = 8;
+    static constexpr int kKept = 8, kLongest = 255;
     long long begin[kTileRows];
     int before[kTileRows + 1];  // entries of the rows before
-    int fits, held;
+    int fits;                   // no list is longer than a count goes
     unsigned counts[kTileRows * kTileClasses / 4];
-    unsigned short cell_of[kEntries];
 
+    // (all threads of the workgroup come here, and to a barrier behind it)
     __device__ __forceinline__ void count(const tgbm_score_rules &rules, long row0, int rows, int c0, int c1) {
         const uint4 zero = {0, 0, 0, 0};
         for (int i = threadIdx.x; i < kTileRows * kTileClasses / 16; i += kAdjustBlock) reinterpret_cast<uint4 *>(counts)[i] = zero;
         if (threadIdx.x < 64) {
             long long b = 0, e = 0;
             if (row0 + threadIdx.x < rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
-            const bool all_short = __all(e - b <= 255);
+            const bool all_short = __all(e - b <= kLongest);
             const int sum = wave_scan_i(all_short ? (int)(e - b) : 0);
             begin[threadIdx.x] = b;
             before[threadIdx.x + 1] = sum;
-            if (threadIdx.x == 0) before[0] = held = 0;
-            if (threadIdx.x == 63) fits = all_short && sum <= kEntries ? 1 : 0;
+            if (threadIdx.x == 0) {
+                before[0] = 0;
+                fits = all_short ? 1 : 0;
+            }
         }
         __syncthreads();
-        if (!fits) return;
-        const int n = before[kTileRows];
+        const int n = before[kTileRows];  // (0 where they do not fit)
         auto entry = [&](int i, int *r) {
             *r = 0;
 #pragma unroll
@@ -151,8 +152,8 @@ struct TileLists {
         };
         auto add = [&](int c, int r) {
             if ((unsigned)c >= (unsigned)(c1 - c0)) return;
-            const int cell = c * kTileRows + r, shift = cell % 4 * 8;
-            if ((atomicAdd(&counts[cell / 4], 1u << shift) >> shift & 0xffu) == 0) cell_of[atomicAdd(&held, 1)] = (unsigned short)cell;
+            const int cell = c * kTileRows + r;
+            atomicAdd(&counts[cell / 4], 1u << cell % 4 * 8);
         };
         int c[kKept], r[kKept];
 #pragma unroll
@@ -169,17 +170,9 @@ struct TileLists {
             add(cls, of);
         }
     }
-    // (behind a barrier)
+    // Where they do not fit, behind the scores without lists: every entry is compared with its list, four threads to a row.
     template <typename T>
     __device__ __forceinline__ void store(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) const {
-        if (fits) {
-            for (int j = threadIdx.x; j < held; j += kAdjustBlock) {
-                const int cell = cell_of[j];
-                store_held_back<T>(in, rules, out, row0 + cell % kTileRows, c0 + cell / kTileRows, counts[cell / 4] >> (cell % 4 * 8) & 0xffu);
-            }
-            return;
-        }
-        // a long list among them: every entry is compared with its list, four threads to a row
         const long row = row0 + threadIdx.x % kTileRows;
         if (row >= in.rows) return;
         long long b, e;
@@ -210,75 +203,137 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores
 }
 
 // ---------------------------------------------------------------------------------------------- bias and allowed sets
-// Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side.
-// ALONG: out is in the same order. LISTS (quad_bits is 4): the workgroup's part of short lists is stored behind it, while the lines that it touches are in
-// the L2.
-template <typename T, bool ALONG, bool LISTS>
+// Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side. ok: a bit for each of
+// the 32 classes, of each of the four rows.
+__device__ __forceinline__ void allowed_of_rows(const tgbm_score_rules &rules, long row, int rows, int classes, int g, unsigned (&ok)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ok[j] = ~0u;
+    if (rules.allowed == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        bool none;
+        const unsigned *words = allowed_words(rules, std::min(row + j, (long)rows - 1), (classes + 31) / 32, &none);
+        ok[j] = none ? 0u : words != nullptr ? words[g / 32] : ~0u;
+    }
+}
+// ALONG: out is in the same order.
+template <typename T, bool ALONG>
 __global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out, int quad_bits) {
     using V = typename ScoreVector<T, 4>::type;
     static_assert(kAdjustBlock / 64 * 32 == kTileClasses);
-    __shared__ __align__(16) typename std::conditional<LISTS, TileLists, char>::type lists;
     const long tile = tile_of_block(blockIdx.x, gridDim.x);
-    if constexpr (LISTS) {
-        quad_bits = 4;
-        const int first = (int)blockIdx.y * kTileClasses;
-        lists.count(rules, tile * kTileRows, in.rows, first, std::min(in.classes, first + kTileClasses));
-    }
     const int lane = threadIdx.x & 63, step = 64 >> quad_bits;
     const int g = ((int)blockIdx.y * (kAdjustBlock / 64) + (int)(threadIdx.x >> 6)) * 32, end = std::min(g + 32, in.classes);
     const long row = ((tile << quad_bits) + (lane & ((1 << quad_bits) - 1))) * 4;
     const int live = (int)std::min(4l, in.rows - row);
-    if (g < in.classes && live > 0) {
-        unsigned ok[4] = {~0u, ~0u, ~0u, ~0u};
-        if (rules.allowed != nullptr) {
-            const int set_words = (in.classes + 31) / 32;
+    if (g >= in.classes || live <= 0) return;
+    unsigned ok[4];
+    allowed_of_rows(rules, row, in.rows, in.classes, g, ok);
+    int c = g + (lane >> quad_bits);
+    const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
+    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
+    if (ALONG && live == 4) {
+        constexpr int kAtOnce = 8;
+        for (; c < end; c += kAtOnce * step) {
+            V x[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bool none;
-                const unsigned *words = allowed_words(rules, std::min(row + j, (long)in.rows - 1), set_words, &none);
-                ok[j] = none ? 0u : words != nullptr ? words[g / 32] : ~0u;
-            }
-        }
-        int c = g + (lane >> quad_bits);
-        const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
-        T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
-        if (ALONG && live == 4) {
-            constexpr int kAtOnce = 8;
-            for (; c < end; c += kAtOnce * step) {
-                V x[kAtOnce];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    if (c + u * step < end) x[u] = *reinterpret_cast<const V *>(from);
-                    from += (size_t)step * in.class_stride;
-                }
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    if (c + u * step < end) {
-                        const float bias = rules.bias != nullptr ? rules.bias[c + u * step] : 0.f;
-                        V v;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (c + u * step - g) & 1u ? score_to_float(x[u][j]) + bias : -__builtin_inff());
-                        *reinterpret_cast<V *>(to) = v;
-                    }
-                    to += (size_t)step * out.class_stride;
-                }
-            }
-        } else {
-            for (; c < end; c += step) {
-                const float bias = rules.bias != nullptr ? rules.bias[c] : 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < live) to[(size_t)j * out.row_stride] = (T)(ok[j] >> (c - g) & 1u ? score_to_float(from[j]) + bias : -__builtin_inff());
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (c + u * step < end) x[u] = *reinterpret_cast<const V *>(from);
                 from += (size_t)step * in.class_stride;
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                if (c + u * step < end) {
+                    const float bias = rules.bias != nullptr ? rules.bias[c + u * step] : 0.f;
+                    V v;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (c + u * step - g) & 1u ? score_to_float(x[u][j]) + bias : -__builtin_inff());
+                    *reinterpret_cast<V *>(to) = v;
+                }
                 to += (size_t)step * out.class_stride;
             }
         }
+    } else {
+        for (; c < end; c += step) {
+            const float bias = rules.bias != nullptr ? rules.bias[c] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < live) to[(size_t)j * out.row_stride] = (T)(ok[j] >> (c - g) & 1u ? score_to_float(from[j]) + bias : -__builtin_inff());
+            from += (size_t)step * in.class_stride;
+            to += (size_t)step * out.class_stride;
+        }
     }
-    if constexpr (LISTS) {
-        __syncthreads();
-        const int first = (int)blockIdx.y * kTileClasses;
-        lists.template store<T>(in, rules, out, tile * kTileRows, first, std::min(in.classes, first + kTileClasses));
+}
+
+// Rows side by side, with lists: a tile's are counted in LDS while its scores are on their way, and a thread takes the counts of four rows of a class with
+// the scores.
+template <typename T, bool ALONG>
+__global__ __launch_bounds__(kAdjustBlock) void k_adjust_tiles(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
+    using V = typename ScoreVector<T, 4>::type;
+    constexpr int kQuads = kTileRows / 4, kStep = 64 / kQuads, kEach = 32 / kStep;
+    __shared__ __align__(16) TileLists lists;
+    const long tile = tile_of_block(blockIdx.x, gridDim.x);
+    const int lane = threadIdx.x & 63, first = (int)blockIdx.y * kTileClasses, last = std::min(in.classes, first + kTileClasses);
+    const int g = first + (int)(threadIdx.x >> 6) * 32, c = g + lane / kQuads, end = std::min(g + 32, last);
+    const long row = tile * kTileRows + lane % kQuads * 4;
+    const int live = (int)std::min(4l, std::max(0l, in.rows - row));
+    V x[kEach];
+    const T *from = static_cast<const T *>(in.data) + (size_t)c * in.class_stride + row;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+        if (c + u * kStep < end) {
+            if (live == 4) {
+                x[u] = *reinterpret_cast<const V *>(from);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < live) x[u][j] = from[j];
+            }
+        }
+        from += (size_t)kStep * in.class_stride;
     }
+    lists.count(rules, tile * kTileRows, in.rows, first, last);
+    __syncthreads();
+    if (g < end && live > 0) {
+        unsigned ok[4];
+        allowed_of_rows(rules, row, in.rows, in.classes, g, ok);
+        T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int cu = c + u * kStep;
+            if (cu < end) {
+                const float bias = rules.bias != nullptr ? rules.bias[cu] : 0.f;
+                float s[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] = score_to_float(x[u][j]) + bias;
+                unsigned times = lists.counts[(cu - first) * kQuads + lane % kQuads];
+                while (times != 0) {  // (few are shown: one at a time)
+                    const int at = (__ffs((int)times) - 1) / 8;
+                    float its = s[0];
+#pragma unroll
+                    for (int j = 1; j < 4; ++j) its = at == j ? s[j] : its;
+                    its = held_back(its, times >> at * 8 & 0xffu, rules);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[j] = at == j ? its : s[j];
+                    times &= ~(0xffu << at * 8);
+                }
+                V v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (cu - g) & 1u ? s[j] : -__builtin_inff());
+                if (ALONG && live == 4) {
+                    *reinterpret_cast<V *>(to) = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < live) to[(size_t)j * out.row_stride] = v[j];
+                }
+            }
+            to += (size_t)kStep * out.class_stride;
+        }
+    }
+    if (lists.fits) return;
+    __syncthreads();
+    lists.store<T>(in, rules, out, tile * kTileRows, first, last);
 }
 
 // Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them. LISTS: a bit in LDS says that a class was shown, and
@@ -473,10 +528,13 @@ void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &
     constexpr int kTogether = 2048;
     const bool together = short_ones && in.classes <= kTogether;
     const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 || together ? 4 : 6;
-    const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << (together ? 4 : quad_bits)) + 1), (in.classes - 1) / (kAdjustBlock / 64 * 32) + 1);
-    if (together) k_adjust_columns<T, ALONG, true><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, 4);
-    else k_adjust_columns<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
-    if (!lists || together) return;
+    const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << quad_bits) + 1), (in.classes - 1) / kTileClasses + 1);
+    if (together) {
+        k_adjust_tiles<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
+        return;
+    }
+    k_adjust_columns<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
+    if (!lists) return;
     if (short_ones) k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
     else k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
 }
