@@ -26,6 +26,7 @@ LENGTHS = {
     "one_of_255": lambda rng, n: np.where(np.arange(n) == n - 1, 255, 1),
     "many_of_90": lambda rng, n: np.full(n, 90),
     "first_rows": lambda rng, n: np.where(np.arange(n) < 20, 400, 0),
+    "one_of_65536": lambda rng, n: np.where(np.arange(n) == n // 2, 65536, 2),
     "all_long": lambda rng, n: rng.integers(150, 2500, n),
 }
 

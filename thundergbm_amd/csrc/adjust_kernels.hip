@@ -1,8 +1,10 @@
-// tgbm_scores_adjust. One read and one write of every score, by 16 bytes of a thread: bias and allowed sets. Classes that a row was
-// shown are few, so a second launch goes through the lists: for every class that is in a row's list it counts how often, by integers, and
-// stores the score as computed from its beginning over what the first launch has stored. Where `out` is `in` that beginning is gone by
-// then: there the lists are counted in LDS, tile by tile, in the one launch that goes over the scores (100003 x 500 float32, 64 sets and 20
-// shown classes a row: 274 us that way).
+// tgbm_scores_adjust. One read and one write of every score, by 16 bytes of a thread (8 of 16-bit scores whose rows lie side by side); memory bounds it.
+//
+// Shown classes are counted in LDS, by integers, while the scores that a workgroup has asked for are on their way, and whoever holds a score looks up
+// its count: no score is stored twice, so `out` may be `in`. A workgroup takes rows' tiles of 64 x 128 classes, or up to 4096 (8192 of 16 bits) classes of a
+// row. Storing the shown classes' scores behind the others, which touches their lines again, took 150 us where this takes 106 (100003 x 500
+// float32, 64 sets, 20 shown classes a row: 3.8 TB/s of the 5 that a copy reaches; rows do not begin at 16 bytes there, which costs 17 us) and 81 where it
+// takes 58 (512 x 65537 bfloat16, a set for each row, 1500 shown classes a row).
 #include <algorithm>
 #include <type_traits>
 
@@ -23,9 +25,9 @@ typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ bool is_in_set(const unsigned *words, bool none, int c) { return !none && (words == nullptr || (words[c / 32] >> (c % 32) & 1u)); }
 
 // ------------------------------------------------------------------------------------------------------- shown classes
-// The score of class c of a row that was shown it `times` times, from its beginning.
+// The score of class c of a row that was shown it `times` times.
 template <typename T>
-__device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row, int c, unsigned times) {
+__device__ __forceinline__ void store_adjusted(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row, int c, unsigned times) {
     bool none;
     const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
     const float z = score_to_float(static_cast<const T *>(in.data)[(size_t)c * in.class_stride + (size_t)row * in.row_stride]);
@@ -33,116 +35,40 @@ __device__ __forceinline__ void store_held_back(const tgbm_scores &in, const tgb
         (T)adjusted(z, rules.bias != nullptr ? rules.bias[c] : 0.f, times, is_in_set(words, none, c), rules);
 }
 
-// The lists of ROWS rows, one behind the other, in LDS where they fit. A thread takes an entry and looks through the entry's list for others of its
-// class; the first one stores. All threads of the workgroup come to stage(), and to a barrier before store().
-constexpr int kStaged = 4096;
-template <int ROWS>
-struct ShortLists {
-    static_assert(ROWS <= 64);
-    long long begin[ROWS];
-    long long before[ROWS + 1];  // entries of the rows before
-    int staged[kStaged + 4];
-
-    __device__ __forceinline__ int row_of(long long i) const {
-        int r = 0;
-#pragma unroll
-        for (int d = ROWS / 2; d > 0; d >>= 1)
-            if (before[r + d] <= i) r += d;
-        return r;
-    }
-    __device__ __forceinline__ void stage(const tgbm_score_rules &rules, long row0, int rows) {
-        if (threadIdx.x < 64) {
-            long long b = 0, e = 0;
-            if (threadIdx.x < ROWS && row0 + threadIdx.x < rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
-            long long sum = e - b;
-#pragma unroll
-            for (int d = 1; d < ROWS; d <<= 1) {
-                const long long o = __shfl_up(sum, d);
-                if ((int)threadIdx.x >= d) sum += o;
-            }
-            if (threadIdx.x < ROWS) {
-                begin[threadIdx.x] = b;
-                before[threadIdx.x + 1] = sum;
-            }
-            if (threadIdx.x == 0) before[0] = 0;
-        }
-        __syncthreads();
-        if (before[ROWS] <= kStaged)
-            for (int i = threadIdx.x; i < (int)before[ROWS]; i += kAdjustBlock) {
-                const int r = row_of(i);
-                staged[i] = rules.shown[begin[r] + (i - (int)before[r])];
-            }
-    }
-    // of the classes [c0, c1)
-    template <typename T>
-    __device__ __forceinline__ void store(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) const {
-        const long long total = before[ROWS];
-        if (total <= kStaged) {
-            const int n = (int)total;
-            for (int i = threadIdx.x; i < n; i += kAdjustBlock) {
-                const int c = staged[i];
-                if (c < c0 || c >= c1) continue;
-                const int r = row_of(i), first = (int)before[r], last = (int)before[r + 1];
-                unsigned times = 0;
-                bool earlier = false;
-                for (int o = first; o < last; o += 4) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {  // (up to three places behind the list may be looked at, and do not count)
-                        const bool same = staged[o + u] == c && o + u < last;
-                        times += same ? 1u : 0u;
-                        earlier |= same && o + u < i;
-                    }
-                }
-                if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
-            }
-            return;
-        }
-        for (long long i = threadIdx.x; i < total; i += kAdjustBlock) {
-            const int r = row_of(i);
-            const int *list = rules.shown + begin[r];
-            const long long mine = i - before[r], length = before[r + 1] - before[r];
-            const int c = list[mine];
-            if (c < c0 || c >= c1) continue;
-            unsigned times = 0;
-            bool earlier = false;
-            for (long long o = 0; o < length; ++o) {
-                const bool same = list[o] == c;
-                times += same ? 1u : 0u;
-                earlier |= same && o < mine;
-            }
-            if (!earlier) store_held_back<T>(in, rules, out, row0 + r, c, times);
-        }
-    }
-};
-
-// The lists of the 64 rows of a tile of kTileClasses classes that begin at c0, as counts in LDS of 8 bits: [classes][rows], those of a class and four rows
-// are one word.
+// The lists of the 64 rows of a tile of kTileClasses classes that begin at c0, as counts in LDS, [classes][rows]: of 16 bits, or, where a list is longer
+// than those go, of 32 bits for half of the classes at a time.
 constexpr int kTileRows = 64, kTileClasses = 128;
 struct TileLists {
-    static constexpr int kKept = 8, kLongest = 255;
+    static constexpr int kKept = 8, kLongest = 65535;
+    __align__(16) unsigned counts[kTileRows * kTileClasses / 2];
     long long begin[kTileRows];
-    int before[kTileRows + 1];  // entries of the rows before
-    int fits;                   // no list is longer than a count goes
-    unsigned counts[kTileRows * kTileClasses / 4];
+    int before[kTileRows + 1], narrow;  // before: entries of the rows before
 
-    // (all threads of the workgroup come here, and to a barrier behind it)
-    __device__ __forceinline__ void count(const tgbm_score_rules &rules, long row0, int rows, int c0, int c1) {
-        const uint4 zero = {0, 0, 0, 0};
-        for (int i = threadIdx.x; i < kTileRows * kTileClasses / 16; i += kAdjustBlock) reinterpret_cast<uint4 *>(counts)[i] = zero;
+    // whether counts of 16 bits do (all threads of the workgroup come here)
+    __device__ __forceinline__ bool look(const tgbm_score_rules &rules, long row0, int rows) {
         if (threadIdx.x < 64) {
             long long b = 0, e = 0;
             if (row0 + threadIdx.x < rows) shown_range(rules, row0 + threadIdx.x, &b, &e);
-            const bool all_short = __all(e - b <= kLongest);
-            const int sum = wave_scan_i(all_short ? (int)(e - b) : 0);
+            const bool fit = __all(e - b <= kLongest);
+            const int sum = wave_scan_i(fit ? (int)(e - b) : 0);
             begin[threadIdx.x] = b;
             before[threadIdx.x + 1] = sum;
             if (threadIdx.x == 0) {
                 before[0] = 0;
-                fits = all_short ? 1 : 0;
+                narrow = fit ? 1 : 0;
             }
         }
+        clear();
         __syncthreads();
-        const int n = before[kTileRows];  // (0 where they do not fit)
+        return narrow != 0;
+    }
+    __device__ __forceinline__ void clear() {
+        const uint4 zero = {0, 0, 0, 0};
+        for (int i = threadIdx.x; i < kTileRows * kTileClasses / 8; i += kAdjustBlock) reinterpret_cast<uint4 *>(counts)[i] = zero;
+    }
+    // behind look(), and in front of a barrier
+    __device__ __forceinline__ void count(const tgbm_score_rules &rules, int c0, int c1) {
+        const int n = before[kTileRows];
         auto entry = [&](int i, int *r) {
             *r = 0;
 #pragma unroll
@@ -153,7 +79,7 @@ struct TileLists {
         auto add = [&](int c, int r) {
             if ((unsigned)c >= (unsigned)(c1 - c0)) return;
             const int cell = c * kTileRows + r;
-            atomicAdd(&counts[cell / 4], 1u << cell % 4 * 8);
+            atomicAdd(&counts[cell / 2], 1u << cell % 2 * 16);
         };
         int c[kKept], r[kKept];
 #pragma unroll
@@ -170,37 +96,27 @@ struct TileLists {
             add(cls, of);
         }
     }
-    // Where they do not fit, behind the scores without lists: every entry is compared with its list, four threads to a row.
+    // how often class c0 + c was shown to rows 4 * quad to 4 * quad + 3
+    __device__ __forceinline__ uint2 of(int c, int quad) const { return reinterpret_cast<const uint2 *>(counts)[c * (kTileRows / 4) + quad]; }
+    // Long lists: the scores of classes [c0, c1), as many as there are counts of 32 bits, behind clear() and a barrier. Four threads go through a row's list.
     template <typename T>
-    __device__ __forceinline__ void store(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) const {
-        const long row = row0 + threadIdx.x % kTileRows;
-        if (row >= in.rows) return;
-        long long b, e;
-        shown_range(rules, row, &b, &e);
-        for (long long i = b + threadIdx.x / kTileRows; i < e; i += kAdjustBlock / kTileRows) {
+    __device__ __forceinline__ void store_long(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out, long row0, int c0, int c1) {
+        const int r = threadIdx.x % kTileRows, slot = threadIdx.x / kTileRows;
+        const bool on = row0 + r < in.rows;
+        long long b = 0, e = 0;
+        if (on) shown_range(rules, row0 + r, &b, &e);
+#pragma unroll 1
+        for (long long i = b + slot; i < e; i += kAdjustBlock / kTileRows) {
             const int c = rules.shown[i];
-            if (c < c0 || c >= c1) continue;
-            unsigned times = 0;
-            bool earlier = false;
-            for (long long o = b; o < e; ++o) {
-                const bool same = rules.shown[o] == c;
-                times += same ? 1u : 0u;
-                earlier |= same && o < i;
-            }
-            if (!earlier) store_held_back<T>(in, rules, out, row, c, times);
+            if (c >= c0 && c < c1) atomicAdd(&counts[(c - c0) * kTileRows + r], 1u);
+        }
+        __syncthreads();
+        if (on) {
+#pragma unroll 1
+            for (int c = c0 + slot; c < c1; c += kAdjustBlock / kTileRows) store_adjusted<T>(in, rules, out, row0 + r, c, counts[(c - c0) * kTileRows + r]);
         }
     }
 };
-
-constexpr int kListRows = 16;
-template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_short_lists(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
-    __shared__ ShortLists<kListRows> lists;
-    const long row0 = (long)blockIdx.x * kListRows;
-    lists.stage(rules, row0, in.rows);
-    __syncthreads();
-    lists.store<T>(in, rules, out, row0, 0, in.classes);
-}
 
 // ---------------------------------------------------------------------------------------------- bias and allowed sets
 // Rows side by side: a wavefront takes 32 classes of 4 << quad_bits rows, four rows to a thread, 64 >> quad_bits classes side by side. ok: a bit for each of
@@ -292,48 +208,53 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_tiles(tgbm_scores in, t
         }
         from += (size_t)kStep * in.class_stride;
     }
-    lists.count(rules, tile * kTileRows, in.rows, first, last);
-    __syncthreads();
-    if (g < end && live > 0) {
-        unsigned ok[4];
-        allowed_of_rows(rules, row, in.rows, in.classes, g, ok);
-        T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
-#pragma unroll
-        for (int u = 0; u < kEach; ++u) {
-            const int cu = c + u * kStep;
-            if (cu < end) {
-                const float bias = rules.bias != nullptr ? rules.bias[cu] : 0.f;
-                float s[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] = score_to_float(x[u][j]) + bias;
-                unsigned times = lists.counts[(cu - first) * kQuads + lane % kQuads];
-                while (times != 0) {  // (few are shown: one at a time)
-                    const int at = (__ffs((int)times) - 1) / 8;
-                    float its = s[0];
-#pragma unroll
-                    for (int j = 1; j < 4; ++j) its = at == j ? s[j] : its;
-                    its = held_back(its, times >> at * 8 & 0xffu, rules);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[j] = at == j ? its : s[j];
-                    times &= ~(0xffu << at * 8);
-                }
-                V v;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (cu - g) & 1u ? s[j] : -__builtin_inff());
-                if (ALONG && live == 4) {
-                    *reinterpret_cast<V *>(to) = v;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < live) to[(size_t)j * out.row_stride] = v[j];
-                }
-            }
-            to += (size_t)kStep * out.class_stride;
+    const bool mine = g < end && live > 0, narrow = lists.look(rules, tile * kTileRows, in.rows);
+    if (!narrow) {
+        for (int half = first; half < last; half += kTileClasses / 2) {
+            lists.store_long<T>(in, rules, out, tile * kTileRows, half, std::min(last, half + kTileClasses / 2));
+            __syncthreads();
+            lists.clear();
+            __syncthreads();
         }
+        return;
     }
-    if (lists.fits) return;
+    lists.count(rules, first, last);
     __syncthreads();
-    lists.store<T>(in, rules, out, tile * kTileRows, first, last);
+    if (!mine) return;
+    unsigned ok[4];
+    allowed_of_rows(rules, row, in.rows, in.classes, g, ok);
+    T *to = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)c * out.class_stride + (size_t)row * out.row_stride;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+        const int cu = c + u * kStep;
+        if (cu < end) {
+            const float bias = rules.bias != nullptr ? rules.bias[cu] : 0.f;
+            float s[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] = score_to_float(x[u][j]) + bias;
+            const uint2 times = lists.of(cu - first, lane % kQuads);
+            unsigned held = (times.x & 0xffffu ? 1u : 0u) | (times.x >> 16 ? 2u : 0u) | (times.y & 0xffffu ? 4u : 0u) | (times.y >> 16 ? 8u : 0u);
+            while (held != 0) {  // (few are shown: one at a time)
+                const int at = __ffs((int)held) - 1;
+                held &= held - 1;
+                float its = at == 0 ? s[0] : at == 1 ? s[1] : at == 2 ? s[2] : s[3];
+                its = held_back(its, (at < 2 ? times.x : times.y) >> at % 2 * 16 & 0xffffu, rules);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] = at == j ? its : s[j];
+            }
+            V v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (T)(ok[j] >> (cu - g) & 1u ? s[j] : -__builtin_inff());
+            if (ALONG && live == 4) {
+                *reinterpret_cast<V *>(to) = v;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < live) to[(size_t)j * out.row_stride] = v[j];
+            }
+        }
+        to += (size_t)kStep * out.class_stride;
+    }
 }
 
 // Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them. LISTS: a bit in LDS says that a class was shown, and
@@ -475,35 +396,10 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_long_lists(tgbm_scores 
     __syncthreads();
     each([&](int c) {
         const unsigned n = atomicExch(&times[c], 0u);
-        if (n != 0) store_held_back<T>(in, rules, out, row, c0 + c, n);
+        if (n != 0) store_adjusted<T>(in, rules, out, row, c0 + c, n);
     });
 }
 
-// In place: a workgroup takes 64 rows and 128 classes (rows side by side), or 2^row_bits threads a row and up to kTableClasses classes of it.
-template <typename T>
-__global__ __launch_bounds__(kAdjustBlock) void k_adjust_columns_in_place(tgbm_scores in, tgbm_score_rules rules, tgbm_scores out) {
-    __shared__ unsigned times[kTileClasses * kTileRows];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long row = (long)blockIdx.x * kTileRows + lane;
-    const int c0 = (int)blockIdx.y * kTileClasses, c1 = row < in.rows ? std::min(in.classes, c0 + kTileClasses) : c0;
-    for (int i = threadIdx.x; i < kTileClasses * kTileRows; i += kAdjustBlock) times[i] = 0;
-    __syncthreads();
-    long long b = 0, e = 0;
-    if (row < in.rows) shown_range(rules, row, &b, &e);
-    for (long long i = b + wave; i < e; i += kAdjustBlock / 64) {
-        const int c = rules.shown[i];
-        if (c >= c0 && c < c1) atomicAdd(&times[(c - c0) * kTileRows + lane], 1u);
-    }
-    __syncthreads();
-    if (row >= in.rows) return;
-    bool none;
-    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-    T *at = static_cast<T *>(const_cast<void *>(out.data)) + (size_t)row * out.row_stride;
-    for (int c = c0 + wave; c < c1; c += kAdjustBlock / 64) {
-        T *z = at + (size_t)c * out.class_stride;
-        *z = (T)adjusted(score_to_float(*z), rules.bias != nullptr ? rules.bias[c] : 0.f, times[(c - c0) * kTileRows + lane], is_in_set(words, none, c), rules);
-    }
-}
 template <typename T, bool ALONG>
 void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_scores &out) {
     const bool columns = rows_side_by_side(in);
@@ -516,27 +412,20 @@ void adjust_slice(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &
         else k_adjust_rows<T, ALONG, false><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, row_bits);
         return;
     }
-    if (rules.shown != nullptr && in.data == out.data) {
-        const dim3 grid((in.rows - 1) / kTileRows + 1, (in.classes - 1) / kTileClasses + 1);
-        k_adjust_columns_in_place<T><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
-        return;
-    }
-    // an entry is compared with its whole list where lists are short, which costs as much as a table for some
-    constexpr int kShort = 96;
-    const bool lists = rules.shown != nullptr, short_ones = lists && rules.n_shown <= (long long)kShort * in.rows;
-    // (and every tile of 128 classes goes through its rows' lists: that pays while there are few)
-    constexpr int kTogether = 2048;
-    const bool together = short_ones && in.classes <= kTogether;
-    const int quad_bits = in.rows <= 32 ? 2 : in.rows <= 128 || together ? 4 : 6;
+    const bool lists = rules.shown != nullptr;
+    // Every tile of 128 classes goes through its rows' lists. For many classes a second launch that goes through them once costs less, and stores the shown
+    // classes' scores again (it cannot where the scores are gone by then). 20011 x 1000, 150 shown classes a row: 82 us by tiles, 156 that way; 400: 169, 244;
+    // 2000 x 5000: 150: 38, 31; 2000 x 20000: 20: 76, 85; 50: 87, 87.
+    constexpr long long kVisits = 1 << 19;  // classes times shown classes of a row
+    const bool tiles = lists && (in.data == out.data || rules.n_shown <= in.rows * kVisits / in.classes);
+    const int quad_bits = tiles ? 4 : in.rows <= 32 ? 2 : in.rows <= 128 ? 4 : 6;
     const dim3 grid(blocks_of_tiles((in.rows - 1) / (4 << quad_bits) + 1), (in.classes - 1) / kTileClasses + 1);
-    if (together) {
+    if (tiles) {
         k_adjust_tiles<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out);
         return;
     }
     k_adjust_columns<T, ALONG><<<grid, kAdjustBlock, 0, s>>>(in, rules, out, quad_bits);
-    if (!lists) return;
-    if (short_ones) k_adjust_short_lists<T><<<(in.rows - 1) / kListRows + 1, kAdjustBlock, 0, s>>>(in, rules, out);
-    else k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
+    if (lists) k_adjust_long_lists<T><<<dim3(in.rows, (in.classes - 1) / kTableClasses + 1), kAdjustBlock, 0, s>>>(in, rules, out);
 }
 
 template <typename T>
