@@ -139,3 +139,21 @@ def test_top_and_distill_on_a_stream():
     check_distill(loss, O.distill(z, best[1].cpu().numpy(), best[0].cpu().numpy(), None, best[2].cpu().numpy()))
     for values, classes, _ in others:
         assert torch.equal(classes, torch.arange(k, dtype=torch.int32, device="cuda").expand(n, k))
+
+
+@pytest.mark.parametrize("C,n,K", [(33, 16_384, 128), (100, 20_011, 10), (120, 16_389, 7), (300, 16_385, 100), (500, 16_400, 32), (1000, 16_390, 5)])
+def test_distill_many_rows(C, n, K):
+    """Tiles of the shapes that many rows are cut into; rows are looked at here and there."""
+    rng = np.random.default_rng(C)
+    at = np.unique(np.r_[0:40, rng.integers(0, n, 150), n - 40:n])
+    where = torch.from_numpy(at).cuda()
+    z = (rng.standard_normal((C, n)) * 2).astype(np.float32)
+    c, t, full = D.teacher(rng, C, n, K, repeated=True)
+    t = rounded(t, torch.bfloat16)
+    lse = np.log(np.exp(full / 2).sum(1)).astype(np.float32) if C % 200 else None
+    y = rng.integers(0, C, n).astype(np.float32)
+    loss, pairs = S.distill(place(z, "class", pad=1), torch.from_numpy(c).cuda(), torch.from_numpy(t).cuda().bfloat16(), torch.from_numpy(y).cuda(),
+                            None if lse is None else torch.from_numpy(lse).cuda(), 2.0, 0.5)
+    want = O.distill(z[:, at], c[at], t[at], y[at], None if lse is None else lse[at], 2.0, 0.5)
+    check_distill((loss[where], pairs[:, where]), want)
+    assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(pairs).all())

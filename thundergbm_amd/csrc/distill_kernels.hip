@@ -463,12 +463,14 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
 
 // How a call goes: rows of a workgroup, chunks of the classes.
 struct DistillPlan {
-    int rows, chunks, chunk;  // rows 0: few classes
+    int rows, threads, chunks, chunk;  // rows 0: few classes
     size_t lds;
 };
 constexpr int kFewClasses = 32;
-constexpr size_t kTileBytes = 72 * 1024;   // two workgroups a CU,
-constexpr size_t kMostBytes = 144 * 1024;  // or one
+constexpr size_t kMostBytes = 144 * 1024;  // one workgroup a CU,
+constexpr size_t kTileBytes = 72 * 1024;   // or two
+constexpr size_t kSmallBytes = 36 * 1024, kMediumBytes = 48 * 1024;
+constexpr int kManyRows = 16384;
 
 DistillPlan plan_distill(int classes, int rows, int entries) {
     DistillPlan p{};
@@ -477,7 +479,17 @@ DistillPlan plan_distill(int classes, int rows, int entries) {
     if (classes <= kFewClasses) return p;
     auto bytes = [&](int chunk, int r) { return sizeof(float) * ((size_t)r * chunk + 3 * (size_t)entries * (r + 1)); };
     p.rows = rows <= 2 ? 1 : rows <= 8 ? 4 : 16;
-    if (rows > 32 && bytes(classes, 64) <= kTileBytes / 2) p.rows = 64;
+    // Much of a workgroup's time goes by at barriers, where another one's work fills in: as many threads as four, three or two workgroups a CU (that LDS has
+    // room for) need to have their loads on their way. 166 666 x 120, 10 entries: 73 us with 32 rows and 256 threads, 183 with 16 and 1024; 100 000 x 200, 32
+    // entries: 76 with 16 and 256, 129 with 16 and 1024; 40 000 x 500: 70 with 16 and 512, 79 with 16 and 1024; 20 000 x 1000: 67, 65.
+    p.threads = 1024;
+    const bool many = rows >= kManyRows;
+    if (many && bytes(classes, 32) <= kSmallBytes) {
+        p.rows = 32;
+        p.threads = 256;
+    } else if (many && bytes(classes, 16) <= kMediumBytes) {
+        p.threads = bytes(classes, 16) <= kSmallBytes ? 256 : 512;
+    }
     const long row_tiles = ((long)rows - 1) / p.rows + 1;
     long chunks = 1;
     if (bytes(classes, p.rows) > kMostBytes) chunks = (classes - 1) / (long)((kTileBytes / sizeof(float) - 3 * (size_t)entries * (p.rows + 1)) / p.rows) + 1;
@@ -501,12 +513,14 @@ void distill_part(hipStream_t s, const DistillPlan &p, const DistillCall &call, 
 
 template <int R, int B>
 void distill_rows(hipStream_t s, const DistillPlan &p, const DistillCall &call, RowSums *sums) {
-    if (p.chunks == 1) {
-        distill_part<R, B, DISTILL_WHOLE>(s, p, call, nullptr);
-    } else {
-        distill_part<R, B, DISTILL_SUMS>(s, p, call, sums);
-        distill_part<R, B, DISTILL_PAIRS>(s, p, call, sums);
+    if constexpr (B == 1024) {  // (tiles of fewer threads hold all classes)
+        if (p.chunks > 1) {
+            distill_part<R, B, DISTILL_SUMS>(s, p, call, sums);
+            distill_part<R, B, DISTILL_PAIRS>(s, p, call, sums);
+            return;
+        }
     }
+    distill_part<R, B, DISTILL_WHOLE>(s, p, call, nullptr);
 }
 
 }  // namespace
@@ -547,8 +561,12 @@ void launch_scores_distill(hipStream_t s, const tgbm_scores &in, const tgbm_teac
                 break;
             case 1: distill_rows<1, 1024>(s, p, call, sums); break;
             case 4: distill_rows<4, 1024>(s, p, call, sums); break;
-            case 16: distill_rows<16, 1024>(s, p, call, sums); break;
-            default: distill_rows<64, 512>(s, p, call, sums); break;
+            case 32: distill_rows<32, 256>(s, p, call, sums); break;
+            default:
+                if (p.threads == 256) distill_rows<16, 256>(s, p, call, sums);
+                else if (p.threads == 512) distill_rows<16, 512>(s, p, call, sums);
+                else distill_rows<16, 1024>(s, p, call, sums);
+                break;
         }
     }
 }
