@@ -157,3 +157,19 @@ def test_distill_many_rows(C, n, K):
     want = O.distill(z[:, at], c[at], t[at], y[at], None if lse is None else lse[at], 2.0, 0.5)
     check_distill((loss[where], pairs[:, where]), want)
     assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(pairs).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("C", [33, 47, 100, 129, 160, 199, 203, 320, 399, 512])
+def test_top_of_short_rows(C, dtype):
+    """Rows of so few classes that the best ones lie in most of the threads that hold any."""
+    rng = np.random.default_rng(C)
+    n = 70
+    z = rounded(D.scores(rng, C, n, special=0.03), dtype)
+    r = D.rules(rng, C, n, sets="some")
+    want = O.adjusted(z, **r)
+    for order in ("row", "class"):
+        x = place(z, order, dtype, pad=3, shift=1)
+        for k in (8, 16, 20, 25, 32, 33, 50, 128):
+            check_top(S.top(x, k), z, k)
+            check_top(S.top(x, k, **on_gpu(r)), want, k)

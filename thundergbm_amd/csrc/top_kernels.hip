@@ -48,7 +48,7 @@ struct TopShared {
 };
 constexpr int kListRoom = 192;                            // candidates: more than kTopMost
 constexpr int kMostThreads = kTopMost + kTopMost / 4;       // that lay their scores out
-constexpr int candidates_wanted(int k) { return k + (k / 4 > 4 ? k / 4 : 4); }
+__host__ __device__ constexpr int candidates_wanted(int k) { return k + (k / 4 > 4 ? k / 4 : 4); }
 
 template <int M>
 __device__ __forceinline__ int count_from(const unsigned (&b)[M], unsigned least) {
@@ -126,6 +126,14 @@ struct Layout {
     int step, extra;
     __device__ __forceinline__ int at(int t, int i) const { return EXTRA && i == N - 1 ? extra + t : t * V + i / V * step + i % V; }
 };
+// As the former, or one by one: score i of thread t at t + i * 64 * W.
+template <int N_, int V, int W>
+struct DealtLayout {
+    static constexpr int N = N_;
+    int extra;
+    bool dealt;
+    __device__ __forceinline__ int at(int t, int i) const { return dealt ? t + i * 64 * W : Layout<N, V, true>{64 * W * V, extra}.at(t, i); }
+};
 // One wavefront, whose lanes count as several threads each, thread t = lane + 64 * part: lane + 64 * (part * N + i).
 template <int N_>
 struct LaneParts {
@@ -191,7 +199,7 @@ template <int W, typename Scores>
 struct LaidOut {
     static constexpr int kRoom = kListRoom, kWords = Scores::kWords;
     static constexpr int kThreads = W == 1 ? 64 : kMostThreads;
-    unsigned word[kThreads * kWords];
+    __align__(16) unsigned word[kThreads * kWords];
     unsigned short owner[kThreads];
     unsigned long long key[kListRoom];
     int better[W == 1 ? 1 : kListRoom];
@@ -550,6 +558,11 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
     constexpr int kGroups = W == 1 ? kTopBlock / 64 : 1;
     constexpr int V = Vector<T>::kOf, N = E + 1, kStep = 64 * W * V;
     constexpr bool kPairs = held_in_pairs<T, E, RULES>();
+    // Short rows: vectors leave most threads without a score. Where too few are left to choose a bound among, all of their scores would be candidates: they are
+    // dealt out one by one then, through LDS (100 000 x 200 bfloat16, k 20: 78 us, 447 without; k 5, where enough are left: 59, 53). Four wavefronts always do:
+    // 100 000 x 200 float32, k 64: 331 us, 1550 without; 13 333 x 1500, k 128: 282, 309; k 64: 54, 52.
+    constexpr bool kSpread = E == 8;
+    __shared__ __align__(16) float spread[kSpread && W > 1 ? 64 * W * E : 4];
     __shared__ TopShared<W> shared[kGroups];
     using Scores = typename std::conditional<held_in_pairs<T, E, RULES>(), HeldPairs<T, E>, Held<N>>::type;
     __shared__ LaidOut<W, Scores> rooms[kGroups];
@@ -565,6 +578,11 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
         const size_t out_at = (size_t)row * chunks + part;
         const int c0 = part * chunk, size = min(in.classes - c0, chunk), whole_size = size / V * V;
         const Layout<N, V, true> at{kStep, whole_size};
+        const bool dealt = kSpread && (W > 1 || whole_size * 4 < candidates_wanted(k) * V * 5);
+        const typename std::conditional<kSpread, DealtLayout<N, V, W>, Layout<N, V, true>>::type choice_at = [&] {
+            if constexpr (kSpread) return DealtLayout<N, V, W>{whole_size, dealt};
+            else return at;
+        }();
         const int base = (int)one_by_one((unsigned)t * V);  // (places are worked out where they are used, not kept over the tiles)
         const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride + c0;
         Scores held_scores;
@@ -647,6 +665,22 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
                 v[E] = ok ? v[E] : kNothing;
             }
         }
+        if constexpr (kSpread) if (dealt) {
+            auto &v = held_scores.v;
+            float *const of_row = W > 1 ? spread : reinterpret_cast<float *>(rooms[group].word);  // (the lists come later)
+#pragma unroll
+            for (int g = 0; g < E / V; ++g)
+                if (base < whole_size - g * kStep) {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(of_row + base + g * kStep + j) = float4{v[g * V + j], v[g * V + j + 1], v[g * V + j + 2], v[g * V + j + 3]};
+                }
+            if (t < size - whole_size) of_row[whole_size + t] = v[E];
+            group_sync<W>();
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = t + i * 64 * W < size ? of_row[t + i * 64 * W] : kNothing;
+            v[E] = kNothing;
+            group_sync<W>();
+        }
         const float best[1] = {best_of<N>(held_scores)};
         float m, s;
         held_scores.look_again();
@@ -667,7 +701,7 @@ __global__ __launch_bounds__(W == 1 ? kTopBlock : 64 * W, (waves_of_top_rows<T, 
                 sh.part_sum[wave_id()] = s;
             }
         }
-        write_top<W, 1, N>(held_scores, best, at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; }, [&] {
+        write_top<W, 1, N>(held_scores, best, choice_at, k, sh, rooms[group], out_at, out, [&](int p) { return c0 + p; }, [&] {
             const bool in = lane_id() < W;
             const float its_max = in ? sh.part_max[lane_id()] : 0.f, its_sum = in ? sh.part_sum[lane_id()] : 0.f;
             const float all = reference_of(wave_max_f(its_sum > 0.f ? its_max : kNothing));
