@@ -3,10 +3,14 @@
 // A group of wavefronts holds a row, or a chunk of it, in registers. The k-th largest of the threads' own maxima is a lower
 // bound of the k-th largest score: the k threads above it hold one such score each. Any bound that between k and a few more
 // maxima reach will do, so it is found by bisection over the maxima (ballots, no memory). Only the threads whose maximum reaches it, about k of
-// them, can hold a score that does: they lay theirs out in LDS, where all threads look through them side by side, and what reaches the bound -
-// a thread rarely holds two of the best - is put in order by counting. Equal scores are told apart by their class, so that no more
-// than k threads are left where many are equal. Rows that go by chunks leave k scores of each, and a launch of its own makes
-// the same choice among those.
+// them, can hold a score that does: they lay theirs out in LDS, and what reaches the bound - a thread rarely holds two of the best - is listed
+// and put in order by counting. Equal scores are told apart by their class, so that no more than k threads are left where
+// many are equal. Where the list overflows all the same, the k-th score is bisected among those laid out. Rows that go by chunks
+// leave k scores of each, and a launch of its own makes the same choice among those.
+//
+// 2048 x 65537 bfloat16, k 64: 92 us and 9 for the join of three parts a row (the memory's share is 54); 877 vector instructions of a wavefront, three quarters
+// of that time, for 3072 scores: an exponential of each, three looks at it (largest, sum, bound), the search and the list. 50021 x 1000 float32, rows
+// side by side, k 10, sets and lists: 110 us of 42, 806 vector instructions to a row.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -969,7 +973,8 @@ struct TopPlan {
     int parts;  // of a lane's scores, rows side by side
 };
 constexpr int kFewClasses = 32;
-// With up to so many best classes the maxima of 64 lanes give a bound that few scores reach: with all of them the lists overflow.
+// With up to so many best classes the maxima of 64 lanes give a bound that few scores reach: with more the lists overflow, and rows go by the 256
+// maxima of four wavefronts (classes side by side) or of a lane's scores in four parts (rows side by side).
 constexpr int kFewBest = 32;
 // Classes side by side: the most scores that a thread has in whole vectors. Looking for the bound, the list and its order cost about as much as
 // the scores of 24, so rows that fill them go by 48.
