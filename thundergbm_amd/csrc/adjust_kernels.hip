@@ -3,7 +3,7 @@
 // Shown classes are counted in LDS, by integers, while the scores that a workgroup has asked for are on their way, and whoever holds a score looks up
 // its count: no score is stored twice, so `out` may be `in`. A workgroup takes rows' tiles of 64 x 128 classes, or up to 4096 (8192 of 16 bits) classes of a
 // row. Storing the shown classes' scores behind the others, which touches their lines again, took 150 us where this takes 106 (100003 x 500
-// float32, 64 sets, 20 shown classes a row: 3.8 TB/s of the 5 that a copy reaches; rows do not begin at 16 bytes there, which costs 17 us) and 81 where it
+// float32, 64 sets, 20 shown classes a row: 3.8 TB/s of the 5 that a copy reaches; rows do not begin at 16 bytes there, which costs 7 us) and 81 where it
 // takes 58 (512 x 65537 bfloat16, a set for each row, 1500 shown classes a row).
 #include <algorithm>
 #include <type_traits>

@@ -974,8 +974,9 @@ struct TopPlan {
 };
 constexpr int kFewClasses = 32;
 // With up to so many best classes the maxima of 64 lanes give a bound that few scores reach: with more the lists overflow, and rows go by the 256
-// maxima of four wavefronts (classes side by side) or of a lane's scores in four parts (rows side by side).
-constexpr int kFewBest = 32;
+// maxima of four wavefronts (classes side by side; 20 000 x 1000 float32, k 40: 31 us, with four 57; 48: 110, 61; 64: 341, 76), or of a lane's scores in four parts
+// (rows side by side; k 26: 30 us, in parts 35; 32: 52, 37; 64: 1206, 76).
+constexpr int kFewBestRows = 42, kFewBest = 28;
 // Classes side by side: the most scores that a thread has in whole vectors. Looking for the bound, the list and its order cost about as much as
 // the scores of 24, so rows that fill them go by 48.
 constexpr int kRowScores = 24, kRowScoresWide = 48;
@@ -1002,7 +1003,7 @@ TopPlan plan_top(bool columns, int classes, int rows, int k) {
         p.per_thread = std::max(p.per_thread, 2);
         p.row_bits = 4;
         while (p.row_bits < 6 && (p.chunk << (p.row_bits + 1)) <= 16384) ++p.row_bits;
-    } else if (k > kFewBest && p.chunk <= 64 * kRowScores) {
+    } else if (k > kFewBestRows && p.chunk <= 64 * kRowScores) {
         p.waves = 4;
         p.per_thread = 8;
     } else {
