@@ -181,3 +181,16 @@ def test_distill_refuses(lib, capfd):
         assert call(**more) == 1 and msg in capfd.readouterr().err, more
     assert call(a=array(rows=0)) == 0
     assert lib.tgbm_scores_distill_workspace(C.byref(large), 0) == lib.tgbm_scores_distill_workspace(C.byref(large), 129) == 0
+
+
+@pytest.mark.parametrize("rules", [dict(repetition=1e-60), dict(repetition=1e60), dict(repetition=-1.0), dict(frequency=1e300), dict(presence=float("nan"))])
+def test_estimator_refuses_numbers_that_32_bits_do_not_hold(rules):
+    """Before the library sees them, which ends the process."""
+    clf = T.TGBMClassifier(objective="multi:softprob", num_class=3)
+    clf.model, clf.tree_per_iter, clf.group_label = C.c_void_p(ADDRESS), 3, [0.0, 1.0, 2.0]
+    try:
+        with pytest.raises(ValueError, match="above 0"):
+            clf._class_rules(2, None, None, [[1.0], [2.0]], **dict(dict(repetition=1.0, frequency=0.0, presence=0.0), **rules))
+        clf._class_rules(2, None, None, [[1.0], [2.0]], 1.5, 0.1, -0.1)
+    finally:
+        clf.model = None

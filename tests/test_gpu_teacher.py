@@ -162,3 +162,24 @@ def test_refusals_of_the_estimator():
                     (dict(shown=[[]] * n, repetition=0), "repetition"), (dict(k=0), "k is 0"), (dict(k=129), "k is 129"), (dict(temperature=0), "temperature")):
         with pytest.raises(ValueError, match=msg):
             clf.top_classes(X, **kw)
+
+
+def test_session_refuses():
+    """What would end the process is said before the library sees it."""
+    X, y, rng = problem(n=300)
+    s = session(X, y)
+    with pytest.raises(ValueError, match="no teacher"):
+        s.teacher_loss()
+    with pytest.raises(ValueError, match="rows"):
+        s.set_teacher(np.zeros((299, 2)), np.zeros((299, 2)))
+    s.set_teacher(np.zeros((300, 2)), np.zeros((300, 2)))
+    assert np.isfinite(s.teacher_loss())
+    s.set_teacher(None)
+    with pytest.raises(ValueError, match="no teacher"):
+        s.teacher_loss()
+    s.close()
+    val, rp, col = datasets.dense_to_csr(X)
+    s = T.Session(val, rp, col, y, depth=2, n_trees=1, objective="reg:linear")
+    with pytest.raises(ValueError, match="objective"):
+        s.set_teacher(np.zeros((300, 2)), np.zeros((300, 2)))
+    s.close()

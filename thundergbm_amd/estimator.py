@@ -224,7 +224,9 @@ class TGBMModel(BaseEstimator):
             labels = np.concatenate([np.asarray(labels, dtype=np.float32) for labels in shown]) if n else np.zeros(0, np.float32)
             at = np.minimum(np.searchsorted(known, labels), classes - 1)
             lists = np.where(known[at] == labels, at, -1).astype(np.int32)
-            if not (repetition > 0 and np.isfinite(repetition) and np.isfinite(frequency) and np.isfinite(presence)):
+            with np.errstate(over="ignore", under="ignore"):  # (as the 32-bit numbers that they become)
+                numbers = np.array([repetition, frequency, presence], np.float64).astype(np.float32)
+            if not (numbers[0] > 0 and np.isfinite(numbers).all()):
                 raise ValueError("repetition %r, frequency %r, presence %r: numbers are wanted, the first above 0" % (repetition, frequency, presence))
             if len(lists):
                 r.shown, r.shown_begin, r.n_shown = lists.ctypes.data, begin.ctypes.data, len(lists)

@@ -68,6 +68,7 @@ class Session:
         self.n = len(row_ptr) - 1
         self.nnz = int(row_ptr[-1])
         self.depth = depth
+        self.objective, self.has_teacher = objective, False
         # groups: sizes of the query groups (consecutive rows) of the ranking objectives
         grp = np.ascontiguousarray(groups if groups is not None else [], dtype=np.int32)
         self.h = self.L.tgbm_trainer_create_grouped(self.n, _p(val), _p(row_ptr), _p(col), _p(y), depth, n_trees,
@@ -102,13 +103,20 @@ class Session:
         """The rounds from here on train on the loss against a teacher's best scores (scores.distill), with the session's labels:
         classes [rows, entries] are numbers of its ascending distinct labels, scores are float32 or float16 (others become
         float32). None: on the labels alone again."""
+        if self.objective not in ("multi:softmax", "multi:softprob"):
+            raise ValueError("a teacher's class scores need the objective multi:softmax or multi:softprob")
         if classes is None:
             self.L.tgbm_trainer_set_teacher(self.h, None, 1.0, 1.0)
+            self.has_teacher = False
             return
         arrays, t = teacher_arrays(self.n, classes, scores, lse, temperature, weight)
         self.L.tgbm_trainer_set_teacher(self.h, C.byref(t), temperature, weight)
+        self.has_teacher = True
 
     def teacher_loss(self):
+        """The mean of that loss over the rows with the current predictions."""
+        if not self.has_teacher:
+            raise ValueError("there is no teacher")
         return self.L.tgbm_trainer_teacher_loss(self.h)
 
     def sample_columns(self):
