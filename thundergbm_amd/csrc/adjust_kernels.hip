@@ -258,7 +258,7 @@ __global__ __launch_bounds__(kAdjustBlock) void k_adjust_tiles(tgbm_scores in, t
 }
 
 // Classes side by side: 2^row_bits threads to a row, kRowVectors vectors of 16 bytes to each of them. LISTS: a bit in LDS says that a class was shown, and
-// a word how often; the row's threads go through its list meanwhile the scores are on their way.
+// a word how often; the row's threads go through its list while the scores are on their way.
 constexpr int kRowVectors = 4;
 template <int CELLS>
 struct ShownTimes {
