@@ -294,11 +294,12 @@ typedef struct tgbm_teacher {
  * With p = softmax(z / T) and the teacher's q = exp(t / T) over their sum, or exp(t / T - lse) where lse is given:
  *   loss = weight * T^2 * [ sum of q (log q - log p) + r (log r - log R) ] + (1 - weight) * -log softmax(z)[label]
  * r = 1 - sum of q (not below 0) is what the teacher left to the classes that it does not name, taken together, R their p;
- * without lse, or where every class is named, there is no such part. A row without entries has no first part, one whose label is no class's
- * number no second.
- *   gradient = weight * T * (p - q) + (1 - weight) * (softmax(z) - [label]), q of a class that is not named being r p / R
- *   hessian = max(2 (weight * p (1 - p) + (1 - weight) * s (1 - s)), 1e-16), s = softmax(z): the factor of two and the
+ * without lse, or where every class is named or the others' scores are all -infinity, there is no such part. A row without entries has no first part,
+ * one whose label is no class's number no second.
+ *   gradient = weight * T * (M p - q) + (1 - weight) * (softmax(z) - [label]), q of a class that is not named being r p / R
+ *   hessian = max(2 (weight * M p (1 - p) + (1 - weight) * s (1 - s)), 1e-16), s = softmax(z): the factor of two and the
  * least value are those of the objective multi:softmax (multiclass_obj.cu:6-35).
+ * M = sum of q + r is 1, but with an lse where there is no part for r (M = sum of q), or where the sum of q is above 1.
  * Where all scores of a row are -infinity every p is 0; a NaN or an infinite score or teacher's score makes its row NaN.
  * in: float scores, the rows of a class side by side. labels (NULL only where weight is 1): [rows] class numbers as floats. loss (may be NULL): [rows].
  * pairs (may be NULL): gradient and hessian of class c in row i at pairs[2 * (c * pair_stride + i)]. temperature: 1e-3 to

@@ -68,11 +68,12 @@ __device__ __forceinline__ int label_of(const DistillCall &call, long row) {  //
 
 // What turns a row's scores into pairs. Every probability is an exponential to one of the two references times a factor: with
 // e = exp((z - max) / T), e1 = exp(z - max): p = e * p_by, the gradient is e * g_by + e1 * g1_by, less b at the label; a named
-// class's has aT * q less.
+// class's is aT * (mass * p - q). mass: of the teacher altogether, entries and rest, as the derivative of -sum q log p is (sum q) p - q over T: 1, but
+// where what is left over has no class to go to, or the entries have more than 1 together.
 struct RowFactors {
     float other_max, other_p, other_p1, other_g;
     float named_max, named_p, named_p1;
-    float a, b, aT;
+    float a, b, aT, mass;  // a: the weight, times the mass for the hessian
 };
 
 // sum: of all classes; any: the teacher names a class; given: the sum of all entries' q; label < 0: none. Returns the loss as well.
@@ -86,12 +87,14 @@ __device__ __forceinline__ RowFactors factors_of(const RowSums &sum, bool any, f
     f.a = !any ? 0.f : given <= FLT_MAX ? weight : __builtin_nanf("");
     f.b = label >= 0 ? 1.f - weight : 0.f;
     f.aT = f.a * temperature;
-    const float rest = has_rest && others && any ? fmaxf(0.f, 1.f - given) : 0.f;  // the teacher's mass on the other classes
+    const bool takes = has_rest && others && any;
+    const float rest = takes ? fmaxf(0.f, 1.f - given) : 0.f;  // the teacher's mass on the other classes
+    f.mass = !has_rest ? 1.f : takes ? fmaxf(given, 1.f) : given;
     f.other_max = sum.other_max;
     f.named_max = sum.named_max;
     f.other_p = other_up * inv;
     f.named_p = named_up * inv;
-    f.other_g = f.aT * (f.other_p - (rest != 0.f ? rest / sum.other_sum : 0.f));
+    f.other_g = f.aT * (f.mass * f.other_p - (rest != 0.f ? rest / sum.other_sum : 0.f));
     f.other_p1 = f.named_p1 = 0.f;
     float log_Z1 = 0.f;
     if (label >= 0) {
@@ -111,6 +114,7 @@ __device__ __forceinline__ RowFactors factors_of(const RowSums &sum, bool any, f
     }
     if (f.b != 0.f) value += f.b * (log_Z1 - (sum.label - higher));
     *loss = value;
+    f.a *= f.mass;
     return f;
 }
 
@@ -195,7 +199,7 @@ __global__ __launch_bounds__(kFewBlock) void k_distill_few(DistillCall call) {
         const bool is_named = there >> c & 1u;
         const float d = z[c] - (is_named ? f.named_max : f.other_max), e = exp2_of(d * by), e1 = hard ? exp2_of(d * kLog2e) : 0.f;
         const float p = e * (is_named ? f.named_p : f.other_p), p1 = e1 * (is_named ? f.named_p1 : f.other_p1);
-        if (c < classes) *to = pair_of(f, p, p1, is_named ? f.aT * (p - q[c]) : e * f.other_g, c == label);
+        if (c < classes) *to = pair_of(f, p, p1, is_named ? f.aT * (f.mass * p - q[c]) : e * f.other_g, c == label);
         to += call.pair_stride;
     }
 }
@@ -461,7 +465,7 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
         }
         const float d = z - (named ? f.named_max : f.other_max), e = exp2_of(d * by), e1 = hard ? exp2_of(d * kLog2e) : 0.f;
         const float p = e * (named ? f.named_p : f.other_p), p1 = e1 * (named ? f.named_p1 : f.other_p1);
-        to[(size_t)i * call.pair_stride] = pair_of(f, p, p1, named ? f.aT * (p - q) : e * f.other_g, c0 + i == label);
+        to[(size_t)i * call.pair_stride] = pair_of(f, p, p1, named ? f.aT * (f.mass * p - q) : e * f.other_g, c0 + i == label);
     }
 }
 

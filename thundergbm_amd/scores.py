@@ -246,8 +246,10 @@ def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature
 
     With p = softmax(z / T) and R its part on the classes that are not named:
       loss = weight * T^2 * (sum(q * (log q - log p)) + r * (log r - log R)) + (1 - weight) * -log softmax(z)[label]
-      gradient = weight * T * (p - q) + (1 - weight) * (softmax(z) - [label]); q of a class that is not named is r * p / R
-      hessian = max(2 * (weight * p * (1 - p) + (1 - weight) * s * (1 - s)), 1e-16), s = softmax(z), like multi:softmax's."""
+      gradient = weight * T * (M * p - q) + (1 - weight) * (softmax(z) - [label]); q of a class that is not named is r * p / R
+      hessian = max(2 * (weight * M * p * (1 - p) + (1 - weight) * s * (1 - s)), 1e-16), s = softmax(z), like multi:softmax's.
+    M = sum(q) + r is 1, but for rows with a teacher_lse where every class is named or the others' scores are all -inf (no class can take r, the loss has
+    no such part, and M = sum(q)), or where sum(q) is above 1."""
     torch = _torch()
     s = _scores(torch, "scores", scores)
     if s.type != 0 or (s.row_stride != 1 and s.rows > 1):
