@@ -495,15 +495,20 @@ __device__ __forceinline__ float rescaled(float sum, float from, float to, float
     return sum <= FLT_MAX ? sum * exp2_of((from - to) * by) : sum;
 }
 
+// Up to here half a step of max / temperature (in powers of two) is 2^-9 at most, and a factor of 1 - off ln 2 stands for 2^-off within 1e-6. Far beyond, that factor
+// becomes negative.
+constexpr float kShiftMost = 65536.f;
+
 // The largest of a wavefront's scores (0 where it is no number) and the sum of exp((v - it) / temperature). A NaN makes the sum
 // NaN, an infinity makes it infinite. best: the thread's largest.
 template <int E, typename Scores>
 __device__ __forceinline__ void sum_exponentials(const Scores &v, float best, float by, float *reference, float *sum) {
     float m = reference_of(wave_max_f(best));
     float part[4] = {0.f, 0.f, 0.f, 0.f};
-    if (fabsf(m) < 1e30f) {
+    const float shift = m * by;
+    if (fabsf(shift) < kShiftMost) {
         // one multiply-add for the argument; what the product m * by was rounded by is put right in the sum
-        const float shift = m * by, off = __builtin_fmaf(m, by, -shift);
+        const float off = __builtin_fmaf(m, by, -shift);
 #pragma unroll
         for (int i = 0; i < E; ++i) part[i % 4] += exp2_of(__builtin_fmaf(v[i], by, -shift));
         const float s = (part[0] + part[1]) + (part[2] + part[3]);
