@@ -128,3 +128,20 @@ def test_session_whose_teacher_knows_more_classes():
         assert abs(s.teacher_loss() - loss.mean()) <= loss_room.mean() + 2.0**-24 * np.abs(loss).mean()
         s.boost(1)
     s.close()
+
+
+@pytest.mark.parametrize("rest", [0.0, 1.0, 40.0, None])
+@pytest.mark.parametrize("C", [8, 16, 32, 60, 3000])
+def test_masses_that_32_bits_hardly_hold(C, rest):
+    """Entries so far below the best one that their q is less than the least normal number, or none: they add nothing to the loss. rest: what the
+    log-sum-exp lies above the entries' own."""
+    rng = np.random.default_rng(C)
+    T, n, K = 0.1, 300, min(C, 8)
+    z = rng.standard_normal((C, n)).astype(np.float32)
+    classes = np.argsort(rng.random((n, C)), axis=1)[:, :K].astype(np.int32)
+    t = np.zeros((n, K), np.float32)
+    t[:, 2:] = -T * rng.uniform(40 if rest else 80, 90, (n, K - 2))
+    t += rng.standard_normal((n, 1)).astype(np.float32)
+    lse = None if rest is None else (np.log(np.exp(t.astype(np.float64) / np.float32(T)).sum(1)) + rest).astype(np.float32)
+    got, want = check(z, classes, t, None, lse, T)
+    assert np.isfinite(want[0]).all() and bool(torch.isfinite(got[0]).all())

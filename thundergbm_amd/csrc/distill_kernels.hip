@@ -29,6 +29,8 @@ __device__ __forceinline__ bool is_mark(unsigned v) { return v - kMark < (unsign
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * kLn2; }
+// Whether q (log q - log p) counts in the loss: below the least normal number it is 1e-38 times a logarithm, and log_of takes such a q for 0.
+__device__ __forceinline__ bool counts_in_loss(float q) { return !(q < FLT_MIN); }  // (a NaN does)
 __device__ __forceinline__ float reference_of(float m) { return fabsf(m) <= FLT_MAX ? m : 0.f; }
 
 // Of a sum of exponentials: 0 is one of scores that are all -inf, no class has any probability then; one that is infinite or NaN has
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(kFewBlock) void k_distill_few(DistillCall call) {
         s.other_sum += is_named || c >= classes ? 0.f : e;
         s.named_sum1 += is_named ? e1 : 0.f;
         s.other_sum1 += is_named || c >= classes ? 0.f : e1;
-        if (is_named && q[c] != 0.f) {
+        if (is_named && counts_in_loss(q[c])) {
             s.cross += q[c] * (log_of(q[c]) - d / call.temperature);
             s.mass += q[c];
         }
