@@ -145,3 +145,25 @@ def test_masses_that_32_bits_hardly_hold(C, rest):
     lse = None if rest is None else (np.log(np.exp(t.astype(np.float64) / np.float32(T)).sum(1)) + rest).astype(np.float32)
     got, want = check(z, classes, t, None, lse, T)
     assert np.isfinite(want[0]).all() and bool(torch.isfinite(got[0]).all())
+
+
+@pytest.mark.parametrize("offset", [1000.0, -1000.0, 20_000.0])
+@pytest.mark.parametrize("T", [1e-3, 0.01, 1.0])
+@pytest.mark.parametrize("C,n,K", [(8, 60, 5), (40, 50, 12), (300, 30, 128), (500, 16_400, 3), (5000, 4, 60), (40_000, 3, 20)])
+def test_what_a_teacher_s_scores_have_in_common(C, n, K, T, offset):
+    """falls out: without a log-sum-exp the q of a row add up to one, and so the gradient to nothing, however large the scores are."""
+    rng = np.random.default_rng(C + K)
+    z = rng.standard_normal((C, n)).astype(np.float32) * np.float32(min(T, 1) * 2)
+    classes, t, _ = D.teacher(rng, C, n, K, short=False)
+    # (steps that the offset leaves whole, few enough of them that several entries count)
+    t = np.round(t * T * 512) / 512 if T * 512 > 1 else np.round(t / 2) / 512
+    t = (t + offset).astype(np.float32)
+    if n < 1000:
+        (_, pairs), _ = check(z, classes, t, None, None, T)
+    else:
+        at = np.r_[0:30, n - 30:n]
+        got = S.distill(place(z, "class"), on_gpu(classes), on_gpu(t), temperature=T)
+        check_distill((got[0][on_gpu(at)], got[1][:, on_gpu(at)]), N.distill(z[:, at], classes[at], t[at], temperature=T))
+        pairs = got[1]
+    # every p and q is off by at most (4 x + 14 + 4 X + 136 + K + 16) half steps of itself, x of what has a part being a few on average: 600 for all that a row holds
+    assert bool((pairs[..., 0].double().sum(0).abs() <= T * 600 * 2.0**-24).all())

@@ -278,7 +278,7 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
                 if (c + j * kSlots < size) cell[(c + j * kSlots) * R + r] = v[j] == v[j] ? __float_as_uint(v[j]) : kNaN;
         }
     }
-    // the entries: their scores over the temperature for now, -1 for the class of one that is left out
+    // the entries: their scores for now, -1 for the class of one that is left out
     for (int i = threadIdx.x; i < R * K; i += B) {
         const int of = i / K, j = i - of * K;
         int c = -1;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
         if (row0 + of < call.in.rows) {
             const size_t at = given_of(row0 + of) * K + j;
             c = call.teacher.classes[at];
-            t = teacher_at(call.teacher, at) / call.temperature;
+            t = teacher_at(call.teacher, at);
         }
         class_of[j * kPitch + of] = (unsigned)c < (unsigned)call.in.classes && t != kNone ? c : -1;
         q_of[j * kPitch + of] = t;
@@ -301,22 +301,23 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
         }
     group.template reduce<2, 2>(first);
     const bool any = first[1] == 1.f;
-    float norm;  // log of what the exponentials are divided by
+    // q = exp((t - top) / T) * scale: below the row's best entry before anything is rounded, as what all scores have in common may be large over T
+    const float top = reference_of(first[0]);
+    float scale;
     if (call.teacher.lse != nullptr) {
-        norm = on ? call.teacher.lse[given_of(row)] : 0.f;
+        scale = on ? exp2_of((top / call.temperature - call.teacher.lse[given_of(row)]) * kLog2e) : 0.f;
     } else {
-        const float top = reference_of(first[0]);
         float s[1] = {0.f};
         for (int j = slot; j < K; j += kSlots)
-            if (class_of[j * kPitch + r] >= 0) s[0] += exp2_of((q_of[j * kPitch + r] - top) * kLog2e);
+            if (class_of[j * kPitch + r] >= 0) s[0] += exp2_of((q_of[j * kPitch + r] - top) * by);
         group.template reduce<1, 0>(s);
-        norm = top + log_of(s[0]);
+        scale = any ? 1.f / s[0] : 0.f;
     }
     float given = 0.f;
     for (int j = slot; j < K; j += kSlots) {
         const int c = class_of[j * kPitch + r] - c0;
         if (c + c0 < 0) continue;
-        const float q = exp2_of((q_of[j * kPitch + r] - norm) * kLog2e);
+        const float q = exp2_of((q_of[j * kPitch + r] - top) * by) * scale;
         given += q;
         q_of[j * kPitch + r] = q;
         if (c >= 0 && c < size) z_of[j * kPitch + r] = __uint_as_float(cell[c * R + r]);
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(B, 8) void k_distill(DistillCall call, RowSums *__r
         const float z = z_of[j * kPitch + r], d = z - sum.named_max, q = q_of[j * kPitch + r];
         s[2] += exp2_of(d * by);
         if (hard) s[3] += exp2_of(d * kLog2e);
-        if (q != 0.f) {
+        if (counts_in_loss(q)) {
             s[4] += q * (log_of(q) - d / call.temperature);
             s[5] += q;
         }
