@@ -120,7 +120,8 @@ def distill(z, classes, teacher, labels=None, lse=None, temperature=1.0, weight=
             mass = sum(np.exp(t - norm) for _, t in entries)
             r = 0.0
             target, dtarget = q.copy(), dq.copy()
-            if entries and lse is not None and not named.all() and np.any(logp[~named, i] > -np.inf):
+            takes_rest = bool(entries) and lse is not None and not named.all() and bool(np.any(logp[~named, i] > -np.inf))
+            if takes_rest:
                 r = max(0.0, 1.0 - mass)
                 dr = sum_dq + u * (len(entries) + 2)
                 log_R = np.log(p[~named].sum()) if p[~named].sum() > 1e-280 else log_sum(logp[~named, i])
@@ -137,7 +138,7 @@ def distill(z, classes, teacher, labels=None, lse=None, temperature=1.0, weight=
                     soft_room += q[c] * u * (6 * abs(np.log(q[c])) + 8 * abs(logp[c, i]) + 2 * adds + 6 * np.log(C) + 30 + 4 * spread / T)
                 if r > 0:
                     soft += r * (np.log(r) - log_R)
-                if lse is not None and not named.all():
+                if takes_rest:
                     soft_room += dr * (abs(np.log(max(r, dr))) + abs(log_R) + 2) if np.isfinite(log_R) else 0
                     soft_room += r * u * (6 * abs(np.log(r)) if r > 0 else 0) + r * u * (8 * abs(log_R) + 2 * adds + 6 * np.log(C) + 30 + 4 * spread / T)
                 soft_room += 4 * u * abs(soft)

@@ -58,3 +58,16 @@ def test_restatements_agree(C, n, K, T, rest):
         a, b = O.distill(z, classes, t, y, lse, T, weight), N.distill(z, classes, t, y, lse, T, weight)
         np.testing.assert_allclose(a[0], b[0], rtol=0, atol=1e-12)
         np.testing.assert_allclose(a[1], b[1], rtol=0, atol=1e-12)
+
+
+@pytest.mark.parametrize("oracle", [O, N])
+def test_rows_whose_others_are_all_out(oracle):
+    """A row's numbers do not hang on the rows before it, and the first row may be one whose classes that are not named are all at -inf."""
+    z, classes, t, _, lse = left_over("others_out")
+    z[:, 4] = np.random.default_rng(1).standard_normal(len(z))
+    together = oracle.distill(z, classes, t, None, lse, 2.0)
+    for i in range(z.shape[1]):
+        alone = oracle.distill(z[:, i:i + 1], classes[i:i + 1], t[i:i + 1], None, lse[i:i + 1], 2.0)
+        for a, b in zip(together, alone):
+            np.testing.assert_array_equal(a[i:i + 1] if a.ndim == 1 else a[:, i:i + 1], b)
+        assert np.isfinite(alone[0]).all()
