@@ -167,3 +167,20 @@ def test_what_a_teacher_s_scores_have_in_common(C, n, K, T, offset):
         pairs = got[1]
     # every p and q is off by at most (4 x + 14 + 4 X + 136 + K + 16) half steps of itself, x of what has a part being a few on average: 600 for all that a row holds
     assert bool((pairs[..., 0].double().sum(0).abs() <= T * 600 * 2.0**-24).all())
+
+
+@pytest.mark.parametrize("T", [1e-3, 0.05, 30.0, 1e3])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("C,n,K", [(3, 50, 2), (8, 60, 5), (16, 40, 16), (32, 40, 7), (60, 50, 12), (300, 30, 128), (2500, 5, 30), (40_000, 3, 20)])
+def test_ends_of_the_temperatures(C, n, K, rest, T):
+    """Scores as far apart as the temperature makes them count, and scores of trees."""
+    rng = np.random.default_rng(C + K)
+    for spread in (min(T, 3.0), 3.0):
+        z = (rng.standard_normal((C, n)) * spread).astype(np.float32)
+        classes, t, full = D.teacher(rng, C, n, K, short=spread == 3.0)
+        t, full = (t * np.float32(spread / 2.5), full * np.float32(spread / 2.5))
+        f = full.astype(np.float64) / np.float32(T)
+        lse = (f.max(1) + np.log(np.exp(f - f.max(1, keepdims=True)).sum(1))).astype(np.float32) if rest else None
+        y = rng.integers(0, C, n).astype(np.float32)
+        got, _ = check(z, classes, t, y, lse, T, 0.6)
+        assert bool(torch.isfinite(got[0]).all())
