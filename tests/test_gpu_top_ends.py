@@ -34,3 +34,9 @@ def test_ends_of_the_temperatures(C, n, k, T, order):
         r = D.rules(rng, C, n, sets="some")
         got = S.top(place(z, order, torch.bfloat16), k, temperature=T, **on_gpu(r))
         check_top(got, O.adjusted(z, **r), k, T32)
+
+
+def test_length_of_the_lists_as_numpy_s_integer():
+    x = place(np.random.default_rng(1).standard_normal((50, 9)).astype(np.float32), "class")
+    for a, b in zip(S.top(x, np.int64(3)), S.top(x, 3)):
+        assert torch.equal(a, b)

@@ -9,7 +9,7 @@ import scipy.sparse as sp
 from sklearn.base import BaseEstimator, ClassifierMixin, RegressorMixin
 
 from . import _lib
-from .scores import _Rules
+from .scores import _Rules, _list_length
 from .session import Session, teacher_arrays
 
 _PARAMS = ("depth", "n_trees", "n_gpus", "min_child_weight", "lambda_tgbm", "gamma", "max_num_bin", "verbose",
@@ -253,8 +253,7 @@ class TGBMModel(BaseEstimator):
         X = _csr(X)
         n = X.shape[0]
         r, keep = self._class_rules(n, bias, allowed, shown, repetition, frequency, presence)
-        if not 1 <= k <= 128:
-            raise ValueError("k is %r: 1 to 128 is wanted" % (k,))
+        k = _list_length(k)
         if not 1e-6 <= temperature <= 1e6:
             raise ValueError("temperature is %r: 1e-6 to 1e6 is wanted" % (temperature,))
         indptr, indices = np.ascontiguousarray(X.indptr, dtype=np.int32), np.ascontiguousarray(X.indices, dtype=np.int32)

@@ -10,6 +10,7 @@ raise ValueError before anything is launched. The calls take no part in autograd
 import ctypes as C
 import functools
 import math
+import operator
 import sys
 
 from . import _lib
@@ -126,6 +127,17 @@ def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repeti
     return r
 
 
+def _list_length(k):
+    """How many classes are listed, as any type of integer."""
+    try:
+        n = operator.index(k)
+    except TypeError:
+        n = 0
+    if not 1 <= n <= 128:
+        raise ValueError("k is %r: 1 to 128 is wanted" % (k,))
+    return n
+
+
 _functions = {}
 
 
@@ -214,8 +226,7 @@ def top(scores, k, bias=None, allowed=None, allowed_set=None, shown=None, shown_
     torch = _torch()
     s = _scores(torch, "scores", scores)
     r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
-    if not isinstance(k, int) or not 1 <= k <= 128:
-        raise ValueError("k is %r: 1 to 128 is wanted" % (k,))
+    k = _list_length(k)
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError("temperature is %r: 1e-6 to 1e6 is wanted" % (temperature,))
     n, device = s.rows, scores.device
