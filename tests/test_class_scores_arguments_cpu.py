@@ -24,3 +24,12 @@ def test_lengths_of_lists_that_are_refused(k):
             clf.top_classes(np.zeros((2, 2), np.float32), k=k)
     finally:
         clf.model = None
+
+
+def test_groups_beside_a_teacher_are_refused():
+    """They would be dropped."""
+    X, y = np.zeros((4, 2), np.float32), np.arange(4, dtype=np.float32)
+    clf = T.TGBMClassifier(objective="multi:softprob", num_class=4)
+    with pytest.raises(ValueError, match="groups"):
+        clf.fit(X, y, groups=[4], teacher=T.Teacher(np.zeros((4, 1)), np.zeros((4, 1))))
+    assert clf.model is None

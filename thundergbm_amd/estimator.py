@@ -105,8 +105,10 @@ class TGBMModel(BaseEstimator):
             self.model = None
 
     def fit(self, X, y, groups=None, teacher=None):
-        """teacher: a Teacher, for the objectives multi:softmax and multi:softprob."""
+        """teacher: a Teacher, for the objectives multi:softmax and multi:softprob, which know no groups."""
         if teacher is not None:
+            if groups is not None:
+                raise ValueError("groups are for the ranking objectives: a teacher's class scores go without")
             return self._fit_teacher(X, y, teacher)
         lib = _lib.load()
         self._release()
