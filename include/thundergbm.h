@@ -273,7 +273,8 @@ int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, con
  * exp(score / temperature) over all classes: exp(value / temperature - lse) is a listed class's probability. values and
  * classes are [rows][k], the best first, of equal scores the lower class; a class whose score is -infinity or NaN is not
  * listed, and what is left of a list is class -1 with -infinity. lse, [rows], is -infinity where nothing is allowed and
- * NaN where a score is that is not taken out. temperature: 1e-6 to 1e6. workspace: as many bytes as
+ * NaN where a score is that is not taken out. It is a 32-bit number: where value / temperature is large, probabilities from it are off by up to 2^-23 of that
+ * (value / temperature of 1000: one part in 8000). temperature: 1e-6 to 1e6. workspace: as many bytes as
  * tgbm_scores_top_workspace says, whose only use is during the call's work on the stream. */
 size_t tgbm_scores_top_workspace(const tgbm_scores *in, int k);
 int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes,
@@ -301,6 +302,8 @@ typedef struct tgbm_teacher {
  * least value are those of the objective multi:softmax (multiclass_obj.cu:6-35).
  * M = sum of q + r is 1, but with an lse where there is no part for r (M = sum of q), or where the sum of q is above 1.
  * Where all scores of a row are -infinity every p is 0; a NaN or an infinite score or teacher's score makes its row NaN.
+ * Everything is 32 bits: terms of the size of log(classes) cancel in the loss of a student that is near its teacher, so about T^2 * 1e-6 of it is rounding;
+ * with an lse, q is off by up to 2^-23 of score / T, and so is M where no class takes r. A q below 1e-38 is not counted in the loss.
  * in: float scores, the rows of a class side by side. labels (NULL only where weight is 1): [rows] class numbers as floats. loss (may be NULL): [rows].
  * pairs (may be NULL): gradient and hessian of class c in row i at pairs[2 * (c * pair_stride + i)]. temperature: 1e-3 to
  * 1e3, weight: 0 to 1. workspace: as for tgbm_scores_top. */

@@ -10,7 +10,8 @@
 //
 // Memory bounds it where there are pairs to write: 120011 x 1000, 32 bfloat16 entries and labels, 384 us, 3.8 TB/s (370 us of 120064 rows: with others the
 // 128 bytes that 16 rows' pairs of a class are straddle lines). 500000 x 8, five float16 entries and labels: 20 us, 3.4 TB/s. The loss alone is bound by
-// the tiles' barriers: 200000 x 100, ten entries, 41 us, 2.4 TB/s. Few rows wait for their chunks' sums: 24 x 50021, 100 entries, 11 and 18 us.
+// the tiles' barriers: 200000 x 100, ten entries, 41 us, 2.4 TB/s. Few rows wait for their chunks' sums: 24 x 50021, 100 entries, 11 and 18 us. The second
+// launch works its own chunk's sums out once more on the way to its marks: 20000 x 5000, 32 entries and labels, takes 483 us where bytes alone take 241.
 #include <algorithm>
 #include <cfloat>
 

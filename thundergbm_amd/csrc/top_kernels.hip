@@ -8,9 +8,11 @@
 // many are equal. Where the list overflows all the same, the k-th score is bisected among those laid out. Rows that go by chunks
 // leave k scores of each, and a launch of its own makes the same choice among those.
 //
-// 2048 x 65537 bfloat16, k 64: 92 us and 9 for the join of three parts a row (the memory's share is 54); 877 vector instructions of a wavefront, three quarters
-// of that time, for 3072 scores: an exponential of each, three looks at it (largest, sum, bound), the search and the list. 50021 x 1000 float32, rows
-// side by side, k 10, sets and lists: 110 us of 42, 806 vector instructions to a row.
+// 2048 x 65537 bfloat16, k 64: 88 us by the profiler and 9 for the join of three parts a row, 92 together where calls follow one another (the memory's share is
+// 54); 877 vector instructions of a wavefront, three quarters of that time, for 48 scores of a lane: an exponential of each, three looks at it (largest, sum, bound),
+// the search and the list. 50021 x 1000 float32, rows side by side, k 10, sets and lists: 106 us where the memory's share is 42; 806 vector and 510
+// scalar instructions to a row of 16 scores a lane, most of them the same whatever the scores: the search, the list and its order. What a longer list costs
+// short rows stands at kFewBestRows and in k_top_rows.
 #include <algorithm>
 #include <cfloat>
 #include <climits>

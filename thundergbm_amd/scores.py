@@ -222,7 +222,8 @@ def top(scores, k, bias=None, allowed=None, allowed_set=None, shown=None, shown_
 
     The best come first, of equal scores the lower class. A class whose score is -inf or NaN is not listed; a list that is
     not filled ends with class -1 and -inf. lse is the logarithm of the sum of exp(score / temperature) over all classes (-inf
-    where nothing is allowed, NaN where a score is NaN), so that exp(values / temperature - lse[:, None]) are probabilities."""
+    where nothing is allowed, NaN where a score is NaN), so that exp(values / temperature - lse[:, None]) are probabilities; lse being a 32-bit number, they
+    are off by up to 2^-23 of values / temperature where that is large."""
     torch = _torch()
     s = _scores(torch, "scores", scores)
     r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
@@ -260,7 +261,10 @@ def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature
       gradient = weight * T * (M * p - q) + (1 - weight) * (softmax(z) - [label]); q of a class that is not named is r * p / R
       hessian = max(2 * (weight * M * p * (1 - p) + (1 - weight) * s * (1 - s)), 1e-16), s = softmax(z), like multi:softmax's.
     M = sum(q) + r is 1, but for rows with a teacher_lse where every class is named or the others' scores are all -inf (no class can take r, the loss has
-    no such part, and M = sum(q)), or where sum(q) is above 1."""
+    no such part, and M = sum(q)), or where sum(q) is above 1.
+
+    Everything is 32 bits: terms of the size of log(classes) cancel in the loss of a student that is near its teacher, so about T^2 * 1e-6 of it is rounding;
+    with a teacher_lse, q is off by up to 2^-23 of teacher / T. A q below 1e-38 is not counted in the loss."""
     torch = _torch()
     s = _scores(torch, "scores", scores)
     if s.type != 0 or (s.row_stride != 1 and s.rows > 1):
