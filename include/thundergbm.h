@@ -280,6 +280,52 @@ size_t tgbm_scores_top_workspace(const tgbm_scores *in, int k);
 int tgbm_scores_top(const tgbm_scores *in, const tgbm_score_rules *rules, int k, float temperature, float *values, int *classes,
                     float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
+/* How a class is drawn. temperature, p, min_p, k: a number for each row, or NULL where all rows have the same one, which stands beside it.
+ * temperature: 0 takes the best class; else 1e-6 to 1e6 (of the rows' own, those below count as 0, those above as 1e6). k: so many of the best classes are
+ * kept, 0 (of the rows' own also what is below) for all. min_p, 0 to 1: of those, the ones with at least min_p of the best one's probability. p, above 0 and up to 1: of those, the fewest best ones
+ * that have at least p of their probability together. (Of the rows' own, what is beyond 0 or 1 counts as that, and a p of 0 leaves the best class.) */
+typedef struct tgbm_sampling {
+    const float *temperature, *p, *min_p;
+    const int *k;
+    float temperature_all, p_all, min_p_all;
+    int k_all;
+} tgbm_sampling;
+
+/* A class of every row, drawn from softmax(score / temperature) of the scores as the rules leave them, as far as `how` keeps them: the first one, in falling order
+ * of the scores and of equal scores the lower class first, where the sum of the probabilities passes u[row]; u from 0 (the best class) up to, not
+ * including, 1, what is beyond counts as the ends. logp, [rows]: the logarithm of the drawn class's probability among those that are kept. Classes whose
+ * score is -infinity or NaN are never drawn; infinite scores share alike. Where nothing is left a row gets class -1 and -infinity, where one of its numbers is NaN
+ * class -1 and NaN. Sums are 64 bits; a probability below 2^-64 of the best one's counts as none. workspace: as for tgbm_scores_top. */
+size_t tgbm_scores_sample_workspace(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how);
+int tgbm_scores_sample(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+#define TGBM_I8 3
+
+/* Rows of numbers, those of a row side by side: floating ones, or signed ones of 8 bits with a scale for each row, which they are multiplied by. pitch: elements
+ * from one row to the next. padded: not 0 says that all of the pitch can be read behind the last row's numbers too (of 8 bits, where pitch and data are
+ * multiples of 16, such rows are taken as they lie; others are copied into the workspace first). 1 to 65536 features. */
+typedef struct tgbm_rows {
+    const void *data;
+    const float *scale; /* of TGBM_I8 */
+    long long pitch;
+    int type; /* TGBM_F32, TGBM_F16, TGBM_BF16, TGBM_I8 */
+    int rows, features;
+    int padded;
+} tgbm_rows;
+
+/* scale = the row's largest magnitude / 127, q = the nearest whole number (of two the even one) to number / scale, both operations in 32 bits; 0 where the
+ * scale is 0. A row that has an infinity or a NaN gets the scale NaN and zeros. q: [rows][q_pitch] bytes, of which a row's first q_width are written, zeros behind its features;
+ * features <= q_width <= q_pitch. */
+int tgbm_rows_quantise(const tgbm_rows *x, signed char *q, long long q_pitch, int q_width, float *scale, void *stream);
+
+/* Class scores as a product: out's score of class c in row i is (sum of x[i] * weights[c] over the features) * x's scale[i] * weights' scale[c] + bias[c], the
+ * sum exact (of 8-bit numbers, in 32 bits), the other steps in 32 bits, rounded once to out's type. x: of TGBM_I8, or floating rows, which are quantised as
+ * tgbm_rows_quantise does first. weights: of TGBM_I8, a row for each class. bias may be NULL. out shares no memory with the others. */
+size_t tgbm_scores_linear_workspace(const tgbm_rows *x, const tgbm_rows *weights);
+int tgbm_scores_linear(const tgbm_rows *x, const tgbm_rows *weights, const float *bias, const tgbm_scores *out, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
 /* A teacher's best scores: [rows][entries] (1 to 128) classes and scores, in any order, as tgbm_scores_top lists them.
  * Entries whose class is negative or no class of the student, or whose score is -infinity, are left out; entries that name the
  * same class add up. lse (may be NULL): the logarithm of the sum of exp(score / temperature) over all of the teacher's classes. */

@@ -63,6 +63,11 @@ SIGNATURES = {
     "tgbm_scores_adjust": (C.c_int, [_P, _P, _P, _P]),
     "tgbm_scores_distill_workspace": (C.c_size_t, [_P, C.c_int]),
     "tgbm_scores_distill": (C.c_int, [_P, _P, _P, C.c_float, C.c_float, _P, _P, C.c_longlong, _P, C.c_size_t, _P]),
+    "tgbm_rows_quantise": (C.c_int, [_P, _P, C.c_longlong, C.c_int, _P, _P]),
+    "tgbm_scores_linear_workspace": (C.c_size_t, [_P, _P]),
+    "tgbm_scores_linear": (C.c_int, [_P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "tgbm_scores_sample_workspace": (C.c_size_t, [_P, _P, _P]),
+    "tgbm_scores_sample": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "tgbm_scores_top_workspace": (C.c_size_t, [_P, C.c_int]),
     "tgbm_scores_top": (C.c_int, [_P, _P, C.c_int, C.c_float, _P, _P, _P, _P, C.c_size_t, _P]),
 }

@@ -10,7 +10,8 @@ CALIBRATION_LIB = os.path.join(HERE, "libtgbm_calibration.so")
 BIN_DIR = os.path.join(HERE, "bin")
 
 HIP_SOURCES = ["tree_kernels.hip", "level_kernels.hip", "sparse_kernels.hip", "prep_kernels.hip", "cut_kernels.hip", "predict_kernels.hip", "rank_kernels.hip", "trainer.hip",
-               "predictor.hip", "capi.hip", "predict_noalloc.hip", "device_memory.hip", "transfer.hip", "adjust_kernels.hip", "top_kernels.hip", "distill_kernels.hip", "scores_api.hip"]
+               "predictor.hip", "capi.hip", "predict_noalloc.hip", "device_memory.hip", "transfer.hip", "adjust_kernels.hip", "top_kernels.hip", "distill_kernels.hip", "sample_kernels.hip",
+               "linear_kernels.hip", "scores_api.hip"]
 CPP_SOURCES = ["host_io.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

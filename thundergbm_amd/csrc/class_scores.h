@@ -1,5 +1,5 @@
-// Operators on class scores that lie on the GPU: adjusting them before an answer, the best classes of every row, and the
-// loss against a teacher's top scores (the tgbm_scores_* entry points). Launchers are stream-ordered, allocate nothing and
+// Operators on class scores that lie on the GPU: adjusting them before an answer, the best classes of every row, a drawn class, the
+// loss against a teacher's top scores, and scores as a product in 8 bits (the tgbm_scores_* entry points). Launchers are stream-ordered, allocate nothing and
 // never synchronise; the entry points (scores_api.hip) have checked the arguments. None has a counterpart in the reference,
 // whose answers are its arg-max and its softmax over the raw scores (multiclass_obj.cu:44-88) and whose multi-class loss
 // knows labels only (multiclass_obj.cu:6-35).
@@ -16,6 +16,7 @@ namespace tgbm {
 constexpr int kClassesMost = 1 << 22;  // (the tiles of a row are one direction of a launch: at most 65 535)
 constexpr int kSliceRows = 1 << 22;  // rows of a launch
 constexpr int kTopMost = 128;      // classes that top lists
+constexpr int kFeaturesMost = 1 << 16;  // of a product in 8 bits: their sum stays within 31 bits
 constexpr int kTeacherMost = 128;  // entries of a teacher's row
 
 // Whether the arguments of an entry point can be worked on; if not, why not is said on stderr (scores_api.hip).
@@ -51,6 +52,15 @@ void launch_scores_adjust(hipStream_t s, const tgbm_scores &in, const tgbm_score
 size_t scores_top_workspace(bool columns, int classes, int rows, int k);
 void launch_scores_top(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, int k, float temperature, float *values, int *classes, float *lse,
                        void *workspace);
+
+size_t scores_sample_workspace(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how);
+void launch_scores_sample(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp,
+                          void *workspace);
+
+// pad: bytes of a row that are written, zeros behind its features
+void launch_rows_quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pitch, int pad, float *scale);
+size_t scores_linear_workspace(const tgbm_rows &x, const tgbm_rows &weights);
+void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &weights, const float *bias, const tgbm_scores &out, void *workspace);
 
 // row_of (may be null): the teacher's row, and the loss's, of every row of the scores, the labels and the pairs.
 size_t scores_distill_workspace(int classes, int rows, int entries);

@@ -2,6 +2,7 @@
 // cannot be done is said on stderr and returned.
 #include <cmath>
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
 
 #include "class_scores.h"
@@ -83,6 +84,37 @@ int check_temperature(const char *entry, float t) {
     return t >= 1e-6f && t <= 1e6f ? 0 : refused(entry, "temperature is %g: 1e-6 to 1e6 is wanted", t);
 }
 
+int check_sampling(const char *entry, const tgbm_sampling *h) {
+    if (h == nullptr) return refused(entry, "how is null");
+    const float t = h->temperature_all;
+    if (h->temperature == nullptr && !(t == 0.f || (t >= 1e-6f && t <= 1e6f))) return refused(entry, "temperature is %g: 0 or 1e-6 to 1e6 is wanted", t);
+    if (h->p == nullptr && !(h->p_all > 0.f && h->p_all <= 1.f)) return refused(entry, "p is %g: above 0 and up to 1 is wanted", h->p_all);
+    if (h->min_p == nullptr && !(h->min_p_all >= 0.f && h->min_p_all <= 1.f)) return refused(entry, "min_p is %g: 0 to 1 is wanted", h->min_p_all);
+    if (h->k == nullptr && h->k_all < 0) return refused(entry, "k is %d: 0 or more is wanted", h->k_all);
+    return 0;
+}
+
+int check_rows(const char *entry, const char *what, const tgbm_rows *r, bool whole_numbers, bool floating) {
+    if (r == nullptr) return refused(entry, "%s is null", what);
+    const bool is_floating = r->type == TGBM_F32 || r->type == TGBM_F16 || r->type == TGBM_BF16;
+    if (!(is_floating && floating) && !(r->type == TGBM_I8 && whole_numbers)) return refused(entry, "%s: type %d", what, r->type);
+    if (r->rows < 0) return refused(entry, "%s: %d rows", what, r->rows);
+    if (r->features < 1 || r->features > kFeaturesMost) return refused(entry, "%s: %d features: 1 to %d are wanted", what, r->features, kFeaturesMost);
+    if (r->rows > 1 ? r->pitch < r->features : r->pitch < 0) return refused(entry, "%s: a pitch of %lld for %d features", what, r->pitch, r->features);
+    if (r->rows > 0 && r->data == nullptr) return refused(entry, "%s: null data", what);
+    if (r->type == TGBM_I8 && r->rows > 0 && r->scale == nullptr) return refused(entry, "%s: no scales", what);
+    return 0;
+}
+
+// (a single row's pitch says nothing but whether what is behind it can be read)
+tgbm_rows with_pitch(tgbm_rows r) {
+    if (r.pitch < r.features) {
+        r.pitch = r.features;
+        r.padded = 0;
+    }
+    return r;
+}
+
 }  // namespace
 
 namespace tgbm {
@@ -151,5 +183,62 @@ extern "C" int tgbm_scores_distill(const tgbm_scores *in, const tgbm_teacher *te
     const size_t needed = scores_distill_workspace(in->classes, in->rows, teacher->entries);
     if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
     launch_scores_distill(static_cast<hipStream_t>(stream), *in, *teacher, labels, temperature, weight, loss, pairs, pair_stride, nullptr, workspace);
+    return launched(entry);
+}
+
+extern "C" size_t tgbm_scores_sample_workspace(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how) {
+    const char *entry = "tgbm_scores_sample_workspace";
+    if (check_scores(entry, "in", in) != 0 || check_rules(entry, rules, in->rows) != 0 || check_sampling(entry, how) != 0 || in->rows == 0) return 0;
+    return scores_sample_workspace(*in, *rules, *how);
+}
+
+extern "C" int tgbm_scores_sample(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+    const char *entry = "tgbm_scores_sample";
+    int rc = check_scores(entry, "in", in);
+    if (rc == 0) rc = check_rules(entry, rules, in->rows);
+    if (rc == 0) rc = check_sampling(entry, how);
+    if (rc != 0) return rc;
+    if (in->rows == 0) return 0;
+    if (u == nullptr) return refused(entry, "u is null");
+    if (classes == nullptr || logp == nullptr) return refused(entry, "an output is null");
+    const size_t needed = scores_sample_workspace(*in, *rules, *how);
+    if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
+    launch_scores_sample(static_cast<hipStream_t>(stream), *in, *rules, *how, u, classes, logp, workspace);
+    return launched(entry);
+}
+
+extern "C" int tgbm_rows_quantise(const tgbm_rows *x, signed char *q, long long q_pitch, int q_width, float *scale, void *stream) {
+    const char *entry = "tgbm_rows_quantise";
+    if (const int rc = check_rows(entry, "x", x, false, true)) return rc;
+    if (q_width < x->features || q_pitch < q_width) return refused(entry, "q: %d of %lld bytes a row for %d features", q_width, q_pitch, x->features);
+    if (x->rows == 0) return 0;
+    if (q == nullptr || scale == nullptr) return refused(entry, "an output is null");
+    launch_rows_quantise(static_cast<hipStream_t>(stream), with_pitch(*x), q, q_pitch, q_width, scale);
+    return launched(entry);
+}
+
+extern "C" size_t tgbm_scores_linear_workspace(const tgbm_rows *x, const tgbm_rows *weights) {
+    const char *entry = "tgbm_scores_linear_workspace";
+    if (check_rows(entry, "x", x, true, true) != 0 || check_rows(entry, "weights", weights, true, false) != 0 || x->rows == 0 || weights->rows == 0) return 0;
+    return scores_linear_workspace(with_pitch(*x), with_pitch(*weights));
+}
+
+extern "C" int tgbm_scores_linear(const tgbm_rows *x, const tgbm_rows *weights, const float *bias, const tgbm_scores *out, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+    const char *entry = "tgbm_scores_linear";
+    int rc = check_rows(entry, "x", x, true, true);
+    if (rc == 0) rc = check_rows(entry, "weights", weights, true, false);
+    if (rc == 0) rc = check_scores(entry, "out", out);
+    if (rc != 0) return rc;
+    if (x->features != weights->features) return refused(entry, "%d features of x, %d of the weights", x->features, weights->features);
+    if (out->classes != weights->rows || out->rows != x->rows)
+        return refused(entry, "out has %d classes and %d rows, the weights have %d and x has %d", out->classes, out->rows, weights->rows, x->rows);
+    if (x->rows == 0) return 0;
+    const tgbm_rows x_ = with_pitch(*x), w_ = with_pitch(*weights);
+    const size_t needed = scores_linear_workspace(x_, w_);
+    if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
+    if (needed > 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return refused(entry, "the workspace does not begin at 16 bytes");
+    launch_scores_linear(static_cast<hipStream_t>(stream), x_, w_, bias, *out, workspace);
     return launched(entry);
 }

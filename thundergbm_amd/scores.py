@@ -1,6 +1,7 @@
 """Operators on class scores that lie on the GPU, as torch tensors (tgbm_scores_*): what is known besides the model is put on
-the scores (`adjust`), the best classes of every row are listed (`top`), and they
-are held against a teacher's best scores (`distill`). torch is imported by the caller, never here.
+the scores (`adjust`), the best classes of every row are listed (`top`) or one is drawn (`sample`), and they
+are held against a teacher's best scores (`distill`). Scores of a linear layer, as a larger model's last one, are a product in
+8 bits (`linear`) of rows that `quantise` makes. torch is imported by the caller, never here.
 
 Scores are [classes, rows], float32, float16 or bfloat16, in either order: the rows of a class side by side, as trainers and
 predictors hold them, or the classes of a row side by side (`x.t()` of a [rows, classes] tensor). Everything is launched on
@@ -25,6 +26,16 @@ class _Rules(C.Structure):
     _fields_ = [("bias", C.c_void_p), ("allowed", C.c_void_p), ("allowed_set", C.c_void_p), ("shown", C.c_void_p),
                 ("shown_begin", C.c_void_p), ("n_shown", C.c_longlong), ("allowed_sets", C.c_int), ("repetition", C.c_float),
                 ("frequency", C.c_float), ("presence", C.c_float)]
+
+
+class _Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("p", C.c_void_p), ("min_p", C.c_void_p), ("k", C.c_void_p), ("temperature_all", C.c_float),
+                ("p_all", C.c_float), ("min_p_all", C.c_float), ("k_all", C.c_int)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scale", C.c_void_p), ("pitch", C.c_longlong), ("type", C.c_int), ("rows", C.c_int), ("features", C.c_int),
+                ("padded", C.c_int)]
 
 
 class _Teacher(C.Structure):
@@ -124,6 +135,35 @@ def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repeti
         if not (math.isfinite(frequency) and math.isfinite(presence)):
             raise ValueError("frequency is %r, presence is %r: numbers are wanted" % (frequency, presence))
         r.repetition, r.frequency, r.presence = repetition, frequency, presence
+    return r
+
+
+def _rows(torch, name, x, scale=None, whole=False, floating=True):
+    """Rows of numbers, [rows, features]; int8 ones with their scales."""
+    _on_gpu(torch, name, x)
+    kind = _types.get(x.dtype) if floating else None
+    if kind is None and whole and x.dtype == torch.int8:
+        kind = 3
+    if kind is None:
+        raise ValueError("%s: %s is wanted, got %s" % (name, " or ".join((["float32, float16, bfloat16"] if floating else []) + (["int8"] if whole else [])), x.dtype))
+    if x.dim() != 2 or not 1 <= x.shape[1] <= 65536 or x.shape[0] >= 1 << 31:
+        raise ValueError("%s: [rows, features] with 1 to 65536 features is wanted, got %s" % (name, tuple(x.shape)))
+    rows, features = x.shape
+    pitch = x.stride(0) if rows > 1 else features
+    if (features > 1 and x.stride(1) != 1) or pitch < features:
+        raise ValueError("%s: strides %s of a tensor %s: the features of a row lie side by side" % (name, tuple(x.stride()), tuple(x.shape)))
+    r = _Rows(x.data_ptr(), None, pitch, kind, rows, features, 0)
+    if kind == 3:
+        if scale is None:
+            raise ValueError("%s: whole numbers go with a scale for each row" % name)
+        r.scale = _plain(torch, name + "_scale", scale, x, torch.float32, (rows,))
+        # (whether the memory goes on behind the last row as it does behind the others)
+        left = x.untyped_storage().nbytes() - x.storage_offset()
+        if rows == 1 and left >= (features + 15) // 16 * 16:
+            r.pitch = (features + 15) // 16 * 16
+        r.padded = 1 if left >= rows * r.pitch else 0
+    elif scale is not None:
+        raise ValueError("%s_scale goes with whole numbers, %s is %s" % (name, name, x.dtype))
     return r
 
 
@@ -294,6 +334,113 @@ def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature
         _call(torch, scores, "tgbm_scores_distill", C.byref(s), C.byref(t), y, temperature, weight, loss.data_ptr(),
               pairs.data_ptr() if gradient else None, n, room.data_ptr() if size else None, size)
     return loss, pairs
+
+
+def _setting(torch, name, v, scores, dtype, fine, wanted):
+    """A setting of `sample`: (address of the rows' own, 0) or (None, everybody's)."""
+    if isinstance(v, torch.Tensor):
+        return _plain(torch, name, v, scores, dtype, (scores.shape[1],)), 0
+    try:
+        number = operator.index(v) if dtype is torch.int32 else float(v)
+    except (TypeError, ValueError):
+        number = None
+    if number is None or not fine(number):
+        raise ValueError("%s is %r: %s is wanted" % (name, v, wanted))
+    return None, number
+
+
+def sample(scores, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed=None, allowed_set=None, shown=None, shown_begin=None,
+           repetition=1.0, frequency=0.0, presence=0.0):
+    """A class of every row, drawn from softmax(score / temperature) of the scores as `adjust` would leave them: classes int32 [rows], and the
+    logarithm of each one's probability among those that were kept, float32 [rows].
+
+    u: float32 [rows], random numbers from 0 up to 1, not included (what is beyond counts as the ends). With the classes in falling order of their scores, of
+      equal scores the lower class first, the first one is drawn where the sum of the probabilities passes u: 0 draws the best class.
+    k: so many of the best classes are kept; 0: all.
+    min_p: of those, the ones with at least min_p (0 to 1) of the best one's probability.
+    p: of those, the fewest best ones that have at least p (above 0, up to 1) of their probability together.
+    temperature: 0 takes the best class; else 1e-6 to 1e6.
+    Each of these may be a tensor [rows], int32 (k) or float32, with a number for each row: there a k below 0 is all, a p of 0 or below leaves the best class, what is
+    above 1 is 1, a min_p below 0 is 0, temperatures below 1e-6 are 0 and above 1e6 are that.
+
+    Classes whose score is -inf or NaN are never drawn. A row that nothing is left of gets class -1 and -inf, one with a NaN among its numbers class -1 and NaN.
+    Sums are 64 bits, and the same call draws the same classes; a class with less than 2^-64 of the best one's probability counts as one without."""
+    torch = _torch()
+    s = _scores(torch, "scores", scores)
+    r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
+    n = s.rows
+    at = _plain(torch, "u", u, scores, torch.float32, (n,))
+    h = _Sampling()
+    h.temperature, h.temperature_all = _setting(torch, "temperature", temperature, scores, torch.float32, lambda v: v == 0 or 1e-6 <= v <= 1e6, "0 or 1e-6 to 1e6")
+    h.p, h.p_all = _setting(torch, "p", p, scores, torch.float32, lambda v: 1e-37 <= v <= 1, "1e-37 to 1")
+    h.min_p, h.min_p_all = _setting(torch, "min_p", min_p, scores, torch.float32, lambda v: 0 <= v <= 1, "0 to 1")
+    h.k, h.k_all = _setting(torch, "k", k, scores, torch.int32, lambda v: v >= 0, "0 or more")
+    h.k_all = min(h.k_all, s.classes) if h.k is None else 0
+    classes = torch.empty(n, dtype=torch.int32, device=scores.device)
+    logp = torch.empty(n, dtype=torch.float32, device=scores.device)
+    if n:
+        size = _lib.load().tgbm_scores_sample_workspace(C.byref(s), C.byref(r), C.byref(h))
+        room = torch.empty(size, dtype=torch.uint8, device=scores.device) if size else None
+        _call(torch, scores, "tgbm_scores_sample", C.byref(s), C.byref(r), C.byref(h), at, classes.data_ptr(), logp.data_ptr(),
+              room.data_ptr() if size else None, size)
+    return classes, logp
+
+
+def quantise(x):
+    """Rows of numbers in 8 bits: (q int8 [rows, features], scale float32 [rows]), x being about q * scale[:, None].
+
+    x: float32, float16 or bfloat16 [rows, features], the features of a row side by side, 1 to 65536 of them.
+    scale is the row's largest magnitude / 127 and q the nearest whole number (of two the even one) to x / scale, 0 where the scale is 0. A row that
+    holds an infinity or a NaN gets the scale NaN and zeros. Rows of q begin at multiples of 128 bytes, with zeros behind their features: as `linear`
+    takes them without copying."""
+    torch = _torch()
+    r = _rows(torch, "x", x)
+    width = (r.features + 127) // 128 * 128
+    q = torch.empty((r.rows, width), dtype=torch.int8, device=x.device)
+    scale = torch.empty(r.rows, dtype=torch.float32, device=x.device)
+    if r.rows:
+        _call(torch, x, "tgbm_rows_quantise", C.byref(r), q.data_ptr(), width, width, scale.data_ptr())
+    return q[:, :r.features], scale
+
+
+def linear(x, weight, weight_scale, bias=None, x_scale=None, order="row", dtype=None):
+    """Class scores of a linear layer in 8 bits, [classes, rows]: (sum of x[i] * weight[c] over the features) * x_scale[i] * weight_scale[c] + bias[c].
+
+    x: [rows, features], int8 with x_scale float32 [rows], or float32, float16 or bfloat16, which are quantised first as `quantise` does.
+    weight, weight_scale: int8 [classes, features] and float32 [classes], as `quantise` makes them of the layer's weights, once. Rows that begin at multiples of 16
+      bytes are read as they lie; others (and int8 rows of x whose features are no multiple of 128) are copied at every call.
+    bias: float32 [classes].
+    order: "row": the classes of a row side by side, "class": the rows of a class, as the trainer's operators want them.
+    dtype: of the scores, float32 (the default), float16 or bfloat16.
+    The sum is exact; the steps behind it are 32 bits, rounded once to the scores' type. A row whose scale is NaN has scores that are."""
+    torch = _torch()
+    r = _rows(torch, "x", x, x_scale, whole=True)
+    w = _rows(torch, "weight", weight, weight_scale, whole=True, floating=False)
+    if weight.device != x.device:
+        raise ValueError("weight is on %s, x is on %s" % (weight.device, x.device))
+    if w.features != r.features:
+        raise ValueError("%d features of x, %d of the weights" % (r.features, w.features))
+    if not 1 <= w.rows <= 1 << 22:
+        raise ValueError("weight: %d classes" % w.rows)
+    dtype = torch.float32 if dtype is None else dtype
+    kind = _types.get(dtype)
+    if kind is None:
+        raise ValueError("dtype: float32, float16 or bfloat16 is wanted, got %s" % (dtype,))
+    if order not in ("row", "class"):
+        raise ValueError("order is %r: \"row\" or \"class\" is wanted" % (order,))
+    b = None if bias is None else _plain(torch, "bias", bias, x, torch.float32, (w.rows,))
+    n, classes = r.rows, w.rows
+    if order == "row":
+        out = torch.empty((n, classes), dtype=dtype, device=x.device).t()
+        o = _Scores(out.data_ptr(), 1, classes, kind, classes, n)
+    else:
+        out = torch.empty((classes, n), dtype=dtype, device=x.device)
+        o = _Scores(out.data_ptr(), max(n, 1), 1, kind, classes, n)
+    if n:
+        size = _lib.load().tgbm_scores_linear_workspace(C.byref(r), C.byref(w))
+        room = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _call(torch, x, "tgbm_scores_linear", C.byref(r), C.byref(w), b, C.byref(o), room.data_ptr() if size else None, size)
+    return out
 
 
 def _apart(s, o, size):
