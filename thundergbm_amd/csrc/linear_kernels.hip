@@ -6,6 +6,8 @@
 //
 // Rows are brought to a common form first, kChunk features at a time with zeros behind the last: where a row of features is zero it does not matter what
 // the weights' rows hold there.
+#include <algorithm>
+
 #include "kernel_common.h"
 #include "score_rules.h"
 
@@ -51,61 +53,230 @@ __global__ __launch_bounds__(kLinearBlock) void k_pack(const signed char *x, lon
     for (int i = threadIdx.x; i < pad; i += kLinearBlock) to[(size_t)blockIdx.x * pad + i] = i < features ? row[i] : (signed char)0;
 }
 
-// 64 classes x 64 rows to a workgroup, 16 classes to a wavefront. Every operand row's next kChunk bytes at a time.
-constexpr int kTile = 64;
 struct Rows8 {
     const signed char *data;
     const float *scale;
     long long pitch;
     int rows;
 };
-template <typename O>
-__global__ __launch_bounds__(kLinearBlock) void k_linear(Rows8 x, Rows8 w, int features, const float *bias, O *out, long long class_stride, long long row_stride) {
-    __shared__ __align__(16) signed char ws[kTile][kChunk + 16], xs[kTile][kChunk + 16];
-    const int c0 = blockIdx.x * kTile, r0 = blockIdx.y * kTile, lane = lane_id(), wave = wave_id();
-    const int whole = (features + 15) / 16 * 16;
-    Int4 sum[4] = {};
-    for (int f0 = 0; f0 < features; f0 += kChunk) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kTile * kChunk / 16; i += kLinearBlock) {
-            const int row = i / (kChunk / 16), f = i % (kChunk / 16) * 16;
-            const Int4 zero = {0, 0, 0, 0};
-            // (what lies behind the features of a weights' row meets zeros)
-            *reinterpret_cast<Int4 *>(&ws[row][f]) =
-                c0 + row < w.rows && f0 + f < whole ? *reinterpret_cast<const Int4 *>(w.data + (size_t)(c0 + row) * w.pitch + f0 + f) : zero;
-            *reinterpret_cast<Int4 *>(&xs[row][f]) = r0 + row < x.rows ? *reinterpret_cast<const Int4 *>(x.data + (size_t)(r0 + row) * x.pitch + f0 + f) : zero;
+typedef int Int16 __attribute__((ext_vector_type(16)));
+typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// (as three operations, whichever kernel does it)
+__device__ __forceinline__ float score_of(int sum, float x_scale, float w_scale, float bias) {
+#pragma clang fp contract(off)
+    return (float)sum * x_scale * w_scale + bias;
+}
+
+// What a tile's lines and columns are: `lines` follow one another in the scores' memory. In one order of the scores those are the classes, in the other the rows.
+struct Product {
+    Rows8 lines, columns;
+    const float *bias;
+    int features;
+    void *out;
+    long long column_stride;
+};
+
+__device__ __forceinline__ void to_lds(const signed char *from, signed char *to) {  // 16 bytes of each lane, to 16 bytes behind the lane below's
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// LDS of a workgroup: two stages, and in their place, when they are done with, 32 columns of each wavefront's scores on their way out and the scales.
+template <typename O, int LINES>
+__host__ __device__ constexpr int line_pitch() { return LINES + 16 / (int)sizeof(O); }
+template <typename O, int BL, int BC, int WL, int WC>
+__host__ __device__ constexpr int lds_of_scores() { return (int)sizeof(O) * WL * WC * 32 * line_pitch<O, BL / WL>(); }
+template <typename O, int BL, int BC, int WL, int WC>
+constexpr size_t lds_of_tiles() { return std::max(2 * (BL + BC) * kChunk, lds_of_scores<O, BL, BC, WL, WC>() + 2 * (BL + BC) * (int)sizeof(float)); }
+
+// BL lines x BC columns to a workgroup of WL * WC wavefronts. Two stages of kChunk bytes of every line and column in LDS: while the wavefronts work on one the
+// other one is on its way there. A line's 16-byte parts lie in an order that goes by the line, so that the lanes of a read, which look at the same part of
+// 32 lines, find them in different banks. CLASSES: the lines are classes.
+template <typename O, int BL, int BC, int WL, int WC, bool CLASSES>
+__global__ __launch_bounds__(64 * WL * WC, 2) void k_linear_tiles(Product p, int line_tiles, int column_tiles) {
+    constexpr int kWaves = WL * WC, kL = BL / WL / 32, kC = BC / WC / 32, kStage = (BL + BC) * kChunk;
+    extern __shared__ __align__(16) signed char lds[];
+    // Neighbouring tiles on one die, by columns of kBand tiles of lines
+    constexpr int kBand = 8;
+    const int tiles = line_tiles * column_tiles, tile = (int)tile_of_block(blockIdx.x, gridDim.x);
+    if (tile >= tiles) return;
+    const int band = tile / (kBand * column_tiles), in_band = tile - band * kBand * column_tiles, high = min(kBand, line_tiles - band * kBand);
+    const int l0 = (band * kBand + in_band % high) * BL, c0 = in_band / high * BC;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const int chunks = (p.features + kChunk - 1) / kChunk, whole = (p.features + 15) / 16 * 16;
+
+    // a wavefront brings eight lines at a time
+    constexpr int kLoadL = BL / 8 / kWaves, kLoadC = BC / 8 / kWaves;
+    const int part = (lane % 8) ^ (lane / 8);
+    const signed char *const of_l = p.lines.data + (size_t)l0 * p.lines.pitch, *const of_c = p.columns.data + (size_t)c0 * p.columns.pitch;
+    unsigned at_l[kLoadL], at_c[kLoadC];  // (from a tile's first line: 256 lines of up to 2^17 bytes)
+#pragma unroll
+    for (int i = 0; i < kLoadL; ++i) at_l[i] = (unsigned)min((wave * kLoadL + i) * 8 + lane / 8, p.lines.rows - 1 - l0) * (unsigned)p.lines.pitch + part * 16;
+#pragma unroll
+    for (int i = 0; i < kLoadC; ++i) at_c[i] = (unsigned)min((wave * kLoadC + i) * 8 + lane / 8, p.columns.rows - 1 - c0) * (unsigned)p.columns.pitch + part * 16;
+    auto bring = [&](int chunk, int stage) {
+        signed char *to = lds + stage * kStage;
+        // weights may end with their features: what is read instead, a line's begin, meets zeros
+        const int f = chunk * kChunk;
+        const unsigned back = f + part * 16 >= whole ? f + part * 16 : 0;
+#pragma unroll
+        for (int i = 0; i < kLoadL; ++i) to_lds(of_l + (at_l[i] + f - (CLASSES ? back : 0u)), to + (wave * kLoadL + i) * 8 * kChunk);
+#pragma unroll
+        for (int i = 0; i < kLoadC; ++i) to_lds(of_c + (at_c[i] + f - (CLASSES ? 0u : back)), to + (BL + (wave * kLoadC + i) * 8) * kChunk);
+    };
+    const int wl = wave / WC * (BL / WL), wc = wave % WC * (BC / WC);
+    Int16 sum[kL][kC] = {};
+    bring(0, 0);
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const signed char *stage = lds + (chunk & 1) * kStage;
+        Int4 a[4][kL], b[4][kC];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = lane % 32 * kChunk + (((k * 2 + lane / 32) ^ (lane % 8)) * 16);
+#pragma unroll
+            for (int i = 0; i < kL; ++i) a[k][i] = *reinterpret_cast<const Int4 *>(stage + (wl + i * 32) * kChunk + at);
+#pragma unroll
+            for (int j = 0; j < kC; ++j) b[k][j] = *reinterpret_cast<const Int4 *>(stage + (BL + wc + j * 32) * kChunk + at);
         }
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        bring(min(chunk + 1, chunks - 1), (chunk + 1) & 1);  // (once more at the end: a branch would wait for the reads)
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < kChunk; k += 64) {
-            const Int4 a = *reinterpret_cast<const Int4 *>(&ws[wave * 16 + lane % 16][k + lane / 16 * 16]);
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const Int4 b = *reinterpret_cast<const Int4 *>(&xs[j * 16 + lane % 16][k + lane / 16 * 16]);
-                sum[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, sum[j], 0, 0, 0);
+            for (int j = 0; j < kC; ++j)
+#pragma unroll
+                for (int i = 0; i < kL; ++i) sum[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[k][i], b[k][j], sum[i][j], 0, 0, 0);
+    }
+    // The scores, 32 columns of a wavefront at a time, by way of LDS: a column's lines are stored side by side.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    constexpr int kPitch = line_pitch<O, BL / WL>(), kThreads = 64 * kWaves;
+    O *const mine = reinterpret_cast<O *>(lds) + wave * 32 * kPitch;
+    float *const l_scale = reinterpret_cast<float *>(lds + lds_of_scores<O, BL, BC, WL, WC>()), *const l_bias = l_scale + BL, *const c_scale = l_bias + BL, *const c_bias = c_scale + BC;
+    for (int i = threadIdx.x; i < BL; i += kThreads) {
+        const int l = min(l0 + i, p.lines.rows - 1);
+        l_scale[i] = p.lines.scale[l];
+        if (CLASSES) l_bias[i] = p.bias != nullptr ? p.bias[l] : 0.f;
+    }
+    for (int i = threadIdx.x; i < BC; i += kThreads) {
+        const int c = min(c0 + i, p.columns.rows - 1);
+        c_scale[i] = p.columns.scale[c];
+        if (!CLASSES) c_bias[i] = p.bias != nullptr ? p.bias[c] : 0.f;
+    }
+    __syncthreads();
+    typedef O Four __attribute__((ext_vector_type(4)));
+    constexpr int kOf = 16 / (int)sizeof(O), kLanes = BL / WL / kOf;  // lanes that store a column
+    typedef O Vec __attribute__((ext_vector_type(16 / sizeof(O))));
+    typedef O Loose __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+        const float by = c_scale[wc + j * 32 + lane % 32], of_column = CLASSES ? 0.f : c_bias[wc + j * 32 + lane % 32];
+#pragma unroll
+        for (int i = 0; i < kL; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = i * 32 + g * 8 + lane / 32 * 4;
+                const float4 its = *reinterpret_cast<const float4 *>(l_scale + wl + at);
+                const float4 bias = CLASSES ? *reinterpret_cast<const float4 *>(l_bias + wl + at) : float4{of_column, of_column, of_column, of_column};
+                Four z;
+                const auto score = [&](int q, float s, float more) { return (O)(CLASSES ? score_of(sum[i][j][g * 4 + q], by, s, more) : score_of(sum[i][j][g * 4 + q], s, by, more)); };
+                z[0] = score(0, its.x, bias.x);
+                z[1] = score(1, its.y, bias.y);
+                z[2] = score(2, its.z, bias.z);
+                z[3] = score(3, its.w, bias.w);
+                *reinterpret_cast<Four *>(mine + lane % 32 * kPitch + at) = z;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int step = 0; step < 32 * kLanes / 64; ++step) {
+            const int c = step * (64 / kLanes) + lane / kLanes, col = c0 + wc + j * 32 + c, at = lane % kLanes * kOf, line = l0 + wl + at;
+            if (col >= p.columns.rows || line >= p.lines.rows) continue;
+            O *to = static_cast<O *>(p.out) + (size_t)col * p.column_stride + line;
+            const Vec v = *reinterpret_cast<const Vec *>(mine + c * kPitch + at);
+            if (line + kOf <= p.lines.rows) {
+                *reinterpret_cast<Loose *>(to) = v;
+            } else {
+#pragma unroll
+                for (int q = 0; q < kOf; ++q)
+                    if (line + q < p.lines.rows) to[q] = v[q];
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// Few rows: 16 classes and 16 * R rows to a wavefront, which reads them as the product wants them, without LDS; S wavefronts share the features.
+template <typename O, int R, int S>
+__global__ __launch_bounds__(kLinearBlock) void k_linear_few(Rows8 x, Rows8 w, int features, const float *bias, O *out, long long class_stride, long long row_stride) {
+    constexpr int kTiles = kLinearBlock / 64 / S;
+    __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * R : 1][64];
+    const int lane = lane_id(), wave = wave_id(), share = wave % S, tile = wave / S;
+    const int c0 = ((int)blockIdx.x * kTiles + tile) * 16, r0 = (int)blockIdx.y * 16 * R;
+    const int chunks = (features + kChunk - 1) / kChunk, whole = (features + 15) / 16 * 16;
+    const signed char *of_class = w.data + (size_t)min(c0 + lane % 16, w.rows - 1) * w.pitch;
+    const signed char *of_row[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) of_row[j] = x.data + (size_t)min(r0 + j * 16 + lane % 16, x.rows - 1) * x.pitch;
+    Int4 sum[R] = {};
+    const int first = chunks * share / S, last = chunks * (share + 1) / S;
+    // (which of the features a lane takes is its own affair, as long as it is the same of both)
+    auto step = [&](int f, bool tail) {
+        Int4 a[2], b[R][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = f + lane / 16 * 32 + h * 16;
+            a[h] = *reinterpret_cast<const Int4 *>(of_class + (tail && at >= whole ? 0 : at));
+#pragma unroll
+            for (int j = 0; j < R; ++j) b[j][h] = *reinterpret_cast<const Int4 *>(of_row[j] + at);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < R; ++j) sum[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h], b[j][h], sum[j], 0, 0, 0);
+    };
+    int c = first;
+    for (; c + 4 < last; c += 4) {  // (the last one apart)
+        step(c * kChunk, false);
+        step((c + 1) * kChunk, false);
+        step((c + 2) * kChunk, false);
+        step((c + 3) * kChunk, false);
+    }
+    for (; c < last; ++c) step(c * kChunk, c == last - 1);
+    if constexpr (S > 1) {
+        if (share > 0) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) shared[(tile * (S - 1) + share - 1) * R + j][lane] = sum[j];
+        }
+        __syncthreads();
+        if (share > 0) return;
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s)
+#pragma unroll
+            for (int j = 0; j < R; ++j) sum[j] += shared[(tile * (S - 1) + s) * R + j][lane];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < R; ++j) {
         const int row = r0 + j * 16 + lane % 16;
         if (row >= x.rows) continue;
         const float by = x.scale[row];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = c0 + wave * 16 + lane / 16 * 4 + i;
-            if (c >= w.rows) continue;
-            float z = (float)sum[j][i] * by * w.scale[c];
-            if (bias != nullptr) z += bias[c];
-            out[(size_t)c * class_stride + (size_t)row * row_stride] = (O)z;
+            const int cls = c0 + lane / 16 * 4 + i;
+            if (cls < w.rows)
+                out[(size_t)cls * class_stride + (size_t)row * row_stride] = (O)score_of(sum[j][i], by, w.scale[cls], bias != nullptr ? bias[cls] : 0.f);
         }
     }
 }
 
 constexpr size_t kPackedBytes = (size_t)512 << 20;  // of a slice's features
 
+constexpr long long kPitchMost = 1 << 17;  // places in a tile are 32 bits
 bool lies_well(const tgbm_rows &r) {
-    return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.pitch % 16 == 0 && (r.features % 16 == 0 || r.padded);
+    return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.pitch % 16 == 0 && r.pitch <= kPitchMost && (r.features % 16 == 0 || r.padded);
 }
 long long pad_of(int features) { return ((long long)features + kChunk - 1) / kChunk * kChunk; }
 bool packs_weights(const tgbm_rows &w) { return !lies_well(w); }
@@ -113,17 +284,50 @@ bool packs_features(const tgbm_rows &x) { return x.type != TGBM_I8 || !lies_well
 int packed_rows(const tgbm_rows &x) { return (int)std::max<long long>(1, std::min<long long>(x.rows, (long long)(kPackedBytes / (size_t)pad_of(x.features)))); }
 size_t in_lines(size_t bytes) { return (bytes + 127) / 128 * 128; }
 
+template <typename O, int BL, int BC, int WL, int WC, bool CLASSES>
+void linear_tiles(hipStream_t s, const Product &p) {
+    const int line_tiles = (p.lines.rows - 1) / BL + 1, column_tiles = (p.columns.rows - 1) / BC + 1;
+    static LdsOptIn opt_in;
+    opt_in({reinterpret_cast<const void *>(&k_linear_tiles<O, BL, BC, WL, WC, CLASSES>)});
+    k_linear_tiles<O, BL, BC, WL, WC, CLASSES><<<blocks_of_tiles((unsigned)(line_tiles * column_tiles)), 64 * WL * WC, lds_of_tiles<O, BL, BC, WL, WC>(), s>>>(p, line_tiles,
+                                                                                                                                                       column_tiles);
+}
+
+template <typename O, int R>
+void linear_few(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, O *out, const tgbm_scores &like) {
+    const long waves = (long)((w.rows - 1) / 16 + 1) * ((x.rows - 1) / (16 * R) + 1);
+    const unsigned rows = (unsigned)((x.rows - 1) / (16 * R) + 1);
+    if (waves >= 4096 || features <= 2 * kChunk) k_linear_few<O, R, 1><<<dim3((w.rows - 1) / 64 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
+    else if (waves >= 2048 || features <= 4 * kChunk) k_linear_few<O, R, 2><<<dim3((w.rows - 1) / 32 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
+    else k_linear_few<O, R, 4><<<dim3((w.rows - 1) / 16 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
+}
+
 template <typename O>
 void linear(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, const tgbm_scores &out, int row0) {
     O *to = static_cast<O *>(const_cast<void *>(out.data)) + (size_t)row0 * out.row_stride;
-    constexpr int kMost = 65535 * kTile;  // (a direction of a launch)
+    constexpr int kMost = 1 << 20;  // rows of a launch
     for (int r = 0; r < x.rows; r += std::min(kMost, x.rows - r)) {
         Rows8 part = x;
         part.data += (size_t)r * x.pitch;
         part.scale += r;
         part.rows = std::min(kMost, x.rows - r);
-        k_linear<O><<<dim3((w.rows - 1) / kTile + 1, (part.rows - 1) / kTile + 1), kLinearBlock, 0, s>>>(part, w, features, bias, to + (size_t)r * out.row_stride,
-                                                                                                         out.class_stride, out.row_stride);
+        O *its = to + (size_t)r * out.row_stride;
+        const long tiles = (long)((w.rows - 1) / 128 + 1) * ((part.rows - 1) / 128 + 1);
+        if (part.rows <= 16) {
+            linear_few<O, 1>(s, part, w, features, bias, its, out);
+        } else if (part.rows <= 32) {
+            linear_few<O, 2>(s, part, w, features, bias, its, out);
+        } else if (tiles < 64) {
+            linear_few<O, 4>(s, part, w, features, bias, its, out);
+        } else if (out.class_stride == 1) {
+            const Product p{w, part, bias, features, its, out.row_stride};
+            if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, true>(s, p);
+            else linear_tiles<O, 128, 128, 2, 2, true>(s, p);
+        } else {
+            const Product p{part, w, bias, features, its, out.class_stride};
+            if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, false>(s, p);
+            else linear_tiles<O, 128, 128, 2, 2, false>(s, p);
+        }
     }
 }
 
