@@ -19,32 +19,113 @@ constexpr int kChunk = 128;
 
 typedef int Int4 __attribute__((ext_vector_type(4)));
 
-template <int BLOCK>
-__device__ __forceinline__ unsigned block_max_u(unsigned v, unsigned *part) {
-    for (int d = 32; d > 0; d /= 2) v = max(v, (unsigned)__shfl_xor((int)v, d));
-    if (lane_id() == 0) part[wave_id()] = v;
-    __syncthreads();
-    for (int w = 0; w < BLOCK / 64; ++w) v = max(v, part[w]);
-    return v;
+// What a row's largest magnitude makes of it. most: its bits; an infinity or a NaN among the numbers is the largest of all, and the row has no scale.
+__device__ __forceinline__ float scale_of(unsigned most) { return most < 0x7f800000u ? __uint_as_float(most) / 127.f : __builtin_nanf(""); }
+__device__ __forceinline__ int whole_of(float v, float scale) { return scale > 0.f ? (int)fminf(fmaxf(rintf(v / scale), -127.f), 127.f) : 0; }
+
+// Whole numbers of several, as bytes. A product with 1 / scale is off by 127 * 2^-23 at most, roundings of the inverse, the product and the quotient that is meant
+// together: only where it lies that near to half a step, one in 12 000, does the quotient itself have to be rounded (65537 x 1024: 83 us with a division for
+// every number).
+constexpr float kNearHalf = 0.5f - 0x1p-14f, kSmallScale = 0x1p-100f;
+template <int N, typename T>
+__device__ __forceinline__ void whole_of_all(const T &v, float scale, float inverse, unsigned (&bytes)[N / 4]) {
+    constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's last byte is the whole number
+    unsigned word[N];
+    bool near = !(scale > kSmallScale);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float x = score_to_float(v[j]), by = x * inverse, sum = by + kMagic;
+        word[j] = __float_as_uint(sum);
+        near |= fabsf(by - (sum - kMagic)) > kNearHalf;
+    }
+    if (near) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) word[j] = (unsigned)whole_of(score_to_float(v[j]), scale);
+    }
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+        const unsigned low = __builtin_amdgcn_perm(word[j * 4 + 1], word[j * 4], 0x0c0c0400), high = __builtin_amdgcn_perm(word[j * 4 + 3], word[j * 4 + 2], 0x0c0c0400);
+        bytes[j] = high << 16 | low;
+    }
 }
 
-// A workgroup takes a row. `pad` bytes from the row's begin on are written: zeros behind its features.
+// G threads take a row (a workgroup takes several rows, or one), N vectors of 16 bytes each, which stay in registers. `pad` bytes from the row's begin on are
+// written: zeros behind its features.
+template <typename T, int G, int N>
+__global__ __launch_bounds__(G > kLinearBlock ? G : kLinearBlock) void k_quantise(const T *x, long long pitch, int rows, int features, signed char *q, long long q_pitch, int pad, float *scales) {
+    constexpr int kBlock = G > kLinearBlock ? G : kLinearBlock, V = 16 / (int)sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    typedef signed char Out __attribute__((ext_vector_type(16 / sizeof(T)), aligned(1)));
+    __shared__ unsigned part[kBlock / 64];
+    const long row = (long)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+    const int t = threadIdx.x % G;
+    const bool on = row < rows;  // (all threads stay for the others)
+    const T *from = x + (size_t)(on ? row : 0) * pitch;
+    Vec v[N];
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = (i * G + t) * V;
+        v[i] = (T)0.f;
+        if (at + V <= features) {
+            v[i] = *reinterpret_cast<const Vec *>(from + at);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (at + j < features) v[i][j] = from[at + j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(score_to_float(v[i][j])) & 0x7fffffffu);
+#pragma unroll
+    for (int d = (G < 64 ? G : 64) / 2; d > 0; d /= 2) most = max(most, (unsigned)__shfl_xor((int)most, d));
+    if constexpr (G > 64) {
+        if (lane_id() == 0) part[wave_id()] = most;
+        __syncthreads();
+        constexpr int kWaves = G / 64;
+        const int first = wave_id() / kWaves * kWaves;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = max(most, part[first + w]);
+    }
+    if (!on) return;
+    const float scale = scale_of(most);
+    if (t == 0) scales[row] = scale;
+    signed char *to = q + (size_t)row * q_pitch;
+    const float inverse = 1.f / scale;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = (i * G + t) * V;
+        unsigned bytes[V / 4];
+        whole_of_all<V>(v[i], scale, inverse, bytes);
+        const Out o = __builtin_bit_cast(Out, bytes);
+        if (at + V <= pad) {
+            *reinterpret_cast<Out *>(to + at) = o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (at + j < pad) to[at + j] = o[j];
+        }
+    }
+    for (int i = N * G * V + t; i < pad; i += G) to[i] = 0;  // (a padding that is longer than what a launch is chosen for)
+}
+
+// Longer rows: a workgroup reads its row twice.
 template <typename T>
-__global__ __launch_bounds__(kLinearBlock) void k_quantise(const T *x, long long pitch, int features, signed char *q, long long q_pitch, int pad, float *scales) {
-    __shared__ unsigned part[kLinearBlock / 64];
+__global__ __launch_bounds__(1024) void k_quantise_long(const T *x, long long pitch, int features, signed char *q, long long q_pitch, int pad, float *scales) {
+    __shared__ unsigned part[16];
     const T *row = x + (size_t)blockIdx.x * pitch;
     unsigned most = 0;
-    for (int i = threadIdx.x; i < features; i += kLinearBlock) most = max(most, __float_as_uint(score_to_float(row[i])) & 0x7fffffffu);
-    most = block_max_u<kLinearBlock>(most, part);
-    const bool fine = most < 0x7f800000u;  // (an infinity or a NaN among them: the row has no scale)
-    const float scale = fine ? __uint_as_float(most) / 127.f : __builtin_nanf("");
+    for (int i = threadIdx.x; i < features; i += 1024) most = max(most, __float_as_uint(score_to_float(row[i])) & 0x7fffffffu);
+    for (int d = 32; d > 0; d /= 2) most = max(most, (unsigned)__shfl_xor((int)most, d));
+    if (lane_id() == 0) part[wave_id()] = most;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) most = max(most, part[w]);
+    const float scale = scale_of(most);
     if (threadIdx.x == 0) scales[blockIdx.x] = scale;
     signed char *to = q + (size_t)blockIdx.x * q_pitch;
-    for (int i = threadIdx.x; i < pad; i += kLinearBlock) {
-        float v = 0.f;
-        if (i < features && scale > 0.f) v = fminf(fmaxf(rintf(score_to_float(row[i]) / scale), -127.f), 127.f);
-        to[i] = (signed char)(int)v;
-    }
+    for (int i = threadIdx.x; i < pad; i += 1024) to[i] = (signed char)(i < features ? whole_of(score_to_float(row[i]), scale) : 0);
 }
 
 // Rows of whole numbers, moved to rows of `pad` bytes.
@@ -107,22 +188,26 @@ __global__ __launch_bounds__(64 * WL * WC, 2) void k_linear_tiles(Product p, int
 
     // a wavefront brings eight lines at a time
     constexpr int kLoadL = BL / 8 / kWaves, kLoadC = BC / 8 / kWaves;
-    const int part = (lane % 8) ^ (lane / 8);
+    static_assert(kLoadL % 2 == 0 && kLoadC % 2 == 0);
+    // (the order of a line's parts: in 64 banks, the 16 lines that a quarter of a wavefront reads have each their own)
+    const auto part_of = [&](int i) { return (lane % 8) ^ (lane / 16 + i % 2 * 4); };
     const signed char *const of_l = p.lines.data + (size_t)l0 * p.lines.pitch, *const of_c = p.columns.data + (size_t)c0 * p.columns.pitch;
     unsigned at_l[kLoadL], at_c[kLoadC];  // (from a tile's first line: 256 lines of up to 2^17 bytes)
 #pragma unroll
-    for (int i = 0; i < kLoadL; ++i) at_l[i] = (unsigned)min((wave * kLoadL + i) * 8 + lane / 8, p.lines.rows - 1 - l0) * (unsigned)p.lines.pitch + part * 16;
+    for (int i = 0; i < kLoadL; ++i) at_l[i] = (unsigned)min((wave * kLoadL + i) * 8 + lane / 8, p.lines.rows - 1 - l0) * (unsigned)p.lines.pitch + part_of(i) * 16;
 #pragma unroll
-    for (int i = 0; i < kLoadC; ++i) at_c[i] = (unsigned)min((wave * kLoadC + i) * 8 + lane / 8, p.columns.rows - 1 - c0) * (unsigned)p.columns.pitch + part * 16;
+    for (int i = 0; i < kLoadC; ++i) at_c[i] = (unsigned)min((wave * kLoadC + i) * 8 + lane / 8, p.columns.rows - 1 - c0) * (unsigned)p.columns.pitch + part_of(i) * 16;
     auto bring = [&](int chunk, int stage) {
         signed char *to = lds + stage * kStage;
         // weights may end with their features: what is read instead, a line's begin, meets zeros
         const int f = chunk * kChunk;
-        const unsigned back = f + part * 16 >= whole ? f + part * 16 : 0;
+        unsigned back[2];
 #pragma unroll
-        for (int i = 0; i < kLoadL; ++i) to_lds(of_l + (at_l[i] + f - (CLASSES ? back : 0u)), to + (wave * kLoadL + i) * 8 * kChunk);
+        for (int i = 0; i < 2; ++i) back[i] = f + part_of(i) * 16 >= whole ? f + part_of(i) * 16 : 0;
 #pragma unroll
-        for (int i = 0; i < kLoadC; ++i) to_lds(of_c + (at_c[i] + f - (CLASSES ? 0u : back)), to + (BL + (wave * kLoadC + i) * 8) * kChunk);
+        for (int i = 0; i < kLoadL; ++i) to_lds(of_l + (at_l[i] + f - (CLASSES ? back[i % 2] : 0u)), to + (wave * kLoadL + i) * 8 * kChunk);
+#pragma unroll
+        for (int i = 0; i < kLoadC; ++i) to_lds(of_c + (at_c[i] + f - (CLASSES ? 0u : back[i % 2])), to + (BL + (wave * kLoadC + i) * 8) * kChunk);
     };
     const int wl = wave / WC * (BL / WL), wc = wave % WC * (BC / WC);
     Int16 sum[kL][kC] = {};
@@ -135,7 +220,7 @@ __global__ __launch_bounds__(64 * WL * WC, 2) void k_linear_tiles(Product p, int
         Int4 a[4][kL], b[4][kC];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int at = lane % 32 * kChunk + (((k * 2 + lane / 32) ^ (lane % 8)) * 16);
+            const int at = lane % 32 * kChunk + (((k * 2 + lane / 32) ^ (lane / 2 % 8)) * 16);
 #pragma unroll
             for (int i = 0; i < kL; ++i) a[k][i] = *reinterpret_cast<const Int4 *>(stage + (wl + i * 32) * kChunk + at);
 #pragma unroll
@@ -223,29 +308,30 @@ __global__ __launch_bounds__(kLinearBlock) void k_linear_few(Rows8 x, Rows8 w, i
     for (int j = 0; j < R; ++j) of_row[j] = x.data + (size_t)min(r0 + j * 16 + lane % 16, x.rows - 1) * x.pitch;
     Int4 sum[R] = {};
     const int first = chunks * share / S, last = chunks * (share + 1) / S;
-    // (which of the features a lane takes is its own affair, as long as it is the same of both)
-    auto step = [&](int f, bool tail) {
-        Int4 a[2], b[R][2];
+    // Loads of several steps are on their way together. (Which of the features a lane takes is its own affair, as long as it is the same of both.)
+    constexpr int kAtOnce = R > 2 ? 2 : 4;
+    for (int c = first; c < last; c += kAtOnce) {
+        Int4 a[kAtOnce][2], b[kAtOnce][R][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = f + lane / 16 * 32 + h * 16;
-            a[h] = *reinterpret_cast<const Int4 *>(of_class + (tail && at >= whole ? 0 : at));
+        for (int s = 0; s < kAtOnce; ++s)
+            if (c + s < last) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) b[j][h] = *reinterpret_cast<const Int4 *>(of_row[j] + at);
-        }
+                for (int h = 0; h < 2; ++h) {
+                    const int at = (c + s) * kChunk + lane / 16 * 32 + h * 16;
+                    a[s][h] = *reinterpret_cast<const Int4 *>(of_class + (at >= whole ? 0 : at));
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+                    for (int j = 0; j < R; ++j) b[s][j][h] = *reinterpret_cast<const Int4 *>(of_row[j] + at);
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < R; ++j) sum[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h], b[j][h], sum[j], 0, 0, 0);
-    };
-    int c = first;
-    for (; c + 4 < last; c += 4) {  // (the last one apart)
-        step(c * kChunk, false);
-        step((c + 1) * kChunk, false);
-        step((c + 2) * kChunk, false);
-        step((c + 3) * kChunk, false);
+        for (int s = 0; s < kAtOnce; ++s)
+            if (c + s < last) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < R; ++j) sum[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s][h], b[s][j][h], sum[j], 0, 0, 0);
+            }
     }
-    for (; c < last; ++c) step(c * kChunk, c == last - 1);
     if constexpr (S > 1) {
         if (share > 0) {
 #pragma unroll
@@ -333,10 +419,28 @@ void linear(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const f
 
 }  // namespace
 
+namespace {
+template <typename T, int G, int N>
+void quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pitch, int pad, float *scale) {
+    constexpr int kBlock = G > kLinearBlock ? G : kLinearBlock;
+    k_quantise<T, G, N><<<(x.rows - 1) / (kBlock / G) + 1, kBlock, 0, s>>>(static_cast<const T *>(x.data), x.pitch, x.rows, x.features, q, q_pitch, pad, scale);
+}
+template <typename T>
+void quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pitch, int pad, float *scale) {
+    const int vectors = (x.features - 1) / (16 / (int)sizeof(T)) + 1;
+    if (vectors <= 16) quantise<T, 8, 2>(s, x, q, q_pitch, pad, scale);
+    else if (vectors <= 64) quantise<T, 16, 4>(s, x, q, q_pitch, pad, scale);
+    else if (vectors <= 256) quantise<T, 64, 4>(s, x, q, q_pitch, pad, scale);
+    else if (vectors <= 1024) quantise<T, 256, 4>(s, x, q, q_pitch, pad, scale);
+    else if (vectors <= 4096) quantise<T, 1024, 4>(s, x, q, q_pitch, pad, scale);
+    else k_quantise_long<T><<<x.rows, 1024, 0, s>>>(static_cast<const T *>(x.data), x.pitch, x.features, q, q_pitch, pad, scale);
+}
+}  // namespace
+
 void launch_rows_quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pitch, int pad, float *scale) {
-    if (x.type == TGBM_F32) k_quantise<float><<<x.rows, kLinearBlock, 0, s>>>(static_cast<const float *>(x.data), x.pitch, x.features, q, q_pitch, pad, scale);
-    else if (x.type == TGBM_F16) k_quantise<_Float16><<<x.rows, kLinearBlock, 0, s>>>(static_cast<const _Float16 *>(x.data), x.pitch, x.features, q, q_pitch, pad, scale);
-    else k_quantise<__bf16><<<x.rows, kLinearBlock, 0, s>>>(static_cast<const __bf16 *>(x.data), x.pitch, x.features, q, q_pitch, pad, scale);
+    if (x.type == TGBM_F32) quantise<float>(s, x, q, q_pitch, pad, scale);
+    else if (x.type == TGBM_F16) quantise<_Float16>(s, x, q, q_pitch, pad, scale);
+    else quantise<__bf16>(s, x, q, q_pitch, pad, scale);
 }
 
 size_t scores_linear_workspace(const tgbm_rows &x, const tgbm_rows &w) {
