@@ -294,66 +294,171 @@ __global__ __launch_bounds__(64 * WL * WC, 2) void k_linear_tiles(Product p, int
     }
 }
 
-// Few rows: 16 classes and 16 * R rows to a wavefront, which reads them as the product wants them, without LDS; S wavefronts share the features.
-template <typename O, int R, int S>
-__global__ __launch_bounds__(kLinearBlock) void k_linear_few(Rows8 x, Rows8 w, int features, const float *bias, O *out, long long class_stride, long long row_stride) {
+// Scores of one or of four classes that lie side by side, in the type that they have.
+struct ScoreOut {
+    void *data;
+    long long class_stride, row_stride;
+    int type;
+    template <typename O>
+    __device__ __forceinline__ void as(const float (&z)[4], int cls, int row, int classes) const {
+        typedef O Four __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+        O *to = static_cast<O *>(data) + (size_t)cls * class_stride + (size_t)row * row_stride;
+        if (class_stride == 1 && cls + 4 <= classes) {
+            *reinterpret_cast<Four *>(to) = Four{(O)z[0], (O)z[1], (O)z[2], (O)z[3]};
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (cls + q < classes) to[(size_t)q * class_stride] = (O)z[q];
+        }
+    }
+    __device__ __forceinline__ void four(const float (&z)[4], int cls, int row, int classes) const {
+        if (type == TGBM_F32) as<float>(z, cls, row, classes);
+        else if (type == TGBM_F16) as<_Float16>(z, cls, row, classes);
+        else as<__bf16>(z, cls, row, classes);
+    }
+};
+
+// Few rows: the rows' features in LDS, `slice` of them at a time, and 16 * A classes to a wavefront, whose weights go from memory to the product; S wavefronts share
+// the features. T: of the rows, which are quantised on the way into LDS if they are floating ones (all of their features at once then).
+template <typename T, int A, int R, int S>
+__global__ __launch_bounds__(kLinearBlock) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
+    constexpr bool kQuantise = sizeof(T) > 1;
     constexpr int kTiles = kLinearBlock / 64 / S;
-    __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * R : 1][64];
-    const int lane = lane_id(), wave = wave_id(), share = wave % S, tile = wave / S;
-    const int c0 = ((int)blockIdx.x * kTiles + tile) * 16, r0 = (int)blockIdx.y * 16 * R;
+    __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * A * R : 1][64];
+    __shared__ float scale_of_row[16 * R];
+    __shared__ unsigned most_of_row[kQuantise ? 16 * R : 1];
+    extern __shared__ __align__(16) signed char of_x[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), share = wave % S, tile = wave / S;
+    const int c0 = ((int)blockIdx.x * kTiles + tile) * 16 * A, r0 = (int)blockIdx.y * 16 * R, live = min(rows - r0, 16 * R), pitch = slice + 16;
     const int chunks = (features + kChunk - 1) / kChunk, whole = (features + 15) / 16 * 16;
-    const signed char *of_class = w.data + (size_t)min(c0 + lane % 16, w.rows - 1) * w.pitch;
-    const signed char *of_row[R];
+    x += (size_t)r0 * x_pitch;
+    const signed char *of_class[A];
 #pragma unroll
-    for (int j = 0; j < R; ++j) of_row[j] = x.data + (size_t)min(r0 + j * 16 + lane % 16, x.rows - 1) * x.pitch;
-    Int4 sum[R] = {};
-    const int first = chunks * share / S, last = chunks * (share + 1) / S;
-    // Loads of several steps are on their way together. (Which of the features a lane takes is its own affair, as long as it is the same of both.)
-    constexpr int kAtOnce = R > 2 ? 2 : 4;
-    for (int c = first; c < last; c += kAtOnce) {
-        Int4 a[kAtOnce][2], b[kAtOnce][R][2];
+    for (int i = 0; i < A; ++i) of_class[i] = w.data + (size_t)min(c0 + i * 16 + lane % 16, w.rows - 1) * w.pitch;
+    Int4 sum[A][R] = {};
+    // (what the scores want besides is on its way from the start)
+    float w_scale[A][4], w_bias[A][4];
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int cls = min(c0 + i * 16 + lane / 16 * 4 + q, w.rows - 1);
+            w_scale[i][q] = w.scale[cls];
+            w_bias[i][q] = bias != nullptr ? bias[cls] : 0.f;
+        }
+    constexpr int kAtOnce = A * R > 2 ? 2 : 4;
+    Int4 a[kAtOnce][2][A];
+    const auto bring = [&](int c) {
 #pragma unroll
         for (int s = 0; s < kAtOnce; ++s)
-            if (c + s < last) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int at = (c + s) * kChunk + lane / 16 * 32 + h * 16;
-                    a[s][h] = *reinterpret_cast<const Int4 *>(of_class + (at >= whole ? 0 : at));
+            for (int h = 0; h < 2; ++h) {
+                const int at = min(c + s * S, chunks - 1) * kChunk + h * 64 + lane / 16 * 16;
 #pragma unroll
-                    for (int j = 0; j < R; ++j) b[s][j][h] = *reinterpret_cast<const Int4 *>(of_row[j] + at);
+                for (int i = 0; i < A; ++i) a[s][h][i] = *reinterpret_cast<const Int4 *>(of_class[i] + (at >= whole ? 0 : at));
+            }
+    };
+    for (int f0 = 0; f0 < features; f0 += slice) {
+        const int first = f0 / kChunk + share, last = min(chunks, (f0 + slice) / kChunk);
+        bring(first);
+        if (f0 != 0) __syncthreads();
+        if constexpr (kQuantise) {
+            // all threads go over the rows' vectors, twice: the second time they come from near
+            constexpr int V = 16 / (int)sizeof(T);
+            typedef T Loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+            typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
+            const int parts = chunks * kChunk / V;
+            const auto each = [&](auto f) {
+#pragma unroll 2
+                for (int i = threadIdx.x; i < live * parts; i += kLinearBlock) {
+                    const int r = i / parts, at = (i - r * parts) * V;
+                    const T *row = x + (size_t)r * x_pitch;
+                    Vec v = (T)0.f;
+                    if (at + V <= features) {
+                        v = *reinterpret_cast<const Loose *>(row + at);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            if (at + j < features) v[j] = row[at + j];
+                    }
+                    f(r, at, v);
                 }
+            };
+            if ((int)threadIdx.x < live) most_of_row[threadIdx.x] = 0;
+            __syncthreads();
+            each([&](int r, int, const Vec &v) {
+                unsigned most = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(score_to_float(v[j])) & 0x7fffffffu);
+                atomicMax(&most_of_row[r], most);
+            });
+            __syncthreads();
+            each([&](int r, int at, const Vec &v) {
+                const float scale = scale_of(most_of_row[r]);
+                unsigned bytes[V / 4];
+                whole_of_all<V>(v, scale, 1.f / scale, bytes);
+                typedef unsigned Words __attribute__((ext_vector_type(V / 4)));
+                *reinterpret_cast<Words *>(of_x + r * pitch + at) = __builtin_bit_cast(Words, bytes);
+            });
+            if ((int)threadIdx.x < live) scale_of_row[threadIdx.x] = scale_of(most_of_row[threadIdx.x]);
+        } else {
+            const int parts = (last * kChunk - f0) / 16;
+            for (int i = threadIdx.x; i < live * parts; i += kLinearBlock) {
+                const int r = i / parts, at = (i - r * parts) * 16;
+                *reinterpret_cast<Int4 *>(of_x + r * pitch + at) = *reinterpret_cast<const Int4 *>(x + (size_t)r * x_pitch + f0 + at);
             }
+            if (f0 == 0 && (int)threadIdx.x < live) scale_of_row[threadIdx.x] = x_scales[r0 + threadIdx.x];
+        }
+        __syncthreads();
+        const signed char *of_row[R];
 #pragma unroll
-        for (int s = 0; s < kAtOnce; ++s)
-            if (c + s < last) {
+        for (int j = 0; j < R; ++j) of_row[j] = of_x + min(j * 16 + lane % 16, live - 1) * pitch + lane / 16 * 16;
+        for (int c = first; c < last; c += kAtOnce * S) {
+            if (c != first) bring(c);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int s = 0; s < kAtOnce; ++s)
+                if (c + s * S < last) {
 #pragma unroll
-                    for (int j = 0; j < R; ++j) sum[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s][h], b[s][j][h], sum[j], 0, 0, 0);
-            }
+                    for (int h = 0; h < 2; ++h) {
+                        Int4 b[R];
+#pragma unroll
+                        for (int j = 0; j < R; ++j) b[j] = *reinterpret_cast<const Int4 *>(of_row[j] + (c + s * S) * kChunk - f0 + h * 64);
+#pragma unroll
+                        for (int i = 0; i < A; ++i)
+#pragma unroll
+                            for (int j = 0; j < R; ++j) sum[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s][h][i], b[j], sum[i][j], 0, 0, 0);
+                    }
+                }
+        }
     }
     if constexpr (S > 1) {
         if (share > 0) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) shared[(tile * (S - 1) + share - 1) * R + j][lane] = sum[j];
+            for (int i = 0; i < A; ++i)
+#pragma unroll
+                for (int j = 0; j < R; ++j) shared[((tile * (S - 1) + share - 1) * A + i) * R + j][lane] = sum[i][j];
         }
         __syncthreads();
         if (share > 0) return;
 #pragma unroll
         for (int s = 0; s < S - 1; ++s)
 #pragma unroll
-            for (int j = 0; j < R; ++j) sum[j] += shared[(tile * (S - 1) + s) * R + j][lane];
+            for (int i = 0; i < A; ++i)
+#pragma unroll
+                for (int j = 0; j < R; ++j) sum[i][j] += shared[((tile * (S - 1) + s) * A + i) * R + j][lane];
     }
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-        const int row = r0 + j * 16 + lane % 16;
-        if (row >= x.rows) continue;
-        const float by = x.scale[row];
+        const int r = j * 16 + lane % 16;
+        if (r >= live) continue;
+        const float by = scale_of_row[r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int cls = c0 + lane / 16 * 4 + i;
-            if (cls < w.rows)
-                out[(size_t)cls * class_stride + (size_t)row * row_stride] = (O)score_of(sum[j][i], by, w.scale[cls], bias != nullptr ? bias[cls] : 0.f);
+        for (int i = 0; i < A; ++i) {
+            const int cls = c0 + i * 16 + lane / 16 * 4;
+            float z[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] = score_of(sum[i][j][q], by, w_scale[i][q], w_bias[i][q]);
+            out.four(z, cls, r0 + r, w.rows);
         }
     }
 }
@@ -379,41 +484,55 @@ void linear_tiles(hipStream_t s, const Product &p) {
                                                                                                                                                        column_tiles);
 }
 
-template <typename O, int R>
-void linear_few(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, O *out, const tgbm_scores &like) {
-    const long waves = (long)((w.rows - 1) / 16 + 1) * ((x.rows - 1) / (16 * R) + 1);
-    const unsigned rows = (unsigned)((x.rows - 1) / (16 * R) + 1);
-    if (waves >= 4096 || features <= 2 * kChunk) k_linear_few<O, R, 1><<<dim3((w.rows - 1) / 64 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
-    else if (waves >= 2048 || features <= 4 * kChunk) k_linear_few<O, R, 2><<<dim3((w.rows - 1) / 32 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
-    else k_linear_few<O, R, 4><<<dim3((w.rows - 1) / 16 + 1, rows), kLinearBlock, 0, s>>>(x, w, features, bias, out, like.class_stride, like.row_stride);
+// Rows in LDS: as many of their features as fit, all of them where the rows are quantised on the way.
+constexpr int kFewLds = 64 * 1024, kFusedMost = 16 * 1024;
+bool quantised_on_the_way(const tgbm_rows &x) { return x.type != TGBM_I8 && x.rows <= 16 && (long long)x.rows * pad_of(x.features) <= kFusedMost; }
+
+template <typename T, int A, int R, int S>
+void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
+    constexpr int kOf = kLinearBlock / 64 / S * 16 * A;
+    const int live = std::min(rows, 16 * R), slice = std::min((int)pad_of(features), (kFewLds / live - 16) / kChunk * kChunk);
+    static LdsOptIn opt_in;
+    opt_in({reinterpret_cast<const void *>(&k_linear_few<T, A, R, S>)});
+    k_linear_few<T, A, R, S><<<dim3((w.rows - 1) / kOf + 1, (rows - 1) / (16 * R) + 1), kLinearBlock, live * (slice + 16), s>>>(x, scale, pitch, rows, w, features, bias, out, slice);
+}
+template <typename T, int A, int R>
+void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
+    const long waves = (long)((w.rows - 1) / (16 * A) + 1) * ((rows - 1) / (16 * R) + 1);
+    if (waves >= (A * R > 1 ? 1024 : 4096) || features <= 2 * kChunk) linear_few<T, A, R, 1>(s, x, scale, pitch, rows, w, features, bias, out);
+    else if (waves >= (A * R > 1 ? 512 : 1024) || features <= 4 * kChunk) linear_few<T, A, R, 2>(s, x, scale, pitch, rows, w, features, bias, out);
+    else linear_few<T, A, R, 4>(s, x, scale, pitch, rows, w, features, bias, out);
 }
 
 template <typename O>
-void linear(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, const tgbm_scores &out, int row0) {
-    O *to = static_cast<O *>(const_cast<void *>(out.data)) + (size_t)row0 * out.row_stride;
+void linear_tiles(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, const ScoreOut &out, long tiles) {
+    if (out.class_stride == 1) {
+        const Product p{w, x, bias, features, out.data, out.row_stride};
+        if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, true>(s, p);
+        else linear_tiles<O, 128, 128, 2, 2, true>(s, p);
+    } else {
+        const Product p{x, w, bias, features, out.data, out.class_stride};
+        if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, false>(s, p);
+        else linear_tiles<O, 128, 128, 2, 2, false>(s, p);
+    }
+}
+
+// The scores of rows in 8 bits.
+void linear(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, ScoreOut out) {
     constexpr int kMost = 1 << 20;  // rows of a launch
     for (int r = 0; r < x.rows; r += std::min(kMost, x.rows - r)) {
         Rows8 part = x;
         part.data += (size_t)r * x.pitch;
         part.scale += r;
         part.rows = std::min(kMost, x.rows - r);
-        O *its = to + (size_t)r * out.row_stride;
         const long tiles = (long)((w.rows - 1) / 128 + 1) * ((part.rows - 1) / 128 + 1);
-        if (part.rows <= 16) {
-            linear_few<O, 1>(s, part, w, features, bias, its, out);
-        } else if (part.rows <= 32) {
-            linear_few<O, 2>(s, part, w, features, bias, its, out);
-        } else if (tiles < 64) {
-            linear_few<O, 4>(s, part, w, features, bias, its, out);
-        } else if (out.class_stride == 1) {
-            const Product p{w, part, bias, features, its, out.row_stride};
-            if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, true>(s, p);
-            else linear_tiles<O, 128, 128, 2, 2, true>(s, p);
-        } else {
-            const Product p{part, w, bias, features, its, out.class_stride};
-            if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, false>(s, p);
-            else linear_tiles<O, 128, 128, 2, 2, false>(s, p);
-        }
+        if (part.rows <= 16) linear_few<signed char, 1, 1>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
+        else if (part.rows <= 32) linear_few<signed char, 2, 2>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
+        else if (tiles < 64) linear_few<signed char, 1, 4>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
+        else if (out.type == TGBM_F32) linear_tiles<float>(s, part, w, features, bias, out, tiles);
+        else if (out.type == TGBM_F16) linear_tiles<_Float16>(s, part, w, features, bias, out, tiles);
+        else linear_tiles<__bf16>(s, part, w, features, bias, out, tiles);
+        out.data = static_cast<char *>(out.data) + (out.type == TGBM_F32 ? 4 : 2) * (size_t)part.rows * out.row_stride;
     }
 }
 
@@ -446,7 +565,7 @@ void launch_rows_quantise(hipStream_t s, const tgbm_rows &x, signed char *q, lon
 size_t scores_linear_workspace(const tgbm_rows &x, const tgbm_rows &w) {
     const size_t pad = (size_t)pad_of(x.features);
     size_t bytes = packs_weights(w) ? in_lines(pad * w.rows) : 0;
-    if (packs_features(x)) bytes += in_lines(pad * packed_rows(x)) + (x.type != TGBM_I8 ? sizeof(float) * (size_t)packed_rows(x) : 0);
+    if (packs_features(x) && !quantised_on_the_way(x)) bytes += in_lines(pad * packed_rows(x)) + (x.type != TGBM_I8 ? sizeof(float) * (size_t)packed_rows(x) : 0);
     return bytes;
 }
 
@@ -459,6 +578,13 @@ void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &w,
         weights.data = room;
         weights.pitch = pad;
         room += in_lines((size_t)pad * w.rows);
+    }
+    ScoreOut to{const_cast<void *>(out.data), out.class_stride, out.row_stride, out.type};
+    if (quantised_on_the_way(x)) {
+        if (x.type == TGBM_F32) linear_few<float, 1, 1>(s, static_cast<const float *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
+        else if (x.type == TGBM_F16) linear_few<_Float16, 1, 1>(s, static_cast<const _Float16 *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
+        else linear_few<__bf16, 1, 1>(s, static_cast<const __bf16 *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
+        return;
     }
     const int most = packs_features(x) ? packed_rows(x) : x.rows;
     for (int row = 0; row < x.rows; row += std::min(most, x.rows - row)) {
@@ -478,9 +604,8 @@ void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &w,
             features.data = room;
             features.pitch = pad;
         }
-        if (out.type == TGBM_F32) linear<float>(s, features, weights, x.features, bias, out, row);
-        else if (out.type == TGBM_F16) linear<_Float16>(s, features, weights, x.features, bias, out, row);
-        else linear<__bf16>(s, features, weights, x.features, bias, out, row);
+        linear(s, features, weights, x.features, bias, to);
+        to.data = static_cast<char *>(to.data) + (out.type == TGBM_F32 ? 4 : 2) * (size_t)part.rows * out.row_stride;
     }
 }
 
