@@ -243,30 +243,28 @@ __global__ __launch_bounds__(kSampleBlock) void k_lay_shown(tgbm_scores in, tgbm
     });
 }
 
-// A score's place on the scale that sums are kept by: 32 parts to a halving of w, 64 halvings. What is further down than that (2^-64 of the best class) is nothing
-// beside a random number's last place, 2^-24, whatever there is of it.
+// A score's place on the scale that sums are kept by: 32 parts to a halving of w, 64 halvings; its bucket is the nearest whole number. What is further down than that
+// (2^-64 of the best class) is nothing beside a random number's last place, 2^-24, whatever there is of it.
 constexpr int kParts = 32, kBuckets = 64 * kParts;
 constexpr double kPartsOfE = kParts * 1.44269504088896340736;  // parts to a factor of e
+constexpr double kToWhole = 6755399441055744.0;                // 1.5 * 2^52: the sum's low word is the nearest whole number
 
-// 2^(-g / 32), g in [0, 1], plus `magic` = 2^(52 - bits): its last `bits` bits are the power of two times 2^bits, rounded. Taylor's series about the middle: the
-// seventh term is below 2^-57.
-__device__ __forceinline__ unsigned long long part_of_two(double g, double magic) {
-    constexpr double a = -0.69314718055994530942 / kParts, mid = 0.98922801319397548413;  // 2^(-1/64)
-    constexpr double c1 = a, c2 = a * a / 2, c3 = c2 * a / 3, c4 = c3 * a / 4, c5 = c4 * a / 5, c6 = c5 * a / 6;
-    const double h = g - 0.5;
-    double e = __builtin_fma(h, mid * c6, mid * c5);
-    e = __builtin_fma(h, e, mid * c4);
-    e = __builtin_fma(h, e, mid * c3);
-    e = __builtin_fma(h, e, mid * c2);
-    e = __builtin_fma(h, e, mid * c1);
-    e = __builtin_fma(h, e, mid);
+// 2^(-h / 32), h in [-1/2, 1/2], plus `magic` = 2^(52 - bits): its last 52 bits are the power of two times 2^bits, rounded. Taylor's series: the sixth term is below
+// 2^-48 of the whole, 2^-46 is what a whole number of a row of 2^16 classes is rounded by.
+__device__ __forceinline__ unsigned long long part_of_two(double h, double magic) {
+    constexpr double a = -0.69314718055994530942 / kParts, c2 = a * a / 2, c3 = c2 * a / 3, c4 = c3 * a / 4, c5 = c4 * a / 5;
+    double e = __builtin_fma(h, c5, c4);
+    e = __builtin_fma(h, e, c3);
+    e = __builtin_fma(h, e, c2);
+    e = __builtin_fma(h, e, a);
+    e = __builtin_fma(h, e, 1.0);
     return (unsigned long long)__double_as_longlong(e + magic) & 0xfffffffffffffull;
 }
 
 constexpr int kListed = 256;
 template <int BLOCK>
 struct DrawShared {
-    unsigned long long mass[kBuckets];
+    unsigned long long mass[kBuckets + 1];  // (the last one takes what does not count)
     unsigned long long key[kListed], weight[kListed], front[kListed];
     double part[BLOCK / 64];
     float part_f[BLOCK / 64];
@@ -276,30 +274,47 @@ struct DrawShared {
     int listed, bucket;
 };
 
-// One workgroup's work on a row. Each: each(f) calls f(score, class) for the thread's scores, NaNs being left out already.
-template <int BLOCK, typename Each>
+// One workgroup's work on a row. Row: row.each(f) calls f(scores, their first class) for the thread's vectors; what is no class or NaN is -infinity there.
+template <int BLOCK, typename Row>
 struct Draw {
+    static constexpr int V = Row::V, kEach = kBuckets / BLOCK;
     DrawShared<BLOCK> &sh;
-    const Each &each;
-    double best, by;      // (the place of a score is (best - score) * by)
-    double least_place;   // from where on scores are not kept
-    unsigned long long cut = 0;  // the last kept of the order, as a key
+    Row &row;
+    double best, by;  // (the place of a score is (best - score) * by)
     double magic;
-    int bits;
+    float least = -FLT_MAX;      // the least score that is kept
+    unsigned long long cut = 0;  // the last one of the order that is kept, as a key
+    double last_place = kBuckets - 0.5;
 
     static __device__ __forceinline__ unsigned long long key_of(float x, int c) { return (unsigned long long)ordered(x) << 32 | (unsigned)~c; }
-    // fmax: equal infinities have a NaN between them, which is to be 0
-    __device__ __forceinline__ double place_of(float x) const { return __builtin_fmax((best - (double)x) * by, 0.0); }
-    __device__ __forceinline__ unsigned long long weight_of(double place, int bucket) const { return part_of_two(place - bucket, magic); }
-    // f(place, bucket, key) for all that are kept
+    __device__ __forceinline__ double place_of(float x) const { return (best - (double)x) * by; }
+    static __device__ __forceinline__ int bucket_of(double place) { return (int)__double_as_longlong(place + kToWhole); }
+    __device__ __forceinline__ unsigned long long weight_of(double place) const { return part_of_two(place - ((place + kToWhole) - kToWhole), magic); }
+    // A score below which none has a place up to `place`; the other way: above which none has one from there on.
+    __device__ __forceinline__ float score_below(double place) const {
+        const double x = best - place / by;
+        return __double2float_rd(x - 0x1p-49 * (fabs(x) + fabs(best)));
+    }
+    __device__ __forceinline__ float score_above(double place) const {
+        const double x = best - place / by;
+        return __double2float_ru(x + 0x1p-49 * (fabs(x) + fabs(best)));
+    }
+    // f(place, bucket, key) for those that are kept and whose score is from lo to hi
     template <typename F>
-    __device__ __forceinline__ void kept(F f) const {
-        each([&](float x, int c) {
-            const double s = place_of(x);
-            if (x > kNothing && s <= least_place) {
-                const unsigned long long key = key_of(x, c);
-                if (key >= cut) f(s, (int)s, key);
-            }
+    __device__ __forceinline__ void kept(float lo, float hi, F f) {
+        lo = fmaxf(lo, least);
+        row.each([&](const float (&x)[V], int c) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < V; ++j) any |= x[j] >= lo && x[j] <= hi;
+            if (!any) return;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (x[j] >= lo && x[j] <= hi) {
+                    const double s = place_of(x[j]);
+                    const unsigned long long key = key_of(x[j], c + j);
+                    if (s <= last_place && key >= cut) f(s, bucket_of(s), key);
+                }
         });
     }
 
@@ -310,6 +325,7 @@ struct Draw {
         if (lane_id() == 63) sh.part[wave_id()] = upto;
         __syncthreads();
         double before = 0, sum = 0;
+#pragma unroll
         for (int w = 0; w < BLOCK / 64; ++w) {
             if (w == wave_id()) before = sum;
             sum += sh.part[w];
@@ -321,6 +337,10 @@ struct Draw {
     __device__ __forceinline__ void clear() {
         __syncthreads();
         for (int i = threadIdx.x; i < kBuckets; i += BLOCK) sh.mass[i] = 0;
+        clear_list();
+    }
+    __device__ __forceinline__ void clear_list() {
+        __syncthreads();
         if (threadIdx.x == 0) {
             sh.bucket = 0;
             sh.listed = 0;
@@ -334,8 +354,7 @@ struct Draw {
     // Whether the order up to `before` leaves the next one in what is looked for: up to a target, or below it.
     static __device__ __forceinline__ bool within(double before, double target, bool below) { return below ? before < target : before <= target; }
 
-    // The bucket where the sum passes the target, and the sum in front of it. unit(b): what the bucket's whole numbers count.
-    static constexpr int kEach = kBuckets / BLOCK;
+    // The buckets' sums, those in front of the thread's, and the sum of all. unit(b): what a bucket's whole numbers count.
     template <typename Unit>
     __device__ __forceinline__ double sums(Unit unit, double (&mass)[kEach], double *all) {
         double mine = 0;
@@ -348,7 +367,9 @@ struct Draw {
         }
         return scan(mine, all);
     }
+    // The bucket where the sum passes the target, and the sum in front of it.
     __device__ __forceinline__ void find(const double (&mass)[kEach], double before, double target, bool below, int *bucket, double *front) {
+        __syncthreads();
         if (threadIdx.x == 0) sh.bucket = 0;
         __syncthreads();
         int at = -1;
@@ -374,19 +395,20 @@ struct Draw {
         unsigned long long key;
         double before, weight;  // in the bucket's unit
     };
-    // The one of a bucket where its sum passes the target (in its unit). weight(place, bucket): of one.
+    // The one of a bucket where its sum passes the target (in its unit). weight(place): of one.
     template <typename Weight>
     __device__ __forceinline__ Found resolve(int bucket, double target, bool below, Weight weight) {
+        const float low = score_below(bucket + 0.5), high = score_above(bucket - 0.5);
         unsigned long long lo = 0, hi = ~0ull;
         double front = 0;
         for (;;) {
-            clear();
-            kept([&](double s, int b, unsigned long long key) {
+            clear_list();
+            kept(low, high, [&](double s, int b, unsigned long long key) {
                 if (b != bucket || key < lo || key > hi) return;
                 const int to = atomicAdd(&sh.listed, 1);
                 if (to < kListed) {
                     sh.key[to] = key;
-                    sh.weight[to] = weight(s, b);
+                    sh.weight[to] = weight(s);
                     sh.front[to] = 0;
                 }
             });
@@ -394,7 +416,7 @@ struct Draw {
             const int n = sh.listed;
             if (n <= kListed) return among(n, front, target, below);
             // too many for a list: by parts of the keys between the least and the largest of them
-            kept([&](double, int b, unsigned long long key) {
+            kept(low, high, [&](double, int b, unsigned long long key) {
                 if (b != bucket || key < lo || key > hi) return;
                 atomicMin(&sh.least, key);
                 atomicMax(&sh.most, key);
@@ -405,8 +427,8 @@ struct Draw {
             const int width = 64 - __clzll((long long)(hi - lo)), shift = width > 11 ? width - 11 : 0;
             static_assert(kBuckets == 1 << 11);
             clear();
-            kept([&](double s, int b, unsigned long long key) {
-                if (b == bucket && key >= lo && key <= hi) atomicAdd(&sh.mass[(hi - key) >> shift], weight(s, b));
+            kept(low, high, [&](double s, int b, unsigned long long key) {
+                if (b == bucket && key >= lo && key <= hi) atomicAdd(&sh.mass[(hi - key) >> shift], weight(s));
             });
             __syncthreads();
             double mass[kEach], all;
@@ -418,7 +440,6 @@ struct Draw {
             hi -= (unsigned long long)part << shift;
             const unsigned long long span = (1ull << shift) - 1;
             lo = hi - lo > span ? hi - span : lo;
-            __syncthreads();
         }
     }
     // The same among n listed ones, which are put in order by what is in front of each.
@@ -443,6 +464,58 @@ struct Draw {
         const int j = sh.listed;
         return Found{sh.key[j], front + (double)its, (double)sh.weight[j]};
     }
+
+    // Leaves the k best. The k-th of the threads' own best scores is a bound: only what reaches it is looked at one by one.
+    __device__ __forceinline__ void keep_best(int k) {
+        double mass[kEach], all, front;
+        int bucket;
+        const auto ones = [](int) { return 1.0; };
+        float bound = least;
+        if (k <= BLOCK) {
+            float mine = kNothing;
+            row.each([&](const float (&x)[V], int) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) mine = fmaxf(mine, x[j]);
+            });
+            clear();
+            if (mine >= least && place_of(mine) <= last_place) atomicAdd(&sh.mass[bucket_of(place_of(mine))], 1ull);
+            __syncthreads();
+            const double before = sums(ones, mass, &all);
+            if (all >= (double)k) {
+                find(mass, before, (double)(k - 1), false, &bucket, &front);
+                bound = fmaxf(bound, score_below(bucket + 0.5));
+            }
+        }
+        clear();
+        kept(bound, __builtin_inff(), [&](double, int b, unsigned long long) { atomicAdd(&sh.mass[b], 1ull); });
+        __syncthreads();
+        const double before = sums(ones, mass, &all);
+        if (all <= (double)k) {  // (all that reach the bound: it is the cut)
+            least = bound;
+            return;
+        }
+        find(mass, before, (double)(k - 1), false, &bucket, &front);
+        const unsigned long long key = resolve(bucket, (double)(k - 1) - front, false, [](double) { return 1ull; }).key;
+        cut = key;
+        const unsigned o = (unsigned)(key >> 32);
+        least = __uint_as_float(o ^ ((o >> 31) - 1u | 0x80000000u));
+    }
+    // The weights of what is kept, into the buckets.
+    __device__ __forceinline__ void add_up(bool all_kept) {
+        clear();
+        if (!all_kept) {
+            kept(least, __builtin_inff(), [&](double s, int b, unsigned long long) { atomicAdd(&sh.mass[b], weight_of(s)); });
+        } else {
+            row.each([&](const float (&x)[V], int) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const double s = __builtin_fmin(place_of(x[j]), (double)kBuckets), at = s + kToWhole;
+                    atomicAdd(&sh.mass[(int)__double_as_longlong(at)], part_of_two(s - (at - kToWhole), magic));
+                }
+            });
+        }
+        __syncthreads();
+    }
 };
 
 template <int BLOCK>
@@ -451,6 +524,7 @@ __device__ __forceinline__ float block_max(float v, float *part) {
     __syncthreads();
     if (lane_id() == 0) part[wave_id()] = v;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < BLOCK / 64; ++w) v = fmaxf(v, part[w]);
     return v;
 }
@@ -460,15 +534,48 @@ __device__ __forceinline__ int block_min(int v, int *part) {
     __syncthreads();
     if (lane_id() == 0) part[wave_id()] = v;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < BLOCK / 64; ++w) v = min(v, part[w]);
     return v;
 }
+template <int BLOCK>
+__device__ __forceinline__ int block_sum(int v, int *part) {
+    v = wave_sum_i(v);
+    __syncthreads();
+    if (lane_id() == 0) part[wave_id()] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; ++w) v += part[w];
+    return v;
+}
+
+// The class of the n-th (from 0) score that is m, by bisection.
+template <int BLOCK, typename Row>
+__device__ __forceinline__ int nth_class(Row &row, float m, int n, int classes, int *part) {
+    int lo = -1, hi = classes - 1;
+    while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        int count = 0;
+        row.each([&](const float (&x)[Row::V], int c) {
+#pragma unroll
+            for (int j = 0; j < Row::V; ++j) count += x[j] == m && c + j <= mid ? 1 : 0;
+        });
+        if (block_sum<BLOCK>(count, part) > n) hi = mid;
+        else lo = mid;
+    }
+    return hi;
+}
 
 // The draw of a row by a workgroup. bits: of a whole number that stands for a w of one, so that the sum of a row's has room in 63.
-template <int BLOCK, typename Each>
-__device__ __forceinline__ void draw_row(const Each &each, const RowSampling &r, int bits, DrawShared<BLOCK> &sh, int *cls, float *logp) {
+template <int BLOCK, typename Row>
+__device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int classes, int bits, DrawShared<BLOCK> &sh, int *cls, float *logp) {
+    constexpr int V = Row::V;
     float m = kNothing;
-    each([&](float x, int) { m = fmaxf(m, x); });
+    row.each([&](const float (&x)[V], int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, x[j]);
+    });
     m = block_max<BLOCK>(m, sh.part_f);
     if (m == kNothing || r.none) {
         if (threadIdx.x == 0) {
@@ -479,7 +586,10 @@ __device__ __forceinline__ void draw_row(const Each &each, const RowSampling &r,
     }
     if (r.greedy) {
         int first = INT_MAX;
-        each([&](float x, int c) { first = x == m ? min(first, c) : first; });
+        row.each([&](const float (&x)[V], int c) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) first = x[j] == m ? min(first, c + j) : first;
+        });
         first = block_min<BLOCK>(first, sh.part_i);
         if (threadIdx.x == 0) {
             *cls = first;
@@ -487,32 +597,38 @@ __device__ __forceinline__ void draw_row(const Each &each, const RowSampling &r,
         }
         return;
     }
-    Draw<BLOCK, Each> d{sh, each};
+    if (m == __builtin_inff()) {  // (infinite scores share alike)
+        int count = 0;
+        row.each([&](const float (&x)[V], int) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) count += x[j] == m ? 1 : 0;
+        });
+        int n = min(block_sum<BLOCK>(count, sh.part_i), r.k);
+        if (r.p < 1.f) n = max(1, (int)ceil((double)fmaxf(r.p, 0.f) * n));
+        const int c = nth_class<BLOCK>(row, m, (int)((double)r.u * n), classes, sh.part_i);
+        if (threadIdx.x == 0) {
+            *cls = c;
+            *logp = (float)-log((double)n);
+        }
+        return;
+    }
+    Draw<BLOCK, Row> d{sh, row};
     d.best = (double)m;
     d.by = kPartsOfE / (double)r.temperature;
-    d.bits = bits;
     d.magic = __longlong_as_double((long long)(1023 + 52 - bits) << 52);
-    d.least_place = 0x1.fffffffffffffp10;  // (just below kBuckets)
-    if (r.min_p > 0.f) d.least_place = fmin(d.least_place, -log2((double)r.min_p) * kParts);
-    const auto weight = [&](double s, int b) { return d.weight_of(s, b); };
-    double mass[Draw<BLOCK, Each>::kEach], all;
-    if (r.k != INT_MAX) {
-        d.clear();
-        d.kept([&](double, int b, unsigned long long) { atomicAdd(&sh.mass[b], 1ull); });
-        __syncthreads();
-        const double before = d.sums([](int) { return 1.0; }, mass, &all);
-        if (all > (double)r.k) {
-            int bucket;
-            double front;
-            const double last = (double)(r.k - 1);
-            d.find(mass, before, last, false, &bucket, &front);
-            const unsigned long long key = d.resolve(bucket, last - front, false, [](double, int) { return 1ull; }).key;
-            d.cut = key;
-        }
+    bool all_kept = true;
+    if (r.min_p > 0.f) {
+        d.last_place = fmin(d.last_place, -log2((double)r.min_p) * kParts);
+        d.least = fmaxf(d.least, d.score_below(d.last_place));
+        all_kept = false;
     }
-    d.clear();
-    d.kept([&](double s, int b, unsigned long long) { atomicAdd(&sh.mass[b], weight(s, b)); });
-    __syncthreads();
+    if (r.k < classes) {
+        d.keep_best(r.k);
+        all_kept = all_kept && d.cut == 0 && d.least == -FLT_MAX;
+    }
+    const auto weight = [&](double s) { return d.weight_of(s); };
+    double mass[Draw<BLOCK, Row>::kEach], all;
+    d.add_up(all_kept);
     const double one = __longlong_as_double((long long)(1023 - bits) << 52);
     const auto unit = [&](int b) { return exp2(-(double)b / kParts) * one; };
     const double before = d.sums(unit, mass, &all);
@@ -535,24 +651,87 @@ __device__ __forceinline__ void draw_row(const Each &each, const RowSampling &r,
     }
 }
 
-// Classes side by side, bias and allowed sets: a workgroup goes over its row's scores as often as it has to.
-template <typename T, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
+// A row's scores, classes side by side, with bias and allowed sets. N vectors of 16 bytes to a thread, which stay in registers as they were read; longer rows (N is
+// 0) are read as often as they are gone over.
+template <typename T, int BLOCK, int N, bool RULES>
+struct ScoreRow {
+    static constexpr int V = 16 / (int)sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    const T *src;
+    const float *bias;
+    const unsigned *words;
+    int classes;
+    bool none;
+    Vec held[N > 0 ? N : 1];
+
+    __device__ __forceinline__ Vec read(int c) const {
+        if (c + V <= classes) return *reinterpret_cast<const Vec *>(src + c);
+        Vec v = (T)kNothing;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j < classes) v[j] = src[c + j];
+        return v;
+    }
+    __device__ __forceinline__ void load() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * BLOCK + (int)threadIdx.x) * V;
+            held[i] = c < classes ? read(c) : (Vec)(T)kNothing;
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void give(const Vec &v, int c, F f) {
+        float x[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = score_to_float(v[j]);
+        if constexpr (RULES) {
+            if (bias != nullptr) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] += bias[min(c + j, classes - 1)];
+            }
+            if (none || words != nullptr) {
+                const unsigned ok = none ? 0u : words[c / 32] >> (c % 32);
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] = ok >> j & 1u ? x[j] : kNothing;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = without_nan(x[j]);
+        f(x, c);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        if constexpr (N > 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                // (one vector at a time, unpacked anew wherever it is looked at: the compiler would keep all of them)
+                __builtin_amdgcn_sched_barrier(0);
+                typedef unsigned Words __attribute__((ext_vector_type(4)));
+                Words w = __builtin_bit_cast(Words, held[i]);
+                asm volatile("" : "+v"(w));
+                const int c = (i * BLOCK + (int)threadIdx.x) * V;
+                if (c < classes) give(__builtin_bit_cast(Vec, w), c, f);
+            }
+        } else {
+            for (int c = (int)threadIdx.x * V; c < classes; c += BLOCK * V) give(read(c), c, f);
+        }
+    }
+};
+
+template <typename T, int BLOCK, int N, bool RULES>
+__global__ __launch_bounds__(BLOCK, BLOCK == 1024 ? 4 : 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
     __shared__ DrawShared<BLOCK> sh;
     const long row = blockIdx.x;
     const RowSampling r = sampling_of(how, u, row);
-    const T *src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
-    bool none;
-    const unsigned *words = allowed_words(rules, row, (in.classes + 31) / 32, &none);
-    const auto each = [&](auto f) {
-        for (int c = threadIdx.x; c < in.classes; c += BLOCK) {
-            float s = score_to_float(src[c]);
-            if (rules.bias != nullptr) s += rules.bias[c];
-            if (none || (words != nullptr && !(words[c / 32] >> (c % 32) & 1u))) s = kNothing;
-            f(without_nan(s), c);
-        }
-    };
-    draw_row<BLOCK>(each, r, bits, sh, classes + row, logp + row);
+    ScoreRow<T, BLOCK, N, RULES> scores;
+    scores.src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
+    scores.classes = in.classes;
+    scores.bias = rules.bias;
+    scores.words = nullptr;
+    scores.none = false;
+    if constexpr (RULES) scores.words = allowed_words(rules, row, (in.classes + 31) / 32, &scores.none);
+    scores.load();
+    draw_row<BLOCK>(scores, r, in.classes, bits, sh, classes + row, logp + row);
 }
 
 // ------------------------------------------------------------------------------------------------------- how a call goes
@@ -586,13 +765,19 @@ void sample_few(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &ru
     else k_sample_few<T, 32><<<blocks, kSampleBlock, 0, s>>>(in, rules, how, u, classes, logp);
 }
 
-template <typename T>
+template <typename T, bool RULES>
 void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
     int log_classes = 0;
     while ((1 << log_classes) < in.classes) ++log_classes;
-    const int bits = std::min(50, 62 - log_classes);
-    if (in.classes <= 8192) k_sample_rows<T, 256><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
-    else k_sample_rows<T, 1024><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    const int bits = std::min(50, 61 - log_classes), vectors = (in.classes - 1) / (16 / (int)sizeof(T)) + 1;
+    if (vectors <= 4 * 256) k_sample_rows<T, 256, 0, RULES><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    else if (getenv("B1") == nullptr) k_sample_rows<T, 512, 0, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    else k_sample_rows<T, 1024, 0, RULES><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
+}
+template <typename T>
+void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
+    if (rules.bias != nullptr || rules.allowed != nullptr) sample_rows<T, true>(s, in, rules, how, u, classes, logp);
+    else sample_rows<T, false>(s, in, rules, how, u, classes, logp);
 }
 
 template <typename T>
