@@ -13,6 +13,7 @@ namespace tgbm {
 namespace {
 
 constexpr int kSampleBlock = 256;
+typedef float Float4 __attribute__((ext_vector_type(4), aligned(4)));
 constexpr float kNothing = -__builtin_inff();
 constexpr float kGreedyBelow = 1e-6f;  // temperatures below take the best class
 constexpr float kLargestBelowOne = 0x1.fffffep-1f;
@@ -243,17 +244,22 @@ __global__ __launch_bounds__(kSampleBlock) void k_lay_shown(tgbm_scores in, tgbm
     });
 }
 
-// A score's place on the scale that sums are kept by: 32 parts to a halving of w, 64 halvings; its bucket is the nearest whole number. What is further down than that
+// A score's place on the scale that sums are kept by: P parts to a halving of w, 64 halvings; its bucket is the nearest whole number. What is further down than that
 // (2^-64 of the best class) is nothing beside a random number's last place, 2^-24, whatever there is of it.
-constexpr int kParts = 32, kBuckets = 64 * kParts;
-constexpr double kPartsOfE = kParts * 1.44269504088896340736;  // parts to a factor of e
-constexpr double kToWhole = 6755399441055744.0;                // 1.5 * 2^52: the sum's low word is the nearest whole number
+template <int P>
+struct Scale {
+    static constexpr int kBuckets = 64 * P;
+    static constexpr double kOfE = P * 1.44269504088896340736;  // parts to a factor of e
+};
+constexpr double kToWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest whole number
 
-// 2^(-h / 32), h in [-1/2, 1/2], plus `magic` = 2^(52 - bits): its last 52 bits are the power of two times 2^bits, rounded. Taylor's series: the sixth term is below
-// 2^-48 of the whole, 2^-46 is what a whole number of a row of 2^16 classes is rounded by.
+// 2^(-h / P), h in [-1/2, 1/2], plus `magic` = 2^(52 - bits): its last 52 bits are the power of two times 2^bits, rounded. Taylor's series, up to where the next term
+// is below 2^-48 of the whole; 2^-46 is what a whole number of a row of 2^16 classes is rounded by.
+template <int P>
 __device__ __forceinline__ unsigned long long part_of_two(double h, double magic) {
-    constexpr double a = -0.69314718055994530942 / kParts, c2 = a * a / 2, c3 = c2 * a / 3, c4 = c3 * a / 4, c5 = c4 * a / 5;
-    double e = __builtin_fma(h, c5, c4);
+    constexpr double a = -0.69314718055994530942 / P, c2 = a * a / 2, c3 = c2 * a / 3, c4 = c3 * a / 4, c5 = c4 * a / 5, c6 = c5 * a / 6, c7 = c6 * a / 7;
+    static_assert(P == 32 || P == 8);
+    double e = P == 32 ? __builtin_fma(h, c5, c4) : __builtin_fma(h, __builtin_fma(h, __builtin_fma(h, c7, c6), c5), c4);
     e = __builtin_fma(h, e, c3);
     e = __builtin_fma(h, e, c2);
     e = __builtin_fma(h, e, a);
@@ -261,24 +267,36 @@ __device__ __forceinline__ unsigned long long part_of_two(double h, double magic
     return (unsigned long long)__double_as_longlong(e + magic) & 0xfffffffffffffull;
 }
 
-constexpr int kListed = 256;
-template <int BLOCK>
+// What is shared by the G threads that work on a row, a workgroup or a wavefront of several.
+template <int G>
+constexpr int parts_of() { return G == 64 ? 8 : 32; }
+template <int G>
+constexpr int listed_of() { return G == 64 ? 64 : 256; }
+template <int G>
 struct DrawShared {
-    unsigned long long mass[kBuckets + 1];  // (the last one takes what does not count)
-    unsigned long long key[kListed], weight[kListed], front[kListed];
-    double part[BLOCK / 64];
-    float part_f[BLOCK / 64];
-    int part_i[BLOCK / 64];
+    unsigned long long mass[Scale<parts_of<G>()>::kBuckets + 1];  // (the last one takes what does not count)
+    unsigned long long key[listed_of<G>()], weight[listed_of<G>()], front[listed_of<G>()];
+    double part[G / 64];
+    float part_f[G / 64];
+    int part_i[G / 64];
     unsigned long long best, least, most;
     double before;
     int listed, bucket;
 };
+template <int G>
+__device__ __forceinline__ void group_sync() {
+    if constexpr (G == 64) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else __syncthreads();
+}
+template <int G>
+__device__ __forceinline__ int in_group() { return G == 64 ? lane_id() : (int)threadIdx.x; }
 
-// One workgroup's work on a row. Row: row.each(f) calls f(scores, their first class) for the thread's vectors; what is no class or NaN is -infinity there.
-template <int BLOCK, typename Row>
+// A group's work on a row. Row: row.each(f) calls f(scores, their first class) for the thread's vectors; what is no class is -infinity there, NaNs stay what they
+// are and are to be let fall by comparisons.
+template <int G, typename Row>
 struct Draw {
-    static constexpr int V = Row::V, kEach = kBuckets / BLOCK;
-    DrawShared<BLOCK> &sh;
+    static constexpr int V = Row::V, P = parts_of<G>(), kBuckets = Scale<P>::kBuckets, kEach = kBuckets / G, kListed = listed_of<G>();
+    DrawShared<G> &sh;
     Row &row;
     double best, by;  // (the place of a score is (best - score) * by)
     double magic;
@@ -289,7 +307,7 @@ struct Draw {
     static __device__ __forceinline__ unsigned long long key_of(float x, int c) { return (unsigned long long)ordered(x) << 32 | (unsigned)~c; }
     __device__ __forceinline__ double place_of(float x) const { return (best - (double)x) * by; }
     static __device__ __forceinline__ int bucket_of(double place) { return (int)__double_as_longlong(place + kToWhole); }
-    __device__ __forceinline__ unsigned long long weight_of(double place) const { return part_of_two(place - ((place + kToWhole) - kToWhole), magic); }
+    __device__ __forceinline__ unsigned long long weight_of(double place) const { return part_of_two<P>(place - ((place + kToWhole) - kToWhole), magic); }
     // A score below which none has a place up to `place`; the other way: above which none has one from there on.
     __device__ __forceinline__ float score_below(double place) const {
         const double x = best - place / by;
@@ -321,12 +339,17 @@ struct Draw {
     // Exclusive sums over the threads, in their order, and the sum of all.
     __device__ __forceinline__ double scan(double v, double *all) {
         const double upto = wave_scan_d(v);
-        __syncthreads();
+        if constexpr (G == 64) {
+            *all = read_lane_d(upto, 63);
+            const double up = shfl_up_d(upto, 1);
+            return lane_id() == 0 ? 0.0 : up;
+        }
+        group_sync<G>();
         if (lane_id() == 63) sh.part[wave_id()] = upto;
-        __syncthreads();
+        group_sync<G>();
         double before = 0, sum = 0;
 #pragma unroll
-        for (int w = 0; w < BLOCK / 64; ++w) {
+        for (int w = 0; w < G / 64; ++w) {
             if (w == wave_id()) before = sum;
             sum += sh.part[w];
         }
@@ -335,20 +358,20 @@ struct Draw {
         return lane_id() == 0 ? before : before + up;
     }
     __device__ __forceinline__ void clear() {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kBuckets; i += BLOCK) sh.mass[i] = 0;
+        group_sync<G>();
+        for (int i = in_group<G>(); i < kBuckets; i += G) sh.mass[i] = 0;
         clear_list();
     }
     __device__ __forceinline__ void clear_list() {
-        __syncthreads();
-        if (threadIdx.x == 0) {
+        group_sync<G>();
+        if (in_group<G>() == 0) {
             sh.bucket = 0;
             sh.listed = 0;
             sh.best = 0;
             sh.least = ~0ull;
             sh.most = 0;
         }
-        __syncthreads();
+        group_sync<G>();
     }
 
     // Whether the order up to `before` leaves the next one in what is looked for: up to a target, or below it.
@@ -360,7 +383,7 @@ struct Draw {
         double mine = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int b = threadIdx.x * kEach + i;
+            const int b = in_group<G>() * kEach + i;
             const unsigned long long m = sh.mass[b];
             mass[i] = m != 0 ? (double)m * unit(b) : 0.0;
             mine += mass[i];
@@ -369,25 +392,25 @@ struct Draw {
     }
     // The bucket where the sum passes the target, and the sum in front of it.
     __device__ __forceinline__ void find(const double (&mass)[kEach], double before, double target, bool below, int *bucket, double *front) {
-        __syncthreads();
-        if (threadIdx.x == 0) sh.bucket = 0;
-        __syncthreads();
+        group_sync<G>();
+        if (in_group<G>() == 0) sh.bucket = 0;
+        group_sync<G>();
         int at = -1;
         double its = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (mass[i] > 0 && within(before, target, below)) {
-                at = threadIdx.x * kEach + i;
+                at = in_group<G>() * kEach + i;
                 its = before;
             }
             before += mass[i];
         }
         if (at >= 0) atomicMax(&sh.bucket, at);
-        __syncthreads();
+        group_sync<G>();
         *bucket = sh.bucket;
         if (at == *bucket) sh.before = its;
-        else if (*bucket == 0 && threadIdx.x == 0) sh.before = 0;  // (roundings may leave none: the first one then)
-        __syncthreads();
+        else if (*bucket == 0 && in_group<G>() == 0) sh.before = 0;  // (roundings may leave none: the first one then)
+        group_sync<G>();
         *front = sh.before;
     }
 
@@ -395,6 +418,7 @@ struct Draw {
         unsigned long long key;
         double before, weight;  // in the bucket's unit
     };
+    static constexpr int kKeyBits = P == 32 ? 11 : 9;
     // The one of a bucket where its sum passes the target (in its unit). weight(place): of one.
     template <typename Weight>
     __device__ __forceinline__ Found resolve(int bucket, double target, bool below, Weight weight) {
@@ -412,7 +436,7 @@ struct Draw {
                     sh.front[to] = 0;
                 }
             });
-            __syncthreads();
+            group_sync<G>();
             const int n = sh.listed;
             if (n <= kListed) return among(n, front, target, below);
             // too many for a list: by parts of the keys between the least and the largest of them
@@ -421,16 +445,16 @@ struct Draw {
                 atomicMin(&sh.least, key);
                 atomicMax(&sh.most, key);
             });
-            __syncthreads();
+            group_sync<G>();
             lo = sh.least;
             hi = sh.most;
-            const int width = 64 - __clzll((long long)(hi - lo)), shift = width > 11 ? width - 11 : 0;
-            static_assert(kBuckets == 1 << 11);
+            const int width = 64 - __clzll((long long)(hi - lo)), shift = width > kKeyBits ? width - kKeyBits : 0;
+            static_assert(kBuckets == 1 << kKeyBits);
             clear();
             kept(low, high, [&](double s, int b, unsigned long long key) {
                 if (b == bucket && key >= lo && key <= hi) atomicAdd(&sh.mass[(hi - key) >> shift], weight(s));
             });
-            __syncthreads();
+            group_sync<G>();
             double mass[kEach], all;
             const double before = sums([](int) { return 1.0; }, mass, &all);
             int part;
@@ -444,42 +468,37 @@ struct Draw {
     }
     // The same among n listed ones, which are put in order by what is in front of each.
     __device__ __forceinline__ Found among(int n, double front, double target, bool below) {
-        constexpr int kShares = BLOCK / kListed > 0 ? BLOCK / kListed : 1;
-        const int share = threadIdx.x / kListed;
-        for (int j = threadIdx.x % kListed; j < n; j += BLOCK < kListed ? BLOCK : kListed) {
+        constexpr int kShares = G / kListed;
+        const int share = in_group<G>() / kListed;
+        if (const int j = in_group<G>() % kListed; j < n) {
             const unsigned long long mine = sh.key[j];
             unsigned long long sum = 0;
             for (int o = share; o < n; o += kShares) sum += sh.key[o] > mine ? sh.weight[o] : 0ull;
             atomicAdd(&sh.front[j], sum);
         }
-        __syncthreads();
+        group_sync<G>();
         // (the first one always is; a larger sum in front comes later in the order, and no two are equal)
-        for (int j = threadIdx.x; j < n; j += BLOCK)
+        for (int j = in_group<G>(); j < n; j += G)
             if (sh.front[j] != 0 && within(front + (double)sh.front[j], target, below)) atomicMax(&sh.best, sh.front[j]);
-        __syncthreads();
+        group_sync<G>();
         const unsigned long long its = sh.best;
-        for (int j = threadIdx.x; j < n; j += BLOCK)
+        for (int j = in_group<G>(); j < n; j += G)
             if (sh.front[j] == its) sh.listed = j;
-        __syncthreads();
+        group_sync<G>();
         const int j = sh.listed;
         return Found{sh.key[j], front + (double)its, (double)sh.weight[j]};
     }
 
     // Leaves the k best. The k-th of the threads' own best scores is a bound: only what reaches it is looked at one by one.
-    __device__ __forceinline__ void keep_best(int k) {
+    __device__ __forceinline__ void keep_best(int k, float mine) {
         double mass[kEach], all, front;
         int bucket;
         const auto ones = [](int) { return 1.0; };
         float bound = least;
-        if (k <= BLOCK) {
-            float mine = kNothing;
-            row.each([&](const float (&x)[V], int) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) mine = fmaxf(mine, x[j]);
-            });
+        if (k <= G) {
             clear();
             if (mine >= least && place_of(mine) <= last_place) atomicAdd(&sh.mass[bucket_of(place_of(mine))], 1ull);
-            __syncthreads();
+            group_sync<G>();
             const double before = sums(ones, mass, &all);
             if (all >= (double)k) {
                 find(mass, before, (double)(k - 1), false, &bucket, &front);
@@ -488,7 +507,7 @@ struct Draw {
         }
         clear();
         kept(bound, __builtin_inff(), [&](double, int b, unsigned long long) { atomicAdd(&sh.mass[b], 1ull); });
-        __syncthreads();
+        group_sync<G>();
         const double before = sums(ones, mass, &all);
         if (all <= (double)k) {  // (all that reach the bound: it is the cut)
             least = bound;
@@ -510,48 +529,51 @@ struct Draw {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const double s = __builtin_fmin(place_of(x[j]), (double)kBuckets), at = s + kToWhole;
-                    atomicAdd(&sh.mass[(int)__double_as_longlong(at)], part_of_two(s - (at - kToWhole), magic));
+                    atomicAdd(&sh.mass[(int)__double_as_longlong(at)], part_of_two<P>(s - (at - kToWhole), magic));
                 }
             });
         }
-        __syncthreads();
+        group_sync<G>();
     }
 };
 
-template <int BLOCK>
+template <int G>
 __device__ __forceinline__ float block_max(float v, float *part) {
     v = wave_max_f(v);
-    __syncthreads();
+    if constexpr (G == 64) return v;
+    group_sync<G>();
     if (lane_id() == 0) part[wave_id()] = v;
-    __syncthreads();
+    group_sync<G>();
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) v = fmaxf(v, part[w]);
+    for (int w = 0; w < G / 64; ++w) v = fmaxf(v, part[w]);
     return v;
 }
-template <int BLOCK>
+template <int G>
 __device__ __forceinline__ int block_min(int v, int *part) {
     v = wave_min_i(v);
-    __syncthreads();
+    if constexpr (G == 64) return v;
+    group_sync<G>();
     if (lane_id() == 0) part[wave_id()] = v;
-    __syncthreads();
+    group_sync<G>();
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) v = min(v, part[w]);
+    for (int w = 0; w < G / 64; ++w) v = min(v, part[w]);
     return v;
 }
-template <int BLOCK>
+template <int G>
 __device__ __forceinline__ int block_sum(int v, int *part) {
     v = wave_sum_i(v);
-    __syncthreads();
+    if constexpr (G == 64) return v;
+    group_sync<G>();
     if (lane_id() == 0) part[wave_id()] = v;
-    __syncthreads();
+    group_sync<G>();
     v = 0;
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) v += part[w];
+    for (int w = 0; w < G / 64; ++w) v += part[w];
     return v;
 }
 
 // The class of the n-th (from 0) score that is m, by bisection.
-template <int BLOCK, typename Row>
+template <int G, typename Row>
 __device__ __forceinline__ int nth_class(Row &row, float m, int n, int classes, int *part) {
     int lo = -1, hi = classes - 1;
     while (hi - lo > 1) {
@@ -561,24 +583,24 @@ __device__ __forceinline__ int nth_class(Row &row, float m, int n, int classes, 
 #pragma unroll
             for (int j = 0; j < Row::V; ++j) count += x[j] == m && c + j <= mid ? 1 : 0;
         });
-        if (block_sum<BLOCK>(count, part) > n) hi = mid;
+        if (block_sum<G>(count, part) > n) hi = mid;
         else lo = mid;
     }
     return hi;
 }
 
 // The draw of a row by a workgroup. bits: of a whole number that stands for a w of one, so that the sum of a row's has room in 63.
-template <int BLOCK, typename Row>
-__device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int classes, int bits, DrawShared<BLOCK> &sh, int *cls, float *logp) {
+template <int G, typename Row>
+__device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int classes, int bits, DrawShared<G> &sh, int *cls, float *logp) {
     constexpr int V = Row::V;
-    float m = kNothing;
+    float mine = kNothing;
     row.each([&](const float (&x)[V], int) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = fmaxf(m, x[j]);
+        for (int j = 0; j < V; ++j) mine = fmaxf(mine, x[j]);
     });
-    m = block_max<BLOCK>(m, sh.part_f);
+    const float m = block_max<G>(mine, sh.part_f);
     if (m == kNothing || r.none) {
-        if (threadIdx.x == 0) {
+        if (in_group<G>() == 0) {
             *cls = -1;
             *logp = r.none ? __builtin_nanf("") : kNothing;
         }
@@ -590,8 +612,8 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
 #pragma unroll
             for (int j = 0; j < V; ++j) first = x[j] == m ? min(first, c + j) : first;
         });
-        first = block_min<BLOCK>(first, sh.part_i);
-        if (threadIdx.x == 0) {
+        first = block_min<G>(first, sh.part_i);
+        if (in_group<G>() == 0) {
             *cls = first;
             *logp = 0.f;
         }
@@ -603,34 +625,35 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
 #pragma unroll
             for (int j = 0; j < V; ++j) count += x[j] == m ? 1 : 0;
         });
-        int n = min(block_sum<BLOCK>(count, sh.part_i), r.k);
+        int n = min(block_sum<G>(count, sh.part_i), r.k);
         if (r.p < 1.f) n = max(1, (int)ceil((double)fmaxf(r.p, 0.f) * n));
-        const int c = nth_class<BLOCK>(row, m, (int)((double)r.u * n), classes, sh.part_i);
-        if (threadIdx.x == 0) {
+        const int c = nth_class<G>(row, m, (int)((double)r.u * n), classes, sh.part_i);
+        if (in_group<G>() == 0) {
             *cls = c;
             *logp = (float)-log((double)n);
         }
         return;
     }
-    Draw<BLOCK, Row> d{sh, row};
+    Draw<G, Row> d{sh, row};
     d.best = (double)m;
-    d.by = kPartsOfE / (double)r.temperature;
+    constexpr int P = parts_of<G>();
+    d.by = Scale<P>::kOfE / (double)r.temperature;
     d.magic = __longlong_as_double((long long)(1023 + 52 - bits) << 52);
     bool all_kept = true;
     if (r.min_p > 0.f) {
-        d.last_place = fmin(d.last_place, -log2((double)r.min_p) * kParts);
+        d.last_place = fmin(d.last_place, -log2((double)r.min_p) * P);
         d.least = fmaxf(d.least, d.score_below(d.last_place));
         all_kept = false;
     }
     if (r.k < classes) {
-        d.keep_best(r.k);
+        d.keep_best(r.k, mine);
         all_kept = all_kept && d.cut == 0 && d.least == -FLT_MAX;
     }
     const auto weight = [&](double s) { return d.weight_of(s); };
-    double mass[Draw<BLOCK, Row>::kEach], all;
+    double mass[Draw<G, Row>::kEach], all;
     d.add_up(all_kept);
     const double one = __longlong_as_double((long long)(1023 - bits) << 52);
-    const auto unit = [&](int b) { return exp2(-(double)b / kParts) * one; };
+    const auto unit = [&](int b) { return exp2(-(double)b / P) * one; };
     const double before = d.sums(unit, mass, &all);
     double kept = all, front;
     int bucket;
@@ -645,15 +668,15 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
     d.find(mass, before, target, false, &bucket, &front);
     const double its = unit(bucket);
     const auto drawn = d.resolve(bucket, (target - front) / its, false, weight);
-    if (threadIdx.x == 0) {
+    if (in_group<G>() == 0) {
         *cls = (int)~(unsigned)drawn.key;
         *logp = (float)log(drawn.weight * its / kept);
     }
 }
 
-// A row's scores, classes side by side, with bias and allowed sets. N vectors of 16 bytes to a thread, which stay in registers as they were read; longer rows (N is
-// 0) are read as often as they are gone over.
-template <typename T, int BLOCK, int N, bool RULES>
+// A row's scores, classes side by side, with bias and allowed sets, read by vectors of 16 bytes as often as they are gone over. (Scores that stay in registers want
+// every loop over them to be written out, and there are a dozen: the compiler did not find registers for it.)
+template <typename T, int G, bool RULES>
 struct ScoreRow {
     static constexpr int V = 16 / (int)sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
@@ -662,7 +685,6 @@ struct ScoreRow {
     const unsigned *words;
     int classes;
     bool none;
-    Vec held[N > 0 ? N : 1];
 
     __device__ __forceinline__ Vec read(int c) const {
         if (c + V <= classes) return *reinterpret_cast<const Vec *>(src + c);
@@ -672,13 +694,6 @@ struct ScoreRow {
             if (c + j < classes) v[j] = src[c + j];
         return v;
     }
-    __device__ __forceinline__ void load() {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = (i * BLOCK + (int)threadIdx.x) * V;
-            held[i] = c < classes ? read(c) : (Vec)(T)kNothing;
-        }
-    }
     template <typename F>
     __device__ __forceinline__ void give(const Vec &v, int c, F f) {
         float x[V];
@@ -687,7 +702,16 @@ struct ScoreRow {
         if constexpr (RULES) {
             if (bias != nullptr) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] += bias[min(c + j, classes - 1)];
+                for (int j = 0; j < V; j += 4) {
+                    if (c + j + 4 <= classes) {
+                        const Float4 b = *reinterpret_cast<const Float4 *>(bias + c + j);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) x[j + q] += b[q];
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) x[j + q] += c + j + q < classes ? bias[c + j + q] : 0.f;
+                    }
+                }
             }
             if (none || words != nullptr) {
                 const unsigned ok = none ? 0u : words[c / 32] >> (c % 32);
@@ -695,55 +719,155 @@ struct ScoreRow {
                 for (int j = 0; j < V; ++j) x[j] = ok >> j & 1u ? x[j] : kNothing;
             }
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = without_nan(x[j]);
         f(x, c);
     }
     template <typename F>
     __device__ __forceinline__ void each(F f) {
-        if constexpr (N > 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                // (one vector at a time, unpacked anew wherever it is looked at: the compiler would keep all of them)
-                __builtin_amdgcn_sched_barrier(0);
-                typedef unsigned Words __attribute__((ext_vector_type(4)));
-                Words w = __builtin_bit_cast(Words, held[i]);
-                asm volatile("" : "+v"(w));
-                const int c = (i * BLOCK + (int)threadIdx.x) * V;
-                if (c < classes) give(__builtin_bit_cast(Vec, w), c, f);
-            }
-        } else {
-            for (int c = (int)threadIdx.x * V; c < classes; c += BLOCK * V) give(read(c), c, f);
+        // (the next vectors are on their way while one is worked on)
+        constexpr int kStep = G * V;
+        int c = (int)threadIdx.x * V;
+        Vec a = (T)kNothing, b = (T)kNothing;
+        if (c < classes) a = read(c);
+        if (c + kStep < classes) b = read(c + kStep);
+        for (; c < classes; c += kStep) {
+            const Vec now = a;
+            a = b;
+            if (c + 2 * kStep < classes) b = read(c + 2 * kStep);
+            give(now, c, f);
         }
     }
 };
 
-template <typename T, int BLOCK, int N, bool RULES>
-__global__ __launch_bounds__(BLOCK, BLOCK == 1024 ? 4 : 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
-    __shared__ DrawShared<BLOCK> sh;
+template <typename T, int G, bool RULES>
+__global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
+    __shared__ DrawShared<G> sh;
     const long row = blockIdx.x;
     const RowSampling r = sampling_of(how, u, row);
-    ScoreRow<T, BLOCK, N, RULES> scores;
+    ScoreRow<T, G, RULES> scores;
     scores.src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
     scores.classes = in.classes;
     scores.bias = rules.bias;
     scores.words = nullptr;
     scores.none = false;
     if constexpr (RULES) scores.words = allowed_words(rules, row, (in.classes + 31) / 32, &scores.none);
-    scores.load();
-    draw_row<BLOCK>(scores, r, in.classes, bits, sh, classes + row, logp + row);
+    draw_row<G>(scores, r, in.classes, bits, sh, classes + row, logp + row);
+}
+
+// A row in LDS, adjusted, for a wavefront; behind its classes -infinity up to a multiple of four.
+struct LdsRow {
+    static constexpr int V = 4;
+    const float *scores;
+    int classes;
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int c = lane_id() * 4; c < classes; c += 256) {
+            const float4 v = *reinterpret_cast<const float4 *>(scores + c);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            f(x, c);
+        }
+    }
+};
+
+// Rows of a middle length: a wavefront to a row, whose adjusted scores lie in LDS. COLUMNS: the rows lie side by side, and a workgroup brings as many as it has
+// wavefronts; else each brings its own. A class that was shown has a bit, and its cell holds how often first; whoever takes the bit away puts the score there.
+// LDS of a wavefront: DrawShared, pitch cells, with lists pitch / 32 + 1 words of bits.
+template <typename T, bool COLUMNS, bool RULES>
+__global__ __launch_bounds__(COLUMNS ? 1024 : 256) void k_sample_middle(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits,
+                                                                       int pitch, int of_wave) {
+    constexpr int kWaves = COLUMNS ? 16 : 4;
+    extern __shared__ __align__(16) char lds[];
+    const auto shared_of = [&](int w) { return reinterpret_cast<DrawShared<64> *>(lds + (size_t)w * of_wave); };
+    const auto cells_of = [&](int w) { return reinterpret_cast<unsigned *>(lds + (size_t)w * of_wave + sizeof(DrawShared<64>)); };
+    const auto bits_of = [&](int w) { return cells_of(w) + pitch; };
+    static_assert(sizeof(DrawShared<64>) % 16 == 0);
+    const int lane = lane_id(), wave = wave_id(), n = in.classes;
+    const long row0 = (COLUMNS ? tile_of_block(blockIdx.x, gridDim.x) : (long)blockIdx.x) * kWaves;
+    if (row0 >= in.rows) return;
+    // who brings what: r: the row of the tile, at, step: its classes
+    const int r = COLUMNS ? (int)threadIdx.x % 16 : wave, at = COLUMNS ? (int)threadIdx.x / 16 : lane, step = 64;
+    const long row = row0 + r;
+    const bool on = row < in.rows;
+    if (!COLUMNS && !on) return;
+    const auto sync = [&] { group_sync<COLUMNS ? 1024 : 64>(); };
+    unsigned *const cell = cells_of(r), *const bit_of = bits_of(r);
+    const T *src = static_cast<const T *>(in.data) + (size_t)(on ? row : 0) * in.row_stride;
+    bool none = false;
+    const unsigned *words = nullptr;
+    long long b = 0, e = 0;
+    if constexpr (RULES) {
+        if (on) words = allowed_words(rules, row, (n + 31) / 32, &none);
+        if (rules.shown != nullptr) {
+            for (int i = at; i < (n + 31) / 32; i += step) bit_of[i] = 0;
+            sync();
+            if (on) shown_range(rules, row, &b, &e);
+            for (long long i = b + at; i < e; i += step) {
+                const int c = rules.shown[i];
+                if ((unsigned)c >= (unsigned)n) continue;
+                cell[c] = 0;
+                atomicOr(&bit_of[c / 32], 1u << (c % 32));
+            }
+            sync();
+            for (long long i = b + at; i < e; i += step) {
+                const int c = rules.shown[i];
+                if ((unsigned)c < (unsigned)n) atomicAdd(&cell[c], 1u);
+            }
+        }
+    }
+    const auto one = [&](int c, T v) {
+        float s = score_to_float(v);
+        if constexpr (RULES) {
+            if (rules.bias != nullptr) s += rules.bias[c];
+            if (none || (words != nullptr && !(words[c / 32] >> (c % 32) & 1u))) s = kNothing;
+            if (rules.shown != nullptr && (bit_of[c / 32] >> (c % 32) & 1u)) return;
+        }
+        cell[c] = __float_as_uint(s);
+    };
+    if (on) {
+        // (eight loads of a thread are on their way together)
+        for (int c = at; c < n; c += 8 * step) {
+            T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = src[(size_t)min(c + i * step, n - 1) * in.class_stride];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i * step < n) one(c + i * step, v[i]);
+        }
+        if (at < (-n & 3)) cell[n + at] = __float_as_uint(kNothing);
+    }
+    if constexpr (RULES) {
+        if (rules.shown != nullptr) {
+            sync();
+            for (long long i = b + at; i < e; i += step) {
+                const int c = rules.shown[i];
+                if ((unsigned)c >= (unsigned)n) continue;
+                const unsigned bit = 1u << (c % 32);
+                if (!(atomicAnd(&bit_of[c / 32], ~bit) & bit)) continue;  // (another mention of the class has come first)
+                const bool ok = !none && (words == nullptr || words[c / 32] & bit);
+                cell[c] = __float_as_uint(adjusted(score_to_float(src[(size_t)c * in.class_stride]), rules.bias != nullptr ? rules.bias[c] : 0.f, cell[c], ok, rules));
+            }
+        }
+    }
+    sync();
+    const long its = row0 + wave;
+    if (its >= in.rows) return;
+    LdsRow scores{reinterpret_cast<const float *>(cells_of(wave)), n};
+    draw_row<64>(scores, sampling_of(how, u, its), n, bits, *shared_of(wave), classes + its, logp + its);
 }
 
 // ------------------------------------------------------------------------------------------------------- how a call goes
-enum Way { kFew, kFromList, kRows, kLaidOut };
+enum Way { kFew, kFromList, kMiddle, kRows, kLaidOut };
 constexpr int kFewClasses = 32;
+constexpr int kMiddleRows = 2048, kMiddleColumns = 1024;  // (16 rows' LDS holds 1050)
 constexpr size_t kLaidBytes = (size_t)128 << 20;  // (half of what the last cache holds)
 
 Way way_of(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how) {
     if (in.classes <= kFewClasses) return kFew;
     if (how.k == nullptr && how.k_all >= 1 && how.k_all <= kTopMost) return kFromList;
+    if (in.classes <= (rows_side_by_side(in) ? kMiddleColumns : kMiddleRows)) return kMiddle;
     return rules.shown != nullptr || rows_side_by_side(in) ? kLaidOut : kRows;
 }
+int middle_pitch(int classes) { return (classes + 3) / 4 * 4; }
+int middle_lds(int classes) { return (int)((sizeof(DrawShared<64>) + sizeof(unsigned) * (middle_pitch(classes) + (classes + 31) / 32) + 15) / 16 * 16); }
 // values, classes and what top leaves beside them, in front of its own workspace
 size_t list_bytes(size_t rows, size_t k) { return (sizeof(float) * rows * (2 * k + 1) + 15) / 16 * 16; }
 long laid_pitch(int classes) { return ((long)classes + 3) / 4 * 4; }
@@ -765,14 +889,37 @@ void sample_few(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &ru
     else k_sample_few<T, 32><<<blocks, kSampleBlock, 0, s>>>(in, rules, how, u, classes, logp);
 }
 
+// Bits of a whole number that stands for a w of one: the sum of a row's, of which w is at most 1.05 in a bucket, has room in 63.
+int weight_bits(int classes) {
+    int log_classes = 0;
+    while ((1 << log_classes) < classes) ++log_classes;
+    return std::min(50, 61 - log_classes);
+}
+
+template <typename T, bool COLUMNS, bool RULES>
+void sample_middle(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
+    constexpr int kWaves = COLUMNS ? 16 : 4;
+    static LdsOptIn opt_in;
+    opt_in({reinterpret_cast<const void *>(&k_sample_middle<T, COLUMNS, RULES>)});
+    // (rows' cells begin four banks apart, so that sixteen rows of four classes are stored at once)
+    const int of_wave = COLUMNS ? (middle_lds(in.classes) + 239) / 256 * 256 + 16 : middle_lds(in.classes);
+    const unsigned tiles = (unsigned)((in.rows - 1) / kWaves + 1);
+    k_sample_middle<T, COLUMNS, RULES><<<COLUMNS ? blocks_of_tiles(tiles) : tiles, 64 * kWaves, of_wave * kWaves, s>>>(in, rules, how, u, classes, logp, weight_bits(in.classes),
+                                                                                                                      middle_pitch(in.classes), of_wave);
+}
+template <typename T>
+void sample_middle(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
+    const bool some = rules.bias != nullptr || rules.allowed != nullptr || rules.shown != nullptr;
+    if (rows_side_by_side(in)) (some ? sample_middle<T, true, true> : sample_middle<T, true, false>)(s, in, rules, how, u, classes, logp);
+    else (some ? sample_middle<T, false, true> : sample_middle<T, false, false>)(s, in, rules, how, u, classes, logp);
+}
+
 template <typename T, bool RULES>
 void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
-    int log_classes = 0;
-    while ((1 << log_classes) < in.classes) ++log_classes;
-    const int bits = std::min(50, 61 - log_classes), vectors = (in.classes - 1) / (16 / (int)sizeof(T)) + 1;
-    if (vectors <= 4 * 256) k_sample_rows<T, 256, 0, RULES><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
-    else if (getenv("B1") == nullptr) k_sample_rows<T, 512, 0, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
-    else k_sample_rows<T, 1024, 0, RULES><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    const int bits = weight_bits(in.classes), vectors = (in.classes - 1) / (16 / (int)sizeof(T)) + 1;
+    if (vectors <= 4 * 256) k_sample_rows<T, 256, RULES><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    else if (in.rows > 256) k_sample_rows<T, 512, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    else k_sample_rows<T, 1024, RULES><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
 }
 template <typename T>
 void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
@@ -801,6 +948,7 @@ void sample(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules,
             void *workspace) {
     switch (way_of(in, rules, how)) {
         case kFew: return sample_few<T>(s, in, rules, how, u, classes, logp);
+        case kMiddle: return sample_middle<T>(s, in, rules, how, u, classes, logp);
         case kRows: return sample_rows<T>(s, in, rules, how, u, classes, logp);
         case kLaidOut: return sample_laid_out<T>(s, in, rules, how, u, classes, logp, static_cast<float *>(workspace));
         case kFromList: {
