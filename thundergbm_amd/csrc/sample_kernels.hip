@@ -129,16 +129,19 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_few(tgbm_scores in, tgb
 
 // ------------------------------------------------------------------------------------------------------- from a list
 // Rows whose best classes are listed in order, as top leaves them: a wavefront takes a row's k of up to 128.
-__device__ __forceinline__ double shfl_up_d(double v, int d) { return __longlong_as_double(shfl_up_ll(__double_as_longlong(v), d)); }
-__device__ __forceinline__ double read_lane_d(double v, int lane) { return __longlong_as_double(read_lane_ll(__double_as_longlong(v), lane)); }
+// (of all lanes: one that does not take part hands nothing on)
+struct WaveSumD {
+    double v;
+    template <int CTRL, int ROWS>
+    __device__ __forceinline__ void at() { v += __longlong_as_double(dpp_ll<CTRL, ROWS>(__double_as_longlong(v))); }
+};
 __device__ __forceinline__ double wave_scan_d(double v) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double o = shfl_up_d(v, d);
-        if (lane_id() >= d) v += o;
-    }
-    return v;
+    WaveSumD s{v};
+    wave_scan_steps(s);
+    return s.v;
 }
+__device__ __forceinline__ double from_below_d(double v) { return __longlong_as_double(dpp_ll<kDppWaveShr1>(__double_as_longlong(v))); }  // (0 in lane 0)
+__device__ __forceinline__ double read_lane_d(double v, int lane) { return __longlong_as_double(read_lane_ll(__double_as_longlong(v), lane)); }
 __global__ __launch_bounds__(kSampleBlock) void k_sample_listed(const float *values, const int *listed, int k, int rows, tgbm_sampling how, const float *u, int *classes,
                                                                 float *logp) {
     const long row = (long)blockIdx.x * (kSampleBlock / 64) + wave_id();
@@ -164,8 +167,7 @@ __global__ __launch_bounds__(kSampleBlock) void k_sample_listed(const float *val
         w[i] = x[i] > kNothing && e >= (double)r.min_p && 2 * lane + i < (r.greedy ? 1 : r.k) ? e : 0.0;
     }
     const double upto1 = wave_scan_d(w[0] + w[1]), sum = read_lane_d(upto1, 63);
-    const double up = shfl_up_d(upto1, 1);  // (of all lanes: one that does not take part hands nothing on)
-    const double front0 = lane == 0 ? 0.0 : up, front1 = front0 + w[0];
+    const double front0 = from_below_d(upto1), front1 = front0 + w[0];
     double kept = sum;
     if (r.p < 1.f) {
         const double most = (double)r.p * sum;
@@ -273,15 +275,14 @@ constexpr int parts_of() { return G == 64 ? 8 : 32; }
 template <int G>
 constexpr int listed_of() { return G == 64 ? 64 : 256; }
 template <int G>
-struct DrawShared {
+struct alignas(16) DrawShared {
     unsigned long long mass[Scale<parts_of<G>()>::kBuckets + 1];  // (the last one takes what does not count)
     unsigned long long key[listed_of<G>()], weight[listed_of<G>()], front[listed_of<G>()];
     double part[G / 64];
     float part_f[G / 64];
     int part_i[G / 64];
     unsigned long long best, least, most;
-    double before;
-    int listed, bucket;
+    int listed;
 };
 template <int G>
 __device__ __forceinline__ void group_sync() {
@@ -341,8 +342,7 @@ struct Draw {
         const double upto = wave_scan_d(v);
         if constexpr (G == 64) {
             *all = read_lane_d(upto, 63);
-            const double up = shfl_up_d(upto, 1);
-            return lane_id() == 0 ? 0.0 : up;
+            return from_below_d(upto);
         }
         group_sync<G>();
         if (lane_id() == 63) sh.part[wave_id()] = upto;
@@ -354,8 +354,7 @@ struct Draw {
             sum += sh.part[w];
         }
         *all = sum;
-        const double up = shfl_up_d(upto, 1);
-        return lane_id() == 0 ? before : before + up;
+        return before + from_below_d(upto);
     }
     __device__ __forceinline__ void clear() {
         group_sync<G>();
@@ -365,7 +364,6 @@ struct Draw {
     __device__ __forceinline__ void clear_list() {
         group_sync<G>();
         if (in_group<G>() == 0) {
-            sh.bucket = 0;
             sh.listed = 0;
             sh.best = 0;
             sh.least = ~0ull;
@@ -377,24 +375,20 @@ struct Draw {
     // Whether the order up to `before` leaves the next one in what is looked for: up to a target, or below it.
     static __device__ __forceinline__ bool within(double before, double target, bool below) { return below ? before < target : before <= target; }
 
-    // The buckets' sums, those in front of the thread's, and the sum of all. unit(b): what a bucket's whole numbers count.
-    template <typename Unit>
-    __device__ __forceinline__ double sums(Unit unit, double (&mass)[kEach], double *all) {
+    // The buckets' sums, those in front of the thread's, and the sum of all. first, ratio: what the whole numbers of the thread's first bucket count, and each
+    // bucket's next to the one before.
+    __device__ __forceinline__ double sums(double first, double ratio, double (&mass)[kEach], double *all) {
         double mine = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int b = in_group<G>() * kEach + i;
-            const unsigned long long m = sh.mass[b];
-            mass[i] = m != 0 ? (double)m * unit(b) : 0.0;
+            mass[i] = (double)sh.mass[in_group<G>() * kEach + i] * first;
+            first *= ratio;
             mine += mass[i];
         }
         return scan(mine, all);
     }
-    // The bucket where the sum passes the target, and the sum in front of it.
+    // The bucket where the sum passes the target, and the sum in front of it (the first one, where roundings leave none).
     __device__ __forceinline__ void find(const double (&mass)[kEach], double before, double target, bool below, int *bucket, double *front) {
-        group_sync<G>();
-        if (in_group<G>() == 0) sh.bucket = 0;
-        group_sync<G>();
         int at = -1;
         double its = 0;
 #pragma unroll
@@ -405,13 +399,27 @@ struct Draw {
             }
             before += mass[i];
         }
-        if (at >= 0) atomicMax(&sh.bucket, at);
-        group_sync<G>();
-        *bucket = sh.bucket;
-        if (at == *bucket) sh.before = its;
-        else if (*bucket == 0 && in_group<G>() == 0) sh.before = 0;  // (roundings may leave none: the first one then)
-        group_sync<G>();
-        *front = sh.before;
+        const unsigned long long who = __ballot(at >= 0);
+        const int lane = who != 0 ? 63 - __clzll((long long)who) : 0;
+        at = read_lane(at, lane);
+        its = read_lane_d(its, lane);
+        if constexpr (G > 64) {
+            group_sync<G>();
+            if (lane_id() == 0) {
+                sh.part_i[wave_id()] = at;
+                sh.part[wave_id()] = its;
+            }
+            group_sync<G>();
+#pragma unroll
+            for (int w = 0; w < G / 64; ++w)
+                if (const int other = sh.part_i[w]; other >= 0) {
+                    at = other;
+                    its = sh.part[w];
+                }
+            group_sync<G>();
+        }
+        *bucket = __builtin_amdgcn_readfirstlane(at >= 0 ? at : 0);
+        *front = at >= 0 ? its : 0.0;
     }
 
     struct Found {
@@ -456,7 +464,7 @@ struct Draw {
             });
             group_sync<G>();
             double mass[kEach], all;
-            const double before = sums([](int) { return 1.0; }, mass, &all);
+            const double before = sums(1.0, 1.0, mass, &all);
             int part;
             double its;
             find(mass, front + before, target, below, &part, &its);
@@ -493,13 +501,12 @@ struct Draw {
     __device__ __forceinline__ void keep_best(int k, float mine) {
         double mass[kEach], all, front;
         int bucket;
-        const auto ones = [](int) { return 1.0; };
         float bound = least;
         if (k <= G) {
             clear();
             if (mine >= least && place_of(mine) <= last_place) atomicAdd(&sh.mass[bucket_of(place_of(mine))], 1ull);
             group_sync<G>();
-            const double before = sums(ones, mass, &all);
+            const double before = sums(1.0, 1.0, mass, &all);
             if (all >= (double)k) {
                 find(mass, before, (double)(k - 1), false, &bucket, &front);
                 bound = fmaxf(bound, score_below(bucket + 0.5));
@@ -508,7 +515,7 @@ struct Draw {
         clear();
         kept(bound, __builtin_inff(), [&](double, int b, unsigned long long) { atomicAdd(&sh.mass[b], 1ull); });
         group_sync<G>();
-        const double before = sums(ones, mass, &all);
+        const double before = sums(1.0, 1.0, mass, &all);
         if (all <= (double)k) {  // (all that reach the bound: it is the cut)
             least = bound;
             return;
@@ -654,7 +661,8 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
     d.add_up(all_kept);
     const double one = __longlong_as_double((long long)(1023 - bits) << 52);
     const auto unit = [&](int b) { return exp2(-(double)b / P) * one; };
-    const double before = d.sums(unit, mass, &all);
+    constexpr double kNext = P == 32 ? 0.97857206208770013451 : 0.91700404320467123174;  // 2^(-1 / P)
+    const double before = d.sums(unit(in_group<G>() * Draw<G, Row>::kEach), kNext, mass, &all);
     double kept = all, front;
     int bucket;
     if (r.p < 1.f) {
