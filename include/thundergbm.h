@@ -374,6 +374,14 @@ void tgbm_predict_adjusted(int row_size, const float *val, const int *row_ptr, c
 void tgbm_predict_top(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees,
                       int trees_per_iter, float learning_rate, const tgbm_score_rules *rules, int k, float temperature, float *values,
                       int *classes, float *lse);
+void tgbm_predict_sample(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees,
+                         int trees_per_iter, float learning_rate, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u,
+                         int *classes, float *logp);
+
+/* The k best classes of a linear layer, as a teacher's: host arrays x [row_size][n_features], weights [n_classes][n_features] and bias [n_classes] (may be NULL), in
+ * 8 bits each with a scale as tgbm_rows_quantise makes them; the outputs as tgbm_scores_top writes them. Wrong arguments abort the process. */
+void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes, const float *weights, const float *bias, int k, float temperature,
+                     float *values, int *classes, float *lse);
 
 #ifdef __cplusplus
 }

@@ -60,6 +60,8 @@ SIGNATURES = {
     "tgbm_trainer_teacher_loss": (C.c_double, [_P]),
     "tgbm_predict_adjusted": (None, [C.c_int, _P, _P, _P, _P, C.c_int, C.c_int, C.c_float, _P, _P]),
     "tgbm_predict_top": (None, [C.c_int, _P, _P, _P, _P, C.c_int, C.c_int, C.c_float, _P, C.c_int, C.c_float, _P, _P, _P]),
+    "tgbm_predict_sample": (None, [C.c_int, _P, _P, _P, _P, C.c_int, C.c_int, C.c_float, _P, _P, _P, _P, _P]),
+    "tgbm_linear_top": (None, [C.c_int, C.c_int, _P, C.c_int, _P, _P, C.c_int, C.c_float, _P, _P, _P]),
     "tgbm_scores_adjust": (C.c_int, [_P, _P, _P, _P]),
     "tgbm_scores_distill_workspace": (C.c_size_t, [_P, C.c_int]),
     "tgbm_scores_distill": (C.c_int, [_P, _P, _P, C.c_float, C.c_float, _P, _P, C.c_longlong, _P, C.c_size_t, _P]),

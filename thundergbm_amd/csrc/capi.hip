@@ -163,7 +163,7 @@ class DeviceRules {
     std::vector<void *> blocks_;
 };
 
-// What tgbm_predict_adjusted and tgbm_predict_top do alike: the scores on the device and the rules beside them.
+// What tgbm_predict_adjusted, tgbm_predict_top and tgbm_predict_sample do alike: the scores on the device and the rules beside them.
 template <typename Use>
 void with_scores(const char *entry, int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees, int trees_per_iter,
                  float learning_rate, const tgbm_score_rules *rules, Use use) {
@@ -538,6 +538,92 @@ void tgbm_predict_top(int row_size, const float *val, const int *row_ptr, const 
                     device_free(d_values);
                     device_free(workspace);
                 });
+}
+
+void tgbm_predict_sample(int row_size, const float *val, const int *row_ptr, const int *col_ptr, tgbm_model *model, int n_trees, int trees_per_iter,
+                         float learning_rate, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp) {
+    std::lock_guard<std::mutex> lock(g_call_mutex);
+    TGBM_CHECK(sampling_ok("tgbm_predict_sample", how), "tgbm_predict_sample: wrong arguments");
+    with_scores("tgbm_predict_sample", row_size, val, row_ptr, col_ptr, model, n_trees, trees_per_iter, learning_rate, rules,
+                [&](hipStream_t s, const tgbm_scores &scores, const tgbm_score_rules &r) {
+                    // the rows' numbers side by side: random numbers, settings, then what comes back
+                    const size_t n = (size_t)row_size;
+                    float *room = static_cast<float *>(device_alloc(sizeof(float) * n * 7));
+                    const auto up = [&](int place, const void *from) {
+                        if (from != nullptr) HIP_CHECK(hipMemcpyAsync(room + n * place, from, sizeof(float) * n, hipMemcpyHostToDevice, s));
+                        return from != nullptr ? room + n * place : nullptr;
+                    };
+                    tgbm_sampling h = *how;
+                    const float *d_u = up(0, u);
+                    h.temperature = up(1, how->temperature);
+                    h.p = up(2, how->p);
+                    h.min_p = up(3, how->min_p);
+                    h.k = reinterpret_cast<const int *>(up(4, how->k));
+                    const size_t bytes = scores_sample_workspace(scores, r, h);
+                    void *workspace = bytes > 0 ? device_alloc(bytes) : nullptr;
+                    int *d_classes = reinterpret_cast<int *>(room + n * 5);
+                    float *d_logp = room + n * 6;
+                    launch_scores_sample(s, scores, r, h, d_u, d_classes, d_logp, workspace);
+                    HIP_CHECK(hipMemcpyAsync(classes, d_classes, sizeof(int) * n, hipMemcpyDeviceToHost, s));
+                    HIP_CHECK(hipMemcpyAsync(logp, d_logp, sizeof(float) * n, hipMemcpyDeviceToHost, s));
+                    HIP_CHECK(hipStreamSynchronize(s));
+                    device_free(room);
+                    device_free(workspace);
+                });
+}
+
+void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes, const float *weights, const float *bias, int k, float temperature, float *values,
+                     int *classes, float *lse) {
+    std::lock_guard<std::mutex> lock(g_call_mutex);
+    const char *entry = "tgbm_linear_top";
+    TGBM_CHECK(k >= 1 && k <= kTopMost, "%s: k is %d: 1 to %d is wanted", entry, k, kTopMost);
+    TGBM_CHECK(temperature >= 1e-6f && temperature <= 1e6f, "%s: temperature is %g: 1e-6 to 1e6 is wanted", entry, temperature);
+    const size_t F = (size_t)std::max(n_features, 1), C = (size_t)std::max(n_classes, 1);
+    const tgbm_rows host_x{x, nullptr, (long long)F, TGBM_F32, row_size, n_features, 0}, host_w{weights, nullptr, (long long)F, TGBM_F32, n_classes, n_features, 0};
+    const tgbm_scores shape{x, 1, (long long)C, TGBM_F32, n_classes, row_size};  // (the address stands for the scores' own)
+    TGBM_CHECK(rows_ok(entry, "x", &host_x) && rows_ok(entry, "weights", &host_w) && scores_ok(entry, "scores", &shape), "%s: wrong arguments", entry);
+    if (row_size == 0) return;
+    hipStream_t s = stream_acquire();
+    const size_t width = (F + 127) / 128 * 128;
+    const auto alloc = [](size_t bytes) { return device_alloc(std::max<size_t>(bytes, 16)); };
+    const auto up = [&](const void *from, size_t bytes) {
+        void *to = alloc(bytes);
+        upload_large(s, to, from, bytes);
+        return to;
+    };
+    // the weights in 8 bits, once
+    tgbm_rows w = host_w;
+    void *d_weights = up(weights, sizeof(float) * C * F);
+    w.data = d_weights;
+    signed char *q = static_cast<signed char *>(alloc(C * width));
+    float *scale = static_cast<float *>(alloc(sizeof(float) * C)), *d_bias = bias != nullptr ? static_cast<float *>(up(bias, sizeof(float) * C)) : nullptr;
+    launch_rows_quantise(s, w, q, (long long)width, (int)width, scale);
+    const tgbm_rows w8{q, scale, (long long)width, TGBM_I8, n_classes, n_features, 1};
+    // rows by slices, whose scores take 256 MB
+    const size_t most = std::min<size_t>((size_t)row_size, std::max<size_t>(1, ((size_t)1 << 26) / C));
+    float *d_x = static_cast<float *>(alloc(sizeof(float) * most * F)), *d_scores = static_cast<float *>(alloc(sizeof(float) * most * C));
+    float *out = static_cast<float *>(alloc(sizeof(float) * most * (2 * (size_t)k + 1)));
+    size_t room = 0;
+    const auto slice = [&](size_t r) { return (int)std::min(most, (size_t)row_size - r); };
+    const auto rows_of = [&](int n) { return tgbm_rows{d_x, nullptr, (long long)F, TGBM_F32, n, n_features, 0}; };
+    for (const int n : {slice(0), slice((size_t)(row_size - 1) / most * most)}) room = std::max({room, scores_linear_workspace(rows_of(n), w8), scores_top_workspace(false, n_classes, n, k)});
+    void *workspace = alloc(room);
+    for (size_t r = 0; r < (size_t)row_size; r += most) {
+        const int n = slice(r);
+        upload_large(s, d_x, x + r * F, sizeof(float) * (size_t)n * F);
+        const tgbm_scores scores{d_scores, 1, (long long)C, TGBM_F32, n_classes, n};
+        launch_scores_linear(s, rows_of(n), w8, d_bias, scores, workspace);
+        int *d_classes = reinterpret_cast<int *>(out + (size_t)n * k);
+        float *d_lse = out + 2 * (size_t)n * k;
+        launch_scores_top(s, scores, tgbm_score_rules{}, k, temperature, out, d_classes, d_lse, workspace);
+        HIP_CHECK_LAUNCHES(entry);
+        HIP_CHECK(hipMemcpyAsync(values + r * k, out, sizeof(float) * (size_t)n * k, hipMemcpyDeviceToHost, s));
+        HIP_CHECK(hipMemcpyAsync(classes + r * k, d_classes, sizeof(int) * (size_t)n * k, hipMemcpyDeviceToHost, s));
+        HIP_CHECK(hipMemcpyAsync(lse + r, d_lse, sizeof(float) * (size_t)n, hipMemcpyDeviceToHost, s));
+        HIP_CHECK(hipStreamSynchronize(s));
+    }
+    for (void *p : {d_weights, (void *)q, (void *)scale, (void *)d_bias, (void *)d_x, (void *)d_scores, (void *)out, workspace}) device_free(p);
+    stream_release(s);
 }
 
 int tgbm_cut_points(int row_size, int n_features, const float *val, const int *row_ptr, const int *col_ptr,

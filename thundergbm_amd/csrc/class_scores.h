@@ -22,6 +22,8 @@ constexpr int kTeacherMost = 128;  // entries of a teacher's row
 // Whether the arguments of an entry point can be worked on; if not, why not is said on stderr (scores_api.hip).
 bool scores_ok(const char *entry, const char *what, const tgbm_scores *s);
 bool rules_ok(const char *entry, const tgbm_score_rules *rules, int rows);
+bool sampling_ok(const char *entry, const tgbm_sampling *how);
+bool rows_ok(const char *entry, const char *what, const tgbm_rows *rows);  // of floating rows
 
 inline bool rows_side_by_side(const tgbm_scores &s) { return !(s.class_stride == 1 && (s.rows == 1 || s.row_stride != 1)); }
 

@@ -120,6 +120,8 @@ tgbm_rows with_pitch(tgbm_rows r) {
 namespace tgbm {
 bool scores_ok(const char *entry, const char *what, const tgbm_scores *s) { return check_scores(entry, what, s) == 0; }
 bool rules_ok(const char *entry, const tgbm_score_rules *rules, int rows) { return check_rules(entry, rules, rows) == 0; }
+bool sampling_ok(const char *entry, const tgbm_sampling *how) { return check_sampling(entry, how) == 0; }
+bool rows_ok(const char *entry, const char *what, const tgbm_rows *rows) { return check_rows(entry, what, rows, false, true) == 0; }
 }  // namespace tgbm
 
 extern "C" int tgbm_scores_adjust(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_scores *out, void *stream) {

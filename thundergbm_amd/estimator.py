@@ -9,7 +9,7 @@ import scipy.sparse as sp
 from sklearn.base import BaseEstimator, ClassifierMixin, RegressorMixin
 
 from . import _lib
-from .scores import _Rules, _list_length
+from .scores import _FINE, _Rules, _Sampling, _list_length, _one_setting
 from .session import Session, teacher_arrays
 
 _PARAMS = ("depth", "n_trees", "n_gpus", "min_child_weight", "lambda_tgbm", "gamma", "max_num_bin", "verbose",
@@ -77,6 +77,31 @@ class Teacher:
 
     def __init__(self, labels, scores, lse=None, temperature=1.0, weight=1.0):
         self.labels, self.scores, self.lse, self.temperature, self.weight = labels, scores, lse, temperature, weight
+
+    @classmethod
+    def linear(cls, x, weights, labels, bias=None, k=20, temperature=1.0, weight=1.0):
+        """A linear layer as the teacher: for every row of x [rows, features] the k best of the classes whose weights are [classes, features] and whose labels are
+        `labels` [classes], by x @ weights.T + bias in 8 bits (scores.quantise, scores.linear), with the log-sum-exp over all of them at the temperature."""
+        x, weights = np.ascontiguousarray(x, dtype=np.float32), np.ascontiguousarray(weights, dtype=np.float32)
+        labels = np.asarray(labels, dtype=np.float32)
+        if x.ndim != 2 or weights.ndim != 2 or x.shape[1] != weights.shape[1] or not 1 <= x.shape[1] <= 65536:
+            raise ValueError("x: [rows, features] and weights: [classes, features] with 1 to 65536 features are wanted, got %s and %s" % (x.shape, weights.shape))
+        (n, features), classes = x.shape, len(weights)
+        if not 1 <= classes <= 1 << 22 or labels.shape != (classes,):
+            raise ValueError("labels: one for each of %d classes is wanted, got the shape %s" % (classes, labels.shape))
+        if bias is not None:
+            bias = np.ascontiguousarray(bias, dtype=np.float32)
+            if bias.shape != (classes,):
+                raise ValueError("bias: a number for each of %d classes is wanted, got the shape %s" % (classes, bias.shape))
+        for name, a in (("x", x), ("weights", weights), ("bias", bias)):
+            if a is not None and not np.isfinite(a).all():
+                raise ValueError("%s: a number is NaN or infinite" % name)
+        k = min(_list_length(k), classes)
+        if not 1e-3 <= temperature <= 1e3:
+            raise ValueError("temperature is %r: 1e-3 to 1e3 is wanted" % (temperature,))
+        values, at, lse = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+        _lib.load().tgbm_linear_top(n, features, _ptr(x), classes, _ptr(weights), None if bias is None else _ptr(bias), k, temperature, _ptr(values), _ptr(at), _ptr(lse))
+        return cls(np.where(at >= 0, labels[np.maximum(at, 0)], np.float32(np.nan)), values, lse, temperature, weight)
 
     def class_numbers(self, known):
         """The entries' places among the ascending labels `known`, -1 for those that are none."""
@@ -266,6 +291,35 @@ class TGBMModel(BaseEstimator):
         labels = np.where(classes >= 0, known[np.maximum(classes, 0)], np.float32(np.nan))
         lse = np.where(np.isneginf(lse), np.float32(0), lse)  # (nothing is allowed: no probability anywhere)
         return labels, np.exp(values / np.float32(temperature) - lse[:, None])
+
+    def sample_classes(self, X, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed=None, shown=None, repetition=1.0, frequency=0.0, presence=0.0):
+        """A label of every row, drawn by the random numbers u [rows] from the softmax of `class_scores` over the temperature, cut as scores.sample says (k, p, min_p and
+        temperature: numbers, or arrays with one for each row), and its probability among what was kept. Where nothing is allowed the label is NaN and
+        the probability 0."""
+        X = _csr(X)
+        n = X.shape[0]
+        r, keep = self._class_rules(n, bias, allowed, shown, repetition, frequency, presence)
+        h = _Sampling()
+        for name, v in (("temperature", temperature), ("p", p), ("min_p", min_p), ("k", k)):
+            if np.ndim(v) == 0:
+                setattr(h, name + "_all", _one_setting(name, v, *_FINE[name]))
+                continue
+            v = np.ascontiguousarray(v, dtype=np.int32 if name == "k" else np.float32)
+            if v.shape != (n,):
+                raise ValueError("%s: a number for each of %d rows is wanted, got the shape %s" % (name, n, v.shape))
+            setattr(h, name, v.ctypes.data if n else None)
+            setattr(h, name + "_all", 0 if name in ("k", "min_p") else 1)
+            keep.append(v)
+        h.k_all = min(h.k_all, self.tree_per_iter)
+        u = np.ascontiguousarray(u, dtype=np.float32)
+        if u.shape != (n,):
+            raise ValueError("u: a number for each of %d rows is wanted, got the shape %s" % (n, u.shape))
+        indptr, indices = np.ascontiguousarray(X.indptr, dtype=np.int32), np.ascontiguousarray(X.indices, dtype=np.int32)
+        classes, logp = np.empty(n, np.int32), np.empty(n, np.float32)
+        _lib.load().tgbm_predict_sample(n, _ptr(X.data), _ptr(indptr), _ptr(indices), self.model, self.n_trees, self.tree_per_iter,
+                                        self.learning_rate, C.byref(r), C.byref(h), _ptr(u), _ptr(classes), _ptr(logp))
+        known = np.asarray(self.group_label, dtype=np.float32)
+        return np.where(classes >= 0, known[np.maximum(classes, 0)], np.float32(np.nan)), np.exp(logp)
 
     def predict(self, X, groups=None):
         if not self.model:

@@ -336,17 +336,26 @@ def distill(scores, classes, teacher, labels=None, teacher_lse=None, temperature
     return loss, pairs
 
 
-def _setting(torch, name, v, scores, dtype, fine, wanted):
-    """A setting of `sample`: (address of the rows' own, 0) or (None, everybody's)."""
-    if isinstance(v, torch.Tensor):
-        return _plain(torch, name, v, scores, dtype, (scores.shape[1],)), 0
+# what a setting of `sample` may be, for all rows alike
+_FINE = {"temperature": (lambda v: v == 0 or 1e-6 <= v <= 1e6, "0 or 1e-6 to 1e6"), "p": (lambda v: 1e-37 <= v <= 1, "above 0 and up to 1"),
+         "min_p": (lambda v: 0 <= v <= 1, "0 to 1"), "k": (lambda v: v >= 0, "0 or more")}
+
+
+def _one_setting(name, v, fine, wanted):
     try:
-        number = operator.index(v) if dtype is torch.int32 else float(v)
+        number = operator.index(v) if name == "k" else float(v)
     except (TypeError, ValueError):
         number = None
     if number is None or not fine(number):
         raise ValueError("%s is %r: %s is wanted" % (name, v, wanted))
-    return None, number
+    return number
+
+
+def _setting(torch, name, v, scores, dtype, fine, wanted):
+    """A setting of `sample`: (address of the rows' own, 0) or (None, everybody's)."""
+    if isinstance(v, torch.Tensor):
+        return _plain(torch, name, v, scores, dtype, (scores.shape[1],)), 0
+    return None, _one_setting(name, v, fine, wanted)
 
 
 def sample(scores, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed=None, allowed_set=None, shown=None, shown_begin=None,
@@ -371,11 +380,11 @@ def sample(scores, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed
     n = s.rows
     at = _plain(torch, "u", u, scores, torch.float32, (n,))
     h = _Sampling()
-    h.temperature, h.temperature_all = _setting(torch, "temperature", temperature, scores, torch.float32, lambda v: v == 0 or 1e-6 <= v <= 1e6, "0 or 1e-6 to 1e6")
-    h.p, h.p_all = _setting(torch, "p", p, scores, torch.float32, lambda v: 1e-37 <= v <= 1, "1e-37 to 1")
-    h.min_p, h.min_p_all = _setting(torch, "min_p", min_p, scores, torch.float32, lambda v: 0 <= v <= 1, "0 to 1")
-    h.k, h.k_all = _setting(torch, "k", k, scores, torch.int32, lambda v: v >= 0, "0 or more")
-    h.k_all = min(h.k_all, s.classes) if h.k is None else 0
+    h.temperature, h.temperature_all = _setting(torch, "temperature", temperature, scores, torch.float32, *_FINE["temperature"])
+    h.p, h.p_all = _setting(torch, "p", p, scores, torch.float32, *_FINE["p"])
+    h.min_p, h.min_p_all = _setting(torch, "min_p", min_p, scores, torch.float32, *_FINE["min_p"])
+    h.k, k = _setting(torch, "k", k, scores, torch.int32, *_FINE["k"])
+    h.k_all = min(k, s.classes)
     classes = torch.empty(n, dtype=torch.int32, device=scores.device)
     logp = torch.empty(n, dtype=torch.float32, device=scores.device)
     if n:
