@@ -308,14 +308,17 @@ constexpr int parts_of() { return G == 64 ? 8 : 32; }
 template <int G>
 constexpr int listed_of() { return G == 64 ? 64 : 256; }
 template <int G>
+constexpr int chosen_of() { return G == 64 ? 1 : G == 256 ? 512 : 2048; }
+template <int G>
 struct alignas(16) DrawShared {
+    unsigned long long chosen[chosen_of<G>()];
     unsigned long long mass[Scale<parts_of<G>()>::kBuckets + 1];  // (the last one takes what does not count)
     unsigned long long key[listed_of<G>()], weight[listed_of<G>()], front[listed_of<G>()];
     double part[G / 64];
     float part_f[G / 64];
     int part_i[G / 64];
     unsigned long long best, least, most;
-    int listed;
+    int listed, count;
 };
 template <int G>
 __device__ __forceinline__ void group_sync() {
@@ -351,10 +354,52 @@ struct Draw {
         const double x = best - place / by;
         return __double2float_ru(x + 0x1p-49 * (fabs(x) + fabs(best)));
     }
+    int chosen = -1;  // how many there are, once all that is kept lies in the list of them
+
+    // Lists all that is kept and whose score is `bound` or more, if there is room for them. A row of 128003 classes is gone over six times where a count and a mass cut it,
+    // two or three times with the list.
+    __device__ __forceinline__ void choose(float bound) {
+        if (G == 64 || chosen >= 0) return;
+        bound = fmaxf(bound, least);
+        group_sync<G>();
+        if (in_group<G>() == 0) sh.count = 0;
+        group_sync<G>();
+        row.each([&](const float (&x)[V], int c) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < V; ++j) any |= x[j] >= bound;
+            if (!__any(any)) return;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const unsigned long long who = __ballot(x[j] >= bound);
+                if (who == 0) continue;
+                const int first = __ffsll((long long)who) - 1;
+                int to = 0;
+                if (lane_id() == first) to = atomicAdd(&sh.count, __popcll(who));
+                to = read_lane(to, first) + lanes_below(who);
+                if (x[j] >= bound && to < chosen_of<G>()) sh.chosen[to] = key_of(x[j], c + j);
+            }
+        });
+        group_sync<G>();
+        const int n = sh.count;
+        chosen = n <= chosen_of<G>() ? n : -1;
+        least = chosen >= 0 ? bound : least;
+    }
     // f(place, bucket, key) for those that are kept and whose score is from lo to hi
     template <typename F>
     __device__ __forceinline__ void kept(float lo, float hi, F f) {
         lo = fmaxf(lo, least);
+        if (G > 64 && chosen >= 0) {
+            for (int i = in_group<G>(); i < chosen; i += G) {
+                const unsigned long long key = sh.chosen[i];
+                const float x = from_ordered((unsigned)(key >> 32));
+                if (x >= lo && x <= hi && key >= cut) {
+                    const double s = place_of(x);
+                    if (s <= last_place) f(s, bucket_of(s), key);
+                }
+            }
+            return;
+        }
         row.each([&](const float (&x)[V], int c) {
             bool any = false;
 #pragma unroll
@@ -543,6 +588,7 @@ struct Draw {
             if (all >= (double)k) {
                 find(mass, before, (double)(k - 1), false, &bucket, &front);
                 bound = fmaxf(bound, score_below(bucket + 0.5));
+                choose(bound);
             }
         }
         clear();
@@ -606,6 +652,18 @@ __device__ __forceinline__ int block_sum(int v, int *part) {
     if (lane_id() == 0) part[wave_id()] = v;
     group_sync<G>();
     v = 0;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) v += part[w];
+    return v;
+}
+
+template <int G>
+__device__ __forceinline__ float block_sum_f(float v, float *part) {
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+    group_sync<G>();
+    if (lane_id() == 0) part[wave_id()] = v;
+    group_sync<G>();
+    v = 0.f;
 #pragma unroll
     for (int w = 0; w < G / 64; ++w) v += part[w];
     return v;
@@ -683,6 +741,7 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
         d.last_place = fmin(d.last_place, -log2((double)r.min_p) * P);
         d.least = fmaxf(d.least, d.score_below(d.last_place));
         all_kept = false;
+        d.choose(d.least);
     }
     if (r.k < classes) {
         d.keep_best(r.k, mine);
@@ -701,6 +760,18 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
         const double most = fmax((double)r.p, 0.0) * all;
         d.find(mass, before, most, true, &bucket, &front);
         const double its = unit(bucket);
+        // The draw is among those up to here. A bucket's weights are nearly the same: its whole numbers say how many they are.
+        float count = 0.f;
+        if (G > 64 && d.chosen < 0) {
+#pragma unroll
+            for (int i = 0; i < Draw<G, Row>::kEach; ++i) {
+                const int b = in_group<G>() * Draw<G, Row>::kEach + i;
+                if (b <= bucket) count += (float)sh.mass[b];
+            }
+            count = block_sum_f<G>(count, sh.part_f) * (float)one;
+            // (more of them cost as much to list as they save: 2048 x 65537, 2300 of a row kept: 249 us, 279 with the list)
+            if (count < fminf(0.95f * chosen_of<G>(), (float)classes / 128.f)) d.choose(d.score_below(bucket + 0.5));
+        }
         const auto last = d.resolve(bucket, (most - front) / its, true, weight);
         kept = front + (last.before + last.weight) * its;
     }
