@@ -335,7 +335,7 @@ struct Draw {
     static constexpr int V = Row::V, P = parts_of<G>(), kBuckets = Scale<P>::kBuckets, kEach = kBuckets / G, kListed = listed_of<G>();
     DrawShared<G> &sh;
     Row &row;
-    double best, by;  // (the place of a score is (best - score) * by)
+    double best, by, step;  // (the place of a score is (best - score) * by; step: 1 / by)
     double magic;
     float least = -FLT_MAX;      // the least score that is kept
     unsigned long long cut = 0;  // the last one of the order that is kept, as a key
@@ -347,11 +347,11 @@ struct Draw {
     __device__ __forceinline__ unsigned long long weight_of(double place) const { return part_of_two<P>(place - ((place + kToWhole) - kToWhole), magic); }
     // A score below which none has a place up to `place`; the other way: above which none has one from there on.
     __device__ __forceinline__ float score_below(double place) const {
-        const double x = best - place / by;
+        const double x = best - place * step;
         return __double2float_rd(x - 0x1p-49 * (fabs(x) + fabs(best)));
     }
     __device__ __forceinline__ float score_above(double place) const {
-        const double x = best - place / by;
+        const double x = best - place * step;
         return __double2float_ru(x + 0x1p-49 * (fabs(x) + fabs(best)));
     }
     int chosen = -1;  // how many there are, once all that is kept lies in the list of them
@@ -735,6 +735,7 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
     d.best = (double)m;
     constexpr int P = parts_of<G>();
     d.by = Scale<P>::kOfE / (double)r.temperature;
+    d.step = (double)r.temperature * (1.0 / Scale<P>::kOfE);
     d.magic = __longlong_as_double((long long)(1023 + 52 - bits) << 52);
     bool all_kept = true;
     if (r.min_p > 0.f) {
@@ -751,7 +752,16 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
     double mass[Draw<G, Row>::kEach], all;
     d.add_up(all_kept);
     const double one = __longlong_as_double((long long)(1023 - bits) << 52);
-    const auto unit = [&](int b) { return exp2(-(double)b / P) * one; };
+    // 2^(-b / P): what a bucket's whole numbers count, beside `one`
+    const auto unit = [&](int b) {
+        constexpr double kPart[8] = {1.0, 0.91700404320467123174, 0.84089641525371454303, 0.77110541270397041180, 0.70710678118654752440, 0.64841977732550483296, 0.59460355750136053336,
+                                     0.54525386633262882960};
+        if constexpr (P == 32) return exp2(-(double)b / P) * one;
+        double part = kPart[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) part = b % 8 == i ? kPart[i] : part;
+        return part * __longlong_as_double((long long)(1023 - b / 8) << 52) * one;
+    };
     constexpr double kNext = P == 32 ? 0.97857206208770013451 : 0.91700404320467123174;  // 2^(-1 / P)
     const double before = d.sums(unit(in_group<G>() * Draw<G, Row>::kEach), kNext, mass, &all);
     double kept = all, front;
