@@ -140,7 +140,8 @@ def _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repeti
 
 def _rows(torch, name, x, scale=None, whole=False, floating=True):
     """Rows of numbers, [rows, features]; int8 ones with their scales."""
-    _on_gpu(torch, name, x)
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.requires_grad:
+        _on_gpu(torch, name, x)
     kind = _types.get(x.dtype) if floating else None
     if kind is None and whole and x.dtype == torch.int8:
         kind = 3
@@ -157,11 +158,11 @@ def _rows(torch, name, x, scale=None, whole=False, floating=True):
         if scale is None:
             raise ValueError("%s: whole numbers go with a scale for each row" % name)
         r.scale = _plain(torch, name + "_scale", scale, x, torch.float32, (rows,))
-        # (whether the memory goes on behind the last row as it does behind the others)
-        left = x.untyped_storage().nbytes() - x.storage_offset()
-        if rows == 1 and left >= (features + 15) // 16 * 16:
-            r.pitch = (features + 15) // 16 * 16
-        r.padded = 1 if left >= rows * r.pitch else 0
+        if features % 16:  # (whether the memory goes on behind the last row as it does behind the others)
+            left = x.untyped_storage().nbytes() - x.storage_offset()
+            if rows == 1 and left >= (features + 15) // 16 * 16:
+                r.pitch = (features + 15) // 16 * 16
+            r.padded = 1 if left >= rows * r.pitch else 0
     elif scale is not None:
         raise ValueError("%s_scale goes with whole numbers, %s is %s" % (name, name, x.dtype))
     return r
@@ -205,6 +206,22 @@ def _stream(torch, device):
 @functools.lru_cache(maxsize=256)
 def _top_workspace(by_class, by_row, classes, rows, k):
     return _lib.load().tgbm_scores_top_workspace(C.byref(_Scores(1, by_class, by_row, 0, classes, rows)), k)
+
+
+@functools.lru_cache(maxsize=256)
+def _sample_workspace(kind, by_class, by_row, classes, rows, shown, k):
+    """shown: whether there are lists; k: the rows' common one, None where each has its own."""
+    r, h = _Rules(repetition=1.0), _Sampling(None, None, None, 1 if k is None else None, 1.0, 1.0, 0.0, k or 0)  # (addresses stand for any)
+    if shown:
+        r.shown, r.shown_begin = 1, 1
+    return _lib.load().tgbm_scores_sample_workspace(C.byref(_Scores(1, by_class, by_row, kind, classes, rows)), C.byref(r), C.byref(h))
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_workspace(features, *rows):
+    """rows: of x and of the weights, the place in 16 bytes, pitch, type, rows, padded."""
+    x, w = (_Rows(16 + at, 16, pitch, kind, n, features, padded) for at, pitch, kind, n, padded in (rows[:5], rows[5:]))
+    return _lib.load().tgbm_scores_linear_workspace(C.byref(x), C.byref(w))
 
 
 @functools.lru_cache(maxsize=256)
@@ -353,6 +370,8 @@ def _one_setting(name, v, fine, wanted):
 
 def _setting(torch, name, v, scores, dtype, fine, wanted):
     """A setting of `sample`: (address of the rows' own, 0) or (None, everybody's)."""
+    if (type(v) is int or (type(v) is float and name != "k")) and fine(v):
+        return None, v
     if isinstance(v, torch.Tensor):
         return _plain(torch, name, v, scores, dtype, (scores.shape[1],)), 0
     return None, _one_setting(name, v, fine, wanted)
@@ -384,11 +403,11 @@ def sample(scores, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed
     h.p, h.p_all = _setting(torch, "p", p, scores, torch.float32, *_FINE["p"])
     h.min_p, h.min_p_all = _setting(torch, "min_p", min_p, scores, torch.float32, *_FINE["min_p"])
     h.k, k = _setting(torch, "k", k, scores, torch.int32, *_FINE["k"])
-    h.k_all = min(k, s.classes)
+    h.k_all = k = min(k, s.classes)
     classes = torch.empty(n, dtype=torch.int32, device=scores.device)
     logp = torch.empty(n, dtype=torch.float32, device=scores.device)
     if n:
-        size = _lib.load().tgbm_scores_sample_workspace(C.byref(s), C.byref(r), C.byref(h))
+        size = _sample_workspace(s.type, s.class_stride, s.row_stride, s.classes, n, r.shown is not None, k if h.k is None else None)
         room = torch.empty(size, dtype=torch.uint8, device=scores.device) if size else None
         _call(torch, scores, "tgbm_scores_sample", C.byref(s), C.byref(r), C.byref(h), at, classes.data_ptr(), logp.data_ptr(),
               room.data_ptr() if size else None, size)
@@ -409,7 +428,7 @@ def quantise(x):
     scale = torch.empty(r.rows, dtype=torch.float32, device=x.device)
     if r.rows:
         _call(torch, x, "tgbm_rows_quantise", C.byref(r), q.data_ptr(), width, width, scale.data_ptr())
-    return q[:, :r.features], scale
+    return (q if r.features == width else q[:, :r.features]), scale
 
 
 def linear(x, weight, weight_scale, bias=None, x_scale=None, order="row", dtype=None):
@@ -446,7 +465,7 @@ def linear(x, weight, weight_scale, bias=None, x_scale=None, order="row", dtype=
         out = torch.empty((classes, n), dtype=dtype, device=x.device)
         o = _Scores(out.data_ptr(), max(n, 1), 1, kind, classes, n)
     if n:
-        size = _lib.load().tgbm_scores_linear_workspace(C.byref(r), C.byref(w))
+        size = _linear_workspace(r.features, r.data % 16, r.pitch, r.type, n, r.padded, w.data % 16, w.pitch, w.type, classes, w.padded)
         room = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         _call(torch, x, "tgbm_scores_linear", C.byref(r), C.byref(w), b, C.byref(o), room.data_ptr() if size else None, size)
     return out
