@@ -316,7 +316,7 @@ typedef struct tgbm_rows {
 
 /* scale = the row's largest magnitude / 127, q = the nearest whole number (of two the even one) to number / scale, both operations in 32 bits; 0 where the
  * scale is 0. A row that has an infinity or a NaN gets the scale NaN and zeros. q: [rows][q_pitch] bytes, of which a row's first q_width are written, zeros behind its features;
- * features <= q_width <= q_pitch. */
+ * features <= q_width <= q_pitch. q shares no memory with x. */
 int tgbm_rows_quantise(const tgbm_rows *x, signed char *q, long long q_pitch, int q_width, float *scale, void *stream);
 
 /* Class scores as a product: out's score of class c in row i is (sum of x[i] * weights[c] over the features) * x's scale[i] * weights' scale[c] + bias[c], the

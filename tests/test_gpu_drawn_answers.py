@@ -37,7 +37,7 @@ def test_drawn_answers(model):
         rules = dict(bias=bias, allowed=allowed[:rows], shown=shown[:rows], repetition=1.5, frequency=0.25, presence=0.5)
         x = O.adjusted(raw[:, :rows], bias, D.bits_of(allowed[:rows]), None, numbers if len(numbers) else None, begin if len(numbers) else None, 1.5, 0.25, 0.5)
         each = dict(temperature=rng.choice([0.0, 0.5, 1.0], rows).astype(np.float32), k=rng.integers(0, 4, rows).astype(np.int32), p=rng.choice([1.0, 0.7], rows).astype(np.float32))
-        for how in (dict(), dict(k=2, temperature=0.7), dict(p=0.8), dict(min_p=0.3), dict(temperature=0), each):
+        for how in (dict(), dict(k=2, temperature=0.7), dict(k=1 << 40), dict(p=0.8), dict(min_p=0.3), dict(temperature=0), each):
             labels, prob = clf.sample_classes(X[:rows], u[:rows], **rules, **how)
             classes, logp = R.sample(x, u[:rows], **how)
             np.testing.assert_array_equal(labels, np.where(classes >= 0, known[np.maximum(classes, 0)], np.nan))

@@ -148,6 +148,48 @@ def test_nothing_else_is_written_and_repeats_are_equal():
             assert torch.equal(S.linear(x, w, w_scale, bias=bias, order="class"), eager)
 
 
+def test_many_rows():
+    """More rows than a launch or a part of the workspace takes."""
+    gen = torch.Generator("cuda").manual_seed(1)
+    for n, F, C in ((1_300_000, 40, 3), (70_000, 9000, 5)):
+        x = torch.randn(n, F, device="cuda", generator=gen, dtype=torch.float32).bfloat16()
+        w, w_scale = S.quantise(torch.randn(C, F, device="cuda", generator=gen))
+        q, scale = S.quantise(x)
+        at = torch.tensor([0, 1, n // 2, (1 << 20) - 1, 1 << 20, 59_578, 59_579, n - 1], device="cuda").clamp(max=n - 1)
+        want_q, want_scale = R.quantise(x[at].float().cpu().numpy())
+        np.testing.assert_array_equal(q[at].cpu().numpy(), want_q)
+        np.testing.assert_array_equal(scale[at].cpu().numpy(), want_scale)
+        for order in ("row", "class"):
+            z = S.linear(x, w, w_scale, order=order)
+            check(z[:, at], torch.from_numpy(want_q), torch.from_numpy(want_scale), w.cpu(), w_scale.cpu(), None, torch.float32)
+            assert torch.equal(z, S.linear(q, w, w_scale, x_scale=scale, order=order))
+
+
+def test_two_streams_at_once():
+    """Calls that run side by side have workspaces of their own."""
+    gen = torch.Generator("cuda").manual_seed(2)
+    x = [torch.randn(700, 300, device="cuda", generator=gen) for _ in range(2)]
+    w, w_scale = S.quantise(torch.randn(900, 300, device="cuda", generator=gen))
+    u = torch.rand(700, device="cuda", generator=gen)
+
+    def chain(v):
+        z = S.linear(v, w, w_scale)
+        return (z, *S.sample(z, u, p=0.9), *S.sample(z, u, k=20))
+
+    want = [chain(v) for v in x]
+    streams = [torch.cuda.Stream() for _ in x]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(chain(x[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
 def test_no_rows():
     w, w_scale = S.quantise(torch.randn(9, 40, device="cuda"))
     assert S.linear(torch.zeros(0, 40, device="cuda"), w, w_scale).shape == (9, 0)

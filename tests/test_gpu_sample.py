@@ -146,6 +146,22 @@ def test_many_rows():
         check(S.sample(x, u, **how), R.sample(x[:, at].cpu().numpy(), u[at].cpu().numpy(), **how), rows)
 
 
+def test_far_apart_rows_and_long_lists():
+    """Rows whose places pass 32 bits, long lists of shown classes, one class many times."""
+    rng = np.random.default_rng(9)
+    C, n, pitch = 9000, 3, 1_500_000_000
+    memory = torch.empty(2 * pitch + C, dtype=torch.bfloat16, device="cuda")
+    x = memory.as_strided((n, C), (pitch, 1))
+    z = rounded(rng.standard_normal((C, n)).astype(np.float32) * 2, torch.bfloat16)
+    x.copy_(torch.from_numpy(z).t())
+    u = numbers(rng, n)
+    lists = [rng.integers(0, C, 20_000), np.full(70_000, 7), rng.integers(0, C, 3)]
+    r = dict(shown=np.concatenate(lists).astype(np.int32), shown_begin=np.cumsum([0] + [len(l) for l in lists]).astype(np.int64), repetition=1.1, frequency=1e-3, presence=0.2)
+    for how in (dict(p=0.9), dict(k=500), dict(k=40, p=0.8)):
+        check(S.sample(x.t(), torch.from_numpy(u).cuda(), **on_gpu(r), **how), R.sample(O.adjusted(z, **r), u, **how))
+        check(S.sample(x.t(), torch.from_numpy(u).cuda(), **how), R.sample(z, u, **how))
+
+
 def test_streams_graphs_and_repeats():
     rng = np.random.default_rng(8)
     for C, n, how in ((8, 500, dict()), (700, 200, dict(k=30, p=0.9)), (700, 200, dict(p=0.9)), (20_000, 9, dict(k=300))):

@@ -320,10 +320,11 @@ struct ScoreOut {
 
 // Few rows: the rows' features in LDS, `slice` of them at a time, and 16 * A classes to a wavefront, whose weights go from memory to the product; S wavefronts share
 // the features. T: of the rows, which are quantised on the way into LDS if they are floating ones (all of their features at once then).
+constexpr int few_block(int shares) { return shares > 4 ? 64 * shares : kLinearBlock; }
 template <typename T, int A, int R, int S>
-__global__ __launch_bounds__(kLinearBlock) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
+__global__ __launch_bounds__(few_block(S)) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
     constexpr bool kQuantise = sizeof(T) > 1;
-    constexpr int kTiles = kLinearBlock / 64 / S;
+    constexpr int kBlock = few_block(S), kTiles = kBlock / 64 / S;
     __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * A * R : 1][64];
     __shared__ float scale_of_row[16 * R];
     __shared__ unsigned most_of_row[kQuantise ? 16 * R : 1];
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(kLinearBlock) void k_linear_few(const T *x, const f
             const int parts = chunks * kChunk / V;
             const auto each = [&](auto f) {
 #pragma unroll 2
-                for (int i = threadIdx.x; i < live * parts; i += kLinearBlock) {
+                for (int i = threadIdx.x; i < live * parts; i += kBlock) {
                     const int r = i / parts, at = (i - r * parts) * V;
                     const T *row = x + (size_t)r * x_pitch;
                     Vec v = (T)0.f;
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(kLinearBlock) void k_linear_few(const T *x, const f
             if ((int)threadIdx.x < live) scale_of_row[threadIdx.x] = scale_of(most_of_row[threadIdx.x]);
         } else {
             const int parts = (last * kChunk - f0) / 16;
-            for (int i = threadIdx.x; i < live * parts; i += kLinearBlock) {
+            for (int i = threadIdx.x; i < live * parts; i += kBlock) {
                 const int r = i / parts, at = (i - r * parts) * 16;
                 *reinterpret_cast<Int4 *>(of_x + r * pitch + at) = *reinterpret_cast<const Int4 *>(x + (size_t)r * x_pitch + f0 + at);
             }
@@ -490,18 +491,22 @@ bool quantised_on_the_way(const tgbm_rows &x) { return x.type != TGBM_I8 && x.ro
 
 template <typename T, int A, int R, int S>
 void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
-    constexpr int kOf = kLinearBlock / 64 / S * 16 * A;
+    constexpr int kOf = few_block(S) / 64 / S * 16 * A;
     const int live = std::min(rows, 16 * R), slice = std::min((int)pad_of(features), (kFewLds / live - 16) / kChunk * kChunk);
     static LdsOptIn opt_in;
     opt_in({reinterpret_cast<const void *>(&k_linear_few<T, A, R, S>)});
-    k_linear_few<T, A, R, S><<<dim3((w.rows - 1) / kOf + 1, (rows - 1) / (16 * R) + 1), kLinearBlock, live * (slice + 16), s>>>(x, scale, pitch, rows, w, features, bias, out, slice);
+    k_linear_few<T, A, R, S><<<dim3((w.rows - 1) / kOf + 1, (rows - 1) / (16 * R) + 1), few_block(S), live * (slice + 16), s>>>(x, scale, pitch, rows, w, features, bias, out, slice);
 }
 template <typename T, int A, int R>
 void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
     const long waves = (long)((w.rows - 1) / (16 * A) + 1) * ((rows - 1) / (16 * R) + 1);
-    if (waves >= (A * R > 1 ? 1024 : 4096) || features <= 2 * kChunk) linear_few<T, A, R, 1>(s, x, scale, pitch, rows, w, features, bias, out);
-    else if (waves >= (A * R > 1 ? 512 : 1024) || features <= 4 * kChunk) linear_few<T, A, R, 2>(s, x, scale, pitch, rows, w, features, bias, out);
-    else linear_few<T, A, R, 4>(s, x, scale, pitch, rows, w, features, bias, out);
+    // More wavefronts share the features where there are few of them (1 x 4096 x 32000, 2000 wavefronts of 16 classes: 26 us, 30 where four share; 8 x 65536 x 100: 62 us
+    // with four, 45 with sixteen).
+    constexpr long kFull = A * R > 1 ? 1024 : 4096;
+    if (waves >= kFull || features <= 2 * kChunk) linear_few<T, A, R, 1>(s, x, scale, pitch, rows, w, features, bias, out);
+    else if (waves >= std::min(kFull / 2, 1024l) || features <= 4 * kChunk) linear_few<T, A, R, 2>(s, x, scale, pitch, rows, w, features, bias, out);
+    else if (waves >= 128 || features <= 16 * kChunk) linear_few<T, A, R, 4>(s, x, scale, pitch, rows, w, features, bias, out);
+    else linear_few<T, A, R, 16>(s, x, scale, pitch, rows, w, features, bias, out);
 }
 
 template <typename O>
@@ -528,7 +533,7 @@ void linear(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const f
         const long tiles = (long)((w.rows - 1) / 128 + 1) * ((part.rows - 1) / 128 + 1);
         if (part.rows <= 16) linear_few<signed char, 1, 1>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
         else if (part.rows <= 32) linear_few<signed char, 2, 2>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
-        else if (tiles < 64) linear_few<signed char, 1, 4>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
+        else if (tiles < 32) linear_few<signed char, 1, 4>(s, part.data, part.scale, part.pitch, part.rows, w, features, bias, out);
         else if (out.type == TGBM_F32) linear_tiles<float>(s, part, w, features, bias, out, tiles);
         else if (out.type == TGBM_F16) linear_tiles<_Float16>(s, part, w, features, bias, out, tiles);
         else linear_tiles<__bf16>(s, part, w, features, bias, out, tiles);
@@ -556,10 +561,19 @@ void quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pit
 }
 }  // namespace
 
+// (a launch has fewer than 2^32 threads in a direction: very many rows go by slices)
 void launch_rows_quantise(hipStream_t s, const tgbm_rows &x, signed char *q, long long q_pitch, int pad, float *scale) {
-    if (x.type == TGBM_F32) quantise<float>(s, x, q, q_pitch, pad, scale);
-    else if (x.type == TGBM_F16) quantise<_Float16>(s, x, q, q_pitch, pad, scale);
-    else quantise<__bf16>(s, x, q, q_pitch, pad, scale);
+    constexpr int kMost = 1 << 20;
+    const size_t size = x.type == TGBM_F32 ? 4 : 2;
+    for (int row = 0; row < x.rows; row += std::min(kMost, x.rows - row)) {
+        tgbm_rows part = x;
+        part.data = static_cast<const char *>(x.data) + size * (size_t)row * x.pitch;
+        part.rows = std::min(kMost, x.rows - row);
+        signed char *to = q + (size_t)row * q_pitch;
+        if (x.type == TGBM_F32) quantise<float>(s, part, to, q_pitch, pad, scale + row);
+        else if (x.type == TGBM_F16) quantise<_Float16>(s, part, to, q_pitch, pad, scale + row);
+        else quantise<__bf16>(s, part, to, q_pitch, pad, scale + row);
+    }
 }
 
 size_t scores_linear_workspace(const tgbm_rows &x, const tgbm_rows &w) {

@@ -302,7 +302,8 @@ class TGBMModel(BaseEstimator):
         h = _Sampling()
         for name, v in (("temperature", temperature), ("p", p), ("min_p", min_p), ("k", k)):
             if np.ndim(v) == 0:
-                setattr(h, name + "_all", _one_setting(name, v, *_FINE[name]))
+                v = _one_setting(name, v, *_FINE[name])
+                setattr(h, name + "_all", min(v, self.tree_per_iter) if name == "k" else v)
                 continue
             v = np.ascontiguousarray(v, dtype=np.int32 if name == "k" else np.float32)
             if v.shape != (n,):
@@ -310,7 +311,6 @@ class TGBMModel(BaseEstimator):
             setattr(h, name, v.ctypes.data if n else None)
             setattr(h, name + "_all", 0 if name in ("k", "min_p") else 1)
             keep.append(v)
-        h.k_all = min(h.k_all, self.tree_per_iter)
         u = np.ascontiguousarray(u, dtype=np.float32)
         if u.shape != (n,):
             raise ValueError("u: a number for each of %d rows is wanted, got the shape %s" % (n, u.shape))

@@ -428,7 +428,7 @@ def quantise(x):
     scale = torch.empty(r.rows, dtype=torch.float32, device=x.device)
     if r.rows:
         _call(torch, x, "tgbm_rows_quantise", C.byref(r), q.data_ptr(), width, width, scale.data_ptr())
-    return (q if r.features == width else q[:, :r.features]), scale
+    return q[:, :r.features], scale
 
 
 def linear(x, weight, weight_scale, bias=None, x_scale=None, order="row", dtype=None):
