@@ -295,7 +295,8 @@ typedef struct tgbm_sampling {
  * of the scores and of equal scores the lower class first, where the sum of the probabilities passes u[row]; u from 0 (the best class) up to, not
  * including, 1, what is beyond counts as the ends. logp, [rows]: the logarithm of the drawn class's probability among those that are kept. Classes whose
  * score is -infinity or NaN are never drawn; infinite scores share alike. Where nothing is left a row gets class -1 and -infinity, where one of its numbers is NaN
- * class -1 and NaN. Sums are 64 bits; a probability below 2^-64 of the best one's counts as none. workspace: as for tgbm_scores_top. */
+ * class -1 and NaN. Sums are 64 bits; a probability below 2^-64 of the best one's counts as none. workspace: as for tgbm_scores_top,
+ * from a multiple of 16 bytes on. */
 size_t tgbm_scores_sample_workspace(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how);
 int tgbm_scores_sample(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp,
                        void *workspace, size_t workspace_bytes, void *stream);
@@ -321,7 +322,8 @@ int tgbm_rows_quantise(const tgbm_rows *x, signed char *q, long long q_pitch, in
 
 /* Class scores as a product: out's score of class c in row i is (sum of x[i] * weights[c] over the features) * x's scale[i] * weights' scale[c] + bias[c], the
  * sum exact (of 8-bit numbers, in 32 bits), the other steps in 32 bits, rounded once to out's type. x: of TGBM_I8, or floating rows, which are quantised as
- * tgbm_rows_quantise does first. weights: of TGBM_I8, a row for each class. bias may be NULL. out shares no memory with the others. */
+ * tgbm_rows_quantise does first. weights: of TGBM_I8, a row for each class. bias may be NULL. out shares no memory with the others. workspace: as for
+ * tgbm_scores_sample. */
 size_t tgbm_scores_linear_workspace(const tgbm_rows *x, const tgbm_rows *weights);
 int tgbm_scores_linear(const tgbm_rows *x, const tgbm_rows *weights, const float *bias, const tgbm_scores *out, void *workspace, size_t workspace_bytes,
                        void *stream);

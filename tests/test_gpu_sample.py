@@ -146,6 +146,26 @@ def test_many_rows():
         check(S.sample(x, u, **how), R.sample(x[:, at].cpu().numpy(), u[at].cpu().numpy(), **how), rows)
 
 
+@pytest.mark.parametrize("C,n", [(16_384, 128), (16_390, 129), (50_001, 17), (140_000, 64), (600_000, 3)])
+def test_few_long_rows(C, n):
+    """Rows that go by parts, some of which end the parts' way: equal scores, infinities, nothing allowed, temperatures of 0, numbers that are NaN."""
+    rng = np.random.default_rng(C)
+    z = rounded(rng.standard_normal((C, n)).astype(np.float32) * rng.choice([0.5, 2.5, 8.0], n).astype(np.float32), torch.bfloat16)
+    z[:, ::5] = rng.standard_normal(z[:, ::5].shape[1]).astype(np.float32)  # all of a row's scores are equal
+    z[C // 2, 1::7] = np.inf
+    z[:, 2] = -np.inf
+    z = rounded(z, torch.bfloat16)
+    u = numbers(rng, n)
+    f = lambda *v: np.array(v, np.float32)[rng.integers(0, len(v), n)]
+    each = dict(temperature=f(0, 0.5, 1, 1, 3, 1e6, np.nan), p=f(1, 0.9, 0.3, 0.999, 0, np.nan), min_p=f(0, 0, 0.1, 1))
+    r = D.rules(rng, C, n, sets="some", shown=n < 20)
+    for how in (dict(), dict(p=0.9), dict(p=0.5, min_p=0.01), dict(min_p=0.2, temperature=2.0), each):
+        some = {k: torch.from_numpy(v).cuda() if isinstance(v, np.ndarray) else v for k, v in how.items()}
+        check(S.sample(place(z, "row", torch.bfloat16, pad=3), torch.from_numpy(u).cuda(), **some), R.sample(z, u, **how))
+    check(S.sample(place(z, "row", torch.bfloat16), torch.from_numpy(u).cuda(), p=0.8, **on_gpu(r)), R.sample(O.adjusted(z, **r), u, p=0.8))
+    check(S.sample(place(z, "class"), torch.from_numpy(u).cuda(), p=0.95), R.sample(z, u, p=0.95))
+
+
 def test_far_apart_rows_and_long_lists():
     """Rows whose places pass 32 bits, long lists of shown classes, one class many times."""
     rng = np.random.default_rng(9)
@@ -164,7 +184,7 @@ def test_far_apart_rows_and_long_lists():
 
 def test_streams_graphs_and_repeats():
     rng = np.random.default_rng(8)
-    for C, n, how in ((8, 500, dict()), (700, 200, dict(k=30, p=0.9)), (700, 200, dict(p=0.9)), (20_000, 9, dict(k=300))):
+    for C, n, how in ((8, 500, dict()), (700, 200, dict(k=30, p=0.9)), (700, 200, dict(p=0.9)), (20_000, 9, dict(k=300)), (20_000, 9, dict(p=0.8))):
         z, u = rng.standard_normal((C, n)).astype(np.float32) * 2, numbers(rng, n)
         r = D.rules(rng, C, n, sets="each")
         want = R.sample(O.adjusted(z, **r), u, **how)

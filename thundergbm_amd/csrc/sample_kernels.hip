@@ -3,6 +3,7 @@
 // The classes of a row in order, the best first and of equal scores the lower class: w = exp((score - best) / T) of each. Every cut keeps a front part of that
 // order, and so the class that is drawn is the one where the sum of w passes u times the sum of what is kept. A sum over all classes decides which of two
 // classes it is, so everything is 64 bits, and what many threads add up is added as whole numbers, whose sum has no order.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 
@@ -686,6 +687,75 @@ __device__ __forceinline__ int nth_class(Row &row, float m, int n, int classes, 
     return hi;
 }
 
+// A row's draw, its largest score being m, a number. False: min_p cuts.
+template <int G, typename Row>
+__device__ __forceinline__ bool begin_draw(Draw<G, Row> &d, const RowSampling &r, float m, int bits) {
+    d.best = (double)m;
+    constexpr int P = parts_of<G>();
+    d.by = Scale<P>::kOfE / (double)r.temperature;
+    d.step = (double)r.temperature * (1.0 / Scale<P>::kOfE);
+    d.magic = __longlong_as_double((long long)(1023 + 52 - bits) << 52);
+    if (r.min_p == 0.f) return true;
+    d.last_place = fmin(d.last_place, -log2((double)r.min_p) * P);
+    d.least = fmaxf(d.least, d.score_below(d.last_place));
+    return false;
+}
+
+// What a bucket's whole numbers count: 2^(-b / P - bits).
+template <int P>
+__device__ __forceinline__ double unit_of(int b, int bits) {
+    const double one = __longlong_as_double((long long)(1023 - bits) << 52);
+    if constexpr (P == 32) return exp2(-(double)b / P) * one;
+    constexpr double kPart[8] = {1.0, 0.91700404320467123174, 0.84089641525371454303, 0.77110541270397041180, 0.70710678118654752440, 0.64841977732550483296, 0.59460355750136053336,
+                                 0.54525386633262882960};
+    double part = kPart[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) part = b % 8 == i ? kPart[i] : part;
+    return part * __longlong_as_double((long long)(1023 - b / 8) << 52) * one;
+}
+template <int P>
+__device__ __forceinline__ constexpr double next_unit() { return P == 32 ? 0.97857206208770013451 : 0.91700404320467123174; }  // 2^(-1 / P)
+
+// The draw, the weights of all that is kept being in their buckets.
+template <int G, typename Row>
+__device__ __forceinline__ void end_draw(Draw<G, Row> &d, const RowSampling &r, int classes, int bits, int *cls, float *logp) {
+    constexpr int P = parts_of<G>();
+    DrawShared<G> &sh = d.sh;
+    const auto weight = [&](double s) { return d.weight_of(s); };
+    double mass[Draw<G, Row>::kEach], all;
+    const auto unit = [&](int b) { return unit_of<P>(b, bits); };
+    const double before = d.sums(unit(in_group<G>() * Draw<G, Row>::kEach), next_unit<P>(), mass, &all);
+    double kept = all, front;
+    int bucket;
+    if (r.p < 1.f) {
+        const double most = fmax((double)r.p, 0.0) * all;
+        d.find(mass, before, most, true, &bucket, &front);
+        const double its = unit(bucket);
+        // The draw is among those up to here. A bucket's weights are nearly the same: its whole numbers say how many they are.
+        float count = 0.f;
+        if (G > 64 && d.chosen < 0) {
+#pragma unroll
+            for (int i = 0; i < Draw<G, Row>::kEach; ++i) {
+                const int b = in_group<G>() * Draw<G, Row>::kEach + i;
+                if (b <= bucket) count += (float)sh.mass[b];
+            }
+            count = block_sum_f<G>(count, sh.part_f) * (float)unit_of<P>(0, bits);
+            // (more of them cost as much to list as they save: 2048 x 65537, 2300 of a row kept: 249 us, 279 with the list)
+            if (count < fminf(0.95f * chosen_of<G>(), (float)classes / 128.f)) d.choose(d.score_below(bucket + 0.5));
+        }
+        const auto last = d.resolve(bucket, (most - front) / its, true, weight);
+        kept = front + (last.before + last.weight) * its;
+    }
+    const double target = (double)r.u * kept;
+    d.find(mass, before, target, false, &bucket, &front);
+    const double its = unit(bucket);
+    const auto drawn = d.resolve(bucket, (target - front) / its, false, weight);
+    if (in_group<G>() == 0) {
+        *cls = (int)~(unsigned)drawn.key;
+        *logp = (float)log(drawn.weight * its / kept);
+    }
+}
+
 // The draw of a row by a workgroup. bits: of a whole number that stands for a w of one, so that the sum of a row's has room in 63.
 template <int G, typename Row>
 __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int classes, int bits, DrawShared<G> &sh, int *cls, float *logp) {
@@ -732,67 +802,14 @@ __device__ __forceinline__ void draw_row(Row &row, const RowSampling &r, int cla
         return;
     }
     Draw<G, Row> d{sh, row};
-    d.best = (double)m;
-    constexpr int P = parts_of<G>();
-    d.by = Scale<P>::kOfE / (double)r.temperature;
-    d.step = (double)r.temperature * (1.0 / Scale<P>::kOfE);
-    d.magic = __longlong_as_double((long long)(1023 + 52 - bits) << 52);
-    bool all_kept = true;
-    if (r.min_p > 0.f) {
-        d.last_place = fmin(d.last_place, -log2((double)r.min_p) * P);
-        d.least = fmaxf(d.least, d.score_below(d.last_place));
-        all_kept = false;
-        d.choose(d.least);
-    }
+    bool all_kept = begin_draw(d, r, m, bits);
+    if (!all_kept) d.choose(d.least);
     if (r.k < classes) {
         d.keep_best(r.k, mine);
         all_kept = all_kept && d.cut == 0 && d.least == -FLT_MAX;
     }
-    const auto weight = [&](double s) { return d.weight_of(s); };
-    double mass[Draw<G, Row>::kEach], all;
     d.add_up(all_kept);
-    const double one = __longlong_as_double((long long)(1023 - bits) << 52);
-    // 2^(-b / P): what a bucket's whole numbers count, beside `one`
-    const auto unit = [&](int b) {
-        constexpr double kPart[8] = {1.0, 0.91700404320467123174, 0.84089641525371454303, 0.77110541270397041180, 0.70710678118654752440, 0.64841977732550483296, 0.59460355750136053336,
-                                     0.54525386633262882960};
-        if constexpr (P == 32) return exp2(-(double)b / P) * one;
-        double part = kPart[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) part = b % 8 == i ? kPart[i] : part;
-        return part * __longlong_as_double((long long)(1023 - b / 8) << 52) * one;
-    };
-    constexpr double kNext = P == 32 ? 0.97857206208770013451 : 0.91700404320467123174;  // 2^(-1 / P)
-    const double before = d.sums(unit(in_group<G>() * Draw<G, Row>::kEach), kNext, mass, &all);
-    double kept = all, front;
-    int bucket;
-    if (r.p < 1.f) {
-        const double most = fmax((double)r.p, 0.0) * all;
-        d.find(mass, before, most, true, &bucket, &front);
-        const double its = unit(bucket);
-        // The draw is among those up to here. A bucket's weights are nearly the same: its whole numbers say how many they are.
-        float count = 0.f;
-        if (G > 64 && d.chosen < 0) {
-#pragma unroll
-            for (int i = 0; i < Draw<G, Row>::kEach; ++i) {
-                const int b = in_group<G>() * Draw<G, Row>::kEach + i;
-                if (b <= bucket) count += (float)sh.mass[b];
-            }
-            count = block_sum_f<G>(count, sh.part_f) * (float)one;
-            // (more of them cost as much to list as they save: 2048 x 65537, 2300 of a row kept: 249 us, 279 with the list)
-            if (count < fminf(0.95f * chosen_of<G>(), (float)classes / 128.f)) d.choose(d.score_below(bucket + 0.5));
-        }
-        const auto last = d.resolve(bucket, (most - front) / its, true, weight);
-        kept = front + (last.before + last.weight) * its;
-    }
-    const double target = (double)r.u * kept;
-    d.find(mass, before, target, false, &bucket, &front);
-    const double its = unit(bucket);
-    const auto drawn = d.resolve(bucket, (target - front) / its, false, weight);
-    if (in_group<G>() == 0) {
-        *cls = (int)~(unsigned)drawn.key;
-        *logp = (float)log(drawn.weight * its / kept);
-    }
+    end_draw(d, r, classes, bits, cls, logp);
 }
 
 // A row's scores, classes side by side, with bias and allowed sets, read by vectors of 16 bytes as often as they are gone over. (Scores that stay in registers want
@@ -804,7 +821,7 @@ struct ScoreRow {
     const T *src;
     const float *bias;
     const unsigned *words;
-    int classes;
+    int begin, classes;  // from where to where
     bool none;
 
     __device__ __forceinline__ Vec read(int c) const {
@@ -846,7 +863,7 @@ struct ScoreRow {
     __device__ __forceinline__ void each(F f) {
         // (the next vectors are on their way while one is worked on)
         constexpr int kStep = G * V;
-        int c = (int)threadIdx.x * V;
+        int c = begin + (int)threadIdx.x * V;
         Vec a = (T)kNothing, b = (T)kNothing;
         if (c < classes) a = read(c);
         if (c + kStep < classes) b = read(c + kStep);
@@ -860,18 +877,137 @@ struct ScoreRow {
 };
 
 template <typename T, int G, bool RULES>
-__global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
-    __shared__ DrawShared<G> sh;
-    const long row = blockIdx.x;
-    const RowSampling r = sampling_of(how, u, row);
+__device__ __forceinline__ ScoreRow<T, G, RULES> row_of(const tgbm_scores &in, const tgbm_score_rules &rules, long row, int begin, int end) {
     ScoreRow<T, G, RULES> scores;
     scores.src = static_cast<const T *>(in.data) + (size_t)row * in.row_stride;
-    scores.classes = in.classes;
+    scores.begin = begin;
+    scores.classes = end;
     scores.bias = rules.bias;
     scores.words = nullptr;
     scores.none = false;
     if constexpr (RULES) scores.words = allowed_words(rules, row, (in.classes + 31) / 32, &scores.none);
-    draw_row<G>(scores, r, in.classes, bits, sh, classes + row, logp + row);
+    return scores;
+}
+template <typename T, int G, bool RULES>
+__global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
+    __shared__ DrawShared<G> sh;
+    const long row = blockIdx.x;
+    auto scores = row_of<T, G, RULES>(in, rules, row, 0, in.classes);
+    draw_row<G>(scores, sampling_of(how, u, row), in.classes, bits, sh, classes + row, logp + row);
+}
+
+// Few long rows whose number of classes is not cut: parts of a row by a workgroup each, in four launches. The largest score; the weights' buckets, added up over the
+// parts as the whole numbers that they are; the scores of the buckets where the sum can pass the target; the draw among those. One workgroup to a row took 58 us
+// for 1 x 128003 bfloat16 and 116 for 8 of them.
+constexpr int kSplitBlock = 512, kSplitParts = 64, kSplitRows = 128, kSplitLeast = 16384, kSplitListed = chosen_of<kSplitBlock>();
+struct SplitRow {
+    unsigned long long mass[Scale<parts_of<kSplitBlock>()>::kBuckets];
+    unsigned long long listed[kSplitListed];
+    float most[kSplitParts];
+    int count, unused[3];
+};
+__device__ __forceinline__ void part_of_row(int classes, int *begin, int *end) {
+    const int size = ((classes - 1) / (int)gridDim.x + 64) / 64 * 64;
+    *begin = min((int)blockIdx.x * size, classes);
+    *end = min(*begin + size, classes);
+}
+__device__ __forceinline__ float most_of(const SplitRow &s, int parts) { return wave_max_f(lane_id() < parts ? s.most[lane_id()] : kNothing); }
+// (rows that have no draw of this kind: the last launch goes over them by itself)
+__device__ __forceinline__ bool goes_by_parts(const RowSampling &r, float m) { return !r.none && !r.greedy && m > kNothing && m < __builtin_inff(); }
+
+template <typename T, bool RULES>
+__global__ __launch_bounds__(kSplitBlock, 4) void k_split_most(tgbm_scores in, tgbm_score_rules rules, SplitRow *splits) {
+    __shared__ float part_f[kSplitBlock / 64];
+    SplitRow &s = splits[blockIdx.y];
+    int begin, end;
+    part_of_row(in.classes, &begin, &end);
+    auto scores = row_of<T, kSplitBlock, RULES>(in, rules, blockIdx.y, begin, end);
+    float mine = kNothing;
+    scores.each([&](const float (&x)[decltype(scores)::V], int) {
+#pragma unroll
+        for (int j = 0; j < decltype(scores)::V; ++j) mine = fmaxf(mine, x[j]);
+    });
+    const float m = block_max<kSplitBlock>(mine, part_f);
+    if (threadIdx.x == 0) {
+        s.most[blockIdx.x] = m;
+        if (blockIdx.x == 0) s.count = 0;
+    }
+    constexpr int kBuckets = Scale<parts_of<kSplitBlock>()>::kBuckets;
+    for (int i = (int)(blockIdx.x * kSplitBlock + threadIdx.x); i < kBuckets; i += (int)gridDim.x * kSplitBlock) s.mass[i] = 0;
+}
+template <typename T, bool RULES>
+__global__ __launch_bounds__(kSplitBlock, 4) void k_split_add(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, SplitRow *splits, int bits) {
+    __shared__ DrawShared<kSplitBlock> sh;
+    const RowSampling r = sampling_of(how, u, blockIdx.y);
+    SplitRow &s = splits[blockIdx.y];
+    const float m = most_of(s, gridDim.x);
+    if (!goes_by_parts(r, m)) return;
+    int begin, end;
+    part_of_row(in.classes, &begin, &end);
+    auto scores = row_of<T, kSplitBlock, RULES>(in, rules, blockIdx.y, begin, end);
+    Draw<kSplitBlock, decltype(scores)> d{sh, scores};
+    const bool all_kept = begin_draw(d, r, m, bits);
+    d.add_up(all_kept);
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock)
+        if (sh.mass[i] != 0) atomicAdd(&s.mass[i], sh.mass[i]);
+}
+template <typename T, bool RULES>
+__global__ __launch_bounds__(kSplitBlock, 4) void k_split_list(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, SplitRow *splits, int bits) {
+    __shared__ DrawShared<kSplitBlock> sh;
+    const RowSampling r = sampling_of(how, u, blockIdx.y);
+    SplitRow &s = splits[blockIdx.y];
+    const float m = most_of(s, gridDim.x);
+    if (!goes_by_parts(r, m)) return;
+    int begin, end;
+    part_of_row(in.classes, &begin, &end);
+    auto scores = row_of<T, kSplitBlock, RULES>(in, rules, blockIdx.y, begin, end);
+    using D = Draw<kSplitBlock, decltype(scores)>;
+    D d{sh, scores};
+    begin_draw(d, r, m, bits);
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = s.mass[i];
+    __syncthreads();
+    double mass[D::kEach], all, front;
+    const double before = d.sums(unit_of<D::P>(threadIdx.x * D::kEach, bits), next_unit<D::P>(), mass, &all);
+    // the bucket where the cut is, and those where the draw can be: what is kept is known but for that bucket's part
+    int cut = -1, first, last;
+    double least = all, most = all;
+    if (r.p < 1.f) {
+        d.find(mass, before, fmax((double)r.p, 0.0) * all, true, &cut, &front);
+        least = front;
+        most = front + (double)s.mass[cut] * unit_of<D::P>(cut, bits);
+    }
+    d.find(mass, before, (double)r.u * least * (1.0 - 0x1p-40), false, &first, &front);
+    d.find(mass, before, (double)r.u * most * (1.0 + 0x1p-40), false, &last, &front);
+    const auto list = [&](int from, int to) {
+        d.kept(d.score_below(to + 0.5), d.score_above(from - 0.5), [&](double, int b, unsigned long long key) {
+            if (b < from || b > to) return;
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kSplitListed) s.listed[at] = key;
+        });
+    };
+    list(first, last);
+    if (cut >= 0 && !(first <= cut && cut <= last)) list(cut, cut);
+}
+template <typename T, bool RULES>
+__global__ __launch_bounds__(kSplitBlock, 4) void k_split_draw(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, const SplitRow *splits, int parts, int *classes,
+                                                               float *logp, int bits) {
+    __shared__ DrawShared<kSplitBlock> sh;
+    const long row = blockIdx.x;
+    const RowSampling r = sampling_of(how, u, row);
+    const SplitRow &s = splits[row];
+    const float m = most_of(s, parts);
+    auto scores = row_of<T, kSplitBlock, RULES>(in, rules, row, 0, in.classes);
+    if (!goes_by_parts(r, m) || s.count > kSplitListed) {
+        draw_row<kSplitBlock>(scores, r, in.classes, bits, sh, classes + row, logp + row);
+        return;
+    }
+    Draw<kSplitBlock, decltype(scores)> d{sh, scores};
+    begin_draw(d, r, m, bits);
+    d.chosen = s.count;  // (not all that is kept, but all of the buckets that are looked into)
+    for (int i = threadIdx.x; i < d.chosen; i += kSplitBlock) sh.chosen[i] = s.listed[i];
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = s.mass[i];
+    __syncthreads();
+    end_draw(d, r, in.classes, bits, classes + row, logp + row);
 }
 
 // A row in LDS, adjusted, for a wavefront; behind its classes -infinity up to a multiple of four.
@@ -1035,17 +1171,31 @@ void sample_middle(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules 
     else (some ? sample_middle<T, false, true> : sample_middle<T, false, false>)(s, in, rules, how, u, classes, logp);
 }
 
+// Few long rows go by parts.
+bool splits_rows(const tgbm_sampling &how, int classes) { return how.k == nullptr && how.k_all == 0 && classes >= kSplitLeast; }
+size_t split_bytes(const tgbm_sampling &how, int classes, int rows) { return splits_rows(how, classes) ? sizeof(SplitRow) * (size_t)std::min(rows, kSplitRows) : 0; }
+
 template <typename T, bool RULES>
-void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
+void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp, void *room) {
+    if (in.rows <= kSplitRows && splits_rows(how, in.classes)) {
+        const int bits = weight_bits(in.classes), parts = std::min({kSplitParts, in.classes / 4096, std::max(2, 1024 / in.rows)});
+        const dim3 grid((unsigned)parts, (unsigned)in.rows);
+        SplitRow *splits = static_cast<SplitRow *>(room);
+        k_split_most<T, RULES><<<grid, kSplitBlock, 0, s>>>(in, rules, splits);
+        k_split_add<T, RULES><<<grid, kSplitBlock, 0, s>>>(in, rules, how, u, splits, bits);
+        k_split_list<T, RULES><<<grid, kSplitBlock, 0, s>>>(in, rules, how, u, splits, bits);
+        k_split_draw<T, RULES><<<in.rows, kSplitBlock, 0, s>>>(in, rules, how, u, splits, parts, classes, logp, bits);
+        return;
+    }
     const int bits = weight_bits(in.classes), vectors = (in.classes - 1) / (16 / (int)sizeof(T)) + 1;
     if (vectors <= 4 * 256) k_sample_rows<T, 256, RULES><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
     else if (in.rows > 256) k_sample_rows<T, 512, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
     else k_sample_rows<T, 1024, RULES><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
 }
 template <typename T>
-void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp) {
-    if (rules.bias != nullptr || rules.allowed != nullptr) sample_rows<T, true>(s, in, rules, how, u, classes, logp);
-    else sample_rows<T, false>(s, in, rules, how, u, classes, logp);
+void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp, void *room) {
+    if (rules.bias != nullptr || rules.allowed != nullptr) sample_rows<T, true>(s, in, rules, how, u, classes, logp, room);
+    else sample_rows<T, false>(s, in, rules, how, u, classes, logp, room);
 }
 
 template <typename T>
@@ -1060,7 +1210,7 @@ void sample_laid_out(hipStream_t s, const tgbm_scores &in, const tgbm_score_rule
         k_lay_out<T><<<dim3((in.classes - 1) / kLaid + 1, (part.rows - 1) / kLaid + 1), kSampleBlock, 0, s>>>(part, r, room, pitch);
         if (rules.shown != nullptr) k_lay_shown<T><<<dim3(part.rows, (in.classes - 1) / kShownClasses + 1), kSampleBlock, 0, s>>>(part, r, room, pitch);
         const tgbm_scores laid{room, 1, pitch, TGBM_F32, in.classes, part.rows};
-        sample_rows<float>(s, laid, tgbm_score_rules{}, take(how, row), u + row, classes + row, logp + row);
+        sample_rows<float>(s, laid, tgbm_score_rules{}, take(how, row), u + row, classes + row, logp + row, room + (size_t)most * pitch);
     }
 }
 
@@ -1070,7 +1220,7 @@ void sample(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules,
     switch (way_of(in, rules, how)) {
         case kFew: return sample_few<T>(s, in, rules, how, u, classes, logp);
         case kMiddle: return sample_middle<T>(s, in, rules, how, u, classes, logp);
-        case kRows: return sample_rows<T>(s, in, rules, how, u, classes, logp);
+        case kRows: return sample_rows<T>(s, in, rules, how, u, classes, logp, workspace);
         case kLaidOut: return sample_laid_out<T>(s, in, rules, how, u, classes, logp, static_cast<float *>(workspace));
         case kFromList: {
             const size_t n = (size_t)in.rows, k = (size_t)how.k_all;
@@ -1091,7 +1241,8 @@ size_t scores_sample_workspace(const tgbm_scores &in, const tgbm_score_rules &ru
     return workspace_of_slices(in.rows, [&](int rows) -> size_t {
         switch (way_of(in, rules, how)) {
             case kFromList: return list_bytes((size_t)rows, (size_t)how.k_all) + scores_top_workspace(rows_side_by_side(in), in.classes, rows, how.k_all);
-            case kLaidOut: return sizeof(float) * (size_t)laid_rows(in.classes, rows) * laid_pitch(in.classes);
+            case kLaidOut: return sizeof(float) * (size_t)laid_rows(in.classes, rows) * laid_pitch(in.classes) + split_bytes(how, in.classes, laid_rows(in.classes, rows));
+            case kRows: return split_bytes(how, in.classes, rows);
             default: return 0;
         }
     });

@@ -206,6 +206,7 @@ extern "C" int tgbm_scores_sample(const tgbm_scores *in, const tgbm_score_rules 
     if (classes == nullptr || logp == nullptr) return refused(entry, "an output is null");
     const size_t needed = scores_sample_workspace(*in, *rules, *how);
     if (needed > workspace_bytes || (needed > 0 && workspace == nullptr)) return refused(entry, "%zu bytes of workspace, %zu are needed", workspace_bytes, needed);
+    if (needed > 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return refused(entry, "the workspace does not begin at 16 bytes");
     launch_scores_sample(static_cast<hipStream_t>(stream), *in, *rules, *how, u, classes, logp, workspace);
     return launched(entry);
 }
