@@ -128,10 +128,30 @@ __global__ __launch_bounds__(1024) void k_quantise_long(const T *x, long long pi
     for (int i = threadIdx.x; i < pad; i += 1024) to[i] = (signed char)(i < features ? whole_of(score_to_float(row[i]), scale) : 0);
 }
 
-// Rows of whole numbers, moved to rows of `pad` bytes.
-__global__ __launch_bounds__(kLinearBlock) void k_pack(const signed char *x, long long pitch, int features, signed char *to, int pad) {
-    const signed char *row = x + (size_t)blockIdx.x * pitch;
-    for (int i = threadIdx.x; i < pad; i += kLinearBlock) to[(size_t)blockIdx.x * pad + i] = i < features ? row[i] : (signed char)0;
+// Rows of whole numbers, moved to rows of `pad` bytes, 16 of them to a thread.
+__global__ __launch_bounds__(kLinearBlock) void k_pack(const signed char *x, long long pitch, int rows, int features, signed char *to, int pad) {
+    typedef Int4 Loose __attribute__((aligned(1)));
+    const int parts = pad / 16;
+    const long at = (long)blockIdx.x * kLinearBlock + threadIdx.x, row = at / parts;
+    const int f = (int)(at - row * parts) * 16;
+    if (row >= rows) return;
+    const signed char *from = x + (size_t)row * pitch + f;
+    Int4 v = {0, 0, 0, 0};
+    if (f + 16 <= features) {
+        v = *reinterpret_cast<const Loose *>(from);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (f + j < features) v[j / 4] |= (int)((unsigned)(unsigned char)from[j] << j % 4 * 8);
+    }
+    *reinterpret_cast<Int4 *>(to + (size_t)row * pad + f) = v;
+}
+void pack(hipStream_t s, const signed char *x, long long pitch, int rows, int features, signed char *to, int pad) {
+    const int most = std::max(1, (1 << 30) / pad);  // (a launch has fewer than 2^32 threads in a direction)
+    for (int row = 0; row < rows; row += std::min(most, rows - row)) {
+        const int n = std::min(most, rows - row);
+        k_pack<<<(unsigned)(((long)n * (pad / 16) - 1) / kLinearBlock + 1), kLinearBlock, 0, s>>>(x + (size_t)row * pitch, pitch, n, features, to + (size_t)row * pad, pad);
+    }
 }
 
 struct Rows8 {
@@ -588,7 +608,7 @@ void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &w,
     signed char *room = static_cast<signed char *>(workspace);
     Rows8 weights{static_cast<const signed char *>(w.data), w.scale, w.pitch, w.rows};
     if (packs_weights(w)) {
-        k_pack<<<w.rows, kLinearBlock, 0, s>>>(weights.data, w.pitch, w.features, room, pad);
+        pack(s, weights.data, w.pitch, w.rows, w.features, room, pad);
         weights.data = room;
         weights.pitch = pad;
         room += in_lines((size_t)pad * w.rows);
@@ -609,7 +629,7 @@ void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &w,
         Rows8 features{static_cast<const signed char *>(part.data), x.type == TGBM_I8 ? x.scale + row : nullptr, x.pitch, part.rows};
         if (packs_features(x)) {
             if (x.type == TGBM_I8) {
-                k_pack<<<part.rows, kLinearBlock, 0, s>>>(features.data, x.pitch, x.features, room, pad);
+                pack(s, features.data, x.pitch, part.rows, x.features, room, pad);
             } else {
                 float *scale = reinterpret_cast<float *>(room + in_lines((size_t)pad * most));
                 launch_rows_quantise(s, part, room, pad, pad, scale);
