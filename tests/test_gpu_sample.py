@@ -158,8 +158,9 @@ def test_few_long_rows(C, n):
     u = numbers(rng, n)
     f = lambda *v: np.array(v, np.float32)[rng.integers(0, len(v), n)]
     each = dict(temperature=f(0, 0.5, 1, 1, 3, 1e6, np.nan), p=f(1, 0.9, 0.3, 0.999, 0, np.nan), min_p=f(0, 0, 0.1, 1))
+    counts = dict(k=np.array([0, 1, 3, 50, 700, 9000, C - 1, C, C + 1], np.int32)[rng.integers(0, 9, n)])
     r = D.rules(rng, C, n, sets="some", shown=n < 20)
-    for how in (dict(), dict(p=0.9), dict(p=0.5, min_p=0.01), dict(min_p=0.2, temperature=2.0), each):
+    for how in (dict(), dict(p=0.9), dict(p=0.5, min_p=0.01), dict(min_p=0.2, temperature=2.0), each, counts, {**counts, **each}, dict(k=500), dict(k=300, p=0.7), dict(k=5000, min_p=0.001, p=0.99)):
         some = {k: torch.from_numpy(v).cuda() if isinstance(v, np.ndarray) else v for k, v in how.items()}
         check(S.sample(place(z, "row", torch.bfloat16, pad=3), torch.from_numpy(u).cuda(), **some), R.sample(z, u, **how))
     check(S.sample(place(z, "row", torch.bfloat16), torch.from_numpy(u).cuda(), p=0.8, **on_gpu(r)), R.sample(O.adjusted(z, **r), u, p=0.8))

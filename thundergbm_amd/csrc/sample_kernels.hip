@@ -896,13 +896,14 @@ __global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score
     draw_row<G>(scores, sampling_of(how, u, row), in.classes, bits, sh, classes + row, logp + row);
 }
 
-// Few long rows whose number of classes is not cut: parts of a row by a workgroup each, in four launches. The largest score; the weights' buckets, added up over the
-// parts as the whole numbers that they are; the scores of the buckets where the sum can pass the target; the draw among those. One workgroup to a row took 58 us
-// for 1 x 128003 bfloat16 and 116 for 8 of them.
-constexpr int kSplitBlock = 512, kSplitParts = 64, kSplitRows = 128, kSplitLeast = 16384, kSplitListed = chosen_of<kSplitBlock>();
+// Few long rows: parts of a row by a workgroup each, in four launches. The largest score; the weights' buckets, added up over the parts as the whole numbers that they
+// are, and where a number of classes cuts how many there are in each; the scores of the buckets where the cuts and the draw can be; the draw among those. One workgroup
+// to a row took 58 us for 1 x 128003 bfloat16, 116 for 8 of them, 167 for 256 with settings of each row.
+constexpr int kSplitBlock = 512, kSplitParts = 64, kSplitRows = 384, kSplitLeast = 16384, kSplitListed = chosen_of<kSplitBlock>();
 struct SplitRow {
     unsigned long long mass[Scale<parts_of<kSplitBlock>()>::kBuckets];
     unsigned long long listed[kSplitListed];
+    unsigned times[Scale<parts_of<kSplitBlock>()>::kBuckets];  // (of rows whose number of classes is cut)
     float most[kSplitParts];
     int count, unused[3];
 };
@@ -933,7 +934,10 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_most(tgbm_scores in, t
         if (blockIdx.x == 0) s.count = 0;
     }
     constexpr int kBuckets = Scale<parts_of<kSplitBlock>()>::kBuckets;
-    for (int i = (int)(blockIdx.x * kSplitBlock + threadIdx.x); i < kBuckets; i += (int)gridDim.x * kSplitBlock) s.mass[i] = 0;
+    for (int i = (int)(blockIdx.x * kSplitBlock + threadIdx.x); i < kBuckets; i += (int)gridDim.x * kSplitBlock) {
+        s.mass[i] = 0;
+        s.times[i] = 0;
+    }
 }
 template <typename T, bool RULES>
 __global__ __launch_bounds__(kSplitBlock, 4) void k_split_add(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, SplitRow *splits, int bits) {
@@ -947,9 +951,36 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_add(tgbm_scores in, tg
     auto scores = row_of<T, kSplitBlock, RULES>(in, rules, blockIdx.y, begin, end);
     Draw<kSplitBlock, decltype(scores)> d{sh, scores};
     const bool all_kept = begin_draw(d, r, m, bits);
-    d.add_up(all_kept);
+    unsigned *const times = reinterpret_cast<unsigned *>(sh.chosen);
+    if (r.k < in.classes) {
+        for (int i = threadIdx.x; i <= d.kBuckets; i += kSplitBlock) times[i] = 0;
+        d.clear();
+        d.kept(d.least, __builtin_inff(), [&](double place, int bucket, unsigned long long) {
+            atomicAdd(&sh.mass[bucket], d.weight_of(place));
+            atomicAdd(&times[bucket], 1u);
+        });
+        __syncthreads();
+    } else {
+        d.add_up(all_kept);
+    }
     for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock)
-        if (sh.mass[i] != 0) atomicAdd(&s.mass[i], sh.mass[i]);
+        if (sh.mass[i] != 0) {
+            atomicAdd(&s.mass[i], sh.mass[i]);
+            if (r.k < in.classes) atomicAdd(&s.times[i], times[i]);
+        }
+}
+// The bucket where the number of classes is cut, -1 where there are no more than that, and how many there are in front of it.
+template <typename D>
+__device__ __forceinline__ int cut_of_times(D &d, const SplitRow &s, int k, double *front) {
+    d.clear();
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) d.sh.mass[i] = s.times[i];
+    __syncthreads();
+    double mass[D::kEach], all;
+    const double before = d.sums(1.0, 1.0, mass, &all);
+    if (all <= (double)k) return -1;
+    int bucket;
+    d.find(mass, before, (double)(k - 1), false, &bucket, front);
+    return bucket;
 }
 template <typename T, bool RULES>
 __global__ __launch_bounds__(kSplitBlock, 4) void k_split_list(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, SplitRow *splits, int bits) {
@@ -964,29 +995,32 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_list(tgbm_scores in, t
     using D = Draw<kSplitBlock, decltype(scores)>;
     D d{sh, scores};
     begin_draw(d, r, m, bits);
-    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = s.mass[i];
+    double front = 0;
+    const int last_bucket = r.k < in.classes ? cut_of_times(d, s, r.k, &front) : -1;
+    d.clear();
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = last_bucket < 0 || i <= last_bucket ? s.mass[i] : 0;
     __syncthreads();
-    double mass[D::kEach], all, front;
+    double mass[D::kEach], all;
     const double before = d.sums(unit_of<D::P>(threadIdx.x * D::kEach, bits), next_unit<D::P>(), mass, &all);
-    // the bucket where the cut is, and those where the draw can be: what is kept is known but for that bucket's part
-    int cut = -1, first, last;
-    double least = all, most = all;
+    const auto of = [&](int bucket) { return (double)s.mass[bucket] * unit_of<D::P>(bucket, bits); };
+    // Sums are known but for the part of a bucket that is cut: from where to where the cut by mass and the draw can be.
+    double least = last_bucket < 0 ? all : all - of(last_bucket), most = all;
+    int cut_first = 0, cut_last = -1, first, last;
     if (r.p < 1.f) {
-        d.find(mass, before, fmax((double)r.p, 0.0) * all, true, &cut, &front);
-        least = front;
-        most = front + (double)s.mass[cut] * unit_of<D::P>(cut, bits);
+        const double p = fmax((double)r.p, 0.0);
+        d.find(mass, before, p * least * (1.0 - 0x1p-40), true, &cut_first, &front);
+        least = fmax(front - 0x1p-40 * all, 0.0);
+        d.find(mass, before, p * most * (1.0 + 0x1p-40), true, &cut_last, &front);
+        most = front + of(cut_last);
     }
     d.find(mass, before, (double)r.u * least * (1.0 - 0x1p-40), false, &first, &front);
     d.find(mass, before, (double)r.u * most * (1.0 + 0x1p-40), false, &last, &front);
-    const auto list = [&](int from, int to) {
-        d.kept(d.score_below(to + 0.5), d.score_above(from - 0.5), [&](double, int b, unsigned long long key) {
-            if (b < from || b > to) return;
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kSplitListed) s.listed[at] = key;
-        });
-    };
-    list(first, last);
-    if (cut >= 0 && !(first <= cut && cut <= last)) list(cut, cut);
+    const int from = min(first, min(cut_last < 0 ? first : cut_first, last_bucket < 0 ? first : last_bucket)), to = max(last, max(cut_last, last_bucket));
+    d.kept(d.score_below(to + 0.5), d.score_above(from - 0.5), [&](double, int b, unsigned long long key) {
+        if ((b < first || b > last) && (b < cut_first || b > cut_last) && b != last_bucket) return;
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kSplitListed) s.listed[at] = key;
+    });
 }
 template <typename T, bool RULES>
 __global__ __launch_bounds__(kSplitBlock, 4) void k_split_draw(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, const SplitRow *splits, int parts, int *classes,
@@ -1005,8 +1039,22 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_draw(tgbm_scores in, t
     begin_draw(d, r, m, bits);
     d.chosen = s.count;  // (not all that is kept, but all of the buckets that are looked into)
     for (int i = threadIdx.x; i < d.chosen; i += kSplitBlock) sh.chosen[i] = s.listed[i];
-    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = s.mass[i];
+    double front = 0;
+    const int last_bucket = r.k < in.classes ? cut_of_times(d, s, r.k, &front) : -1;
+    if (last_bucket >= 0) {
+        const unsigned long long key = d.resolve(last_bucket, (double)(r.k - 1) - front, false, [](double) { return 1ull; }).key;
+        d.cut = key;
+        d.least = from_ordered((unsigned)(key >> 32));
+    }
+    d.clear();
+    for (int i = threadIdx.x; i < d.kBuckets; i += kSplitBlock) sh.mass[i] = last_bucket < 0 || i < last_bucket ? s.mass[i] : 0;
     __syncthreads();
+    if (last_bucket >= 0) {
+        d.kept(d.least, __builtin_inff(), [&](double place, int b, unsigned long long) {
+            if (b == last_bucket) atomicAdd(&sh.mass[b], d.weight_of(place));
+        });
+        __syncthreads();
+    }
     end_draw(d, r, in.classes, bits, classes + row, logp + row);
 }
 
@@ -1172,12 +1220,11 @@ void sample_middle(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules 
 }
 
 // Few long rows go by parts.
-bool splits_rows(const tgbm_sampling &how, int classes) { return how.k == nullptr && how.k_all == 0 && classes >= kSplitLeast; }
-size_t split_bytes(const tgbm_sampling &how, int classes, int rows) { return splits_rows(how, classes) ? sizeof(SplitRow) * (size_t)std::min(rows, kSplitRows) : 0; }
+size_t split_bytes(int classes, int rows) { return classes >= kSplitLeast ? sizeof(SplitRow) * (size_t)std::min(rows, kSplitRows) : 0; }
 
 template <typename T, bool RULES>
 void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp, void *room) {
-    if (in.rows <= kSplitRows && splits_rows(how, in.classes)) {
+    if (in.rows <= kSplitRows && in.classes >= kSplitLeast) {
         const int bits = weight_bits(in.classes), parts = std::min({kSplitParts, in.classes / 4096, std::max(2, 1024 / in.rows)});
         const dim3 grid((unsigned)parts, (unsigned)in.rows);
         SplitRow *splits = static_cast<SplitRow *>(room);
@@ -1241,8 +1288,8 @@ size_t scores_sample_workspace(const tgbm_scores &in, const tgbm_score_rules &ru
     return workspace_of_slices(in.rows, [&](int rows) -> size_t {
         switch (way_of(in, rules, how)) {
             case kFromList: return list_bytes((size_t)rows, (size_t)how.k_all) + scores_top_workspace(rows_side_by_side(in), in.classes, rows, how.k_all);
-            case kLaidOut: return sizeof(float) * (size_t)laid_rows(in.classes, rows) * laid_pitch(in.classes) + split_bytes(how, in.classes, laid_rows(in.classes, rows));
-            case kRows: return split_bytes(how, in.classes, rows);
+            case kLaidOut: return sizeof(float) * (size_t)laid_rows(in.classes, rows) * laid_pitch(in.classes) + split_bytes(in.classes, laid_rows(in.classes, rows));
+            case kRows: return split_bytes(in.classes, rows);
             default: return 0;
         }
     });
