@@ -531,13 +531,14 @@ void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, 
 
 template <typename O>
 void linear_tiles(hipStream_t s, const Rows8 &x, const Rows8 &w, int features, const float *bias, const ScoreOut &out, long tiles) {
+    const bool large = tiles >= 2048 && features > 4 * kChunk;
     if (out.class_stride == 1) {
         const Product p{w, x, bias, features, out.data, out.row_stride};
-        if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, true>(s, p);
+        if (large) linear_tiles<O, 256, 256, 2, 4, true>(s, p);
         else linear_tiles<O, 128, 128, 2, 2, true>(s, p);
     } else {
         const Product p{x, w, bias, features, out.data, out.class_stride};
-        if (tiles >= 2048) linear_tiles<O, 256, 256, 2, 4, false>(s, p);
+        if (large) linear_tiles<O, 256, 256, 2, 4, false>(s, p);
         else linear_tiles<O, 128, 128, 2, 2, false>(s, p);
     }
 }

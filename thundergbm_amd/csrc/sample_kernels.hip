@@ -909,7 +909,7 @@ struct SplitRow {
     unsigned long long listed[kSplitListed];
     unsigned times[Scale<parts_of<kSplitBlock>()>::kBuckets];  // (of rows whose number of classes is cut)
     float most[kSplitParts];
-    int count, unused[3];
+    int count, first, unused[2];  // first: the first class of the largest score, where that is the answer
 };
 __device__ __forceinline__ void part_of_row(int classes, int *begin, int *end) {
     const int size = ((classes - 1) / (int)gridDim.x + 64) / 64 * 64;
@@ -935,7 +935,10 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_most(tgbm_scores in, t
     const float m = block_max<kSplitBlock>(mine, part_f);
     if (threadIdx.x == 0) {
         s.most[blockIdx.x] = m;
-        if (blockIdx.x == 0) s.count = 0;
+        if (blockIdx.x == 0) {
+            s.count = 0;
+            s.first = INT_MAX;
+        }
     }
     constexpr int kBuckets = Scale<parts_of<kSplitBlock>()>::kBuckets;
     for (int i = (int)(blockIdx.x * kSplitBlock + threadIdx.x); i < kBuckets; i += (int)gridDim.x * kSplitBlock) {
@@ -992,11 +995,21 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_list(tgbm_scores in, t
     const RowSampling r = sampling_of(how, u, blockIdx.y);
     SplitRow &s = splits[blockIdx.y];
     const float m = most_of(s, gridDim.x);
-    if (!goes_by_parts(r, m)) return;
+    if (!(goes_by_parts(r, m) || (r.greedy && !r.none && m > kNothing))) return;
     int begin, end;
     part_of_row(in.classes, &begin, &end);
     auto scores = row_of<T, kSplitBlock, RULES>(in, rules, blockIdx.y, begin, end);
     using D = Draw<kSplitBlock, decltype(scores)>;
+    if (r.greedy) {
+        int its = INT_MAX;
+        scores.each([&](const float (&x)[D::V], int c) {
+#pragma unroll
+            for (int j = 0; j < D::V; ++j) its = x[j] == m ? min(its, c + j) : its;
+        });
+        its = wave_min_i(its);
+        if (lane_id() == 0 && its != INT_MAX) atomicMin(&s.first, its);
+        return;
+    }
     D d{sh, scores};
     begin_draw(d, r, m, bits);
     double front = 0;
@@ -1035,6 +1048,13 @@ __global__ __launch_bounds__(kSplitBlock, 4) void k_split_draw(tgbm_scores in, t
     const SplitRow &s = splits[row];
     const float m = most_of(s, parts);
     auto scores = row_of<T, kSplitBlock, RULES>(in, rules, row, 0, in.classes);
+    if (r.greedy && !r.none && m > kNothing) {
+        if (threadIdx.x == 0) {
+            classes[row] = s.first;
+            logp[row] = 0.f;
+        }
+        return;
+    }
     if (!goes_by_parts(r, m) || s.count > kSplitListed) {
         draw_row<kSplitBlock>(scores, r, in.classes, bits, sh, classes + row, logp + row);
         return;
