@@ -344,8 +344,9 @@ struct ScoreOut {
 // Few rows: the rows' features in LDS, `slice` of them at a time, and 16 * A classes to a wavefront, whose weights go from memory to the product; S wavefronts share
 // the features. T: of the rows, which are quantised on the way into LDS if they are floating ones (all of their features at once then).
 constexpr int few_block(int shares) { return shares > 4 ? 64 * shares : kLinearBlock; }
+// (Two wavefronts to a SIMD at least: with more than 256 registers the compiler puts sums into the accumulation registers.)
 template <typename T, int A, int R, int S>
-__global__ __launch_bounds__(few_block(S)) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
+__global__ __launch_bounds__(few_block(S), S > 4 ? 4 : 2) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
     constexpr bool kQuantise = sizeof(T) > 1;
     constexpr int kBlock = few_block(S), kTiles = kBlock / 64 / S;
     __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * A * R : 1][64];
