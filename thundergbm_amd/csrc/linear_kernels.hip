@@ -509,9 +509,14 @@ void linear_tiles(hipStream_t s, const Product &p) {
                                                                                                                                                        column_tiles);
 }
 
-// Rows in LDS: as many of their features as fit, all of them where the rows are quantised on the way.
+// Rows in LDS: as many of their features as fit, all of them where the rows are quantised on the way. Every workgroup does that again: it pays where they are few
+// (1 x 4096 x 32000: 25 us, 27 with a launch before; 2 rows: 28 both; 16 x 1024 x 4000: 11, 15; 16 x 1024 x 32000: 20, 14).
 constexpr int kFewLds = 64 * 1024, kFusedMost = 16 * 1024;
-bool quantised_on_the_way(const tgbm_rows &x) { return x.type != TGBM_I8 && x.rows <= 16 && (long long)x.rows * pad_of(x.features) <= kFusedMost; }
+constexpr long long kFusedWork = 200000000;
+bool quantised_on_the_way(const tgbm_rows &x, const tgbm_rows &w) {
+    const long long numbers = (long long)x.rows * pad_of(x.features);
+    return x.type != TGBM_I8 && x.rows <= 16 && numbers <= kFusedMost && numbers * w.rows <= kFusedWork;
+}
 
 template <typename T, int A, int R, int S>
 void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
@@ -604,7 +609,7 @@ void launch_rows_quantise(hipStream_t s, const tgbm_rows &x, signed char *q, lon
 size_t scores_linear_workspace(const tgbm_rows &x, const tgbm_rows &w) {
     const size_t pad = (size_t)pad_of(x.features);
     size_t bytes = packs_weights(w) ? in_lines(pad * w.rows) : 0;
-    if (packs_features(x) && !quantised_on_the_way(x)) bytes += in_lines(pad * packed_rows(x)) + (x.type != TGBM_I8 ? sizeof(float) * (size_t)packed_rows(x) : 0);
+    if (packs_features(x) && !quantised_on_the_way(x, w)) bytes += in_lines(pad * packed_rows(x)) + (x.type != TGBM_I8 ? sizeof(float) * (size_t)packed_rows(x) : 0);
     return bytes;
 }
 
@@ -619,7 +624,7 @@ void launch_scores_linear(hipStream_t s, const tgbm_rows &x, const tgbm_rows &w,
         room += in_lines((size_t)pad * w.rows);
     }
     ScoreOut to{const_cast<void *>(out.data), out.class_stride, out.row_stride, out.type};
-    if (quantised_on_the_way(x)) {
+    if (quantised_on_the_way(x, w)) {
         if (x.type == TGBM_F32) linear_few<float, 1, 1>(s, static_cast<const float *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
         else if (x.type == TGBM_F16) linear_few<_Float16, 1, 1>(s, static_cast<const _Float16 *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
         else linear_few<__bf16, 1, 1>(s, static_cast<const __bf16 *>(x.data), nullptr, x.pitch, x.rows, weights, x.features, bias, to);
