@@ -183,6 +183,22 @@ def test_far_apart_rows_and_long_lists():
         check(S.sample(x.t(), torch.from_numpy(u).cuda(), **how), R.sample(z, u, **how))
 
 
+@pytest.mark.parametrize("order", ["class", "row"])
+@pytest.mark.parametrize("C,n", [(20, 20_000), (20, 300), (100, 17_000), (100, 16_384), (128, 50), (129, 257)])
+def test_ways_of_few_classes(C, n, order):
+    """Few classes with long and short lists of shown ones, many and few rows, counts that cut: each goes another way and wants another workspace."""
+    rng = np.random.default_rng(C + n)
+    z, u = rng.standard_normal((C, n)).astype(np.float32) * 2, numbers(rng, n)
+    rows = np.r_[0:20, n // 2:n // 2 + 10, n - 20:n]
+    at = torch.from_numpy(rows).cuda()
+    for longest in (0, 10, 120):
+        r = D.rules(rng, C, n, sets="some", shown=longest > 0, longest=longest)
+        x = O.adjusted(z, **r)[:, rows]
+        for how in (dict(k=5), dict(k=15, p=0.8), dict(k=40), dict(p=0.6)):
+            got = S.sample(place(z, order), torch.from_numpy(u).cuda(), **on_gpu(r), **how)
+            check([v[at] for v in got], R.sample(x, u[rows], **how))
+
+
 def test_streams_graphs_and_repeats():
     rng = np.random.default_rng(8)
     for C, n, how in ((8, 500, dict()), (700, 200, dict(k=30, p=0.9)), (700, 200, dict(p=0.9)), (20_000, 9, dict(k=300)), (20_000, 9, dict(p=0.8))):

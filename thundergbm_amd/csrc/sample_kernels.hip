@@ -6,7 +6,7 @@
 //
 // 2048 x 65537 bfloat16 cut at a mass of 0.9: 250 us where the memory's share is 53. 47 vector instructions of a wavefront to a score of each lane, 18 of them its
 // weight and place in 64 bits, take two thirds of that; the row is gone over four times (largest score, weights, cut, draw), behind the first from the last cache.
-// 200000 x 100: 442 us (16), about 1100 instructions a row whatever its length. 256 x 128003 bfloat16 with settings of each row: 118 us (13).
+// 50000 x 1000: 190 us (39), 200000 x 100: 234 (16): about 1000 and 600 instructions of a row that its length has no part in. 256 x 128003 bfloat16 with settings of each row: 118 us (13).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -1238,7 +1238,7 @@ constexpr size_t kLaidBytes = (size_t)128 << 20;  // (half of what the last cach
 
 Way way_of(const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how) {
     // (a thread that goes through a long list alone: 24 x 26 with 300 shown classes a row, 172 us)
-    if (in.classes <= kFewClasses && (rules.shown == nullptr || rules.n_shown <= 32ll * in.rows)) return kFew;
+    if (in.classes <= kFewClasses) return rules.shown == nullptr || rules.n_shown <= 32ll * in.rows ? kFew : kMiddle;
     // top's lists where they are short, or the rows long: with more best classes shorter rows' scores overflow them (10343 x 3310, rows side by side, k 120: 1086 us).
     // Two or three launches more: not for few rows (200 x 100, k 20: 22 us, 11 without), and up to 128 classes only for the shortest lists (200000 x 100, k 20: 181 us,
     // 232 without; k 40: 243, 222). A count that cuts nothing is none.
