@@ -165,6 +165,18 @@ def test_many_rows():
             assert torch.equal(z, S.linear(q, w, w_scale, x_scale=scale, order=order))
 
 
+@pytest.mark.parametrize("n,C", [(1024, 32_769), (1024, 32_768 + 130), (33_000, 1000)])
+def test_large_tiles_and_what_is_left_behind_them(n, C):
+    """Lines behind the last whole tile, which go by smaller ones where they would fill no round of their own; the sums as exact numbers of 64 bits."""
+    gen = torch.Generator("cuda").manual_seed(n)
+    q, w = (torch.randint(-127, 128, (r, 640), device="cuda", generator=gen, dtype=torch.int32).to(torch.int8) for r in (n, C))
+    scale, w_scale, bias = torch.rand(n, device="cuda", generator=gen) + 0.5, torch.rand(C, device="cuda", generator=gen) + 0.5, torch.randn(C, device="cuda", generator=gen)
+    total = w.double() @ q.double().t().contiguous()
+    for order in ("row", "class"):
+        z = S.linear(q, w, w_scale, bias=bias, x_scale=scale, order=order)
+        assert torch.equal(z, total.float() * scale * w_scale[:, None] + bias[:, None])
+
+
 def test_two_streams_at_once():
     """Calls that run side by side have workspaces of their own."""
     gen = torch.Generator("cuda").manual_seed(2)
