@@ -544,6 +544,8 @@ void tgbm_predict_sample(int row_size, const float *val, const int *row_ptr, con
                          float learning_rate, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp) {
     std::lock_guard<std::mutex> lock(g_call_mutex);
     TGBM_CHECK(sampling_ok("tgbm_predict_sample", how), "tgbm_predict_sample: wrong arguments");
+    TGBM_CHECK(row_size <= 0 || u != nullptr, "tgbm_predict_sample: u is null");
+    TGBM_CHECK(row_size <= 0 || (classes != nullptr && logp != nullptr), "tgbm_predict_sample: an output is null");
     with_scores("tgbm_predict_sample", row_size, val, row_ptr, col_ptr, model, n_trees, trees_per_iter, learning_rate, rules,
                 [&](hipStream_t s, const tgbm_scores &scores, const tgbm_score_rules &r) {
                     // the rows' numbers side by side: random numbers, settings, then what comes back
