@@ -28,3 +28,20 @@ def refusal(code):
 @pytest.mark.parametrize("arrays,msg", [("None, room, room", "u is null"), ("room, None, room", "an output is null"), ("room, room, None", "an output is null")])
 def test_drawn_answers(arrays, msg):
     assert "tgbm_predict_sample: " + msg in refusal(SAMPLE % (ROOT, arrays))
+
+
+LINEAR = r"""
+import ctypes as C, sys
+sys.path.insert(0, %r)
+import thundergbm_amd as T
+room = (C.c_float * 64)()
+x, weights, values, classes, lse = %s
+T.load().tgbm_linear_top(2, 4, x, 3, weights, None, 2, 1.0, values, classes, lse)
+"""
+
+
+@pytest.mark.parametrize("arrays,msg", [("None, room, room, room, room", "x: null data"), ("room, None, room, room, room", "weights: null data"),
+                                        ("room, room, None, room, room", "an output is null"), ("room, room, room, None, room", "an output is null"),
+                                        ("room, room, room, room, None", "an output is null")])
+def test_a_linear_layer_as_a_teacher(arrays, msg):
+    assert "tgbm_linear_top: " + msg in refusal(LINEAR % (ROOT, arrays))

@@ -585,6 +585,7 @@ void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes
     const tgbm_scores shape{x, 1, (long long)C, TGBM_F32, n_classes, row_size};  // (the address stands for the scores' own)
     TGBM_CHECK(rows_ok(entry, "x", &host_x) && rows_ok(entry, "weights", &host_w) && scores_ok(entry, "scores", &shape), "%s: wrong arguments", entry);
     if (row_size == 0) return;
+    TGBM_CHECK(values != nullptr && classes != nullptr && lse != nullptr, "%s: an output is null", entry);
     hipStream_t s = stream_acquire();
     const size_t width = (F + 127) / 128 * 128;
     const auto alloc = [](size_t bytes) { return device_alloc(std::max<size_t>(bytes, 16)); };
