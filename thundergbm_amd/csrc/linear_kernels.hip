@@ -111,7 +111,8 @@ __global__ __launch_bounds__(G > kLinearBlock ? G : kLinearBlock) void k_quantis
                 if (at + j < pad) to[at + j] = o[j];
         }
     }
-    for (int i = N * G * V + t; i < pad; i += G) to[i] = 0;  // (a padding that is longer than what a launch is chosen for)
+    // (a padding that is longer than what a launch is chosen for; of 2^31 bytes nearly, a place as an int would go round)
+    for (unsigned i = N * G * V + t; i < (unsigned)pad; i += G) to[i] = 0;
 }
 
 // Longer rows: a workgroup reads its row twice.
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(1024) void k_quantise_long(const T *x, long long pi
     const float scale = scale_of(most);
     if (threadIdx.x == 0) scales[blockIdx.x] = scale;
     signed char *to = q + (size_t)blockIdx.x * q_pitch;
-    for (int i = threadIdx.x; i < pad; i += 1024) to[i] = (signed char)(i < features ? whole_of(score_to_float(row[i]), scale) : 0);
+    for (unsigned i = threadIdx.x; i < (unsigned)pad; i += 1024) to[i] = (signed char)(i < (unsigned)features ? whole_of(score_to_float(row[i]), scale) : 0);
 }
 
 // Rows of whole numbers, moved to rows of `pad` bytes, 16 of them to a thread.
