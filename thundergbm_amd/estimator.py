@@ -294,7 +294,7 @@ class TGBMModel(BaseEstimator):
 
     def sample_classes(self, X, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed=None, shown=None, repetition=1.0, frequency=0.0, presence=0.0):
         """A label of every row, drawn by the random numbers u [rows] from the softmax of `class_scores` over the temperature, cut as scores.sample says (k, p, min_p and
-        temperature: numbers, or arrays with one for each row), and its probability among what was kept. Where nothing is allowed the label is NaN and
+        temperature: numbers, or arrays with one for each row, k's of whole numbers), and its probability among what was kept. Where nothing is allowed the label is NaN and
         the probability 0."""
         X = _csr(X)
         n = X.shape[0]
@@ -305,6 +305,11 @@ class TGBMModel(BaseEstimator):
                 v = _one_setting(name, v, *_FINE[name])
                 setattr(h, name + "_all", min(v, self.tree_per_iter) if name == "k" else v)
                 continue
+            if name == "k":  # (of any type of integer: what is below 0 is all classes, like 0, and so is what is above their number)
+                v = np.asarray(v)
+                if v.size and not np.issubdtype(v.dtype, np.integer):
+                    raise ValueError("k: whole numbers are wanted, got an array of %s" % v.dtype)
+                v = np.minimum(np.maximum(v, 0).astype(np.uint64), self.tree_per_iter)
             v = np.ascontiguousarray(v, dtype=np.int32 if name == "k" else np.float32)
             if v.shape != (n,):
                 raise ValueError("%s: a number for each of %d rows is wanted, got the shape %s" % (name, n, v.shape))
