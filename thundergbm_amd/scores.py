@@ -361,7 +361,7 @@ _FINE = {"temperature": (lambda v: v == 0 or 1e-6 <= v <= 1e6, "0 or 1e-6 to 1e6
 def _one_setting(name, v, fine, wanted):
     try:
         number = operator.index(v) if name == "k" else float(v)
-    except (TypeError, ValueError):
+    except (TypeError, ValueError, OverflowError):
         number = None
     if number is None or not fine(number):
         raise ValueError("%s is %r: %s is wanted" % (name, v, wanted))
