@@ -1303,11 +1303,12 @@ void sample_middle(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules 
 }
 
 // Few long rows go by parts.
-size_t split_bytes(int classes, int rows) { return classes >= kSplitLeast ? sizeof(SplitRow) * (size_t)std::min(rows, kSplitRows) : 0; }
+bool goes_by_splits(int classes, int rows) { return rows <= kSplitRows && classes >= kSplitLeast; }
+size_t split_bytes(int classes, int rows) { return goes_by_splits(classes, rows) ? sizeof(SplitRow) * (size_t)rows : 0; }
 
 template <typename T, bool RULES>
 void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &rules, const tgbm_sampling &how, const float *u, int *classes, float *logp, void *room) {
-    if (in.rows <= kSplitRows && in.classes >= kSplitLeast) {
+    if (goes_by_splits(in.classes, in.rows)) {
         const int bits = weight_bits(in.classes), parts = std::min({kSplitParts, in.classes / 4096, std::max(2, 1024 / in.rows)});
         const dim3 grid((unsigned)parts, (unsigned)in.rows);
         SplitRow *splits = static_cast<SplitRow *>(room);
@@ -1371,7 +1372,11 @@ size_t scores_sample_workspace(const tgbm_scores &in, const tgbm_score_rules &ru
     return workspace_of_slices(in.rows, [&](int rows) -> size_t {
         switch (way_of(in, rules, how)) {
             case kFromList: return list_bytes((size_t)rows, (size_t)how.k_all) + scores_top_workspace(rows_side_by_side(in), in.classes, rows, how.k_all);
-            case kLaidOut: return sizeof(float) * (size_t)laid_rows(in.classes, rows) * laid_pitch(in.classes) + split_bytes(in.classes, laid_rows(in.classes, rows));
+            case kLaidOut: {
+                // (as many rows as are laid out at a time, or what is left of them, may go by parts of a row)
+                const int most = laid_rows(in.classes, rows);
+                return sizeof(float) * (size_t)most * laid_pitch(in.classes) + std::max(split_bytes(in.classes, most), split_bytes(in.classes, rows % most));
+            }
             case kRows: return split_bytes(in.classes, rows);
             default: return 0;
         }
