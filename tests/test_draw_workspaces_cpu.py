@@ -1,4 +1,4 @@
-"""The workspace of `sample`: what it is for. Nothing is launched, so no GPU is needed."""
+"""The workspace of `sample`: what it is for, and that less of it is refused. Nothing is launched, so no GPU is needed."""
 import ctypes as C
 
 import pytest
@@ -58,3 +58,19 @@ def test_rows_that_are_laid_out(lib, classes, rows):
     parts = max((SPLIT_ROW * n for n in sizes if n <= SPLIT_ROWS and classes >= 16_384), default=0)
     assert workspace(lib, by_class(classes, rows)) == 4 * most * pitch + parts
     assert workspace(lib, by_row(classes, rows), r=rules(shown=ADDRESS, shown_begin=ADDRESS, n_shown=10 * rows, repetition=1.0)) == 4 * most * pitch + parts
+
+
+WANTED = [(by_class(3000, 10), how(p_all=0.5), rules()), (by_class(3000, 10), how(k_all=5), rules()), (by_row(3000, 10), how(k_all=60), rules()), (by_row(20_000, 3), how(), rules()),
+          (by_class(40_000, 7), how(min_p_all=0.1), rules()), (by_row(40_000, 700), how(), rules(shown=ADDRESS, shown_begin=ADDRESS, n_shown=9, repetition=1.0)), (by_class(100, 100_000), how(k_all=5), rules())]
+
+
+@pytest.mark.parametrize("a,h,r", WANTED)
+def test_less_than_is_needed_is_refused(lib, capfd, a, h, r):
+    need = workspace(lib, a, h, r)
+    assert need > 0
+    call = lambda room, size: lib.tgbm_scores_sample(C.byref(a), C.byref(r), C.byref(h), ADDRESS, ADDRESS, ADDRESS, room, size, None)
+    for room, size, msg in ((ADDRESS, need - 1, "%d bytes of workspace, %d are needed" % (need - 1, need)), (ADDRESS, 0, "0 bytes of workspace"), (None, need, "are needed"),
+                            (None, 0, "are needed"), (ADDRESS + 8, need, "16 bytes"), (ADDRESS + 1, 2 * need, "16 bytes")):
+        assert call(room, size) == 1
+        err = capfd.readouterr().err
+        assert err.startswith("tgbm_scores_sample: ") and msg in err
