@@ -347,7 +347,7 @@ struct ScoreOut {
 constexpr int few_block(int shares) { return shares > 4 ? 64 * shares : kLinearBlock; }
 // (Two wavefronts to a SIMD at least: with more than 256 registers the compiler puts sums into the accumulation registers.)
 template <typename T, int A, int R, int S>
-__global__ __launch_bounds__(few_block(S), S > 4 ? 4 : 2) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
+__global__ __launch_bounds__(few_block(S), S > 8 ? 4 : 2) void k_linear_few(const T *x, const float *x_scales, long long x_pitch, int rows, Rows8 w, int features, const float *bias, ScoreOut out, int slice) {
     constexpr bool kQuantise = sizeof(T) > 1;
     constexpr int kBlock = few_block(S), kTiles = kBlock / 64 / S;
     __shared__ Int4 shared[S > 1 ? kTiles * (S - 1) * A * R : 1][64];
@@ -531,12 +531,13 @@ template <typename T, int A, int R>
 void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, int rows, const Rows8 &w, int features, const float *bias, const ScoreOut &out) {
     const long waves = (long)((w.rows - 1) / (16 * A) + 1) * ((rows - 1) / (16 * R) + 1);
     // More wavefronts share the features where there are few of them (1 x 4096 x 32000, 2000 wavefronts of 16 classes: 26 us, 30 where four share; 8 x 65536 x 100: 62 us
-    // with four, 45 with sixteen).
+    // with four, 45 with sixteen). Where a wavefront has several sums, sixteen of them have too few registers: 24 x 8192 x 1000 takes 24 us with sixteen and 18 with eight,
+    // 100 x 8192 x 500 33 and 26, 64 x 65536 x 100 235 and 250, and the sixteen's scratch of 604 bytes a lane is 320 MB of the device's memory.
     constexpr long kFull = A * R > 1 ? 1024 : 4096;
     if (waves >= kFull || features <= 2 * kChunk) linear_few<T, A, R, 1>(s, x, scale, pitch, rows, w, features, bias, out);
     else if (waves >= std::min(kFull / 2, 1024l) || features <= 4 * kChunk) linear_few<T, A, R, 2>(s, x, scale, pitch, rows, w, features, bias, out);
     else if (waves >= 128 || features <= 16 * kChunk) linear_few<T, A, R, 4>(s, x, scale, pitch, rows, w, features, bias, out);
-    else linear_few<T, A, R, 16>(s, x, scale, pitch, rows, w, features, bias, out);
+    else linear_few<T, A, R, (A * R > 1 ? 8 : 16)>(s, x, scale, pitch, rows, w, features, bias, out);
 }
 
 // Large tiles; the lines behind the last whole one go by small tiles where they would make a round of their own on the chip's 256 CUs (2048 x 4096 x 65537: 565 us, 550
