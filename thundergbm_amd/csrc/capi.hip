@@ -8,6 +8,7 @@
 #include "../../include/thundergbm.h"
 #include "class_scores.h"
 #include "model_handle.h"
+#include "score_slices.h"
 #include "trainer.h"
 
 using namespace tgbm;
@@ -602,8 +603,8 @@ void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes
     float *scale = static_cast<float *>(alloc(sizeof(float) * C)), *d_bias = bias != nullptr ? static_cast<float *>(up(bias, sizeof(float) * C)) : nullptr;
     launch_rows_quantise(s, w, q, (long long)width, (int)width, scale);
     const tgbm_rows w8{q, scale, (long long)width, TGBM_I8, n_classes, n_features, 1};
-    // rows by slices, whose scores take 256 MB
-    const size_t most = std::min<size_t>((size_t)row_size, std::max<size_t>(1, ((size_t)1 << 26) / C));
+    // rows by slices: of their features, scores and lists none takes more than 256 MB
+    const size_t most = (size_t)rows_of_a_slice(row_size, (long long)std::max({F, C, 2 * (size_t)k + 1}));
     float *d_x = static_cast<float *>(alloc(sizeof(float) * most * F)), *d_scores = static_cast<float *>(alloc(sizeof(float) * most * C));
     float *out = static_cast<float *>(alloc(sizeof(float) * most * (2 * (size_t)k + 1)));
     size_t room = 0;

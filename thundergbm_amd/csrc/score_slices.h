@@ -20,4 +20,9 @@ inline std::vector<int> score_slices(const int *row_ptr, int n, long entries, in
     return first;
 }
 
+// Rows of a slice whose widest array has `widest` numbers a row: 256 MB of those, one row at least.
+inline int rows_of_a_slice(long long rows, long long widest) {
+    return (int)std::max(1ll, std::min(rows, (1ll << 26) / std::max(1ll, widest)));
+}
+
 }  // namespace tgbm
