@@ -50,3 +50,18 @@ def test_wide_rows_go_by_slices(device_memory):
     order = np.argsort(-scores, 1, kind="stable")[:, :k]
     np.testing.assert_array_equal(teacher.labels, order.astype(np.float32))
     np.testing.assert_array_equal(teacher.scores, np.take_along_axis(scores, order, 1))
+
+
+def test_weights_go_by_slices(device_memory):
+    """Weights of 1.5 slices: what stays of them is their 8 bits."""
+    n, F, C_, k = 4096, 4096, 24_576, 5
+    x, w = whole_numbers(n, F, 0), whole_numbers(C_, F, 3)
+    bias = (np.arange(C_) % 5).astype(np.float32)
+    teacher, bytes_held = held(device_memory, lambda: T.Teacher.linear(x, w, np.arange(C_), bias=bias, k=k))
+    # the slice that either of them comes through, the weights in 8 bits, 2730 rows' scores, their features in 8 bits; lists, what top wants beside them and the like
+    assert bytes_held < (1 << 28) + C_ * F + (1 << 28) + (1 << 24) + (1 << 25), bytes_held
+    some = np.array([0, 1, 2729, 2730, 2731, n - 1])
+    scores = (x[some] @ w.T + bias).astype(np.float64)
+    order = np.argsort(-scores, 1, kind="stable")[:, :k]
+    np.testing.assert_array_equal(teacher.labels[some], order.astype(np.float32))
+    np.testing.assert_array_equal(teacher.scores[some], np.take_along_axis(scores, order, 1))

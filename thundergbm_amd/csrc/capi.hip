@@ -590,33 +590,33 @@ void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes
     hipStream_t s = stream_acquire();
     const size_t width = (F + 127) / 128 * 128;
     const auto alloc = [](size_t bytes) { return device_alloc(std::max<size_t>(bytes, 16)); };
-    const auto up = [&](const void *from, size_t bytes) {
-        void *to = alloc(bytes);
-        upload_large(s, to, from, bytes);
-        return to;
-    };
-    // the weights in 8 bits, once
-    tgbm_rows w = host_w;
-    void *d_weights = up(weights, sizeof(float) * C * F);
-    w.data = d_weights;
+    // Rows by slices: of their features, scores and lists none takes more than 256 MB. The weights come the same way first, through the same memory: once they are
+    // in 8 bits nothing else of them is wanted.
+    const size_t most = (size_t)rows_of_a_slice(row_size, (long long)std::max({F, C, 2 * (size_t)k + 1})), classes_of_one = (size_t)rows_of_a_slice(n_classes, (long long)F);
+    float *d_x = static_cast<float *>(alloc(sizeof(float) * std::max(most, classes_of_one) * F)), *d_scores = static_cast<float *>(alloc(sizeof(float) * most * C));
+    const auto rows_of = [&](size_t n) { return tgbm_rows{d_x, nullptr, (long long)F, TGBM_F32, (int)n, n_features, 0}; };
     signed char *q = static_cast<signed char *>(alloc(C * width));
-    float *scale = static_cast<float *>(alloc(sizeof(float) * C)), *d_bias = bias != nullptr ? static_cast<float *>(up(bias, sizeof(float) * C)) : nullptr;
-    launch_rows_quantise(s, w, q, (long long)width, (int)width, scale);
+    float *scale = static_cast<float *>(alloc(sizeof(float) * C)), *d_bias = nullptr;
+    for (size_t c = 0; c < C; c += classes_of_one) {
+        const size_t n = std::min(classes_of_one, C - c);
+        upload_large(s, d_x, weights + c * F, sizeof(float) * n * F);
+        launch_rows_quantise(s, rows_of(n), q + c * width, (long long)width, (int)width, scale + c);
+    }
+    if (bias != nullptr) {
+        d_bias = static_cast<float *>(alloc(sizeof(float) * C));
+        upload_large(s, d_bias, bias, sizeof(float) * C);
+    }
     const tgbm_rows w8{q, scale, (long long)width, TGBM_I8, n_classes, n_features, 1};
-    // rows by slices: of their features, scores and lists none takes more than 256 MB
-    const size_t most = (size_t)rows_of_a_slice(row_size, (long long)std::max({F, C, 2 * (size_t)k + 1}));
-    float *d_x = static_cast<float *>(alloc(sizeof(float) * most * F)), *d_scores = static_cast<float *>(alloc(sizeof(float) * most * C));
     float *out = static_cast<float *>(alloc(sizeof(float) * most * (2 * (size_t)k + 1)));
     size_t room = 0;
     const auto slice = [&](size_t r) { return (int)std::min(most, (size_t)row_size - r); };
-    const auto rows_of = [&](int n) { return tgbm_rows{d_x, nullptr, (long long)F, TGBM_F32, n, n_features, 0}; };
-    for (const int n : {slice(0), slice((size_t)(row_size - 1) / most * most)}) room = std::max({room, scores_linear_workspace(rows_of(n), w8), scores_top_workspace(false, n_classes, n, k)});
+    for (const int n : {slice(0), slice((size_t)(row_size - 1) / most * most)}) room = std::max({room, scores_linear_workspace(rows_of((size_t)n), w8), scores_top_workspace(false, n_classes, n, k)});
     void *workspace = alloc(room);
     for (size_t r = 0; r < (size_t)row_size; r += most) {
         const int n = slice(r);
         upload_large(s, d_x, x + r * F, sizeof(float) * (size_t)n * F);
         const tgbm_scores scores{d_scores, 1, (long long)C, TGBM_F32, n_classes, n};
-        launch_scores_linear(s, rows_of(n), w8, d_bias, scores, workspace);
+        launch_scores_linear(s, rows_of((size_t)n), w8, d_bias, scores, workspace);
         int *d_classes = reinterpret_cast<int *>(out + (size_t)n * k);
         float *d_lse = out + 2 * (size_t)n * k;
         launch_scores_top(s, scores, tgbm_score_rules{}, k, temperature, out, d_classes, d_lse, workspace);
@@ -626,7 +626,7 @@ void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes
         HIP_CHECK(hipMemcpyAsync(lse + r, d_lse, sizeof(float) * (size_t)n, hipMemcpyDeviceToHost, s));
         HIP_CHECK(hipStreamSynchronize(s));
     }
-    for (void *p : {d_weights, (void *)q, (void *)scale, (void *)d_bias, (void *)d_x, (void *)d_scores, (void *)out, workspace}) device_free(p);
+    for (void *p : {(void *)q, (void *)scale, (void *)d_bias, (void *)d_x, (void *)d_scores, (void *)out, workspace}) device_free(p);
     stream_release(s);
 }
 
