@@ -9,7 +9,7 @@ from thundergbm_amd import scores as S
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("C,n", [(20_000, 1677 + 3), (20_000, 1677 + 385), (40_000, 838 + 384)])
+@pytest.mark.parametrize("C,n", [(20_000, 1677 + 3), (70_000, 479 + 3), (70_000, 479 + 385), (65_536, 512 + 384)])
 def test_what_is_left_of_the_slices(C, n):
     gen = torch.Generator("cuda").manual_seed(n)
     z = torch.randn(C, n, device="cuda", generator=gen) * 3

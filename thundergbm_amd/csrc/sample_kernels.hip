@@ -948,7 +948,11 @@ __global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score
 // Few long rows: parts of a row by a workgroup each, in four launches. The largest score; the weights' buckets, added up over the parts as the whole numbers that they
 // are, and where a number of classes cuts how many there are in each; the scores of the buckets where the cuts and the draw can be; the draw among those. One workgroup
 // to a row took 58 us for 1 x 128003 bfloat16, 116 for 8 of them, 167 for 256 with settings of each row.
-constexpr int kSplitBlock = 512, kSplitParts = 64, kSplitRows = 384, kSplitLeast = 16384, kSplitListed = chosen_of<kSplitBlock>();
+// Where it pays hangs on the length first (bfloat16, us by parts and by whole rows). Cut at a mass of 0.9: 64 x 16384 33 and 23, 64 x 32768 42 and 34, 256 x 32768 56 and 37,
+// 1 x 65536 36 and 43, 64 x 65536 56 and 50, 64 x 100000 63 and 98, 384 x 128003 154 and 241. With settings of each row: 256 x 32768 61 and 44, 64 x 65536 61 and 83,
+// 256 x 128003 137 and 235, 384 x 128003 172 and 198. Beyond that many rows the chip is full either way, and whole rows launch once (512 x 32768 72 and 49).
+// (A least probability or a count alone leave so little of a row that it does not pay up to 250 000 classes: 256 x 128003 62 and 34, 92 and 46.)
+constexpr int kSplitBlock = 512, kSplitParts = 64, kSplitRows = 384, kSplitLeast = 65536, kSplitListed = chosen_of<kSplitBlock>();
 struct SplitRow {
     unsigned long long mass[Scale<parts_of<kSplitBlock>()>::kBuckets];
     unsigned long long listed[kSplitListed];
