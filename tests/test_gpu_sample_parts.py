@@ -18,6 +18,18 @@ def test_around_the_length(C, n):
     G.test_few_long_rows(C, n)
 
 
+@pytest.mark.parametrize("C,n", [(16_383, 3), (16_384, 3), (9000, 256), (9000, 257), (20_000, 256), (20_000, 257)])
+def test_threads_of_a_row(C, n):
+    """A workgroup has more threads where rows are long, and as few as there are CUs."""
+    rng = np.random.default_rng(C)
+    z = G.rounded(rng.standard_normal((C, n)).astype(np.float32) * 2, torch.float16)
+    u = G.numbers(rng, n)
+    rows = np.r_[0:3, n // 2, n - 2:n]
+    for how in (dict(), dict(p=0.9), dict(k=600, p=0.7, temperature=0.8), dict(min_p=0.05)):
+        got = S.sample(place(z, "row", torch.float16, pad=1), torch.from_numpy(u).cuda(), **how)
+        G.check(got, R.sample(z[:, rows], u[rows], **how), rows)
+
+
 @pytest.mark.parametrize("order", ["class", "row"])
 @pytest.mark.parametrize("how", [dict(k=300), dict(p=0.8), dict(k=700, p=0.9, min_p=1e-4)])
 def test_streams_graphs_and_repeats(how, order):

@@ -1322,9 +1322,12 @@ void sample_rows(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &r
         k_split_draw<T, RULES><<<in.rows, kSplitBlock, 0, s>>>(in, rules, how, u, splits, parts, classes, logp, bits);
         return;
     }
+    // Threads of a row's workgroup. 256 for a few vectors each (cut at a mass of 0.9, us with 256 and 512: 20000 x 4096 float32 353 and 460, 300 x 4096 17 and 15); 1024 where each CU has a row at
+    // most, and that is long (us with 512 and 1024: 256 x 5000 float32 14 and 16, 256 x 16384 bfloat16 25 and 26, with k 500 33 and 24, 256 x 32768 39 and 37, with k 500 50 and 27;
+    // 384 x 32768, more rows than CUs, 47 and 61).
     const int bits = weight_bits(in.classes), vectors = (in.classes - 1) / (16 / (int)sizeof(T)) + 1;
     if (vectors <= 4 * 256) k_sample_rows<T, 256, RULES><<<in.rows, 256, 0, s>>>(in, rules, how, u, classes, logp, bits);
-    else if (in.rows > 256) k_sample_rows<T, 512, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
+    else if (in.rows > 256 || in.classes < 16384) k_sample_rows<T, 512, RULES><<<in.rows, 512, 0, s>>>(in, rules, how, u, classes, logp, bits);
     else k_sample_rows<T, 1024, RULES><<<in.rows, 1024, 0, s>>>(in, rules, how, u, classes, logp, bits);
 }
 template <typename T>
