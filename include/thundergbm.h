@@ -295,7 +295,7 @@ typedef struct tgbm_sampling {
  * of the scores and of equal scores the lower class first, where the sum of the probabilities passes u[row]; u from 0 (the best class) up to, not
  * including, 1, what is beyond counts as the ends. logp, [rows]: the logarithm of the drawn class's probability among those that are kept. Classes whose
  * score is -infinity or NaN are never drawn; infinite scores share alike. Where nothing is left a row gets class -1 and -infinity, where one of its numbers is NaN
- * class -1 and NaN. Sums are 64 bits; a probability below 2^-64 of the best one's counts as none. workspace: as for tgbm_scores_top,
+ * class -1 and NaN. Sums are 64 bits, of weights that are rounded by about 2^-46 of themselves at most (beyond 2^16 classes by more, 2^-40 at 2^22); a probability below 2^-64 of the best one's counts as none. workspace: as for tgbm_scores_top,
  * from a multiple of 16 bytes on. */
 size_t tgbm_scores_sample_workspace(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how);
 int tgbm_scores_sample(const tgbm_scores *in, const tgbm_score_rules *rules, const tgbm_sampling *how, const float *u, int *classes, float *logp,
@@ -381,7 +381,8 @@ void tgbm_predict_sample(int row_size, const float *val, const int *row_ptr, con
                          int *classes, float *logp);
 
 /* The k best classes of a linear layer, as a teacher's: host arrays x [row_size][n_features], weights [n_classes][n_features] and bias [n_classes] (may be NULL), in
- * 8 bits each with a scale as tgbm_rows_quantise makes them; the outputs as tgbm_scores_top writes them. Wrong arguments abort the process. */
+ * 8 bits each with a scale as tgbm_rows_quantise makes them; the outputs as tgbm_scores_top writes them. The device holds the weights in 8 bits and a slice of rows, of whose features,
+ * scores and lists none takes more than 256 MB. Wrong arguments, null outputs among them, abort the process. */
 void tgbm_linear_top(int row_size, int n_features, const float *x, int n_classes, const float *weights, const float *bias, int k, float temperature,
                      float *values, int *classes, float *lse);
 

@@ -7,7 +7,7 @@
 // Rows are brought to a common form first, kChunk features at a time with zeros behind the last: where a row of features is zero it does not matter what
 // the weights' rows hold there.
 //
-// 8192 x 8192 x 32000: 1.89 ms, 2.27 POP/s (the library's 8-bit product of 8192^3: 2.13). The matrix units are busy 62 % of the cycles, and the clock is at 1.53 GHz: power bounds
+// 8192 x 8192 x 32000: 1.85 ms, 2.32 POP/s (the library's 8-bit product of 8192^3: 2.13). The matrix units are busy 62 % of the cycles, and the clock is at 1.53 GHz: power bounds
 // it. 1 x 4096 x 32000: 25 us of the kernel for 131 MB, 5.2 TB/s. 100003 x 200 x 500 float32: 88 us, of which the rows' quantisation takes 24, where the memory's share is 55.
 #include <algorithm>
 
@@ -532,7 +532,7 @@ void linear_few(hipStream_t s, const T *x, const float *scale, long long pitch, 
     const long waves = (long)((w.rows - 1) / (16 * A) + 1) * ((rows - 1) / (16 * R) + 1);
     // More wavefronts share the features where there are few of them (1 x 4096 x 32000, 2000 wavefronts of 16 classes: 26 us, 30 where four share; 8 x 65536 x 100: 62 us
     // with four, 45 with sixteen). Where a wavefront has several sums, sixteen of them have too few registers: 24 x 8192 x 1000 takes 24 us with sixteen and 18 with eight,
-    // 100 x 8192 x 500 33 and 26, 64 x 65536 x 100 235 and 250, and the sixteen's scratch of 604 bytes a lane is 320 MB of the device's memory.
+    // 100 x 8192 x 500 33 and 26, 64 x 65536 x 100 235 and 250 (with the weights in the last cache), and the sixteen's scratch of 604 bytes a lane is 320 MB of the device's memory.
     constexpr long kFull = A * R > 1 ? 1024 : 4096;
     if (waves >= kFull || features <= 2 * kChunk) linear_few<T, A, R, 1>(s, x, scale, pitch, rows, w, features, bias, out);
     else if (waves >= std::min(kFull / 2, 1024l) || features <= 4 * kChunk) linear_few<T, A, R, 2>(s, x, scale, pitch, rows, w, features, bias, out);

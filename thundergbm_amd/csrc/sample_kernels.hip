@@ -4,9 +4,10 @@
 // order, and so the class that is drawn is the one where the sum of w passes u times the sum of what is kept. A sum over all classes decides which of two
 // classes it is, so everything is 64 bits, and what many threads add up is added as whole numbers, whose sum has no order.
 //
-// 2048 x 65537 bfloat16 cut at a mass of 0.9: 250 us where the memory's share is 53. 47 vector instructions of a wavefront to a score of each lane, 18 of them its
+// 2048 x 65537 bfloat16 cut at a mass of 0.9: 248 us where the memory's share is 53. 47 vector instructions of a wavefront to a score of each lane, 18 of them its
 // weight and place in 64 bits, take two thirds of that; the row is gone over four times (largest score, weights, cut, draw), behind the first from the last cache.
-// 50000 x 1000: 190 us (39), 200000 x 100: 234 (16): about 1000 and 600 instructions of a row that its length has no part in. 256 x 128003 bfloat16 with settings of each row: 118 us (13).
+// 50000 x 1000: 195 us (39), 200000 x 100: 204 (16): about 1000 and 600 instructions of a row that its length has no part in. 256 x 128003 bfloat16 with settings of each row: 122 us (13).
+// Rows of equal scores are one bucket's, and all of their additions go to one place: 1305 us for 50000 x 1000, 9.7 ms for 2048 x 65537, 3.6 for 1 x 128003.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -339,7 +340,7 @@ struct Scale {
 constexpr double kToWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest whole number
 
 // 2^(-h / P), h in [-1/2, 1/2], plus `magic` = 2^(52 - bits): its last 52 bits are the power of two times 2^bits, rounded. Taylor's series, up to where the next term
-// is below 2^-48 of the whole; 2^-46 is what a whole number of a row of 2^16 classes is rounded by.
+// is below 2^-48 of the whole; 2^-46 is what a whole number of a row of 2^16 classes is rounded by (weight_bits).
 template <int P>
 __device__ __forceinline__ unsigned long long part_of_two(double h, double magic) {
     constexpr double a = -0.69314718055994530942 / P, c2 = a * a / 2, c3 = c2 * a / 3, c4 = c3 * a / 4, c5 = c4 * a / 5, c6 = c5 * a / 6, c7 = c6 * a / 7;
@@ -937,6 +938,7 @@ __device__ __forceinline__ ScoreRow<T, G, RULES> row_of(const tgbm_scores &in, c
     if constexpr (RULES) scores.words = allowed_words(rules, row, (in.classes + 31) / 32, &scores.none);
     return scores;
 }
+// (128 registers a lane are a few too few for all that a row may need: 1 to 37 are spilled)
 template <typename T, int G, bool RULES>
 __global__ __launch_bounds__(G, 4) void k_sample_rows(tgbm_scores in, tgbm_score_rules rules, tgbm_sampling how, const float *u, int *classes, float *logp, int bits) {
     __shared__ DrawShared<G> sh;
@@ -1275,7 +1277,8 @@ void sample_few(hipStream_t s, const tgbm_scores &in, const tgbm_score_rules &ru
     else k_sample_few<T, 32><<<blocks, kSampleBlock, 0, s>>>(in, rules, how, u, classes, logp);
 }
 
-// Bits of a whole number that stands for a w of one: the sum of a row's, of which w is at most 1.05 in a bucket, has room in 63.
+// Bits of a whole number that stands for a w of one: the sum of a row's, of which w is at most 1.05 in a bucket, has room in 63. 50 up to 2^11 classes, 45 at 2^16, 39 at 2^22: a weight is
+// rounded by 2^-40 of itself at most, where a random number's last place is 2^-24.
 int weight_bits(int classes) {
     int log_classes = 0;
     while ((1 << log_classes) < classes) ++log_classes;

@@ -392,7 +392,8 @@ def sample(scores, u, k=0, p=1.0, min_p=0.0, temperature=1.0, bias=None, allowed
     above 1 is 1, a min_p below 0 is 0, temperatures below 1e-6 are 0 and above 1e6 are that.
 
     Classes whose score is -inf or NaN are never drawn. A row that nothing is left of gets class -1 and -inf, one with a NaN among its numbers class -1 and NaN.
-    Sums are 64 bits, and the same call draws the same classes; a class with less than 2^-64 of the best one's probability counts as one without."""
+    Sums are 64 bits, of probabilities that are rounded by about 2^-46 of themselves at most (beyond 2^16 classes by more, 2^-40 at 2^22), and the same call draws the same
+    classes; a class with less than 2^-64 of the best one's probability counts as one without."""
     torch = _torch()
     s = _scores(torch, "scores", scores)
     r = _rules(torch, scores, bias, allowed, allowed_set, shown, shown_begin, repetition, frequency, presence)
